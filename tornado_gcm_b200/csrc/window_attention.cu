@@ -1,0 +1,428 @@
+// Attention in a sliding window with a few first tokens always in sight:
+// the CUDA-core kernels (any head size up to 128, bf16 or fp32) and the
+// operators' host side.
+//
+// With z_ij = q_i . k_j * scale over the keys in sight of query i:
+//   m = max_j z,  l = sum_j exp(z - m),  o_i = sum_j exp(z - m) v_j / l,
+//   lse_i = m + log l  (kept in base 2; a row that sees nothing: o = 0, lse = inf).
+// Backward, with p_ij = exp(z_ij - lse_i) and delta_i = dO_i . O_i:
+//   dv_j = sum_i p_ij dO_i,   ds_ij = p_ij (dO_i . v_j - delta_i) * scale,
+//   dq_i = sum_j ds_ij k_j,   dk_j = sum_i ds_ij q_i,
+// the sums over i running over every query head that shares the key head.
+//
+// These kernels are bound by fp32 FMAs (2 D per pair and product).  Four
+// threads share a row (query rows forward and for dq, key rows for dk and dv)
+// and hold its vectors in registers, float4 pieces dealt out in turn, so a
+// row of the other side, staged in shared memory as fp32, is read as four
+// 16-byte broadcasts per step.  dk and dv take every query that sees the key
+// in one block: no atomics, so gradients have the same bits every time.
+#include "alloc.h"
+
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+
+#include <algorithm>
+#include <cmath>
+#include <string>
+
+#include "common.cuh"
+#include "window_attention.h"
+
+namespace tgcm {
+
+namespace {
+
+constexpr int kRows = 32;                // rows of a block
+constexpr int kTile = 32;                // staged rows of the other side
+constexpr int kWinThreads = 4 * kRows;
+
+template <typename T>
+__device__ __forceinline__ float ldw(const T* p) {
+  if constexpr (std::is_same<T, float>::value)
+    return *p;
+  else
+    return __bfloat162float(*p);
+}
+template <typename T>
+__device__ __forceinline__ void stw(T* p, float v) {
+  if constexpr (std::is_same<T, float>::value)
+    *p = v;
+  else
+    *p = __float2bfloat16(v);
+}
+
+// The thread's share of one row: float4 pieces part, part + 4, ...
+template <typename T, int N>
+__device__ __forceinline__ void load_share(const T* row, int D, int part, bool on, float (&v)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = 4 * (part + 4 * (i / 4)) + i % 4;
+    v[i] = (on && d < D) ? ldw(row + d) : 0.f;
+  }
+}
+template <typename T, int N>
+__device__ __forceinline__ void store_share(T* row, int D, int part, bool on, const float (&v)[N], float f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = 4 * (part + 4 * (i / 4)) + i % 4;
+    if (on && d < D) stw(row + d, v[i] * f);
+  }
+}
+
+// Rows [j0, j0 + kTile) below `end` into shared memory, zero elsewhere.
+template <typename T, int DP>
+__device__ __forceinline__ void stage_rows(float* s, const T* g, long long stride, int j0, int end, int D) {
+  for (int e = threadIdx.x; e < kTile * DP; e += kWinThreads) {
+    const int r = e / DP, d = e % DP;
+    const int j = j0 + r;
+    s[e] = (j < end && d < D) ? ldw(g + j * stride + d) : 0.f;
+  }
+}
+
+template <int N>
+__device__ __forceinline__ float dot_share(const float (&a)[N], const float* row, int part) {
+  float s = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(row + 4 * (part + i));
+    s = fmaf(a[i], b.x, s);
+    s = fmaf(a[i + 1], b.y, s);
+    s = fmaf(a[i + 2], b.z, s);
+    s = fmaf(a[i + 3], b.w, s);
+  }
+  s += __shfl_xor_sync(0xffffffffu, s, 1);
+  s += __shfl_xor_sync(0xffffffffu, s, 2);
+  return s;
+}
+template <int N>
+__device__ __forceinline__ void axpy_share(float (&a)[N], float f, const float* row, int part) {
+#pragma unroll
+  for (int i = 0; i < N; i += 4) {
+    const float4 b = *reinterpret_cast<const float4*>(row + 4 * (part + i));
+    a[i] = fmaf(f, b.x, a[i]);
+    a[i + 1] = fmaf(f, b.y, a[i + 1]);
+    a[i + 2] = fmaf(f, b.z, a[i + 2]);
+    a[i + 3] = fmaf(f, b.w, a[i + 3]);
+  }
+}
+
+// Keys in sight of some query of [i0, i0 + n): sinks [0, *se) and window [*lo, *hi).
+__device__ __forceinline__ void key_ranges(const WinParams& p, int L, int i0, int n, int* se, int* lo, int* hi) {
+  const int last = min(i0 + n, p.S) - 1;
+  *lo = max(0, i0 - (p.window - 1));
+  *hi = min(L, p.causal ? last + 1 : last + p.window);
+  *se = min(min(p.sinks, *lo), L);
+}
+
+template <typename T, int DP>
+__global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(const WinParams p) {
+  constexpr int N = DP / 4;
+  __shared__ __align__(16) float ks[kTile * DP];
+  __shared__ __align__(16) float vs[kTile * DP];
+  const int part = threadIdx.x & 3, r = threadIdx.x >> 2;
+  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+  const int i0 = blockIdx.x * kRows, i = i0 + r;
+  const bool on = i < p.S;
+  const int L = win_length(p, b);
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  float q[N], acc[N];
+  load_share<T, N>(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + h * p.q_sh, p.D, part, on, q);
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    q[e] *= p.scale * kLog2e;
+    acc[e] = 0.f;
+  }
+  float m = -INFINITY, l = 0.f;
+  int se, lo, hi;
+  key_ranges(p, L, i0, kRows, &se, &lo, &hi);
+  for (int phase = 0; phase < 2; ++phase) {
+    const int end = phase ? hi : se;
+    for (int j0 = phase ? lo : 0; j0 < end; j0 += kTile) {
+      __syncthreads();
+      stage_rows<T, DP>(ks, kb, p.k_ss, j0, end, p.D);
+      stage_rows<T, DP>(vs, vb, p.v_ss, j0, end, p.D);
+      __syncthreads();
+      const int n = min(kTile, end - j0);
+      for (int t = 0; t < n; ++t) {
+        const float z = dot_share<N>(q, ks + t * DP, part);
+        if (!win_sees(p, L, i, j0 + t)) continue;  // the four threads of a row agree
+        const float mn = fmaxf(m, z);
+        if (mn > m) {
+          const float c = exp2f(m - mn);  // 0 for the row's first key
+          l *= c;
+#pragma unroll
+          for (int e = 0; e < N; ++e) acc[e] *= c;
+          m = mn;
+        }
+        const float w = z == -INFINITY ? 0.f : exp2f(z - m);  // m may be -inf still
+        l += w;
+        axpy_share<N>(acc, w, vs + t * DP, part);
+      }
+      __syncwarp();
+    }
+  }
+  const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+  store_share<T, N>(static_cast<T*>(p.o) + ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D, p.D, part, on, acc,
+                    inv);
+  if (on && part == 0)
+    p.lse[(static_cast<long long>(b) * p.H + h) * p.S + i] = l == 0.f ? INFINITY : m + log2f(l);
+}
+
+// dq and delta; rows are queries.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kWinThreads) win_dq_kernel(const WinParams p) {
+  constexpr int N = DP / 4;
+  __shared__ __align__(16) float ks[kTile * DP];
+  __shared__ __align__(16) float vs[kTile * DP];
+  const int part = threadIdx.x & 3, r = threadIdx.x >> 2;
+  const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+  const int i0 = blockIdx.x * kRows, i = i0 + r;
+  const bool on = i < p.S;
+  const int L = win_length(p, b);
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
+  const long long orow = ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D;
+  const long long srow = (static_cast<long long>(b) * p.H + h) * p.S + i;
+  float q[N], g[N], acc[N];
+  load_share<T, N>(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_ss + h * p.q_sh, p.D, part, on, q);
+  load_share<T, N>(static_cast<const T*>(p.dout) + b * p.g_sb + i * p.g_ss + h * p.g_sh, p.D, part, on, g);
+  load_share<T, N>(static_cast<const T*>(p.o) + orow, p.D, part, on, acc);
+  float delta = 0.f;
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    delta = fmaf(g[e], acc[e], delta);
+    q[e] *= p.scale * kLog2e;
+    acc[e] = 0.f;
+  }
+  delta += __shfl_xor_sync(0xffffffffu, delta, 1);
+  delta += __shfl_xor_sync(0xffffffffu, delta, 2);
+  const float lse = on ? p.lse[srow] : INFINITY;
+  if (on && part == 0) p.delta[srow] = delta;
+  int se, lo, hi;
+  key_ranges(p, L, i0, kRows, &se, &lo, &hi);
+  for (int phase = 0; phase < 2; ++phase) {
+    const int end = phase ? hi : se;
+    for (int j0 = phase ? lo : 0; j0 < end; j0 += kTile) {
+      __syncthreads();
+      stage_rows<T, DP>(ks, kb, p.k_ss, j0, end, p.D);
+      stage_rows<T, DP>(vs, vb, p.v_ss, j0, end, p.D);
+      __syncthreads();
+      const int n = min(kTile, end - j0);
+      for (int t = 0; t < n; ++t) {
+        const float z = dot_share<N>(q, ks + t * DP, part);
+        const float dp = dot_share<N>(g, vs + t * DP, part);
+        if (!win_sees(p, L, i, j0 + t)) continue;
+        axpy_share<N>(acc, exp2f(z - lse) * (dp - delta), ks + t * DP, part);
+      }
+      __syncwarp();
+    }
+  }
+  store_share<T, N>(static_cast<T*>(p.dq) + orow, p.D, part, on, acc, p.scale);
+}
+
+// dk and dv; rows are keys, the staged side the queries of each head that shares them.
+template <typename T, int DP>
+__global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(const WinParams p) {
+  constexpr int N = DP / 4;
+  __shared__ __align__(16) float qs[kTile * DP];
+  __shared__ __align__(16) float gs[kTile * DP];
+  __shared__ float ls[kTile], ds[kTile];
+  const int part = threadIdx.x & 3, r = threadIdx.x >> 2;
+  const int hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hk;
+  const int j0 = blockIdx.x * kRows, j = j0 + r;
+  const int L = win_length(p, b);
+  const bool on = j < L;
+  float k[N], v[N], dk[N], dv[N];
+  load_share<T, N>(static_cast<const T*>(p.k) + b * p.k_sb + j * p.k_ss + hk * p.k_sh, p.D, part, on, k);
+  load_share<T, N>(static_cast<const T*>(p.v) + b * p.v_sb + j * p.v_ss + hk * p.v_sh, p.D, part, on, v);
+#pragma unroll
+  for (int e = 0; e < N; ++e) {
+    k[e] *= p.scale * kLog2e;
+    dk[e] = dv[e] = 0.f;
+  }
+  const bool sink = j0 < p.sinks;
+  const int lo = p.causal ? j0 : (sink ? 0 : max(0, j0 - (p.window - 1)));
+  const int hi = j0 >= L ? 0
+                         : (sink ? p.S
+                                 : static_cast<int>(min(static_cast<long long>(p.S),
+                                                        static_cast<long long>(j0) + kRows - 1 + p.window)));
+  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+    const T* qb = static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
+    const T* gb = static_cast<const T*>(p.dout) + b * p.g_sb + h * p.g_sh;
+    const long long srow = (static_cast<long long>(b) * p.H + h) * p.S;
+    for (int i0 = lo; i0 < hi; i0 += kTile) {
+      __syncthreads();
+      stage_rows<T, DP>(qs, qb, p.q_ss, i0, hi, p.D);
+      stage_rows<T, DP>(gs, gb, p.g_ss, i0, hi, p.D);
+      const int n = min(kTile, hi - i0);
+      if (static_cast<int>(threadIdx.x) < n) {
+        ls[threadIdx.x] = p.lse[srow + i0 + threadIdx.x];
+        ds[threadIdx.x] = p.delta[srow + i0 + threadIdx.x];
+      }
+      __syncthreads();
+      for (int t = 0; t < n; ++t) {
+        const float z = dot_share<N>(k, qs + t * DP, part);
+        const float dp = dot_share<N>(v, gs + t * DP, part);
+        if (!win_sees(p, L, i0 + t, j)) continue;
+        const float w = exp2f(z - ls[t]);
+        axpy_share<N>(dv, w, gs + t * DP, part);
+        axpy_share<N>(dk, w * (dp - ds[t]), qs + t * DP, part);
+      }
+      __syncwarp();
+    }
+  }
+  const bool in = j < p.S;
+  const long long row = ((static_cast<long long>(b) * p.S + j) * p.Hk + hk) * p.D;
+  store_share<T, N>(static_cast<T*>(p.dk) + row, p.D, part, in, dk, p.scale);
+  store_share<T, N>(static_cast<T*>(p.dv) + row, p.D, part, in, dv, 1.f);
+}
+
+template <typename F>
+void by_dim(int D, F&& f) {
+  if (D <= 16)
+    f(std::integral_constant<int, 16>());
+  else if (D <= 32)
+    f(std::integral_constant<int, 32>());
+  else if (D <= 64)
+    f(std::integral_constant<int, 64>());
+  else
+    f(std::integral_constant<int, 128>());
+}
+
+dim3 row_grid(const WinParams& p, int heads) {
+  return dim3((p.S + kRows - 1) / kRows, heads, p.B);
+}
+
+void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks) {
+  for (const auto* t : {&q, &k, &v}) {
+    TORCH_CHECK(t->is_cuda() && t->device() == q.device(), "window_attention: CUDA tensors of one device expected");
+    TORCH_CHECK(t->dim() == 4, "window_attention: (batch, sequence, heads, head_dim) tensors expected");
+    TORCH_CHECK(t->scalar_type() == q.scalar_type() &&
+                    (t->scalar_type() == at::kBFloat16 || t->scalar_type() == at::kFloat),
+                "window_attention: q, k and v share one type, bf16 or fp32");
+    TORCH_CHECK(t->size(3) == 1 || t->stride(3) == 1, "window_attention: head_dim must be contiguous");
+  }
+  TORCH_CHECK(k.sizes() == v.sizes(), "window_attention: k and v differ in shape");
+  TORCH_CHECK(q.size(0) == k.size(0) && q.size(1) == k.size(1) && q.size(3) == k.size(3),
+              "window_attention: q and k differ in batch, sequence or head_dim");
+  TORCH_CHECK(k.size(2) >= 1 && q.size(2) % k.size(2) == 0,
+              "window_attention: the query heads must be a multiple of the key heads");
+  TORCH_CHECK(q.size(3) >= 1 && q.size(3) <= 128, "window_attention: head_dim 1 to 128 expected, got " + std::to_string(q.size(3)));
+  TORCH_CHECK(window >= 1, "window_attention: the window must hold at least the token itself, got " + std::to_string(window));
+  TORCH_CHECK(sinks >= 0, "window_attention: sinks must not be negative, got " + std::to_string(sinks));
+  TORCH_CHECK(q.size(0) <= 65535 && q.size(2) <= 65535 && q.size(1) <= (1ll << 30),
+              "window_attention: batch and heads up to 65535, sequences up to 2^30");
+}
+
+WinParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks,
+                    bool causal, const c10::optional<at::Tensor>& lengths, double scale) {
+  check_qkv(q, k, v, window, sinks);
+  WinParams p{};
+  p.q = q.data_ptr();
+  p.k = k.data_ptr();
+  p.v = v.data_ptr();
+  p.q_sb = q.stride(0), p.q_ss = q.stride(1), p.q_sh = q.stride(2);
+  p.k_sb = k.stride(0), p.k_ss = k.stride(1), p.k_sh = k.stride(2);
+  p.v_sb = v.stride(0), p.v_ss = v.stride(1), p.v_sh = v.stride(2);
+  p.B = static_cast<int>(q.size(0));
+  p.S = static_cast<int>(q.size(1));
+  p.H = static_cast<int>(q.size(2));
+  p.Hk = static_cast<int>(k.size(2));
+  p.D = static_cast<int>(q.size(3));
+  p.window = static_cast<int>(std::min<int64_t>(window, 1ll << 30));
+  p.sinks = static_cast<int>(std::min<int64_t>(sinks, p.S));
+  p.causal = causal;
+  p.scale = static_cast<float>(scale);
+  if (lengths.has_value() && lengths->defined()) {
+    TORCH_CHECK(lengths->device() == q.device() && lengths->scalar_type() == at::kInt && lengths->is_contiguous() &&
+                    lengths->dim() == 1 && lengths->size(0) == q.size(0),
+                "window_attention: lengths must be a contiguous int32 vector of one value for each sequence");
+    p.lengths = lengths->data_ptr<int>();
+  }
+  return p;
+}
+
+}  // namespace
+
+std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                             int64_t window, int64_t sinks, bool causal,
+                                             const c10::optional<at::Tensor>& lengths, double scale,
+                                             const c10::optional<at::Tensor>& err) {
+  WinParams p = params_of(q, k, v, window, sinks, causal, lengths, scale);
+  c10::cuda::CUDAGuard guard(q.device());
+  auto o = out_empty(q.sizes(), q.options());
+  auto lse = out_empty({p.B, p.H, p.S}, q.options().dtype(at::kFloat));
+  if (o.numel() == 0) return {o, lse};
+  p.o = o.data_ptr();
+  p.lse = lse.data_ptr<float>();
+  auto st = at::cuda::getCurrentCUDAStream();
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  by_dim(p.D, [&](auto dc) {
+    constexpr int DP = decltype(dc)::value;
+    if (bf16)
+      win_fwd_kernel<__nv_bfloat16, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
+    else
+      win_fwd_kernel<float, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {o, lse};
+}
+
+std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                                             const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
+                                             int64_t window, int64_t sinks, bool causal,
+                                             const c10::optional<at::Tensor>& lengths, double scale,
+                                             const c10::optional<at::Tensor>& err) {
+  WinParams p = params_of(q, k, v, window, sinks, causal, lengths, scale);
+  TORCH_CHECK(dout.sizes() == q.sizes() && dout.scalar_type() == q.scalar_type() && dout.device() == q.device() &&
+                  (dout.size(3) == 1 || dout.stride(3) == 1),
+              "window_attention backward: the gradient must match q, contiguous along head_dim");
+  TORCH_CHECK(o.sizes() == q.sizes() && o.is_contiguous() && o.scalar_type() == q.scalar_type() &&
+                  lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
+                  lse.numel() == q.size(0) * q.size(1) * q.size(2),
+              "window_attention backward: o and lse must be the forward's");
+  c10::cuda::CUDAGuard guard(q.device());
+  auto dq = out_empty(q.sizes(), q.options()), dk = out_empty(k.sizes(), k.options()),
+       dv = out_empty(v.sizes(), v.options());
+  if (q.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
+  auto delta = out_empty({p.B, p.H, p.S}, lse.options());
+  p.o = o.data_ptr();
+  p.lse = lse.data_ptr<float>();
+  p.dout = dout.data_ptr();
+  p.g_sb = dout.stride(0), p.g_ss = dout.stride(1), p.g_sh = dout.stride(2);
+  p.delta = delta.data_ptr<float>();
+  p.dq = dq.data_ptr();
+  p.dk = dk.data_ptr();
+  p.dv = dv.data_ptr();
+  auto st = at::cuda::getCurrentCUDAStream();
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  by_dim(p.D, [&](auto dc) {
+    constexpr int DP = decltype(dc)::value;
+    if (bf16) {
+      win_dq_kernel<__nv_bfloat16, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
+      win_dkv_kernel<__nv_bfloat16, DP><<<row_grid(p, p.Hk), kWinThreads, 0, st>>>(p);
+    } else {
+      win_dq_kernel<float, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
+      win_dkv_kernel<float, DP><<<row_grid(p, p.Hk), kWinThreads, 0, st>>>(p);
+    }
+  });
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  return {dq, dk, dv};
+}
+
+}  // namespace tgcm
+
+TORCH_LIBRARY_FRAGMENT(tgcm, m) {
+  m.def("window_attention_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks, bool causal, Tensor? lengths, "
+        "float scale, Tensor? err) -> Tensor[]");
+  m.def("window_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, int window, int sinks, "
+        "bool causal, Tensor? lengths, float scale, Tensor? err) -> Tensor[]");
+}
+
+TORCH_LIBRARY_IMPL(tgcm, CUDA, m) {
+  m.impl("window_attention_fwd", &tgcm::window_attention_fwd);
+  m.impl("window_attention_bwd", &tgcm::window_attention_bwd);
+}

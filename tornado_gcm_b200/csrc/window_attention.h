@@ -1,0 +1,46 @@
+// Shared declarations of the window-attention kernels.
+//
+// Query i and key j of one sequence with L valid keys see each other when
+//   j < L,  j <= i (causal),  and  |i - j| < window  or  j < sinks.
+#pragma once
+
+#include <cstdint>
+#include <cuda_bf16.h>
+#include <cuda_runtime.h>
+
+namespace tgcm {
+
+constexpr float kLog2e = 1.4426950408889634f;
+
+struct WinParams {
+  const void *q, *k, *v;         // (B, S, heads, D), unit stride along D
+  long long q_sb, q_ss, q_sh;    // element strides
+  long long k_sb, k_ss, k_sh;
+  long long v_sb, v_ss, v_sh;
+  void* o;                       // (B, S, H, D) contiguous
+  float* lse;                    // (B, H, S): log2 of the softmax sum, +inf for rows that see nothing
+  // backward
+  const void* dout;              // (B, S, H, D), unit stride along D
+  long long g_sb, g_ss, g_sh;
+  float* delta;                  // (B, H, S): sum_d dO O
+  void *dq, *dk, *dv;            // contiguous, shapes of q, k, v
+  const int* lengths;            // (B,) or null
+  int B, S, H, Hk, D;
+  int window, sinks, causal;
+  float scale;
+};
+
+#ifdef __CUDACC__
+__device__ __forceinline__ int win_length(const WinParams& p, int b) {
+  if (p.lengths == nullptr) return p.S;
+  const int l = p.lengths[b];
+  return l < 0 ? 0 : (l > p.S ? p.S : l);
+}
+
+__device__ __forceinline__ bool win_sees(const WinParams& p, int L, int i, int j) {
+  const int far = i - j;
+  return j < L && !(p.causal && far < 0) && (j < p.sinks || (far < p.window && -far < p.window));
+}
+#endif
+
+}  // namespace tgcm

@@ -1,0 +1,144 @@
+"""Sliding-window attention with sinks, and its single-token form over a ring cache.
+
+Query ``i`` of a sequence attends to key ``j`` when both lie inside ``window`` of each other (``i - window < j <= i``
+for ``causal``, ``|i - j| < window`` otherwise) or ``j`` is one of the first ``sinks`` tokens (static fields, forcings:
+whatever every step has to see).  Query heads may share key heads.  Cost and memory grow with ``sequence x window``:
+no score matrix is stored, and key tiles out of sight are never read.
+
+Kernels: ``csrc/window_attention_sm100.cu`` (bf16, tcgen05), ``csrc/window_attention.cu`` (fp32 and the shapes that
+the tensor cores do not take) and ``csrc/window_step.cu`` (one token over the cache).  Softmax statistics and sums
+are fp32; the gradients use no atomics, so a pass gives the same bits every time.
+"""
+
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+
+from tornado_gcm_b200.ops import _ext
+
+
+class WindowAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, window: int, sinks: int, causal: bool, lengths, scale: float):
+        ops = _ext.require("window attention")
+        o, lse = ops.window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, _ext.error_flag(q.device))
+        ctx.save_for_backward(q, k, v, o, lse, lengths)
+        ctx.cfg = (window, sinks, causal, scale)
+        return o
+
+    @staticmethod
+    def backward(ctx, g):
+        ops = _ext.require("window attention backward")
+        q, k, v, o, lse, lengths = ctx.saved_tensors
+        window, sinks, causal, scale = ctx.cfg
+        g = g if g.stride(-1) == 1 and g.dtype == o.dtype else g.to(o.dtype).contiguous()
+        dq, dk, dv = ops.window_attention_bwd(g, q, k, v, o, lse, window, sinks, causal, lengths, scale,
+                                              _ext.error_flag(q.device))
+        return dq, dk, dv, None, None, None, None, None
+
+
+def window_mask(sequence: int, window: int, sinks: int = 0, causal: bool = True,
+                lengths: Optional[torch.Tensor] = None, device=None) -> torch.Tensor:
+    """``(…, sequence, sequence)`` truth values: query (row) sees key (column)."""
+    i = torch.arange(sequence, device=device)[:, None]
+    j = torch.arange(sequence, device=device)[None, :]
+    see = ((i - j).abs() < window) | (j < sinks)
+    if causal:
+        see = see & (j <= i)
+    if lengths is not None:
+        see = see & (j < lengths.to(j.device)[:, None, None])
+    return see
+
+
+def _torch_form(q, k, v, window, sinks, causal, lengths, scale):
+    """Dense masked attention in elementary torch operations (CPU tensors)."""
+    see = window_mask(q.shape[1], window, sinks, causal, lengths, q.device)
+    see = see[:, None] if see.ndim == 3 else see
+    n = q.shape[2] // k.shape[2]
+    c = torch.float64 if q.dtype == torch.float64 else torch.float32
+    qh, kh, vh = (t.transpose(1, 2).to(c) for t in (q, k.repeat_interleave(n, 2), v.repeat_interleave(n, 2)))
+    s = (qh @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
+    dead = ~see.any(-1, keepdim=True)
+    p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
+    if lengths is not None:  # what lies behind the end may hold anything
+        at = torch.arange(q.shape[1], device=q.device)[None, None, :, None]
+        vh = vh.masked_fill(at >= lengths.to(q.device)[:, None, None, None], 0.0)
+    return (p @ vh).transpose(1, 2).to(q.dtype)
+
+
+def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, sinks: int = 0,
+                     causal: bool = True, lengths: Optional[torch.Tensor] = None,
+                     scale: Optional[float] = None) -> torch.Tensor:
+    """``(B, S, H, D)`` attention of ``q (B, S, H, D)`` over ``k, v (B, S, Hk, D)``; ``Hk`` divides ``H``.
+
+    bf16 or fp32, ``D`` up to 128, any strides with a contiguous last axis.  ``lengths``: int32 ``(B,)``, the number
+    of valid keys of every sequence (what lies behind may hold anything, NaN included); a query that sees no key
+    gives zeros and no gradient.  ``scale`` defaults to ``D ** -0.5``.
+    """
+    if window < 1:
+        raise ValueError(f"window_attention: the window must hold at least the token itself, got {window}")
+    if sinks < 0:
+        raise ValueError(f"window_attention: sinks must not be negative, got {sinks}")
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if not q.is_cuda:
+        if q.ndim != 4 or k.shape != v.shape or q.shape[2] % k.shape[2]:
+            raise ValueError("window_attention: q (B, S, H, D) and k, v (B, S, Hk, D) with Hk dividing H expected")
+        return _torch_form(q, k, v, window, sinks, causal, lengths, scale)
+    q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
+    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
+        return WindowAttentionFn.apply(q, k, v, int(window), int(sinks), bool(causal), lengths, scale)
+    return _ext.require("window attention").window_attention_fwd(
+        q, k, v, int(window), int(sinks), bool(causal), lengths, scale, _ext.error_flag(q.device))[0]
+
+
+def window_slot(token: torch.Tensor, slots: int, sinks: int) -> torch.Tensor:
+    """The cache slot of a token number: itself at first, then round and round behind the sinks."""
+    return torch.where(token < slots, token, sinks + (token - sinks) % (slots - sinks))
+
+
+def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor,
+                          v_cache: torch.Tensor, lengths: torch.Tensor, *, sinks: int = 0,
+                          scale: Optional[float] = None) -> torch.Tensor:
+    """One new token of every sequence: puts ``k, v (B, Hk, D)`` in the caches and returns the attention of
+    ``q (B, H, D)`` over what they then hold.
+
+    ``k_cache, v_cache``: ``(B, sinks + window, Hk, D)``, changed in place.  ``lengths``: int32 ``(B,)``, the tokens
+    that each sequence had before this one (the caller adds one afterwards; calling again with the same lengths
+    writes the same slots).  A negative length marks a sequence that takes no part: zeros, its cache untouched.
+    The result equals the last row of :func:`window_attention` with ``causal`` over the whole history.
+    """
+    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    if q.is_cuda:
+        return _ext.require("window attention step").window_attention_step(q, k, v, k_cache, v_cache, lengths,
+                                                                           int(sinks), scale)
+    cap = k_cache.shape[1]
+    if not 0 <= sinks < cap:
+        raise ValueError("window_attention_step: sinks must lie between 0 and the cache's slots")
+    at = lengths.long()
+    on = (at >= 0).nonzero().flatten()
+    slot = window_slot(at[on], cap, sinks)
+    k_cache[on, slot], v_cache[on, slot] = k[on], v[on]
+    see = torch.arange(cap)[None, None, None] <= at[:, None, None, None]
+    n = q.shape[1] // k.shape[1]
+    kh, vh = (t.repeat_interleave(n, 2).transpose(1, 2).float() for t in (k_cache, v_cache))
+    s = (q.float()[:, :, None] @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
+    dead = ~see.any(-1, keepdim=True)
+    p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
+    vh = vh.masked_fill(~see.transpose(-1, -2), 0.0)
+    return (p @ vh)[:, :, 0].to(q.dtype)
+
+
+def fill_window_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
+                      sinks: int = 0) -> None:
+    """Puts a whole history ``k, v (B, S, Hk, D)`` in the caches, as that many steps would have left them."""
+    S, cap = k.shape[1], k_cache.shape[1]
+    if not 0 <= sinks < cap:
+        raise ValueError("fill_window_cache: sinks must lie between 0 and the cache's slots")
+    keep = torch.arange(S, device=k.device)
+    if S > cap:
+        keep = torch.cat([keep[:sinks], keep[S - (cap - sinks):]])
+    slot = window_slot(keep, cap, sinks)
+    k_cache[:, slot], v_cache[:, slot] = k[:, keep].to(k_cache.dtype), v[:, keep].to(v_cache.dtype)
