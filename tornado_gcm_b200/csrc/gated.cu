@@ -1,0 +1,897 @@
+// Gated linear layer:  h = act(x Wg^T + bg) * (x Wu^T + bu)
+//   x (T, K), Wg and Wu (F, K), h (T, F), all bf16; fp32 accumulation.
+// Backward from dh, with zg, zu the two projections (recomputed, not kept):
+//   dg = dh zu act'(zg),  du = dh act(zg),
+//   dx = dg Wg + du Wu,   dWg = dg^T x,  dWu = du^T x,  dbg, dbu = column sums.
+//
+// Four matrix products on one engine (pair_gemm_kernel), all bound by the
+// tensor cores at sizes worth speaking of (4 T K F FLOP forward, 12 T K F with
+// the gradients against a few bytes for each of T K + 2 F K + T F values):
+//   forward    both projections in one tile: of its 256 accumulator columns 128
+//              are the gate's and 128 the other's, so the epilogue finds both
+//              in its own TMEM lane and h is all that is written;
+//   recompute  the same product again with dg and du for an epilogue.  Keeping
+//              zg and zu instead would cost 8 bytes of traffic for each pair of
+//              values and 4 F bytes a token of memory, and their rounding to
+//              bf16 would reach every gradient; at K = 384 (this model family's
+//              towers) the second product takes less time than those bytes;
+//   dx         one product over the 2 F values of (dg, du) against (Wg; Wu);
+//   dW         (dg, du)^T x, split over tokens where the tiles are few; the
+//              parts are fp32 and are added in order by a second kernel.
+// dg and du are rounded to bf16 between the products (operands of the tensor
+// cores); everything else is rounded once, when it is written.
+//
+// Engine: clusters of two CTAs (cta_group::2) share a 256 x 256 tile: each
+// loads its 128 rows of A and its 128 rows of B (TMA, 128-byte swizzle, no
+// multicast; completion on the even CTA's barrier), the even CTA issues
+// tcgen05.mma over both, each keeps its 128 x 256 half of the accumulator in
+// its own TMEM, double buffered so that the epilogue of one tile runs under the
+// products of the next.  Each SM then reads 128 + 128 operand rows for 256 x
+// 128 outputs: half the shared-memory traffic of one CTA alone.  Warp roles
+// (320 threads): warp 0 TMA, warp 1 MMA, warps 2-9 epilogue.  Waits are bounded.
+//
+// A few tokens (T <= 8) take skinny_kernel instead: bound by reading the
+// weights once, a warp to each hidden value, both weight rows in flight.
+#include "alloc.h"
+#include "tmap.h"
+
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <torch/library.h>
+
+#include <algorithm>
+
+#include "pair_sm100.cuh"
+
+namespace tgcm {
+namespace {
+
+constexpr int kPairThreads = 320;
+constexpr int kPairStages = 6;
+constexpr int kOperand = 128 * 128;             // bytes: 128 rows of 64 bf16
+constexpr int kPairStage = 2 * kOperand;
+constexpr int kWarpStage = 32 * 128;            // bytes: one epilogue warp's 32 x 64 bf16 tile
+constexpr int kPairSmem = kPairStages * kPairStage + 8 * kWarpStage + 256 + 1024;
+constexpr int kSkinnyTokens = 8;
+
+enum PairMode : int { kFwd = 0, kDact = 1, kDx = 2, kDw = 3 };
+
+struct PairMaps {
+  CUtensorMap a[2], b[2];
+};
+
+struct PairParams {
+  int M, N;                 // rows and columns of the output (kFwd, kDact: N = F)
+  int tiles_m, tiles_n;     // 256 rows; 128 (kFwd, kDact) or 256 columns
+  int kb;                   // 64-wide blocks of the reduction (kDx: of each half)
+  int splits;               // kDw: parts of the reduction
+  int act;
+  const __nv_bfloat16 *bias_g, *bias_u;
+  __nv_bfloat16* out[2];    // kFwd: h; kDact: dg, du; kDx: dx; kDw: dWg, dWu
+  long long ld;             // of out
+  const __nv_bfloat16* dh;  // kDact
+  long long dh_ld;
+  float* bias_part;         // kDact: [row groups of 32][2][F] column sums, or null
+  float* part;              // kDw with splits > 1: [split][2][M][part_ld]
+  long long part_ld;
+  int* err;
+};
+
+// act(z) and act'(z).  __expf and the fast division are good to a few units of
+// 1e-7 relative: far below the rounding of the bf16 result.
+template <int ACT>
+__device__ __forceinline__ float act_val(float z) {
+  if constexpr (ACT == kActRelu) return fmaxf(z, 0.f);
+  else if constexpr (ACT == kActGelu) return gelu_erf_f(z);
+  else if constexpr (ACT == kActGeluTanh) {  // z sigmoid(2u) = z (1 + tanh u) / 2
+    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z, z * z, z);
+    return __fdividef(z, 1.f + __expf(-u2));
+  } else if constexpr (ACT == kActSilu) return __fdividef(z, 1.f + __expf(-z));
+  else if constexpr (ACT == kActTanh) return tanhf(z);
+  else return z;
+}
+
+template <int ACT>
+__device__ __forceinline__ void act_both(float z, float* a, float* da) {
+  if constexpr (ACT == kActRelu) {
+    *a = fmaxf(z, 0.f);
+    *da = z > 0.f ? 1.f : 0.f;
+  } else if constexpr (ACT == kActGelu) {
+    const float c = 0.5f * (1.f + erff(z * 0.7071067811865476f));
+    *a = z * c;
+    *da = fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z), c);
+  } else if constexpr (ACT == kActGeluTanh) {
+    const float z2 = z * z;
+    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z, z2, z);
+    const float s = __fdividef(1.f, 1.f + __expf(-u2));
+    *a = z * s;
+    *da = s + z * s * (1.f - s) * 1.5957691216057308f * fmaf(3.f * 0.044715f, z2, 1.f);
+  } else if constexpr (ACT == kActSilu) {
+    const float s = __fdividef(1.f, 1.f + __expf(-z));
+    *a = z * s;
+    *da = s * fmaf(z, 1.f - s, 1.f);
+  } else if constexpr (ACT == kActTanh) {
+    const float t = tanhf(z);
+    *a = t;
+    *da = 1.f - t * t;
+  } else {
+    *a = z;
+    *da = 1.f;
+  }
+}
+
+// One switch for 32 values, so the epilogue is compiled once, not once an activation.
+#define TGCM_GATED_ACTS(CASE) \
+  CASE(kActRelu) CASE(kActGelu) CASE(kActGeluTanh) CASE(kActSilu) CASE(kActTanh) CASE(kActNone)
+
+__device__ __forceinline__ void gate32(int act, uint32_t (&g)[32], const uint32_t (&u)[32]) {
+  switch (act) {
+#define TGCM_CASE(A)                                                                               \
+  case A:                                                                                          \
+    _Pragma("unroll") for (int j = 0; j < 32; ++j) g[j] =                                          \
+        __float_as_uint(act_val<A>(__uint_as_float(g[j])) * __uint_as_float(u[j]));                \
+    break;
+    TGCM_GATED_ACTS(TGCM_CASE)
+#undef TGCM_CASE
+  }
+}
+
+// (zg, zu, dh) -> (dg, du)
+__device__ __forceinline__ void dgate32(int act, uint32_t (&g)[32], uint32_t (&u)[32], const uint32_t (&dh)[16]) {
+  switch (act) {
+#define TGCM_CASE(A)                                                                               \
+  case A:                                                                                          \
+    _Pragma("unroll") for (int j = 0; j < 32; ++j) {                                               \
+      const uint32_t w = dh[j >> 1];                                                               \
+      const float d = __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));                    \
+      float a, da;                                                                                 \
+      act_both<A>(__uint_as_float(g[j]), &a, &da);                                                 \
+      g[j] = __float_as_uint(d * __uint_as_float(u[j]) * da);                                      \
+      u[j] = __float_as_uint(d * a);                                                               \
+    }                                                                                              \
+    break;
+    TGCM_GATED_ACTS(TGCM_CASE)
+#undef TGCM_CASE
+  }
+}
+
+__device__ __forceinline__ uint32_t pack2(uint32_t a, uint32_t b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b));
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Epilogue tiles are 32 rows of eight 16-byte pieces; piece c of row r sits at
+// c ^ (r & 7), so a lane writing its own row and eight lanes reading one row
+// both spread over all banks.
+__device__ __forceinline__ uint4* piece(uint8_t* stage, int row, int c) {
+  return reinterpret_cast<uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+}
+
+// 32 x 64 bf16 tile to global memory, clipped to nrows x ncols.
+__device__ __forceinline__ void tile_out(uint8_t* stage, __nv_bfloat16* g, long long ld, int nrows, int ncols,
+                                         int lane) {
+  const bool vec = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  const int c = lane & 7;
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int row = it * 4 + (lane >> 3);
+    if (row >= nrows || c * 8 >= ncols) continue;
+    const uint4 v = *piece(stage, row, c);
+    __nv_bfloat16* dst = g + row * ld + c * 8;
+    if (vec && c * 8 + 8 <= ncols) {
+      *reinterpret_cast<uint4*>(dst) = v;
+    } else {
+      const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&v);
+#pragma unroll
+      for (int k = 0; k < 8; ++k)
+        if (c * 8 + k < ncols) dst[k] = e[k];
+    }
+  }
+}
+
+__device__ __forceinline__ void tile_in(uint8_t* stage, const __nv_bfloat16* g, long long ld, int nrows, int ncols,
+                                        int lane) {
+  const bool vec = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
+  const int c = lane & 7;
+  uint4 v[8];
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int row = it * 4 + (lane >> 3);
+    v[it] = make_uint4(0, 0, 0, 0);
+    if (row >= nrows || c * 8 >= ncols) continue;
+    const __nv_bfloat16* src = g + row * ld + c * 8;
+    if (vec && c * 8 + 8 <= ncols) {
+      v[it] = __ldg(reinterpret_cast<const uint4*>(src));
+    } else {
+      alignas(16) __nv_bfloat16 e[8];
+#pragma unroll
+      for (int k = 0; k < 8; ++k) e[k] = c * 8 + k < ncols ? src[k] : __float2bfloat16(0.f);
+      v[it] = *reinterpret_cast<uint4*>(e);
+    }
+  }
+#pragma unroll
+  for (int it = 0; it < 8; ++it) *piece(stage, it * 4 + (lane >> 3), c) = v[it];
+}
+
+// 32 x 32 fp32 tile (same 128-byte rows) to global memory.
+__device__ __forceinline__ void tile_out_f32(uint8_t* stage, float* g, long long ld, int nrows, int ncols, int lane) {
+  const int c = lane & 7;  // part_ld is a multiple of 4
+#pragma unroll
+  for (int it = 0; it < 8; ++it) {
+    const int row = it * 4 + (lane >> 3);
+    if (row >= nrows || c * 4 >= ncols) continue;
+    *reinterpret_cast<uint4*>(g + row * ld + c * 4) = *piece(stage, row, c);
+  }
+}
+
+// Column sums of a 32 x 32 block held one row to a lane: after the halving
+// steps lane j has the sum of column j.
+__device__ __forceinline__ float column_sums(const uint32_t (&v)[32], int lane) {
+  float a[32];
+#pragma unroll
+  for (int j = 0; j < 32; ++j) a[j] = __uint_as_float(v[j]);
+#pragma unroll
+  for (int n = 16; n >= 1; n >>= 1) {
+    const bool up = lane & n;
+#pragma unroll
+    for (int j = 0; j < n; ++j) {
+      const float keep = up ? a[j + n] : a[j], give = up ? a[j] : a[j + n];
+      a[j] = keep + __shfl_xor_sync(0xffffffffu, give, n);
+    }
+  }
+  return a[0];
+}
+
+struct PairTile {
+  int tm, tn, which, split, kb0, nkb;
+};
+
+template <int MODE>
+__device__ __forceinline__ PairTile pair_tile(const PairParams& p, int t) {
+  PairTile c;
+  c.tn = t % p.tiles_n;
+  int r = t / p.tiles_n;
+  c.tm = r % p.tiles_m;
+  r /= p.tiles_m;
+  c.which = 0;
+  c.split = 0;
+  c.kb0 = 0;
+  c.nkb = p.kb;
+  if constexpr (MODE == kDx) c.nkb = 2 * p.kb;
+  if constexpr (MODE == kDw) {
+    c.which = r & 1;
+    c.split = r >> 1;
+    const int per = (p.kb + p.splits - 1) / p.splits;
+    c.kb0 = c.split * per;
+    c.nkb = max(0, min(per, p.kb - c.kb0));
+  }
+  return c;
+}
+
+template <int MODE>
+__device__ __forceinline__ int pair_tiles(const PairParams& p) {
+  return p.tiles_m * p.tiles_n * (MODE == kDw ? 2 * p.splits : 1);
+}
+
+template <int MODE>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
+    pair_gemm_kernel(const __grid_constant__ PairMaps maps, const __grid_constant__ PairParams p) {
+  constexpr bool A_MN = MODE == kDw;
+  constexpr bool B_MN = MODE == kDx || MODE == kDw;
+  constexpr uint32_t kIdesc = make_idesc(1, A_MN ? 1 : 0, B_MN ? 1 : 0, 256, 256);
+  constexpr int kTileN = (MODE == kFwd || MODE == kDact) ? 128 : 256;
+
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* staging = smem + kPairStages * kPairStage;
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + 8 * kWarpStage);  // the leader's are used
+  uint64_t* empty_bar = full_bar + kPairStages;
+  uint64_t* acc_full = empty_bar + kPairStages;   // [2]
+  uint64_t* acc_empty = acc_full + 2;             // [2], the leader's are used
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(acc_empty + 2);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = pair_rank();
+  const int n_tiles = pair_tiles<MODE>(p);
+  const int first = blockIdx.x >> 1, step = gridDim.x >> 1;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < kPairStages; ++s) {
+      mbar_init(&full_bar[s], 1);
+      mbar_init(&empty_bar[s], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&acc_full[i], 1);
+      mbar_init(&acc_empty[i], 16);  // eight epilogue warps of each CTA
+    }
+    *abort_flag = 0;
+    fence_barrier_init();
+    tma_prefetch_desc(&maps.a[0]);
+    tma_prefetch_desc(&maps.b[0]);
+  }
+  if (warp == 1) pair_tmem_alloc(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  pair_sync();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      int it = 0;
+      for (int t = first; t < n_tiles && !*abort_flag; t += step) {
+        const PairTile c = pair_tile<MODE>(p, t);
+        for (int i = 0; i < c.nkb; ++i, ++it) {
+          const int s = it % kPairStages;
+          if (!mbar_wait(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
+            *abort_flag = 1;
+            break;
+          }
+          uint8_t* sa = smem + s * kPairStage;
+          uint8_t* sb = sa + kOperand;
+          const uint32_t bar = leader_addr(&full_bar[s]);
+          if (rank == 0) mbar_arrive_expect_tx(&full_bar[s], 2 * kPairStage);  // both CTAs' bytes
+          if constexpr (MODE == kFwd || MODE == kDact) {
+            tma_load_2d_pair(sa, &maps.a[0], bar, i * 64, c.tm * 256 + rank * 128);
+            // the even CTA brings the gate's rows, the odd one the other projection's
+            tma_load_2d_pair(sb, &maps.b[rank], bar, i * 64, c.tn * 128);
+          } else if constexpr (MODE == kDx) {
+            const int half = i >= p.kb, k0 = (i - half * p.kb) * 64;
+            tma_load_2d_pair(sa, &maps.a[half], bar, k0, c.tm * 256 + rank * 128);
+            tma_load_2d_pair(sb, &maps.b[half], bar, c.tn * 256 + rank * 128, k0);
+            tma_load_2d_pair(sb + kOperand / 2, &maps.b[half], bar, c.tn * 256 + rank * 128 + 64, k0);
+          } else {
+            const int k0 = (c.kb0 + i) * 64, m0 = c.tm * 256 + rank * 128, n0 = c.tn * 256 + rank * 128;
+            tma_load_2d_pair(sa, &maps.a[c.which], bar, m0, k0);
+            tma_load_2d_pair(sa + kOperand / 2, &maps.a[c.which], bar, m0 + 64, k0);
+            tma_load_2d_pair(sb, &maps.b[0], bar, n0, k0);
+            tma_load_2d_pair(sb + kOperand / 2, &maps.b[0], bar, n0 + 64, k0);
+          }
+        }
+      }
+      // no load is in flight when the CTA leaves
+      if (rank == 0)
+        for (int i = max(0, it - kPairStages); i < it; ++i)
+          mbar_wait(&full_bar[i % kPairStages], (i / kPairStages) & 1, p.err, kErrTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && rank == 0) {
+      int it = 0, n = 0;
+      for (int t = first; t < n_tiles && !*abort_flag; t += step) {
+        const PairTile c = pair_tile<MODE>(p, t);
+        if (c.nkb == 0) continue;
+        const int acc = n & 1;
+        if (!mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
+          *abort_flag = 1;
+          break;
+        }
+        tc_fence_after();
+        for (int i = 0; i < c.nkb; ++i, ++it) {
+          const int s = it % kPairStages;
+          if (!mbar_wait(&full_bar[s], (it / kPairStages) & 1, p.err, kErrTimeoutFull)) {
+            *abort_flag = 1;
+            break;
+          }
+          tc_fence_after();
+          const uint32_t sa = smem_u32(smem + s * kPairStage), sb = sa + kOperand;
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            const uint64_t ad = A_MN ? make_sw128_desc(sa + k * 2048, kOperand / 2, 1024)
+                                     : make_sw128_desc(sa + k * 32, 16, 1024);
+            const uint64_t bd = B_MN ? make_sw128_desc(sb + k * 2048, kOperand / 2, 1024)
+                                     : make_sw128_desc(sb + k * 32, 16, 1024);
+            pair_umma_bf16(tmem + acc * 256, ad, bd, kIdesc, (i | k) ? 1u : 0u);
+          }
+          pair_commit(&empty_bar[s]);
+        }
+        pair_commit(&acc_full[acc]);  // also after a timeout: the epilogue does not wait for nothing
+        ++n;
+      }
+    }
+  } else {
+    const int q = warp & 3, half = (warp - 2) >> 2;
+    uint8_t* stage = staging + (warp - 2) * kWarpStage;
+    int n = 0;
+    for (int t = first; t < n_tiles; t += step) {
+      const PairTile c = pair_tile<MODE>(p, t);
+      const int row0 = c.tm * 256 + rank * 128 + q * 32;
+      const int nrows = min(32, p.M - row0);
+      const int colw = half * (kTileN / 2);            // this warp's columns of the tile
+      const int col0 = c.tn * kTileN + colw;
+      if (MODE == kDact) {
+        __syncwarp();
+        tile_in(stage, p.dh + static_cast<long long>(row0) * p.dh_ld + col0, p.dh_ld, nrows, p.N - col0, lane);
+        __syncwarp();
+      }
+      const int acc = n & 1;
+      if (c.nkb > 0) {
+        const bool have = mbar_wait(&acc_full[acc], (n >> 1) & 1, p.err, kErrTimeoutTmemFull);
+        if (__any_sync(0xffffffffu, !have || *abort_flag)) break;
+        tc_fence_after();
+        ++n;
+      }
+      const uint32_t ta = tmem + acc * 256 + (static_cast<uint32_t>(q * 32) << 16);
+      if constexpr (MODE == kFwd || MODE == kDact) {
+        uint32_t keep[2][16];  // kDact: du, packed
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          uint32_t g[32], u[32];
+          tmem_ld_32x32b_x32(ta + colw + ch * 32, g);
+          tmem_ld_32x32b_x32(ta + 128 + colw + ch * 32, u);
+          tmem_ld_wait();
+          if (p.bias_g != nullptr) {
+            const int col = col0 + ch * 32 + lane;
+            const float bg = col < p.N ? __bfloat162float(p.bias_g[col]) : 0.f;
+            const float bu = col < p.N ? __bfloat162float(p.bias_u[col]) : 0.f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              g[j] = __float_as_uint(__uint_as_float(g[j]) + __shfl_sync(0xffffffffu, bg, j));
+              u[j] = __float_as_uint(__uint_as_float(u[j]) + __shfl_sync(0xffffffffu, bu, j));
+            }
+          }
+          if constexpr (MODE == kFwd) {
+            gate32(p.act, g, u);
+          } else {
+            uint32_t dh[16];
+#pragma unroll
+            for (int v = 0; v < 4; ++v) {
+              const uint4 w = *piece(stage, lane, ch * 4 + v);
+              dh[4 * v] = w.x, dh[4 * v + 1] = w.y, dh[4 * v + 2] = w.z, dh[4 * v + 3] = w.w;
+            }
+            dgate32(p.act, g, u, dh);
+            if (p.bias_part != nullptr) {
+              const float sg = column_sums(g, lane), su = column_sums(u, lane);
+              const int col = col0 + ch * 32 + lane;
+              if (col < p.N) {
+                float* bp = p.bias_part + static_cast<long long>(row0 >> 5) * 2 * p.N + col;
+                bp[0] = sg;
+                bp[p.N] = su;
+              }
+            }
+#pragma unroll
+            for (int v = 0; v < 16; ++v) keep[ch][v] = pack2(u[2 * v], u[2 * v + 1]);
+          }
+#pragma unroll
+          for (int v = 0; v < 4; ++v)
+            *piece(stage, lane, ch * 4 + v) =
+                make_uint4(pack2(g[8 * v], g[8 * v + 1]), pack2(g[8 * v + 2], g[8 * v + 3]),
+                           pack2(g[8 * v + 4], g[8 * v + 5]), pack2(g[8 * v + 6], g[8 * v + 7]));
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) arrive_cluster(leader_addr(&acc_empty[acc]));
+        tile_out(stage, p.out[0] + static_cast<long long>(row0) * p.ld + col0, p.ld, nrows, p.N - col0, lane);
+        __syncwarp();
+        if constexpr (MODE == kDact) {
+#pragma unroll
+          for (int v = 0; v < 8; ++v)
+            *piece(stage, lane, v) = make_uint4(keep[v >> 2][4 * (v & 3)], keep[v >> 2][4 * (v & 3) + 1],
+                                                keep[v >> 2][4 * (v & 3) + 2], keep[v >> 2][4 * (v & 3) + 3]);
+          __syncwarp();
+          tile_out(stage, p.out[1] + static_cast<long long>(row0) * p.ld + col0, p.ld, nrows, p.N - col0, lane);
+        }
+      } else {
+        const bool parts = MODE == kDw && p.splits > 1;
+        if (parts) {
+          float* dst = p.part + (static_cast<long long>(c.split * 2 + c.which) * p.M + row0) * p.part_ld;
+#pragma unroll 1
+          for (int ch = 0; ch < 4; ++ch) {
+            uint32_t v[32];
+            tmem_ld_32x32b_x32(ta + colw + ch * 32, v);
+            tmem_ld_wait();
+            if (c.nkb == 0) {
+#pragma unroll
+              for (int j = 0; j < 32; ++j) v[j] = 0u;
+            }
+            __syncwarp();
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+              *piece(stage, lane, j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+            __syncwarp();
+            const int col = col0 + ch * 32;
+            tile_out_f32(stage, dst + col, p.part_ld, nrows, static_cast<int>(p.part_ld) - col, lane);
+          }
+        } else {
+          __nv_bfloat16* dst = p.out[c.which] + static_cast<long long>(row0) * p.ld;
+#pragma unroll 1
+          for (int c2 = 0; c2 < 2; ++c2) {
+            __syncwarp();
+#pragma unroll
+            for (int ch = 0; ch < 2; ++ch) {
+              uint32_t v[32];
+              tmem_ld_32x32b_x32(ta + colw + c2 * 64 + ch * 32, v);
+              tmem_ld_wait();
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                *piece(stage, lane, ch * 4 + j) =
+                    make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
+                               pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
+            }
+            __syncwarp();
+            const int col = col0 + c2 * 64;
+            tile_out(stage, dst + col, p.ld, nrows, p.N - col, lane);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0 && c.nkb > 0) arrive_cluster(leader_addr(&acc_empty[acc]));
+      }
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  pair_sync();
+  if (warp == 1) {
+    tc_fence_after();
+    pair_tmem_dealloc(tmem, 512);
+  }
+}
+
+// dW = sum of the parts, rounded once.  Four columns to a thread.
+__global__ void __launch_bounds__(256) join_parts_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ wg,
+                                                        __nv_bfloat16* __restrict__ wu, int F, int K, long long pld,
+                                                        int splits) {
+  const long long i = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 4;
+  const long long row = i / pld;
+  const int col = static_cast<int>(i - row * pld);
+  if (row >= 2ll * F) return;
+  float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int s = 0; s < splits; ++s) {
+    const float4 v = *reinterpret_cast<const float4*>(part + (s * 2ll * F + row) * pld + col);
+    a.x += v.x, a.y += v.y, a.z += v.z, a.w += v.w;
+  }
+  __nv_bfloat16* o = row < F ? wg + row * K : wu + (row - F) * K;
+  const float r[4] = {a.x, a.y, a.z, a.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (col + e < K) o[col + e] = __float2bfloat16(r[e]);
+}
+
+// db = column sums over the row groups, in order.
+__global__ void __launch_bounds__(256) join_bias_kernel(const float* __restrict__ part, __nv_bfloat16* __restrict__ bg,
+                                                       __nv_bfloat16* __restrict__ bu, int F, int groups) {
+  __shared__ float acc[8][32];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int c = blockIdx.x * 32 + lane;
+  float a = 0.f;
+  if (c < 2 * F)
+    for (int g = warp; g < groups; g += 8) a += part[static_cast<long long>(g) * 2 * F + c];
+  acc[warp][lane] = a;
+  __syncthreads();
+  if (warp == 0 && c < 2 * F) {
+    float t = 0.f;
+    for (int w = 0; w < 8; ++w) t += acc[w][lane];
+    (c < F ? bg[c] : bu[c - F]) = __float2bfloat16(t);
+  }
+}
+
+// A few tokens: a warp to each hidden value.  x stays in shared memory (bf16);
+// a lane reads 16 bytes of both weight rows and meets them with every token.
+template <int TT>
+__global__ void __launch_bounds__(256) skinny_kernel(const __nv_bfloat16* __restrict__ x, long long x_ld,
+                                                    const __nv_bfloat16* __restrict__ wg,
+                                                    const __nv_bfloat16* __restrict__ wu, long long w_ld,
+                                                    long long u_ld, const __nv_bfloat16* __restrict__ bg,
+                                                    const __nv_bfloat16* __restrict__ bu,
+                                                    __nv_bfloat16* __restrict__ h, int T, int K, int F, int act) {
+  const int lane = threadIdx.x & 31;
+  const int f = (blockIdx.x * 256 + threadIdx.x) >> 5;
+  if (f >= F) return;
+  float ag[TT], au[TT];
+#pragma unroll
+  for (int t = 0; t < TT; ++t) ag[t] = au[t] = 0.f;
+  const __nv_bfloat16* g = wg + f * w_ld;
+  const __nv_bfloat16* u = wu + f * u_ld;
+#pragma unroll 4
+  for (int k = lane * 8; k < K; k += 256) {
+    const uint4 gv = __ldg(reinterpret_cast<const uint4*>(g + k)), uv = __ldg(reinterpret_cast<const uint4*>(u + k));
+    const uint32_t gw[4] = {gv.x, gv.y, gv.z, gv.w}, uw[4] = {uv.x, uv.y, uv.z, uv.w};
+#pragma unroll
+    for (int t = 0; t < TT; ++t) {
+      if (t >= T) break;
+      const uint4 xv = __ldg(reinterpret_cast<const uint4*>(x + t * x_ld + k));
+      const uint32_t xw[4] = {xv.x, xv.y, xv.z, xv.w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const float x0 = __uint_as_float(xw[e] << 16), x1 = __uint_as_float(xw[e] & 0xffff0000u);
+        ag[t] = fmaf(x0, __uint_as_float(gw[e] << 16), ag[t]);
+        ag[t] = fmaf(x1, __uint_as_float(gw[e] & 0xffff0000u), ag[t]);
+        au[t] = fmaf(x0, __uint_as_float(uw[e] << 16), au[t]);
+        au[t] = fmaf(x1, __uint_as_float(uw[e] & 0xffff0000u), au[t]);
+      }
+    }
+  }
+#pragma unroll
+  for (int t = 0; t < TT; ++t) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+      ag[t] += __shfl_xor_sync(0xffffffffu, ag[t], o);
+      au[t] += __shfl_xor_sync(0xffffffffu, au[t], o);
+    }
+  }
+  float zg = 0.f, zu = 0.f;  // lane t finishes token t
+#pragma unroll
+  for (int t = 0; t < TT; ++t)
+    if (lane == t) zg = ag[t], zu = au[t];
+  if (lane >= T) return;
+  if (bg != nullptr) {
+    zg += __bfloat162float(bg[f]);
+    zu += __bfloat162float(bu[f]);
+  }
+  float a = zg;
+  switch (act) {
+#define TGCM_CASE(A) \
+  case A: a = act_val<A>(zg); break;
+    TGCM_GATED_ACTS(TGCM_CASE)
+#undef TGCM_CASE
+  }
+  h[static_cast<long long>(lane) * F + f] = __float2bfloat16(a * zu);
+}
+
+// Rows of 64 (K-major operands: 128 of them; MN-major ones: 64 steps of the reduction).
+CUtensorMap matrix_map(const at::Tensor& t, uint32_t box_rows) {
+  const uint64_t dims[2] = {static_cast<uint64_t>(t.size(1)), static_cast<uint64_t>(t.size(0))};
+  const uint64_t strides[1] = {static_cast<uint64_t>(t.size(0) > 1 ? t.stride(0) : (t.size(1) + 7) / 8 * 8) * 2};
+  const uint32_t box[2] = {64, box_rows};
+  return tmap_bf16<2>(t.data_ptr(), dims, strides, box);
+}
+
+// CTA pairs that run at once: a GPC with an odd number of free SMs leaves one idle,
+// and a pair that has to wait for another to end would double the time.
+int resident_pairs() {
+  static int pairs[64] = {0};
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && pairs[dev] > 0) return pairs[dev];
+  auto kern = pair_gemm_kernel<kFwd>;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+  const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3(sms / 2 * 2);
+  cfg.blockDim = dim3(kPairThreads);
+  cfg.dynamicSmemBytes = kPairSmem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  C10_CUDA_CHECK(cudaOccupancyMaxActiveClusters(&n, kern, &cfg));
+  TORCH_CHECK(n >= 1, "gated_linear: no room for a pair of CTAs on this device");
+  if (dev < 64) pairs[dev] = n;
+  return n;
+}
+
+template <int MODE>
+void launch_pair(const PairMaps& maps, const PairParams& p, int tiles, cudaStream_t st) {
+  auto kern = pair_gemm_kernel<MODE>;
+  static bool set[64] = {false};  // the attribute is per device and per kernel
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    if (dev < 64) set[dev] = true;
+  }
+  kern<<<2 * std::max(1, std::min(tiles, resident_pairs())), kPairThreads, kPairSmem, st>>>(maps, p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+int ceil_div(int64_t a, int64_t b) { return static_cast<int>((a + b - 1) / b); }
+
+// TMA rows: unit inner stride, 16-byte row pitch and base.
+bool tma_ok(const at::Tensor& t) {
+  return t.stride(1) == 1 && (t.size(0) == 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1))) &&
+         reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0 && t.size(1) % 8 == 0;
+}
+
+// A copy with the inner extent padded to a multiple of 8 with zeros, where TMA cannot read the tensor as it is.
+at::Tensor tma_rows(const at::Tensor& t) {
+  if (tma_ok(t)) return t;
+  const int64_t w = (t.size(1) + 7) / 8 * 8;
+  auto c = at::empty({t.size(0), w}, t.options());
+  if (w != t.size(1)) c.narrow(1, t.size(1), w - t.size(1)).zero_();
+  c.narrow(1, 0, t.size(1)).copy_(t);
+  return c;
+}
+
+void check_gated(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const c10::optional<at::Tensor>& bg,
+                 const c10::optional<at::Tensor>& bu, int64_t act) {
+  for (const auto* t : {&x, &wg, &wu})
+    TORCH_CHECK(t->is_cuda() && t->device() == x.device() && t->dim() == 2 && t->scalar_type() == at::kBFloat16,
+                "gated_linear: bf16 CUDA matrices of one device expected");
+  TORCH_CHECK(wg.sizes() == wu.sizes() && wg.size(1) == x.size(1),
+              "gated_linear: both weights must be (hidden, features) and match x");
+  TORCH_CHECK(x.size(1) >= 1 && wg.size(0) >= 1, "gated_linear: empty weights");
+  TORCH_CHECK(x.size(0) < (1ll << 31) - 256 && x.size(1) < (1ll << 31) - 256 && wg.size(0) < (1ll << 30),
+              "gated_linear: sizes beyond 2^31");
+  const bool a = bg.has_value() && bg->defined(), b = bu.has_value() && bu->defined();
+  TORCH_CHECK(a == b, "gated_linear: both biases or none");
+  if (a)
+    for (const auto& t : {*bg, *bu})
+      TORCH_CHECK(t.device() == x.device() && t.scalar_type() == at::kBFloat16 && t.is_contiguous() &&
+                      t.numel() == wg.size(0),
+                  "gated_linear: biases must be contiguous bf16 vectors of the hidden size");
+  TORCH_CHECK(act >= kActNone && act <= kActTanh, "gated_linear: unknown activation");
+}
+
+const __nv_bfloat16* bf16_or_null(const c10::optional<at::Tensor>& t) {
+  return t.has_value() && t->defined() ? reinterpret_cast<const __nv_bfloat16*>(t->data_ptr()) : nullptr;
+}
+__nv_bfloat16* bf16_ptr(const at::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
+
+}  // namespace
+
+at::Tensor gated_fwd(const at::Tensor& x_in, const at::Tensor& wg_in, const at::Tensor& wu_in,
+                     const c10::optional<at::Tensor>& bg, const c10::optional<at::Tensor>& bu, int64_t act,
+                     const c10::optional<at::Tensor>& err) {
+  check_gated(x_in, wg_in, wu_in, bg, bu, act);
+  c10::cuda::CUDAGuard guard(x_in.device());
+  const int64_t T = x_in.size(0), F = wg_in.size(0);
+  auto h = out_empty({T, F}, x_in.options());
+  if (T == 0) return h;
+  const at::Tensor x = tma_rows(x_in), wg = tma_rows(wg_in), wu = tma_rows(wu_in);
+  const int64_t K = x.size(1);
+  auto st = at::cuda::getCurrentCUDAStream();
+  if (T <= kSkinnyTokens) {
+    const dim3 grid(ceil_div(F, 8));
+    auto run = [&](auto tt) {
+      skinny_kernel<decltype(tt)::value><<<grid, 256, 0, st>>>(
+          bf16_ptr(x), x.stride(0), bf16_ptr(wg), bf16_ptr(wu), wg.stride(0), wu.stride(0), bf16_or_null(bg),
+          bf16_or_null(bu), bf16_ptr(h), static_cast<int>(T), static_cast<int>(K), static_cast<int>(F),
+          static_cast<int>(act));
+    };
+    if (T == 1)
+      run(std::integral_constant<int, 1>());
+    else if (T == 2)
+      run(std::integral_constant<int, 2>());
+    else if (T <= 4)
+      run(std::integral_constant<int, 4>());
+    else
+      run(std::integral_constant<int, 8>());
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+    return h;
+  }
+  PairMaps maps;
+  maps.a[0] = maps.a[1] = matrix_map(x, 128);
+  maps.b[0] = matrix_map(wg, 128);
+  maps.b[1] = matrix_map(wu, 128);
+  PairParams p{};
+  p.M = static_cast<int>(T), p.N = static_cast<int>(F);
+  p.tiles_m = ceil_div(T, 256), p.tiles_n = ceil_div(F, 128), p.kb = ceil_div(K, 64), p.splits = 1;
+  p.act = static_cast<int>(act);
+  p.bias_g = bf16_or_null(bg), p.bias_u = bf16_or_null(bu);
+  p.out[0] = bf16_ptr(h);
+  p.ld = F;
+  p.err = err.has_value() && err->defined() ? err->data_ptr<int>() : nullptr;
+  launch_pair<kFwd>(maps, p, p.tiles_m * p.tiles_n, st);
+  return h;
+}
+
+// dx, dWg, dWu, dbg, dbu; the ones not asked for are empty tensors.
+std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_in, const at::Tensor& wg_in,
+                                  const at::Tensor& wu_in, const c10::optional<at::Tensor>& bg,
+                                  const c10::optional<at::Tensor>& bu, int64_t act, bool need_x, bool need_w,
+                                  bool need_b, const c10::optional<at::Tensor>& err) {
+  check_gated(x_in, wg_in, wu_in, bg, bu, act);
+  const int64_t T = x_in.size(0), F = wg_in.size(0), K0 = x_in.size(1);
+  TORCH_CHECK(dh_in.dim() == 2 && dh_in.size(0) == T && dh_in.size(1) == F && dh_in.device() == x_in.device() &&
+                  dh_in.scalar_type() == at::kBFloat16 && (F == 1 || dh_in.stride(1) == 1),
+              "gated_linear backward: the gradient must be bf16 (tokens, hidden) with contiguous rows");
+  c10::cuda::CUDAGuard guard(x_in.device());
+  need_b = need_b && bg.has_value() && bg->defined();
+  auto opt = x_in.options();
+  auto dx = need_x ? out_empty({T, K0}, opt) : at::Tensor();
+  auto dwg = need_w ? out_empty({F, K0}, opt) : at::Tensor(), dwu = need_w ? out_empty({F, K0}, opt) : at::Tensor();
+  auto dbg = need_b ? out_empty({F}, opt) : at::Tensor(), dbu = need_b ? out_empty({F}, opt) : at::Tensor();
+  auto result = [&] {
+    auto e = at::empty({0}, opt);
+    return std::vector<at::Tensor>{need_x ? dx : e, need_w ? dwg : e, need_w ? dwu : e, need_b ? dbg : e,
+                                   need_b ? dbu : e};
+  };
+  if (T == 0) {
+    for (auto* t : {&dwg, &dwu, &dbg, &dbu})
+      if (t->defined()) t->zero_();
+    return result();
+  }
+  const at::Tensor x = tma_rows(x_in), wg = tma_rows(wg_in), wu = tma_rows(wu_in);
+  const int64_t K = x.size(1), Fp = (F + 7) / 8 * 8;
+  auto st = at::cuda::getCurrentCUDAStream();
+  int* flag = err.has_value() && err->defined() ? err->data_ptr<int>() : nullptr;
+  auto dgu = out_empty({2, T, Fp}, opt);
+  const at::Tensor dg = dgu[0].narrow(1, 0, F), du = dgu[1].narrow(1, 0, F);
+  at::Tensor bias_part;
+  const int groups = ceil_div(T, 256) * 8;
+  {
+    PairMaps maps;
+    maps.a[0] = maps.a[1] = matrix_map(x, 128);
+    maps.b[0] = matrix_map(wg, 128);
+    maps.b[1] = matrix_map(wu, 128);
+    PairParams p{};
+    p.M = static_cast<int>(T), p.N = static_cast<int>(F);
+    p.tiles_m = ceil_div(T, 256), p.tiles_n = ceil_div(F, 128), p.kb = ceil_div(K, 64), p.splits = 1;
+    p.act = static_cast<int>(act);
+    p.bias_g = bf16_or_null(bg), p.bias_u = bf16_or_null(bu);
+    p.out[0] = bf16_ptr(dg), p.out[1] = bf16_ptr(du);
+    p.ld = Fp;
+    p.dh = bf16_ptr(dh_in);
+    p.dh_ld = T > 1 ? dh_in.stride(0) : F;
+    if (need_b) {
+      bias_part = out_empty({groups, 2, F}, opt.dtype(at::kFloat));
+      p.bias_part = bias_part.data_ptr<float>();
+    }
+    p.err = flag;
+    launch_pair<kDact>(maps, p, p.tiles_m * p.tiles_n, st);
+  }
+  if (need_b) {
+    join_bias_kernel<<<ceil_div(2 * F, 32), 256, 0, st>>>(bias_part.data_ptr<float>(), bf16_ptr(dbg), bf16_ptr(dbu),
+                                                          static_cast<int>(F), groups);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  if (need_x) {
+    PairMaps maps;
+    maps.a[0] = matrix_map(dg, 128);
+    maps.a[1] = matrix_map(du, 128);
+    maps.b[0] = matrix_map(wg, 64);
+    maps.b[1] = matrix_map(wu, 64);
+    PairParams p{};
+    p.M = static_cast<int>(T), p.N = static_cast<int>(K0);
+    p.tiles_m = ceil_div(T, 256), p.tiles_n = ceil_div(K0, 256), p.kb = ceil_div(F, 64), p.splits = 1;
+    p.out[0] = bf16_ptr(dx);
+    p.ld = K0;
+    p.err = flag;
+    launch_pair<kDx>(maps, p, p.tiles_m * p.tiles_n, st);
+  }
+  if (need_w) {
+    PairMaps maps;
+    maps.a[0] = matrix_map(dg, 64);
+    maps.a[1] = matrix_map(du, 64);
+    maps.b[0] = maps.b[1] = matrix_map(x, 64);
+    PairParams p{};
+    p.M = static_cast<int>(F), p.N = static_cast<int>(K0);
+    p.tiles_m = ceil_div(F, 256), p.tiles_n = ceil_div(K0, 256), p.kb = ceil_div(T, 64);
+    // Parts of the reduction: the fewest steps of the slowest pair, counting a part's write and
+    // its share of the joining kernel as eight steps; at least eight steps to a part.
+    const int pairs = resident_pairs();
+    const int64_t tiles = 2ll * p.tiles_m * p.tiles_n;
+    int64_t best = -1;
+    p.splits = 1;
+    for (int s = 1; s <= 32 && (s == 1 || p.kb / s >= 8); ++s) {
+      const int64_t cost = ((tiles * s + pairs - 1) / pairs) * (ceil_div(p.kb, s) + (s > 1 ? 8 : 0));
+      if (best < 0 || cost < best) best = cost, p.splits = s;
+    }
+    p.out[0] = bf16_ptr(dwg), p.out[1] = bf16_ptr(dwu);
+    p.ld = K0;
+    p.err = flag;
+    at::Tensor part;
+    if (p.splits > 1) {
+      p.part_ld = (K0 + 3) / 4 * 4;
+      part = out_empty({p.splits, 2, F, p.part_ld}, opt.dtype(at::kFloat));
+      p.part = part.data_ptr<float>();
+    }
+    launch_pair<kDw>(maps, p, static_cast<int>(tiles * p.splits), st);
+    if (p.splits > 1) {
+      join_parts_kernel<<<ceil_div(2 * F * p.part_ld / 4, 256), 256, 0, st>>>(
+          p.part, bf16_ptr(dwg), bf16_ptr(dwu), static_cast<int>(F), static_cast<int>(K0), p.part_ld, p.splits);
+      C10_CUDA_KERNEL_LAUNCH_CHECK();
+    }
+  }
+  return result();
+}
+
+}  // namespace tgcm
+
+TORCH_LIBRARY_FRAGMENT(tgcm, m) {
+  m.def("gated_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act, Tensor? err) -> Tensor");
+  m.def("gated_bwd(Tensor dh, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act, bool need_x, "
+        "bool need_w, bool need_b, Tensor? err) -> Tensor[]");
+}
+
+TORCH_LIBRARY_IMPL(tgcm, CUDA, m) {
+  m.impl("gated_fwd", &tgcm::gated_fwd);
+  m.impl("gated_bwd", &tgcm::gated_bwd);
+}

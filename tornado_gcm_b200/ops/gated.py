@@ -1,0 +1,71 @@
+"""Gated linear layer ``act(x Wgᵀ + bg) * (x Wuᵀ + bu)`` in BF16 on the tensor cores (``csrc/gated.cu``).
+
+Both projections, the activation and the product are one kernel: the two accumulators of a hidden value sit side
+by side in tensor memory and only the product is written.  The backward pass recomputes the projections (nothing
+of the hidden size is kept for it), gets both pre-activation gradients in that kernel's epilogue and needs one
+product for ``dx`` and one for both weight gradients.  A few tokens (a forecast step) take a kernel that streams
+the weights once.
+
+Like the column MLPs (:mod:`tornado_gcm_b200.ops.linear`) the layer computes in the BF16 zone: fp32 inputs and
+master weights are rounded to BF16 on entry, and the gradients reach them through that cast.
+"""
+
+from __future__ import annotations
+
+from typing import Optional
+
+import torch
+
+from tornado_gcm_b200.ops import _ext
+from tornado_gcm_b200.ops.linear import ACT_CODES
+
+
+class GatedLinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, wg, wu, bg, bu, act: int):
+        ops = _ext.require("gated linear layer")
+        ctx.save_for_backward(x, wg, wu, bg, bu)
+        ctx.act = act
+        return ops.gated_fwd(x, wg, wu, bg, bu, act, _ext.error_flag(x.device))
+
+    @staticmethod
+    def backward(ctx, g):
+        ops = _ext.require("gated linear layer (backward)")
+        x, wg, wu, bg, bu = ctx.saved_tensors
+        if g.dtype != torch.bfloat16 or g.stride(-1) != 1:
+            g = g.to(torch.bfloat16).contiguous()
+        need = ctx.needs_input_grad
+        dx, dwg, dwu, dbg, dbu = ops.gated_bwd(g, x, wg, wu, bg, bu, ctx.act, need[0], need[1] or need[2],
+                                               need[3] or need[4], _ext.error_flag(g.device))
+        pick = lambda t, on: t if on else None  # noqa: E731
+        return pick(dx, need[0]), pick(dwg, need[1]), pick(dwu, need[2]), pick(dbg, need[3]), pick(dbu, need[4]), None
+
+
+def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
+                 b_up: Optional[torch.Tensor] = None, *, activation: str = "silu") -> torch.Tensor:
+    """``(…, F)`` from ``x (…, K)`` and the weights ``(F, K)``; ``activation`` one of ``ops.linear.ACT_CODES``.
+
+    On the GPU the result is BF16 and so is the arithmetic's input; on the CPU it has ``x``'s type.
+    """
+    if activation not in ACT_CODES:
+        raise ValueError(f"gated_linear: activation must be one of {sorted(ACT_CODES)}, got {activation!r}")
+    if w_gate.ndim != 2 or w_gate.shape != w_up.shape or x.shape[-1] != w_gate.shape[1]:
+        raise ValueError(f"gated_linear: weights (hidden, features) that match x expected, got x {tuple(x.shape)}, "
+                         f"{tuple(w_gate.shape)} and {tuple(w_up.shape)}")
+    if (b_gate is None) != (b_up is None):
+        raise ValueError("gated_linear: both biases or none")
+    if not x.is_cuda:
+        from tornado_gcm_b200.neural.standard_layers import apply_activation
+
+        lin = torch.nn.functional.linear
+        return apply_activation(activation, lin(x, w_gate, b_gate)) * lin(x, w_up, b_up)
+    bf = torch.bfloat16
+    args = [t if t is None or t.dtype == bf else t.to(bf) for t in (x, w_gate, w_up, b_gate, b_up)]
+    if x.ndim != 2:
+        args[0] = args[0].reshape(-1, x.shape[-1])
+    act = ACT_CODES[activation]
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
+        h = GatedLinearFn.apply(*args, act)
+    else:
+        h = _ext.require("gated linear layer").gated_fwd(*args, act, _ext.error_flag(x.device))
+    return h if x.ndim == 2 else h.reshape(*x.shape[:-1], h.shape[-1])
