@@ -293,6 +293,9 @@ ATTN = [  # B, S, H, Hk, D, window, sinks, causal, lengths
     (2, 257, 2, 2, 16, 300, 0, True, None), (1, 384, 2, 2, 80, 128, 129, False, (200,)),
     (2, 65, 2, 1, 13, 20, 3, True, (65, 30)), (1, 1100, 4, 4, 64, 256, 5, True, None),
     (1, 900, 2, 1, 96, 77, 0, True, (850,)), (1, 520, 8, 1, 64, 90, 300, True, None), (2, 200, 2, 2, 24, 64, 64, True, (7, 150)),
+    # sinks ahead of the queries that see them, beyond their window
+    (1, 600, 2, 1, 64, 20, 300, False, None), (2, 230, 2, 2, 128, 100, 200, False, (230, 180)), (1, 200, 1, 1, 64, 1, 200, False, None),
+    (1, 640, 2, 2, 128, 500, 1, True, None),
 ]
 
 

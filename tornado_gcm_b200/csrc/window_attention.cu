@@ -1,6 +1,7 @@
 // Attention in a sliding window with a few first tokens always in sight:
 // the CUDA-core kernels (any head size up to 128, bf16 or fp32) and the
-// operators' host side.
+// operators' host side.  bf16 problems whose shapes the tensor cores take go
+// to window_attention_sm100.cu.
 //
 // With z_ij = q_i . k_j * scale over the keys in sight of query i:
 //   m = max_j z,  l = sum_j exp(z - m),  o_i = sum_j exp(z - m) v_j / l,
@@ -31,6 +32,11 @@
 #include "window_attention.h"
 
 namespace tgcm {
+
+// window_attention_sm100.cu
+bool window_sm100_takes(const WinParams& p, bool bf16);
+void window_sm100_fwd(const WinParams& p, cudaStream_t st, int* err);
+void window_sm100_bwd(const WinParams& p, cudaStream_t st, int* err);
 
 namespace {
 
@@ -112,7 +118,7 @@ __device__ __forceinline__ void axpy_share(float (&a)[N], float f, const float* 
 __device__ __forceinline__ void key_ranges(const WinParams& p, int L, int i0, int n, int* se, int* lo, int* hi) {
   const int last = min(i0 + n, p.S) - 1;
   *lo = max(0, i0 - (p.window - 1));
-  *hi = min(L, p.causal ? last + 1 : last + p.window);
+  *hi = min(L, p.causal ? last + 1 : max(last + p.window, p.sinks));
   *se = min(min(p.sinks, *lo), L);
 }
 
@@ -345,6 +351,10 @@ WinParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   return p;
 }
 
+int* flag_of(const c10::optional<at::Tensor>& err) {
+  return err.has_value() && err->defined() ? err->data_ptr<int>() : nullptr;
+}
+
 }  // namespace
 
 std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
@@ -360,6 +370,10 @@ std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tens
   p.lse = lse.data_ptr<float>();
   auto st = at::cuda::getCurrentCUDAStream();
   const bool bf16 = q.scalar_type() == at::kBFloat16;
+  if (window_sm100_takes(p, bf16)) {
+    window_sm100_fwd(p, st, flag_of(err));
+    return {o, lse};
+  }
   by_dim(p.D, [&](auto dc) {
     constexpr int DP = decltype(dc)::value;
     if (bf16)
@@ -399,6 +413,10 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
   p.dv = dv.data_ptr();
   auto st = at::cuda::getCurrentCUDAStream();
   const bool bf16 = q.scalar_type() == at::kBFloat16;
+  if (window_sm100_takes(p, bf16)) {
+    window_sm100_bwd(p, st, flag_of(err));
+    return {dq, dk, dv};
+  }
   by_dim(p.D, [&](auto dc) {
     constexpr int DP = decltype(dc)::value;
     if (bf16) {

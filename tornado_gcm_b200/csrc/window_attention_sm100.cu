@@ -1,0 +1,1138 @@
+// Window attention with sinks on the tensor cores: bf16, head sizes that are
+// multiples of 8 up to 128 (formulas in window_attention.cu).
+//
+// Three kernels: forward, dq (with delta), dk and dv.  Each gives a CTA 128
+// rows of one head (queries; keys for dk and dv) and walks the tiles of the
+// other side that are in sight of them: a run of tiles through the window,
+// and the sinks.  Warp 0 feeds a ring of shared-memory slots by TMA, one
+// thread of warp 1 issues tcgen05.mma, warps 2-5 own one row to a thread and
+// do the softmax arithmetic on accumulators read from TMEM; the weights (or
+// their gradients) go back to TMEM as bf16, where they are the A operand of the
+// next product.  Nothing of the size of the score matrix leaves the SM.
+//
+// What bounds them: 128 x 128 scores are 16 384 exponentials, 1024 cycles of
+// the SM's 16 a cycle, against 512 cycles of products at D = 64; so two CTAs
+// share an SM (tiles sized for half of its TMEM and shared memory) and one's
+// products run under the other's exponentials.  Only at D = 128 do dk and dv
+// need all of TMEM; that kernel keeps two score tiles in flight instead.
+//   D <= 64:  forward 128-key tiles (S 128, P 64, O 64 columns),
+//             dq 64-key tiles (S 64, dP 64, dS 32, dQ 64),
+//             dk/dv 64-query tiles (S, dP, dV, dK 64 each; P and dS over S and dP)
+//   D <= 128: forward 64-key tiles (S 64, P 32, O 128),
+//             dq 64-key tiles (S, under dS, 64, dP 64, dQ 128),
+//             dk/dv 64-query tiles (2 x (S, dP 64), dV, dK 128)
+// A head narrower than its tile is filled with zeros by TMA; products run over
+// the columns that are there, rounded up to 16.
+//
+// The forward keeps a running maximum that is only raised (and O rescaled)
+// when a row exceeds it by 2^8: the weights stay below 256 and the sums are
+// fp32, so nothing is lost.  dq and dk/dv recompute the weights from lse; they
+// are separate kernels, at the price of two more products, so that every sum
+// has one owner: no atomics, the same bits every time, and shared key heads are
+// summed over their query heads in the accumulator.  The sinks are seen by
+// every query, so their gradients would be one CTA's work over the whole
+// sequence: the queries outside the sink tile's own window are split over
+// extra CTAs whose fp32 parts are added in order by a small kernel.
+#include "alloc.h"
+#include "tmap.h"
+
+#include <ATen/ATen.h>
+#include <ATen/cuda/CUDAContext.h>
+#include <torch/library.h>
+
+#include <algorithm>
+
+#include "pair_sm100.cuh"
+#include "window_attention.h"
+
+namespace tgcm {
+namespace {
+
+constexpr int kAttnThreads = 192;
+constexpr int kAtom = 128;  // bytes of a swizzled row: 64 bf16
+
+struct AttnMaps {
+  CUtensorMap q, k, v, g;
+};
+
+// ── instructions ───────────────────────────────────────────────────────────
+__device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1, int c2,
+                                            int c3) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5, %6}], [%2];"
+      ::"r"(smem_u32(dst)),
+      "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(c0), "r"(c1), "r"(c2), "r"(c3)
+      : "memory");
+}
+
+// D(tmem) (+)= A(tmem) * B(smem desc), bf16.
+__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
+                                             uint32_t accumulate) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
+      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ uint32_t pack_f2(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+__device__ __forceinline__ void load_row32(uint32_t taddr, float* s) {
+  uint32_t r[32];
+  tmem_ld_32x32b_x32(taddr, r);
+#pragma unroll
+  for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(r[i]);
+}
+
+// K-major operand (rows x 64-value atoms) and the same tile read the other way
+// round (MN-major: the rows are the reduction).  `rows`: of the whole tile.
+__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int rows, int k16) {
+  return make_sw128_desc(tile + (k16 >> 2) * rows * kAtom + (k16 & 3) * 32, 16, 1024);
+}
+__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int rows, int k16) {
+  return make_sw128_desc(tile + k16 * 16 * kAtom, rows * kAtom, 1024);
+}
+
+// Bounded wait of a whole warp: false in all lanes when one gave up.
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
+  const bool ok = mbar_wait(bar, parity, err, code);
+  return !__any_sync(0xffffffffu, !ok || *abort_flag);
+}
+
+// One row of D <= 64 * A values in bf16 from this thread to the staging tile
+// (atoms of 128 rows), then 32 rows of the warp to global memory, eight lanes
+// to a row's 128 bytes.
+__device__ __forceinline__ uint4* stage_piece(uint8_t* stage, int atom, int row, int c) {
+  return reinterpret_cast<uint4*>(stage + atom * (128 * kAtom) + row * kAtom + ((c ^ (row & 7)) << 4));
+}
+template <int DP>
+__device__ __forceinline__ void store_rows(uint8_t* stage, __nv_bfloat16* dst, long long row_stride, int D, int row0,
+                                           int lo, int hi, int lane) {
+#pragma unroll
+  for (int a = 0; a < DP / 64; ++a)
+#pragma unroll
+    for (int it = 0; it < 8; ++it) {
+      const int row = row0 + it * 4 + (lane >> 3), d = a * 64 + (lane & 7) * 8;
+      if (row >= lo && row < hi && d < D)
+        *reinterpret_cast<uint4*>(dst + row * row_stride + d) = *stage_piece(stage, a, row, lane & 7);
+    }
+}
+// TMEM columns [col, col + DP) of this thread's row, times f, to the staging tile.
+template <int DP>
+__device__ __forceinline__ void stage_row(uint8_t* stage, uint32_t taddr, bool have, float f, int row) {
+#pragma unroll
+  for (int c = 0; c < DP / 32; ++c) {
+    float v[32];
+    if (have) {
+      load_row32(taddr + c * 32, v);
+      tmem_ld_wait();
+    } else {
+#pragma unroll
+      for (int i = 0; i < 32; ++i) v[i] = 0.f;
+    }
+#pragma unroll
+    for (int p = 0; p < 4; ++p)
+      *stage_piece(stage, c >> 1, row, (c & 1) * 4 + p) =
+          make_uint4(pack_f2(v[8 * p] * f, v[8 * p + 1] * f), pack_f2(v[8 * p + 2] * f, v[8 * p + 3] * f),
+                     pack_f2(v[8 * p + 4] * f, v[8 * p + 5] * f), pack_f2(v[8 * p + 6] * f, v[8 * p + 7] * f));
+  }
+}
+
+// Key tiles of the queries [i0, i0 + 128): tiles of the sinks below the window's
+// first key, then tiles through the window (and up to the last sink).
+struct KeyTiles {
+  int sink_end, lo, hi, n_sink, n;  // keys [0, sink_end) and [lo, hi); tiles
+};
+template <int KT>
+__device__ __forceinline__ KeyTiles key_tiles(const WinParams& p, int L, int i0) {
+  KeyTiles t;
+  const int last = min(i0 + 128, p.S) - 1;
+  t.lo = max(0, i0 - (p.window - 1));
+  t.hi = min(L, p.causal ? last + 1 : max(last + p.window, p.sinks));  // not causal: sinks may lie ahead
+  t.sink_end = min(min(p.sinks, t.lo), L);
+  t.n_sink = (t.sink_end + KT - 1) / KT;
+  t.n = t.n_sink + (t.hi > t.lo ? (t.hi - t.lo + KT - 1) / KT : 0);
+  return t;
+}
+// First key of tile j and its columns, rounded up to 16.
+template <int KT>
+__device__ __forceinline__ void key_tile(const KeyTiles& t, int j, int* j0, int* cols) {
+  const bool sink = j < t.n_sink;
+  *j0 = sink ? j * KT : t.lo + (j - t.n_sink) * KT;
+  *cols = min(KT, ((sink ? t.sink_end : t.hi) - *j0 + 15) & ~15);
+}
+
+// What query i sees of a key tile starting at j0: columns [a, b) and [0, c).
+struct Sight {
+  int a, b, c;
+};
+__device__ __forceinline__ Sight sight_of(const WinParams& p, const KeyTiles& t, int L, int i, int j, int j0) {
+  Sight s;
+  if (j < t.n_sink) {
+    s.a = s.b = 0;
+    s.c = t.sink_end - j0;  // sinks below the window of every query of the tile: none is ahead of a query
+  } else {
+    s.a = i - (p.window - 1) - j0;
+    s.b = min(L, p.causal ? i + 1 : i + p.window) - j0;
+    s.c = min(min(p.sinks, L), p.causal ? i + 1 : L) - j0;
+  }
+  return s;
+}
+__device__ __forceinline__ bool in_sight(const Sight& s, int c) { return (c >= s.a && c < s.b) || c < s.c; }
+
+// Zeroes the rows [first, n) of a tile of `rows` rows: keys behind the end may
+// hold NaN, which a weight of zero would not remove from a product.
+template <int DP>
+__device__ __forceinline__ void clear_rows(uint8_t* tile, int rows, int first, int n, int thread) {
+  const int pieces = (n - first) * 8;
+#pragma unroll
+  for (int a = 0; a < DP / 64; ++a)
+    for (int e = thread; e < pieces; e += 128)
+      *reinterpret_cast<uint4*>(tile + a * rows * kAtom + first * kAtom + e * 16) = make_uint4(0, 0, 0, 0);
+  fence_async_smem();
+}
+
+// ── forward ────────────────────────────────────────────────────────────────
+template <int DP>
+struct FwdCfg {
+  static constexpr int KT = DP == 64 ? 128 : 64;
+  static constexpr int kSlots = 4;
+  static constexpr int kSlot = KT * DP * 2;  // 16 KB
+  static constexpr int kQ = 128 * DP * 2;
+  static constexpr int kSmem = kQ + kSlots * kSlot + 256 + 1024;
+  static constexpr uint32_t kP = KT;                        // TMEM columns: S at 0
+  static constexpr uint32_t kO = DP == 64 ? 192 : 128;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kAttnThreads, 2)
+    win_fwd_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, int* err) {
+  using C = FwdCfg<DP>;
+  constexpr int KT = C::KT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + C::kQ;
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kSlot);
+  uint64_t* empty = full + C::kSlots;
+  uint64_t* q_full = empty + C::kSlots;
+  uint64_t* s_full = q_full + 1;
+  uint64_t* s_empty = s_full + 1;
+  uint64_t* p_full = s_empty + 1;
+  uint64_t* pv_done = p_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i0 = blockIdx.x * 128, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+  const int L = win_length(p, b);
+  const KeyTiles kt = key_tiles<KT>(p, L, i0);
+  const int kd = (p.D + 15) / 16;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 4);
+    mbar_init(p_full, 4);
+    mbar_init(pv_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && kt.n > 0) {
+      mbar_arrive_expect_tx(q_full, C::kQ);
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a) tma_load_4d(smem + a * 128 * kAtom, &maps.q, q_full, a * 64, i0, h, b);
+      int it = 0;
+      bool go = true;
+      for (int j = 0; j < kt.n && go; ++j) {
+        int j0, cols;
+        key_tile<KT>(kt, j, &j0, &cols);
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int s = it % C::kSlots;
+          if (!mbar_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+            *abort_flag = 1;
+            go = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], C::kSlot);
+#pragma unroll
+          for (int a = 0; a < DP / 64; ++a)
+            tma_load_4d(ring + s * C::kSlot + a * KT * kAtom, kv ? &maps.v : &maps.k, &full[s], a * 64, j0, hk, b);
+        }
+      }
+      mbar_wait(q_full, 0, err, kErrTimeoutDrain);
+      for (int i = max(0, it - C::kSlots); i < it; ++i)
+        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && kt.n > 0) {
+      const uint32_t idesc_s = make_idesc(1, 0, 0, 128, 0), idesc_o = make_idesc(1, 0, 1, 128, 16 * kd);
+      const uint32_t sq = smem_u32(smem), sr = smem_u32(ring);
+      auto scores = [&](int j) {  // S = Q K^T
+        const int it = 2 * j, s = it % C::kSlots;
+        int j0, cols;
+        key_tile<KT>(kt, j, &j0, &cols);
+        if (!mbar_wait(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (j > 0 && !mbar_wait(s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
+        tc_fence_after();
+        for (int k = 0; k < kd; ++k)
+          umma_bf16(tmem, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), idesc_s | ((cols >> 3) << 17),
+                    k ? 1u : 0u);
+        tc_commit(&empty[s]);
+        tc_commit(s_full);
+        return true;
+      };
+      bool go = mbar_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
+      for (int j = 0; j < kt.n && go; ++j) {
+        if (j + 1 < kt.n && !scores(j + 1)) {
+          go = false;
+          break;
+        }
+        const int it = 2 * j + 1, s = it % C::kSlots;
+        int j0, cols;
+        key_tile<KT>(kt, j, &j0, &cols);
+        if (!mbar_wait(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull) ||
+            !mbar_wait(p_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
+          go = false;
+          break;
+        }
+        tc_fence_after();
+        for (int k = 0; k < cols / 16; ++k)  // O += P V
+          umma_bf16_ts(tmem + C::kO, tmem + C::kP + k * 8, desc_mn(sr + s * C::kSlot, KT, k), idesc_o,
+                       (j | k) ? 1u : 0u);
+        tc_commit(&empty[s]);
+        tc_commit(pv_done);
+      }
+      if (!go) *abort_flag = 1;
+    }
+  } else {
+    const int q4 = warp & 3, row = q4 * 32 + lane, i = i0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const int w0 = i0 + q4 * 32, w1 = w0 + 31;  // this warp's queries
+    float m = -INFINITY, l = 0.f;               // m in the scaled base-2 domain
+    bool ok = true;
+    for (int j = 0; j < kt.n; ++j) {
+      int j0, cols;
+      key_tile<KT>(kt, j, &j0, &cols);
+      if (!(ok = warp_wait(s_full, j & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+      tc_fence_after();
+      float s[KT];
+#pragma unroll
+      for (int ch = 0; ch < KT / 32; ++ch)
+        if (ch * 32 < cols) load_row32(tmem + lanes + ch * 32, s + ch * 32);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_empty);
+      // columns in sight
+      const bool whole = j >= kt.n_sink && (cols & 31) == 0 && j0 + cols <= L && j0 > w1 - p.window &&
+                         j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
+      float mx = -INFINITY;
+      if (whole) {
+#pragma unroll
+        for (int ch = 0; ch < KT / 32; ++ch)
+          if (ch * 32 < cols) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[ch * 32 + e]);
+          }
+      } else {
+        const Sight si = sight_of(p, kt, L, i, j, j0);
+#pragma unroll
+        for (int ch = 0; ch < KT / 32; ++ch)
+          if (ch * 32 < cols) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const int col = ch * 32 + e;
+              s[col] = in_sight(si, col) ? s[col] : -INFINITY;
+              mx = fmaxf(mx, s[col]);
+            }
+          }
+      }
+      mx *= c;
+      float f = 1.f;
+      bool raise = false;
+      if (m == -INFINITY) {
+        m = mx;
+      } else if (mx > m + 8.f) {
+        f = ex2(m - mx);
+        m = mx;
+        l *= f;
+        raise = true;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      uint32_t pk[KT / 2];
+      float sum = 0.f;
+#pragma unroll
+      for (int ch = 0; ch < KT / 32; ++ch)
+        if (ch * 32 < cols) {
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            const float a0 = ex2(fmaf(s[ch * 32 + e], c, -base)), a1 = ex2(fmaf(s[ch * 32 + e + 1], c, -base));
+            sum += a0 + a1;
+            pk[ch * 16 + e / 2] = pack_f2(a0, a1);
+          }
+        }
+      l += sum;
+      // the weights of the tile before have been used
+      if (j > 0) {
+        if (!(ok = warp_wait(pv_done, (j - 1) & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+        tc_fence_after();
+        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll
+          for (int ch = 0; ch < DP / 32; ++ch) {
+            uint32_t o[32];
+            tmem_ld_32x32b_x32(tmem + C::kO + lanes + ch * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+            tmem_st_32x32b_x32(tmem + C::kO + lanes + ch * 32, o);
+          }
+        }
+      }
+#pragma unroll
+      for (int ch = 0; ch < KT / 32; ++ch)
+        if (ch * 32 < cols) tmem_st_32x32b_x16(tmem + C::kP + lanes + ch * 16, pk + ch * 16);
+      if (j0 + cols > L) {
+        const int it = 2 * j + 1, sl = it % C::kSlots;
+        if (!(ok = warp_wait(&full[sl], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull))) break;
+        clear_rows<DP>(ring + sl * C::kSlot, KT, max(0, L - j0), cols, threadIdx.x - 64);
+      }
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(p_full);
+    }
+    if (ok && kt.n > 0) ok = warp_wait(pv_done, (kt.n - 1) & 1, abort_flag, err, kErrTimeoutTmemFull);
+    tc_fence_after();
+    if (!ok) {
+      *abort_flag = 1;
+    } else {
+      const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
+      // every product has read the queries: their tile is the staging tile now
+      stage_row<DP>(smem, tmem + C::kO + lanes, kt.n > 0, inv, row);
+      __syncwarp();
+      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o) +
+                         ((static_cast<long long>(b) * p.S + i0) * p.H + h) * p.D;
+      store_rows<DP>(smem, o, static_cast<long long>(p.H) * p.D, p.D, q4 * 32, 0, p.S - i0, lane);
+      if (i < p.S)
+        p.lse[(static_cast<long long>(b) * p.H + h) * p.S + i] = l == 0.f ? INFINITY : m + log2f(l);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// ── dq and delta ───────────────────────────────────────────────────────────
+template <int DP>
+struct DqCfg {
+  static constexpr int KT = 64;
+  static constexpr bool kAlias = DP == 128;  // dS over S: no room for its own columns
+  static constexpr int kSlots = DP == 64 ? 4 : 2;
+  static constexpr int kSlot = KT * DP * 2;
+  static constexpr int kQ = 128 * DP * 2;
+  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 256 + 1024;
+  static constexpr uint32_t kDp = 64, kDs = kAlias ? 0 : 192, kDq = 128;
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kAttnThreads, 2)
+    win_dq_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, int* err) {
+  using C = DqCfg<DP>;
+  constexpr int KT = C::KT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + 2 * C::kQ;  // queries, dO, then the ring
+  uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kSlot);
+  uint64_t* empty = full + C::kSlots;
+  uint64_t* q_full = empty + C::kSlots;
+  uint64_t* s_full = q_full + 1;   // S and dP
+  uint64_t* s_empty = s_full + 1;
+  uint64_t* ds_full = s_empty + 1;
+  uint64_t* dq_done = ds_full + 1;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(dq_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int i0 = blockIdx.x * 128, h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
+  const int L = win_length(p, b);
+  const KeyTiles kt = key_tiles<KT>(p, L, i0);
+  const int kd = (p.D + 15) / 16;
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(q_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(s_empty, 4);
+    mbar_init(ds_full, 4);
+    mbar_init(dq_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, 256);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && kt.n > 0) {
+      mbar_arrive_expect_tx(q_full, 2 * C::kQ);
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a) {
+        tma_load_4d(smem + a * 128 * kAtom, &maps.q, q_full, a * 64, i0, h, b);
+        tma_load_4d(smem + C::kQ + a * 128 * kAtom, &maps.g, q_full, a * 64, i0, h, b);
+      }
+      int it = 0;
+      bool go = true;
+      for (int j = 0; j < kt.n && go; ++j) {
+        int j0, cols;
+        key_tile<KT>(kt, j, &j0, &cols);
+        for (int kv = 0; kv < 2; ++kv, ++it) {
+          const int s = it % C::kSlots;
+          if (!mbar_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+            *abort_flag = 1;
+            go = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], C::kSlot);
+#pragma unroll
+          for (int a = 0; a < DP / 64; ++a)
+            tma_load_4d(ring + s * C::kSlot + a * KT * kAtom, kv ? &maps.v : &maps.k, &full[s], a * 64, j0, hk, b);
+        }
+      }
+      mbar_wait(q_full, 0, err, kErrTimeoutDrain);
+      for (int i = max(0, it - C::kSlots); i < it; ++i)
+        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && kt.n > 0) {
+      const uint32_t idesc_s = make_idesc(1, 0, 0, 128, 0), idesc_q = make_idesc(1, 0, 1, 128, 16 * kd);
+      const uint32_t sq = smem_u32(smem), sg = sq + C::kQ, sr = smem_u32(ring);
+      auto scores = [&](int j) {  // S = Q K^T, dP = dO V^T
+        int j0, cols;
+        key_tile<KT>(kt, j, &j0, &cols);
+        const uint32_t id = idesc_s | ((cols >> 3) << 17);
+        const int ik = 2 * j, iv = ik + 1, s = ik % C::kSlots, sv = iv % C::kSlots;
+        // S lies over dS at D = 128: then the product that reads dS has to be over, not only the reading of S
+        if (j > 0 && !mbar_wait(C::kAlias ? dq_done : s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
+        if (!mbar_wait(&full[s], (ik / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        tc_fence_after();
+        for (int k = 0; k < kd; ++k)
+          umma_bf16(tmem, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), id, k ? 1u : 0u);
+        if (!mbar_wait(&full[sv], (iv / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        tc_fence_after();
+        for (int k = 0; k < kd; ++k)
+          umma_bf16(tmem + C::kDp, desc_k(sg, 128, k), desc_k(sr + sv * C::kSlot, KT, k), id, k ? 1u : 0u);
+        tc_commit(&empty[sv]);
+        tc_commit(s_full);
+        return true;
+      };
+      bool go = mbar_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
+      for (int j = 0; j < kt.n && go; ++j) {
+        if (!C::kAlias && j + 1 < kt.n && !scores(j + 1)) {
+          go = false;
+          break;
+        }
+        int j0, cols;
+        key_tile<KT>(kt, j, &j0, &cols);
+        const int s = (2 * j) % C::kSlots;
+        if (!mbar_wait(ds_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
+          go = false;
+          break;
+        }
+        tc_fence_after();
+        for (int k = 0; k < cols / 16; ++k)  // dQ += dS K
+          umma_bf16_ts(tmem + C::kDq, tmem + C::kDs + k * 8, desc_mn(sr + s * C::kSlot, KT, k), idesc_q,
+                       (j | k) ? 1u : 0u);
+        tc_commit(&empty[s]);
+        tc_commit(dq_done);
+        if (C::kAlias && j + 1 < kt.n && !scores(j + 1)) go = false;
+      }
+      if (!go) *abort_flag = 1;
+    }
+  } else {
+    const int q4 = warp & 3, row = q4 * 32 + lane, i = i0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const int w0 = i0 + q4 * 32, w1 = w0 + 31;
+    const long long srow = (static_cast<long long>(b) * p.H + h) * p.S + i;
+    float delta = 0.f, lse = INFINITY;
+    if (i < p.S) {
+      lse = p.lse[srow];
+      const uint4* o = reinterpret_cast<const uint4*>(
+          static_cast<const __nv_bfloat16*>(p.o) + ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D);
+      const uint4* g = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.dout) + b * p.g_sb +
+                                                      i * p.g_ss + h * p.g_sh);
+      for (int d = 0; d < p.D / 8; ++d) {
+        const uint4 x = o[d], y = g[d];
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          delta = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), delta);
+          delta = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), delta);
+        }
+      }
+      p.delta[srow] = delta;
+    }
+    bool ok = true;
+    for (int j = 0; j < kt.n; ++j) {
+      int j0, cols;
+      key_tile<KT>(kt, j, &j0, &cols);
+      if (!(ok = warp_wait(s_full, j & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+      tc_fence_after();
+      const bool whole = j >= kt.n_sink && (cols & 31) == 0 && j0 + cols <= L && j0 > w1 - p.window &&
+                         j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
+      const Sight si = sight_of(p, kt, L, i, j, j0);
+      uint32_t ds[KT / 2];
+#pragma unroll
+      for (int ch = 0; ch < KT / 32; ++ch)
+        if (ch * 32 < cols) {
+          float s[32], dp[32];
+          load_row32(tmem + lanes + ch * 32, s);
+          load_row32(tmem + C::kDp + lanes + ch * 32, dp);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; ++e) s[e] = ex2(fmaf(s[e], c, -lse)) * (dp[e] - delta);
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) s[e] = in_sight(si, ch * 32 + e) ? s[e] : 0.f;
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) ds[ch * 16 + e / 2] = pack_f2(s[e], s[e + 1]);
+        }
+      tc_fence_before();
+      if (!C::kAlias) {
+        __syncwarp();
+        if (lane == 0) mbar_arrive(s_empty);
+        if (j > 0) {  // the product before has read dS
+          if (!(ok = warp_wait(dq_done, (j - 1) & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+          tc_fence_after();
+        }
+      }
+#pragma unroll
+      for (int ch = 0; ch < KT / 32; ++ch)
+        if (ch * 32 < cols) tmem_st_32x32b_x16(tmem + C::kDs + lanes + ch * 16, ds + ch * 16);
+      if (j0 + cols > L)  // K has arrived: S was made from it
+        clear_rows<DP>(ring + ((2 * j) % C::kSlots) * C::kSlot, KT, max(0, L - j0), cols, threadIdx.x - 64);
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    if (ok && kt.n > 0) ok = warp_wait(dq_done, (kt.n - 1) & 1, abort_flag, err, kErrTimeoutTmemFull);
+    tc_fence_after();
+    if (!ok) {
+      *abort_flag = 1;
+    } else {
+      stage_row<DP>(smem, tmem + C::kDq + lanes, kt.n > 0, p.scale, row);
+      __syncwarp();
+      __nv_bfloat16* dq = static_cast<__nv_bfloat16*>(p.dq) +
+                          ((static_cast<long long>(b) * p.S + i0) * p.H + h) * p.D;
+      store_rows<DP>(smem, dq, static_cast<long long>(p.H) * p.D, p.D, q4 * 32, 0, p.S - i0, lane);
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, 256);
+  }
+}
+
+// ── dk and dv ──────────────────────────────────────────────────────────────
+template <int DP>
+struct DkvCfg {
+  static constexpr int QT = 64;
+  static constexpr int kBufs = DP == 64 ? 1 : 2;  // score tiles in flight
+  static constexpr int kSlots = 4;
+  static constexpr int kSlot = QT * DP * 2;
+  static constexpr int kK = 128 * DP * 2;
+  static constexpr int kSmem = 2 * kK + kSlots * kSlot + 2 * 2 * QT * 4 + 256 + 1024;
+  static constexpr uint32_t kCols = DP == 64 ? 256 : 512;
+  static constexpr uint32_t kDv = kBufs * 128, kDk = kDv + DP;  // S at 0, dP at 64 of each buffer
+  static constexpr int kPerSm = DP == 64 ? 2 : 1;
+};
+
+// Parts of the sinks' gradients: [B][Hk][sink tile][1 + extra][dk, dv][rows][D] fp32.
+struct SinkParts {
+  float* part;
+  int tiles, extra, rows;  // sink tiles, extra CTAs for each, rows kept of a tile (at most 128)
+};
+
+template <int DP>
+__global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
+    win_dkv_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, const SinkParts sp,
+                  int* err) {
+  using C = DkvCfg<DP>;
+  constexpr int QT = C::QT;
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint8_t* ring = smem + 2 * C::kK;  // keys, values, then the ring
+  float* stat = reinterpret_cast<float*>(ring + C::kSlots * C::kSlot);  // [2][lse, delta][QT]
+  uint64_t* full = reinterpret_cast<uint64_t*>(stat + 4 * QT);
+  uint64_t* empty = full + C::kSlots;
+  uint64_t* k_full = empty + C::kSlots;
+  uint64_t* s_full = k_full + 1;   // S and dP
+  uint64_t* ds_full = s_full + 1;  // P and dS
+  uint64_t* d_done = ds_full + 1;   // dV and dK of an iteration
+  uint64_t* all_done = d_done + 1;  // of the last one
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hk;
+  // the first CTAs of a head are the extra ones of its sink tiles
+  const int n_extra = sp.tiles * sp.extra;
+  const bool extra = static_cast<int>(blockIdx.x) < n_extra;
+  const int tile = extra ? blockIdx.x / sp.extra : blockIdx.x - n_extra;
+  const int j0 = tile * 128;
+  const int L = win_length(p, b);
+  const int kd = (p.D + 15) / 16;
+  // Queries of the tile's window, [lo, hi), are the tile's own; of what is left,
+  // [0, lo) (not causal) and [hi, S), each extra CTA takes a run of query tiles.
+  const int lo = p.causal ? j0 : max(0, j0 - (p.window - 1));
+  const int hi = min(p.S, j0 + 127 + p.window);
+  const int before = p.causal ? 0 : (lo + QT - 1) / QT, after = (p.S - hi + QT - 1) / QT;
+  int n, first = 0;  // iterations: query tiles x heads of the group
+  int span;          // query tiles of one head
+  if (extra) {
+    span = before + after;
+    const int all = span * group, per = (all + sp.extra - 1) / sp.extra;
+    first = min(all, static_cast<int>(blockIdx.x - tile * sp.extra) * per);
+    n = min(all, first + per) - first;
+  } else {
+    span = (hi - lo + QT - 1) / QT;
+    n = span * group;
+  }
+  if (j0 >= L) n = 0;
+  // head and first query of iteration it, and where its queries end
+  auto query_tile = [&](int it, int* h, int* i0, int* end) {
+    const int u = first + it, t = u % span;
+    *h = hk * group + u / span;
+    if (!extra) {
+      *i0 = lo + t * QT;
+      *end = hi;
+    } else if (t < before) {
+      *i0 = t * QT;
+      *end = lo;
+    } else {
+      *i0 = hi + (t - before) * QT;
+      *end = p.S;
+    }
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < C::kSlots; ++s) {
+      mbar_init(&full[s], 1);
+      mbar_init(&empty[s], 1);
+    }
+    mbar_init(k_full, 1);
+    mbar_init(s_full, 1);
+    mbar_init(ds_full, 4);
+    mbar_init(d_done, 1);
+    mbar_init(all_done, 1);
+    *abort_flag = 0;
+    fence_barrier_init();
+  }
+  if (warp == 1) {
+    tmem_alloc(tmem_slot, C::kCols);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0 && n > 0) {
+      mbar_arrive_expect_tx(k_full, 2 * C::kK);
+#pragma unroll
+      for (int a = 0; a < DP / 64; ++a)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {  // the keys' map has boxes of 64 rows
+          tma_load_4d(smem + (a * 128 + r * 64) * kAtom, &maps.k, k_full, a * 64, j0 + r * 64, hk, b);
+          tma_load_4d(smem + C::kK + (a * 128 + r * 64) * kAtom, &maps.v, k_full, a * 64, j0 + r * 64, hk, b);
+        }
+      int it = 0;
+      bool go = true;
+      for (int t = 0; t < n && go; ++t) {
+        int h, i0, end;
+        query_tile(t, &h, &i0, &end);
+        for (int qg = 0; qg < 2; ++qg, ++it) {
+          const int s = it % C::kSlots;
+          if (!mbar_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+            *abort_flag = 1;
+            go = false;
+            break;
+          }
+          mbar_arrive_expect_tx(&full[s], C::kSlot);
+#pragma unroll
+          for (int a = 0; a < DP / 64; ++a)
+            tma_load_4d(ring + s * C::kSlot + a * QT * kAtom, qg ? &maps.g : &maps.q, &full[s], a * 64, i0, h, b);
+        }
+      }
+      mbar_wait(k_full, 0, err, kErrTimeoutDrain);
+      for (int i = max(0, it - C::kSlots); i < it; ++i)
+        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
+    }
+  } else if (warp == 1) {
+    if (lane == 0 && n > 0) {
+      const uint32_t idesc_s = make_idesc(1, 0, 0, 128, QT), idesc_d = make_idesc(1, 0, 1, 128, 16 * kd);
+      const uint32_t sk = smem_u32(smem), sv = sk + C::kK, sr = smem_u32(ring);
+      // S^T = K Q^T and dP^T = V dO^T, once the products that read P and dS from this buffer are over
+      auto scores = [&](int t) {
+        if (t >= C::kBufs && !mbar_wait(d_done, (t - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
+        const uint32_t buf = tmem + (t % C::kBufs) * 128;
+        const int iq = 2 * t, ig = iq + 1, s = iq % C::kSlots, sg = ig % C::kSlots;
+        if (!mbar_wait(&full[s], (iq / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        tc_fence_after();
+        for (int k = 0; k < kd; ++k)
+          umma_bf16(buf, desc_k(sk, 128, k), desc_k(sr + s * C::kSlot, QT, k), idesc_s, k ? 1u : 0u);
+        if (!mbar_wait(&full[sg], (ig / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        tc_fence_after();
+        for (int k = 0; k < kd; ++k)
+          umma_bf16(buf + 64, desc_k(sv, 128, k), desc_k(sr + sg * C::kSlot, QT, k), idesc_s, k ? 1u : 0u);
+        tc_commit(s_full);
+        return true;
+      };
+      bool go = mbar_wait(k_full, 0, err, kErrTimeoutFull) && scores(0);
+      for (int t = 0; t < n && go; ++t) {
+        if (C::kBufs == 2 && t + 1 < n && !scores(t + 1)) {
+          go = false;
+          break;
+        }
+        if (!mbar_wait(ds_full, t & 1, err, kErrTimeoutFull) || *abort_flag) {
+          go = false;
+          break;
+        }
+        tc_fence_after();
+        const uint32_t buf = tmem + (t % C::kBufs) * 128;
+        const int s = (2 * t) % C::kSlots, sg = (2 * t + 1) % C::kSlots;
+#pragma unroll
+        for (int k = 0; k < QT / 16; ++k)  // dV += P^T dO
+          umma_bf16_ts(tmem + C::kDv, buf + k * 8, desc_mn(sr + sg * C::kSlot, QT, k), idesc_d, (t | k) ? 1u : 0u);
+        tc_commit(&empty[sg]);
+#pragma unroll
+        for (int k = 0; k < QT / 16; ++k)  // dK += dS^T Q
+          umma_bf16_ts(tmem + C::kDk, buf + 64 + k * 8, desc_mn(sr + s * C::kSlot, QT, k), idesc_d,
+                       (t | k) ? 1u : 0u);
+        tc_commit(&empty[s]);
+        tc_commit(d_done);
+        if (t + 1 == n) tc_commit(all_done);
+        if (C::kBufs == 1 && t + 1 < n && !scores(t + 1)) go = false;
+      }
+      if (!go) *abort_flag = 1;
+    }
+  } else {
+    const int q4 = warp & 3, row = q4 * 32 + lane, j = j0 + row;
+    const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
+    const float c = p.scale * kLog2e;
+    const int tid = threadIdx.x - 64;
+    const int w0 = j0 + q4 * 32, w1 = w0 + 31;
+    // an extra CTA's rows behind the sinks are nobody's: their warps only keep step
+    const bool idle = extra && w0 >= p.sinks;
+    const bool sink = j < p.sinks, valid = j < L;
+    const bool part_rows = sp.extra > 0 && tile < sp.tiles;
+    auto load_stat = [&](int t) {  // this thread's value of iteration t's lse (threads 0-63) or delta
+      int h, i0, end;
+      query_tile(t, &h, &i0, &end);
+      const int i = i0 + (tid & 63);
+      const long long at = (static_cast<long long>(b) * p.H + h) * p.S + i;
+      return tid < 64 ? (i < end ? p.lse[at] : INFINITY) : (i < end ? p.delta[at] : 0.f);
+    };
+    float next = n > 0 ? load_stat(0) : 0.f;
+    bool ok = true;
+    for (int t = 0; t < n; ++t) {
+      int h, i0, end;
+      query_tile(t, &h, &i0, &end);
+      float* st = stat + (t & 1) * 2 * QT;
+      st[tid] = next;
+      asm volatile("bar.sync 1, 128;" ::: "memory");  // also: everyone is done with the buffer of t - 1
+      if (t + 1 < n) next = load_stat(t + 1);
+      // after a wait that gave up the loop goes on empty: the other warps count on this one at the barrier
+      if (ok) ok = warp_wait(s_full, t & 1, abort_flag, err, kErrTimeoutTmemFull);
+      if (!ok) continue;
+      tc_fence_after();
+      if (!idle) {
+        const uint32_t buf = tmem + lanes + (t % C::kBufs) * 128;
+        // queries [qa, qb) of the tile see this thread's key
+        int qa, qb;
+        if (extra) {
+          qa = 0;
+          qb = sink && valid ? QT : 0;
+        } else {
+          qa = (p.causal ? j : (sink ? i0 : j - (p.window - 1))) - i0;
+          qb = valid ? (sink ? QT : j + p.window - i0) : 0;
+        }
+        const bool whole = !extra && w1 < L && i0 >= (p.causal ? w1 : w1 - (p.window - 1)) &&
+                           i0 + QT <= w0 + p.window;
+        uint32_t pk[QT / 2], dk[QT / 2];
+#pragma unroll
+        for (int ch = 0; ch < QT / 32; ++ch) {
+          float s[32], dp[32];
+          load_row32(buf + ch * 32, s);
+          load_row32(buf + 64 + ch * 32, dp);
+          tmem_ld_wait();
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            const float4 ls = *reinterpret_cast<const float4*>(st + ch * 32 + e);
+            const float4 de = *reinterpret_cast<const float4*>(st + QT + ch * 32 + e);
+            const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {de.x, de.y, de.z, de.w};
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+              s[e + u] = ex2(fmaf(s[e + u], c, -lv[u]));
+              dp[e + u] = s[e + u] * (dp[e + u] - dv[u]);
+            }
+          }
+          if (!whole) {
+#pragma unroll
+            for (int e = 0; e < 32; ++e) {
+              const bool on = ch * 32 + e >= qa && ch * 32 + e < qb;
+              s[e] = on ? s[e] : 0.f;
+              dp[e] = on ? dp[e] : 0.f;
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 32; e += 2) {
+            pk[ch * 16 + e / 2] = pack_f2(s[e], s[e + 1]);
+            dk[ch * 16 + e / 2] = pack_f2(dp[e], dp[e + 1]);
+          }
+        }
+        tmem_st_32x32b_x32(buf, pk);
+        tmem_st_32x32b_x32(buf + 64, dk);
+        tmem_st_wait();
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
+    }
+    if (ok && n > 0) ok = warp_wait(all_done, 0, abort_flag, err, kErrTimeoutTmemFull);
+    tc_fence_after();
+    if (!ok) {
+      *abort_flag = 1;
+    } else {
+      const uint32_t tk = tmem + lanes + C::kDk, tv = tmem + lanes + C::kDv;
+      if (part_rows && w0 < p.sinks) {  // the sinks' rows, in fp32
+        const int slot = extra ? 1 + static_cast<int>(blockIdx.x) - tile * sp.extra : 0;
+        float* dst = sp.part + ((((static_cast<long long>(b) * p.Hk + hk) * sp.tiles + tile) * (1 + sp.extra) + slot) *
+                                    2 * sp.rows + row) * p.D;
+#pragma unroll 1
+        for (int kv = 0; kv < 2; ++kv) {
+#pragma unroll 1
+          for (int ch = 0; ch < DP / 32; ++ch) {
+            float v[32];
+            if (n > 0) {
+              load_row32((kv ? tv : tk) + ch * 32, v);
+              tmem_ld_wait();
+            }
+            if (!sink) continue;
+#pragma unroll
+            for (int e = 0; e < 32; e += 4) {
+              if (ch * 32 + e >= p.D) break;
+              const float f = kv ? 1.f : p.scale;
+              *reinterpret_cast<float4*>(dst + static_cast<long long>(kv) * sp.rows * p.D + ch * 32 + e) =
+                  n > 0 ? make_float4(v[e] * f, v[e + 1] * f, v[e + 2] * f, v[e + 3] * f)
+                        : make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+          }
+        }
+      }
+      if (!extra) {
+        const int from = part_rows ? min(128, max(0, p.sinks - j0)) : 0;
+        const long long stride = static_cast<long long>(p.Hk) * p.D;
+        const long long at = ((static_cast<long long>(b) * p.S + j0) * p.Hk + hk) * p.D;
+        // every product has read the keys and values: their tiles are the staging tiles now
+        stage_row<DP>(smem, tk, n > 0, p.scale, row);
+        stage_row<DP>(smem + C::kK, tv, n > 0, 1.f, row);
+        __syncwarp();
+        store_rows<DP>(smem, static_cast<__nv_bfloat16*>(p.dk) + at, stride, p.D, q4 * 32, from, p.S - j0, lane);
+        store_rows<DP>(smem + C::kK, static_cast<__nv_bfloat16*>(p.dv) + at, stride, p.D, q4 * 32, from, p.S - j0,
+                       lane);
+      }
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, C::kCols);
+  }
+}
+
+// dk and dv of the sinks from their parts, added in order.
+__global__ void __launch_bounds__(128) join_sinks_kernel(const WinParams p, const SinkParts sp) {
+  const int j = blockIdx.x, hk = blockIdx.y, b = blockIdx.z;
+  const int tile = j / 128, row = j % 128;
+  const long long step = 2ll * sp.rows * p.D;
+  const float* src = sp.part + ((static_cast<long long>(b) * p.Hk + hk) * sp.tiles + tile) * (1 + sp.extra) * step +
+                     static_cast<long long>(row) * p.D;
+  const long long at = ((static_cast<long long>(b) * p.S + j) * p.Hk + hk) * p.D;
+  for (int e = threadIdx.x; e < 2 * p.D; e += 128) {
+    const int kv = e / p.D, d = e - kv * p.D;
+    float a = 0.f;
+    for (int s = 0; s <= sp.extra; ++s) a += src[s * step + static_cast<long long>(kv) * sp.rows * p.D + d];
+    static_cast<__nv_bfloat16*>(kv ? p.dv : p.dk)[at + d] = __float2bfloat16(a);
+  }
+}
+
+// ── host ───────────────────────────────────────────────────────────────────
+CUtensorMap head_map(const void* ptr, int D, int S, int H, int B, long long ss, long long sh, long long sb, int rows) {
+  // a dimension of one element may carry any stride: give it a valid one
+  const uint64_t row = static_cast<uint64_t>((D + 7) / 8 * 8) * 2;
+  const uint64_t dims[4] = {static_cast<uint64_t>(D), static_cast<uint64_t>(S), static_cast<uint64_t>(H),
+                            static_cast<uint64_t>(B)};
+  const uint64_t strides[3] = {S > 1 ? static_cast<uint64_t>(ss) * 2 : row, H > 1 ? static_cast<uint64_t>(sh) * 2 : row,
+                               B > 1 ? static_cast<uint64_t>(sb) * 2 : row};
+  const uint32_t box[4] = {64, static_cast<uint32_t>(rows), 1, 1};
+  return tmap_bf16<4>(ptr, dims, strides, box);
+}
+
+bool tma_heads(const void* ptr, int S, int H, int B, long long ss, long long sh, long long sb) {
+  auto ok = [](int n, long long s) { return n <= 1 || (s > 0 && s % 8 == 0); };
+  return reinterpret_cast<uintptr_t>(ptr) % 16 == 0 && ok(S, ss) && ok(H, sh) && ok(B, sb);
+}
+
+template <typename K>
+void allow_smem(K kern, int bytes, bool (&set)[64]) {
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev < 64 && set[dev]) return;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes));
+  if (dev < 64) set[dev] = true;
+}
+
+AttnMaps maps_of(const WinParams& p, int q_rows, int k_rows) {
+  AttnMaps m;
+  m.q = head_map(p.q, p.D, p.S, p.H, p.B, p.q_ss, p.q_sh, p.q_sb, q_rows);
+  m.k = head_map(p.k, p.D, p.S, p.Hk, p.B, p.k_ss, p.k_sh, p.k_sb, k_rows);
+  m.v = head_map(p.v, p.D, p.S, p.Hk, p.B, p.v_ss, p.v_sh, p.v_sb, k_rows);
+  m.g = p.dout ? head_map(p.dout, p.D, p.S, p.H, p.B, p.g_ss, p.g_sh, p.g_sb, q_rows) : m.q;
+  return m;
+}
+
+template <int DP>
+void fwd(const WinParams& p, cudaStream_t st, int* err) {
+  using C = FwdCfg<DP>;
+  static bool set[64] = {false};
+  allow_smem(win_fwd_sm100<DP>, C::kSmem, set);
+  win_fwd_sm100<DP><<<dim3((p.S + 127) / 128, p.H, p.B), kAttnThreads, C::kSmem, st>>>(maps_of(p, 128, C::KT), p, err);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+}
+
+template <int DP>
+void bwd(const WinParams& p, cudaStream_t st, int* err) {
+  {
+    using C = DqCfg<DP>;
+    static bool set[64] = {false};
+    allow_smem(win_dq_sm100<DP>, C::kSmem, set);
+    win_dq_sm100<DP><<<dim3((p.S + 127) / 128, p.H, p.B), kAttnThreads, C::kSmem, st>>>(maps_of(p, 128, C::KT), p, err);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  using C = DkvCfg<DP>;
+  static bool set[64] = {false};
+  allow_smem(win_dkv_sm100<DP>, C::kSmem, set);
+  SinkParts sp{};
+  at::Tensor part;
+  const int k_tiles = (p.S + 127) / 128;
+  // Queries that the sinks' own tiles leave over, in CTAs of an ordinary tile's size.
+  const int own = 127 + p.window + (p.causal ? 0 : p.window);
+  const int sink_tiles = (p.sinks + 127) / 128;
+  if (p.sinks > 0 && (p.S > 127 + p.window || (!p.causal && (sink_tiles - 1) * 128 > p.window - 1))) {
+    sp.tiles = sink_tiles;
+    sp.rows = std::min(p.sinks, 128);
+    sp.extra = static_cast<int>(std::max(1ll, (p.S - 127ll - p.window + own - 1) / own));
+    sp.extra = std::min(sp.extra, std::max(1, 512 / sink_tiles));  // enough to fill the SMs; bounds the parts
+    part = out_empty({p.B, p.Hk, sp.tiles, 1 + sp.extra, 2, sp.rows, p.D},
+                     at::TensorOptions().dtype(at::kFloat).device(at::kCUDA, at::cuda::current_device()));
+    sp.part = part.data_ptr<float>();
+  }
+  win_dkv_sm100<DP><<<dim3(k_tiles + sp.tiles * sp.extra, p.Hk, p.B), kAttnThreads, C::kSmem, st>>>(
+      maps_of(p, C::QT, 64), p, sp, err);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
+  if (sp.extra > 0) {
+    join_sinks_kernel<<<dim3(p.sinks, p.Hk, p.B), 128, 0, st>>>(p, sp);
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+}
+
+}  // namespace
+
+// bf16 operands that TMA can read in place; a positive scale (the running
+// maximum is taken before scaling).
+bool window_sm100_takes(const WinParams& p, bool bf16) {
+  return bf16 && p.D % 8 == 0 && p.scale > 0.f && reinterpret_cast<uintptr_t>(p.o) % 16 == 0 && tma_heads(p.q, p.S, p.H, p.B, p.q_ss, p.q_sh, p.q_sb) &&
+         tma_heads(p.k, p.S, p.Hk, p.B, p.k_ss, p.k_sh, p.k_sb) &&
+         tma_heads(p.v, p.S, p.Hk, p.B, p.v_ss, p.v_sh, p.v_sb) &&
+         (!p.dout || tma_heads(p.dout, p.S, p.H, p.B, p.g_ss, p.g_sh, p.g_sb));
+}
+
+void window_sm100_fwd(const WinParams& p, cudaStream_t st, int* err) {
+  if (p.D <= 64)
+    fwd<64>(p, st, err);
+  else
+    fwd<128>(p, st, err);
+}
+
+void window_sm100_bwd(const WinParams& p, cudaStream_t st, int* err) {
+  if (p.D <= 64)
+    bwd<64>(p, st, err);
+  else
+    bwd<128>(p, st, err);
+}
+
+}  // namespace tgcm
