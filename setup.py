@@ -19,7 +19,7 @@ NVCC_FLAGS = [
     "-Xptxas=-v" if os.environ.get("TGCM_PTXAS_VERBOSE") else "-Xptxas=-O3",
 ]
 
-sources = sorted(glob.glob(os.path.join(CSRC, "*.cu"))) + [os.path.join(CSRC, "bindings.cpp")]
+sources = sorted(glob.glob(os.path.join(CSRC, "*.cu"))) + sorted(glob.glob(os.path.join(CSRC, "*.cpp")))
 
 setup(
     name="tornado_gcm_b200",

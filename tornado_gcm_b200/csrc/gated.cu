@@ -33,12 +33,12 @@
 // A few tokens (T <= 8) take skinny_kernel instead: bound by reading the
 // weights once, a warp to each hidden value, both weight rows in flight.
 #include "alloc.h"
+#include "sequence_ops.h"
 #include "tmap.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/library.h>
 
 #include <algorithm>
 
@@ -772,7 +772,7 @@ at::Tensor gated_fwd(const at::Tensor& x_in, const at::Tensor& wg_in, const at::
   return h;
 }
 
-// dx, dWg, dWu, dbg, dbu; the ones not asked for are empty tensors.
+// dx, dWg, dWu, dbg, dbu; the ones not asked for are undefined.
 std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_in, const at::Tensor& wg_in,
                                   const at::Tensor& wu_in, const c10::optional<at::Tensor>& bg,
                                   const c10::optional<at::Tensor>& bu, int64_t act, bool need_x, bool need_w,
@@ -789,9 +789,7 @@ std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_i
   auto dwg = need_w ? out_empty({F, K0}, opt) : at::Tensor(), dwu = need_w ? out_empty({F, K0}, opt) : at::Tensor();
   auto dbg = need_b ? out_empty({F}, opt) : at::Tensor(), dbu = need_b ? out_empty({F}, opt) : at::Tensor();
   auto result = [&] {
-    auto e = at::empty({0}, opt);
-    return std::vector<at::Tensor>{need_x ? dx : e, need_w ? dwg : e, need_w ? dwu : e, need_b ? dbg : e,
-                                   need_b ? dbu : e};
+    return std::vector<at::Tensor>{dx, dwg, dwu, dbg, dbu};
   };
   if (T == 0) {
     for (auto* t : {&dwg, &dwu, &dbg, &dbu})
@@ -884,14 +882,3 @@ std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_i
 }
 
 }  // namespace tgcm
-
-TORCH_LIBRARY_FRAGMENT(tgcm, m) {
-  m.def("gated_fwd(Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act, Tensor? err) -> Tensor");
-  m.def("gated_bwd(Tensor dh, Tensor x, Tensor w_gate, Tensor w_up, Tensor? b_gate, Tensor? b_up, int act, bool need_x, "
-        "bool need_w, bool need_b, Tensor? err) -> Tensor[]");
-}
-
-TORCH_LIBRARY_IMPL(tgcm, CUDA, m) {
-  m.impl("gated_fwd", &tgcm::gated_fwd);
-  m.impl("gated_bwd", &tgcm::gated_bwd);
-}

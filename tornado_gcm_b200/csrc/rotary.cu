@@ -25,11 +25,11 @@
 // sums them in registers; blocks leave one partial each and a second kernel
 // adds the partials in order (no atomics).
 #include "alloc.h"
+#include "sequence_ops.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/library.h>
 
 #include <algorithm>
 #include <string>
@@ -621,16 +621,3 @@ std::vector<at::Tensor> qk_norm_rotary_bwd(const at::Tensor& dyq, const at::Tens
 }
 
 }  // namespace tgcm
-
-TORCH_LIBRARY_FRAGMENT(tgcm, m) {
-  m.def("qk_norm_rotary_fwd(Tensor q, Tensor k, Tensor? table, Tensor? positions, Tensor? q_weight, Tensor? k_weight, "
-        "Tensor? q_bias, Tensor? k_bias, int norm, bool interleaved, float eps, Tensor? err) -> Tensor[]");
-  m.def("qk_norm_rotary_bwd(Tensor dyq, Tensor dyk, Tensor q, Tensor k, Tensor? table, Tensor? positions, "
-        "Tensor? q_weight, Tensor? k_weight, int norm, bool interleaved, float eps, bool params, Tensor? err) "
-        "-> Tensor[]");
-}
-
-TORCH_LIBRARY_IMPL(tgcm, CUDA, m) {
-  m.impl("qk_norm_rotary_fwd", &tgcm::qk_norm_rotary_fwd);
-  m.impl("qk_norm_rotary_bwd", &tgcm::qk_norm_rotary_bwd);
-}

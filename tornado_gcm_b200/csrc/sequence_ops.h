@@ -1,0 +1,39 @@
+// Kernel entry points of the sequence operators that have a backward pass.
+#pragma once
+
+#include <ATen/ATen.h>
+
+#include <vector>
+
+namespace tgcm {
+
+using OptTensor = c10::optional<at::Tensor>;
+
+at::Tensor gated_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const OptTensor& bg,
+                     const OptTensor& bu, int64_t act, const OptTensor& err);
+// dx, dWg, dWu, dbg, dbu; the ones not asked for are undefined
+std::vector<at::Tensor> gated_bwd(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg,
+                                  const at::Tensor& wu, const OptTensor& bg, const OptTensor& bu, int64_t act,
+                                  bool need_x, bool need_w, bool need_b, const OptTensor& err);
+
+std::vector<at::Tensor> qk_norm_rotary_fwd(const at::Tensor& q, const at::Tensor& k, const OptTensor& table,
+                                           const OptTensor& positions, const OptTensor& qw, const OptTensor& kw,
+                                           const OptTensor& qb, const OptTensor& kb, int64_t norm, bool interleaved,
+                                           double eps, const OptTensor& err);
+// dq, dk and, with `params`, (2, 2, D): dw and db of q, then of k
+std::vector<at::Tensor> qk_norm_rotary_bwd(const at::Tensor& dyq, const at::Tensor& dyk, const at::Tensor& q,
+                                           const at::Tensor& k, const OptTensor& table, const OptTensor& positions,
+                                           const OptTensor& qw, const OptTensor& kw, int64_t norm, bool interleaved,
+                                           double eps, bool params, const OptTensor& err);
+
+// o, lse
+std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                             int64_t window, int64_t sinks, bool causal, const OptTensor& lengths,
+                                             double scale, const OptTensor& err);
+// dq, dk, dv
+std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
+                                             const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
+                                             int64_t window, int64_t sinks, bool causal, const OptTensor& lengths,
+                                             double scale, const OptTensor& err);
+
+}  // namespace tgcm

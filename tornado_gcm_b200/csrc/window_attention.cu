@@ -18,11 +18,11 @@
 // 16-byte broadcasts per step.  dk and dv take every query that sees the key
 // in one block: no atomics, so gradients have the same bits every time.
 #include "alloc.h"
+#include "sequence_ops.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <torch/library.h>
 
 #include <algorithm>
 #include <cmath>
@@ -432,15 +432,3 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
 }
 
 }  // namespace tgcm
-
-TORCH_LIBRARY_FRAGMENT(tgcm, m) {
-  m.def("window_attention_fwd(Tensor q, Tensor k, Tensor v, int window, int sinks, bool causal, Tensor? lengths, "
-        "float scale, Tensor? err) -> Tensor[]");
-  m.def("window_attention_bwd(Tensor dout, Tensor q, Tensor k, Tensor v, Tensor o, Tensor lse, int window, int sinks, "
-        "bool causal, Tensor? lengths, float scale, Tensor? err) -> Tensor[]");
-}
-
-TORCH_LIBRARY_IMPL(tgcm, CUDA, m) {
-  m.impl("window_attention_fwd", &tgcm::window_attention_fwd);
-  m.impl("window_attention_bwd", &tgcm::window_attention_bwd);
-}

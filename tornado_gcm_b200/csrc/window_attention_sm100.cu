@@ -38,7 +38,6 @@
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
-#include <torch/library.h>
 
 #include <algorithm>
 

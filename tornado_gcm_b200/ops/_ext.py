@@ -89,15 +89,20 @@ def _flag_key(device) -> str:
 
 def error_flag(device) -> torch.Tensor:
     """Per-device int32 flag that kernels set on a bounded-wait timeout."""
+    if device in _FLAG_OF_DEVICE:  # a tensor's device: no key to build
+        return _FLAG_OF_DEVICE[device]
     key = _flag_key(device)
     t = _FLAGS.get(key)
     if t is None:
         t = torch.zeros(1, dtype=torch.int32, device=device)
         _FLAGS[key] = t
+    if isinstance(device, torch.device) and device.index is not None:
+        _FLAG_OF_DEVICE[device] = t
     return t
 
 
 _FLAGS: dict = {}
+_FLAG_OF_DEVICE: dict = {}
 
 
 def check_error_flag(device) -> int:

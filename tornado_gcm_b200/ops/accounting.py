@@ -89,6 +89,15 @@ def _flops(name: str, args) -> tuple:
             I = N.shape[2] if args[7] else N.shape[1]
             M2 = 2 * Mw - 1
             return 2 * S * J * I * M2 + 2 * S * J * (2 * _tri(Lo, Mw)), "tf32"
+        if name == "gated_linear":
+            x, w = args[0], args[1]
+            return (12 if _trained(args) else 4) * x.shape[0] * w.shape[0] * w.shape[1], "bf16"
+        if name == "window_attention":
+            q, window, sinks, causal = args[0], int(args[3]), int(args[4]), bool(args[5])
+            B, S, H, D = q.shape
+            near = min(window, S) if causal else min(2 * window - 1, S)
+            return (14 if _trained(args) else 4) * B * S * H * D * min(S, near + sinks), (
+                "bf16" if q.dtype == torch.bfloat16 else "fp32")
         if name == "column_attention_fwd":
             q, k = args[0], args[1]
             return 4 * q.shape[0] * q.shape[1] * k.shape[1] * q.shape[2], "fp32"
@@ -100,13 +109,24 @@ def _flops(name: str, args) -> tuple:
     return 0, None
 
 
+#: Ops whose backward pass is native too and runs unseen: one call stands for both.
+_WITH_BACKWARD = ("gated_linear", "qk_norm_rotary", "window_attention")
+
+
+def _trained(args) -> bool:
+    return torch.is_grad_enabled() and any(isinstance(a, torch.Tensor) and a.requires_grad for a in args)
+
+
 def record(name: str, args, kwargs, result) -> None:
     table = _ACTIVE
     if table is None:
         return
     row = table.setdefault(name, {"calls": 0, "bytes": 0, "flops": 0, "cls": None})
     row["calls"] += 1
-    row["bytes"] += _device_bytes(list(args) + list(kwargs.values())) + _device_bytes(result)
+    nbytes = _device_bytes(list(args) + list(kwargs.values())) + _device_bytes(result)
+    # the backward pass reads the inputs and the result's gradient and writes the inputs' gradients
+    row["bytes"] += nbytes if name not in _WITH_BACKWARD or not _trained(args) else (
+        2 * nbytes + _device_bytes([a for a in args if isinstance(a, torch.Tensor) and a.requires_grad]))
     fl, cls = _flops(name, args)
     if fl:
         row["flops"] += fl
@@ -129,6 +149,7 @@ class CountingOps:
             record(name, args, kwargs, out)
             return out
 
+        call.default = call
         return call
 
 

@@ -20,27 +20,6 @@ from tornado_gcm_b200.ops import _ext
 from tornado_gcm_b200.ops.linear import ACT_CODES
 
 
-class GatedLinearFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, wg, wu, bg, bu, act: int):
-        ops = _ext.require("gated linear layer")
-        ctx.save_for_backward(x, wg, wu, bg, bu)
-        ctx.act = act
-        return ops.gated_fwd(x, wg, wu, bg, bu, act, _ext.error_flag(x.device))
-
-    @staticmethod
-    def backward(ctx, g):
-        ops = _ext.require("gated linear layer (backward)")
-        x, wg, wu, bg, bu = ctx.saved_tensors
-        if g.dtype != torch.bfloat16 or g.stride(-1) != 1:
-            g = g.to(torch.bfloat16).contiguous()
-        need = ctx.needs_input_grad
-        dx, dwg, dwu, dbg, dbu = ops.gated_bwd(g, x, wg, wu, bg, bu, ctx.act, need[0], need[1] or need[2],
-                                               need[3] or need[4], _ext.error_flag(g.device))
-        pick = lambda t, on: t if on else None  # noqa: E731
-        return pick(dx, need[0]), pick(dwg, need[1]), pick(dwu, need[2]), pick(dbg, need[3]), pick(dbu, need[4]), None
-
-
 def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_gate: Optional[torch.Tensor] = None,
                  b_up: Optional[torch.Tensor] = None, *, activation: str = "silu") -> torch.Tensor:
     """``(…, F)`` from ``x (…, K)`` and the weights ``(F, K)``; ``activation`` one of ``ops.linear.ACT_CODES``.
@@ -63,9 +42,5 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
     args = [t if t is None or t.dtype == bf else t.to(bf) for t in (x, w_gate, w_up, b_gate, b_up)]
     if x.ndim != 2:
         args[0] = args[0].reshape(-1, x.shape[-1])
-    act = ACT_CODES[activation]
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in args):
-        h = GatedLinearFn.apply(*args, act)
-    else:
-        h = _ext.require("gated linear layer").gated_fwd(*args, act, _ext.error_flag(x.device))
+    h = _ext.require("gated linear layer").gated_linear.default(*args, ACT_CODES[activation], _ext.error_flag(x.device))
     return h if x.ndim == 2 else h.reshape(*x.shape[:-1], h.shape[-1])

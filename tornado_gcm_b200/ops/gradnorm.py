@@ -31,7 +31,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
     if not grads[0].is_cuda:
         return _plain_norm(grads)
     grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
-    return _ext.require("gradient norm").grad_norm(grads)
+    return _ext.require("gradient norm").grad_norm.default(grads)
 
 
 def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
@@ -67,11 +67,11 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
         ops = _ext.require("gradient clipping")
         dense = [g.is_contiguous() and o.is_contiguous() for g, o in zip(grads, out)]
         if all(dense):
-            return ops.clip_grad_norm(grads, out, float(max_norm))
+            return ops.clip_grad_norm.default(grads, out, float(max_norm))
         # strided gradients or outputs pass through contiguous copies
         g2 = [g.contiguous() for g in grads]
         o2 = [o if d else torch.empty_like(g, dtype=o.dtype) for g, o, d in zip(g2, out, dense)]
-        norm = ops.clip_grad_norm(g2, o2, float(max_norm))
+        norm = ops.clip_grad_norm.default(g2, o2, float(max_norm))
         for o, t, d in zip(out, o2, dense):
             if not d:
                 o.copy_(t)

@@ -48,32 +48,6 @@ def rotary_table(positions, rotary_dim: int, base: float = 10000.0, *, scaling: 
     return torch.stack([ang.cos(), ang.sin()], -1).float().to(device or pos.device)
 
 
-class QKNormRotaryFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, table, positions, qw, kw, qb, kb, norm: int, interleaved: bool, eps: float):
-        ops = _ext.require("head norm and rotation")
-        yq, yk = ops.qk_norm_rotary_fwd(q, k, table, positions, qw, kw, qb, kb, norm, interleaved, eps,
-                                        _ext.error_flag(q.device))
-        ctx.save_for_backward(q, k, table, positions, qw, kw)
-        ctx.cfg = (norm, interleaved, eps, qb is not None, kb is not None)
-        return yq, yk
-
-    @staticmethod
-    def backward(ctx, gq, gk):
-        ops = _ext.require("head norm and rotation (adjoint)")
-        q, k, table, positions, qw, kw = ctx.saved_tensors
-        norm, interleaved, eps, has_qb, has_kb = ctx.cfg
-        gq, gk = (g if g.stride(-1) == 1 else g.contiguous() for g in (gq, gk))
-        params = any(ctx.needs_input_grad[4:8])
-        out = ops.qk_norm_rotary_bwd(gq, gk, q, k, table, positions, qw, kw, norm, interleaved, eps, params,
-                                     _ext.error_flag(q.device))
-        dp = out[2].unbind(0) if params else None
-        pick = lambda i, j, on: dp[i][j] if on else None  # noqa: E731
-        need = ctx.needs_input_grad
-        return (out[0], out[1], None, None, pick(0, 0, need[4]), pick(1, 0, need[5]),
-                pick(0, 1, need[6] and has_qb), pick(1, 1, need[7] and has_kb), None, None, None)
-
-
 def _torch_form(q, k, table, positions, qw, kw, qb, kb, norm, interleaved, eps):
     """The same in elementary torch operations (CPU tensors)."""
     out = []
@@ -129,9 +103,6 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tenso
         q = q.contiguous()
     if k.stride(-1) != 1:
         k = k.contiguous()
-    args = (q, k, table, positions, q_weight, k_weight, q_bias, k_bias, NORM_CODES[norm], bool(interleaved), float(eps))
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad
-                                       for t in (q, k, q_weight, k_weight, q_bias, k_bias)):
-        return QKNormRotaryFn.apply(*args)
-    yq, yk = _ext.require("head norm and rotation").qk_norm_rotary_fwd(*args, _ext.error_flag(q.device))
-    return yq, yk
+    return _ext.require("head norm and rotation").qk_norm_rotary.default(
+        q, k, table, positions, q_weight, k_weight, q_bias, k_bias, NORM_CODES[norm], bool(interleaved), float(eps),
+        _ext.error_flag(q.device))

@@ -20,26 +20,6 @@ import torch
 from tornado_gcm_b200.ops import _ext
 
 
-class WindowAttentionFn(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, q, k, v, window: int, sinks: int, causal: bool, lengths, scale: float):
-        ops = _ext.require("window attention")
-        o, lse = ops.window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, _ext.error_flag(q.device))
-        ctx.save_for_backward(q, k, v, o, lse, lengths)
-        ctx.cfg = (window, sinks, causal, scale)
-        return o
-
-    @staticmethod
-    def backward(ctx, g):
-        ops = _ext.require("window attention backward")
-        q, k, v, o, lse, lengths = ctx.saved_tensors
-        window, sinks, causal, scale = ctx.cfg
-        g = g if g.stride(-1) == 1 and g.dtype == o.dtype else g.to(o.dtype).contiguous()
-        dq, dk, dv = ops.window_attention_bwd(g, q, k, v, o, lse, window, sinks, causal, lengths, scale,
-                                              _ext.error_flag(q.device))
-        return dq, dk, dv, None, None, None, None, None
-
-
 def window_mask(sequence: int, window: int, sinks: int = 0, causal: bool = True,
                 lengths: Optional[torch.Tensor] = None, device=None) -> torch.Tensor:
     """``(…, sequence, sequence)`` truth values: query (row) sees key (column)."""
@@ -88,10 +68,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
             raise ValueError("window_attention: q (B, S, H, D) and k, v (B, S, Hk, D) with Hk dividing H expected")
         return _torch_form(q, k, v, window, sinks, causal, lengths, scale)
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
-    if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad):
-        return WindowAttentionFn.apply(q, k, v, int(window), int(sinks), bool(causal), lengths, scale)
-    return _ext.require("window attention").window_attention_fwd(
-        q, k, v, int(window), int(sinks), bool(causal), lengths, scale, _ext.error_flag(q.device))[0]
+    return _ext.require("window attention").window_attention.default(
+        q, k, v, int(window), int(sinks), bool(causal), lengths, scale, _ext.error_flag(q.device))
 
 
 def window_slot(token: torch.Tensor, slots: int, sinks: int) -> torch.Tensor:
@@ -112,8 +90,8 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     """
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if q.is_cuda:
-        return _ext.require("window attention step").window_attention_step(q, k, v, k_cache, v_cache, lengths,
-                                                                           int(sinks), scale)
+        return _ext.require("window attention step").window_attention_step.default(
+            q, k, v, k_cache, v_cache, lengths, int(sinks), scale)
     cap = k_cache.shape[1]
     if not 0 <= sinks < cap:
         raise ValueError("window_attention_step: sinks must lie between 0 and the cache's slots")
