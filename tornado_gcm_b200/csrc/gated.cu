@@ -325,7 +325,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const PairTile c = pair_tile<MODE>(p, t);
         for (int i = 0; i < c.nkb; ++i, ++it) {
           const int s = it % kPairStages;
-          if (!mbar_wait(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
+          if (!mbar_park(&empty_bar[s], ((it / kPairStages) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
             *abort_flag = 1;
             break;
           }
@@ -354,7 +354,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       // no load is in flight when the CTA leaves
       if (rank == 0)
         for (int i = max(0, it - kPairStages); i < it; ++i)
-          mbar_wait(&full_bar[i % kPairStages], (i / kPairStages) & 1, p.err, kErrTimeoutDrain);
+          mbar_park(&full_bar[i % kPairStages], (i / kPairStages) & 1, p.err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
     if (lane == 0 && rank == 0) {
@@ -363,14 +363,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         const PairTile c = pair_tile<MODE>(p, t);
         if (c.nkb == 0) continue;
         const int acc = n & 1;
-        if (!mbar_wait(&acc_empty[acc], ((n >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
+        if (!mbar_park(&acc_empty[acc], ((n >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
           *abort_flag = 1;
           break;
         }
         tc_fence_after();
         for (int i = 0; i < c.nkb; ++i, ++it) {
           const int s = it % kPairStages;
-          if (!mbar_wait(&full_bar[s], (it / kPairStages) & 1, p.err, kErrTimeoutFull)) {
+          if (!mbar_park(&full_bar[s], (it / kPairStages) & 1, p.err, kErrTimeoutFull)) {
             *abort_flag = 1;
             break;
           }
@@ -407,7 +407,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       const int acc = n & 1;
       if (c.nkb > 0) {
-        const bool have = mbar_wait(&acc_full[acc], (n >> 1) & 1, p.err, kErrTimeoutTmemFull);
+        const bool have = mbar_park(&acc_full[acc], (n >> 1) & 1, p.err, kErrTimeoutTmemFull);
         if (__any_sync(0xffffffffu, !have || *abort_flag)) break;
         tc_fence_after();
         ++n;

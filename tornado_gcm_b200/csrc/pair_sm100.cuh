@@ -7,6 +7,30 @@
 
 namespace tgcm {
 
+// Bounded wait that sleeps: a thread whose phase is not over is suspended by the
+// hardware for up to 100 us a try instead of asking again at once, so waiting
+// warps leave the issue slots to the ones that compute.
+__device__ __forceinline__ bool mbar_park(uint64_t* bar, uint32_t parity, int* err, int code) {
+  const uint32_t addr = smem_u32(bar);
+  if (mbar_try_wait(addr, parity)) return true;
+  const uint64_t t0 = global_timer_ns();
+  while (true) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(100000u)
+        : "memory");
+    if (ok) return true;
+    if (global_timer_ns() - t0 > kWaitBudgetNs) {
+      record_error(err, code);
+      return false;
+    }
+  }
+}
+
 __device__ __forceinline__ uint32_t pair_rank() {
   uint32_t r;
   asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));

@@ -47,6 +47,10 @@
 namespace tgcm {
 namespace {
 
+#ifndef TGCM_FB
+#define TGCM_FB 1
+#define TGCM_FP 3
+#endif
 constexpr int kAttnThreads = 192;
 constexpr int kAtom = 128;  // bytes of a swizzled row: 64 bf16
 
@@ -102,6 +106,38 @@ __device__ __forceinline__ float ex2(float x) {
   return y;
 }
 
+// Two fp32 operations in one instruction.
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, c, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+      "fma.rn.f32x2 d, a, b, c;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+  return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "add.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+  float2 d;
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\t"
+      "mul.rn.f32x2 d, a, b;\n\t"
+      "mov.b64 {%0, %1}, d;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+  return d;
+}
+
 __device__ __forceinline__ uint32_t pack_f2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -125,7 +161,7 @@ __device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int rows, int k16) {
 
 // Bounded wait of a whole warp: false in all lanes when one gave up.
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
-  const bool ok = mbar_wait(bar, parity, err, code);
+  const bool ok = mbar_park(bar, parity, err, code);
   return !__any_sync(0xffffffffu, !ok || *abort_flag);
 }
 
@@ -192,23 +228,26 @@ __device__ __forceinline__ void key_tile(const KeyTiles& t, int j, int* j0, int*
   *cols = min(KT, ((sink ? t.sink_end : t.hi) - *j0 + 15) & ~15);
 }
 
-// What query i sees of a key tile starting at j0: columns [a, b) and [0, c).
+// What query i sees of a key tile starting at j0: bit c of the pair of words for column c.
 struct Sight {
-  int a, b, c;
+  uint32_t w[2];
 };
-__device__ __forceinline__ Sight sight_of(const WinParams& p, const KeyTiles& t, int L, int i, int j, int j0) {
+__device__ __forceinline__ unsigned long long bits_below(int x) {
+  return x <= 0 ? 0ull : (x >= 64 ? ~0ull : (1ull << x) - 1);
+}
+__device__ __forceinline__ Sight words(unsigned long long m) {
   Sight s;
-  if (j < t.n_sink) {
-    s.a = s.b = 0;
-    s.c = t.sink_end - j0;  // sinks below the window of every query of the tile: none is ahead of a query
-  } else {
-    s.a = i - (p.window - 1) - j0;
-    s.b = min(L, p.causal ? i + 1 : i + p.window) - j0;
-    s.c = min(min(p.sinks, L), p.causal ? i + 1 : L) - j0;
-  }
+  s.w[0] = static_cast<uint32_t>(m);
+  s.w[1] = static_cast<uint32_t>(m >> 32);
   return s;
 }
-__device__ __forceinline__ bool in_sight(const Sight& s, int c) { return (c >= s.a && c < s.b) || c < s.c; }
+__device__ __forceinline__ Sight sight_of(const WinParams& p, const KeyTiles& t, int L, int i, int j, int j0) {
+  // sinks below the window of every query of the tile: none is ahead of a query
+  if (j < t.n_sink) return words(bits_below(t.sink_end - j0));
+  const int a = i - (p.window - 1), b = min(L, p.causal ? i + 1 : i + p.window);
+  const int c = min(min(p.sinks, L), p.causal ? i + 1 : L);
+  return words((bits_below(b - j0) & ~bits_below(a - j0)) | bits_below(c - j0));
+}
 
 // Zeroes the rows [first, n) of a tile of `rows` rows: keys behind the end may
 // hold NaN, which a weight of zero would not remove from a product.
@@ -225,17 +264,19 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int rows, int first, i
 // ── forward ────────────────────────────────────────────────────────────────
 template <int DP>
 struct FwdCfg {
-  static constexpr int KT = DP == 64 ? 128 : 64;
+  static constexpr int KT = 64;
+  static constexpr int kBufs = DP == 64 ? TGCM_FB : 2;  // score tiles in flight
+  static constexpr int kPerSm = DP == 64 ? TGCM_FP : 2;
   static constexpr int kSlots = 4;
-  static constexpr int kSlot = KT * DP * 2;  // 16 KB
+  static constexpr int kSlot = KT * DP * 2;
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kSmem = kQ + kSlots * kSlot + 256 + 1024;
-  static constexpr uint32_t kP = KT;                        // TMEM columns: S at 0
-  static constexpr uint32_t kO = DP == 64 ? 192 : 128;
+  static constexpr uint32_t kO = kBufs * 64;                // TMEM columns: the scores first, P over them
+  static constexpr uint32_t kCols = kO + DP <= 128 ? 128 : 256;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kAttnThreads, 2)
+__global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
     win_fwd_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, int* err) {
   using C = FwdCfg<DP>;
   constexpr int KT = C::KT;
@@ -246,8 +287,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   uint64_t* empty = full + C::kSlots;
   uint64_t* q_full = empty + C::kSlots;
   uint64_t* s_full = q_full + 1;
-  uint64_t* s_empty = s_full + 1;
-  uint64_t* p_full = s_empty + 1;
+  uint64_t* p_full = s_full + 1;
   uint64_t* pv_done = p_full + 1;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -265,14 +305,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     }
     mbar_init(q_full, 1);
     mbar_init(s_full, 1);
-    mbar_init(s_empty, 4);
     mbar_init(p_full, 4);
     mbar_init(pv_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, 256);
+    tmem_alloc(tmem_slot, C::kCols);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -292,7 +331,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         key_tile<KT>(kt, j, &j0, &cols);
         for (int kv = 0; kv < 2; ++kv, ++it) {
           const int s = it % C::kSlots;
-          if (!mbar_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+          if (!mbar_park(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
             *abort_flag = 1;
             go = false;
             break;
@@ -303,48 +342,51 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             tma_load_4d(ring + s * C::kSlot + a * KT * kAtom, kv ? &maps.v : &maps.k, &full[s], a * 64, j0, hk, b);
         }
       }
-      mbar_wait(q_full, 0, err, kErrTimeoutDrain);
+      mbar_park(q_full, 0, err, kErrTimeoutDrain);
       for (int i = max(0, it - C::kSlots); i < it; ++i)
-        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
+        mbar_park(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
     if (lane == 0 && kt.n > 0) {
       const uint32_t idesc_s = make_idesc(1, 0, 0, 128, 0), idesc_o = make_idesc(1, 0, 1, 128, 16 * kd);
       const uint32_t sq = smem_u32(smem), sr = smem_u32(ring);
-      auto scores = [&](int j) {  // S = Q K^T
+      // S = Q K^T, once the product that read the weights of this buffer is over
+      auto scores = [&](int j) {
         const int it = 2 * j, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
-        if (!mbar_wait(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
-        if (j > 0 && !mbar_wait(s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
+        if (!mbar_park(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (j >= C::kBufs && !mbar_park(pv_done, (j - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
         tc_fence_after();
+        const uint32_t buf = tmem + (j % C::kBufs) * 64;
         for (int k = 0; k < kd; ++k)
-          umma_bf16(tmem, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), idesc_s | ((cols >> 3) << 17),
+          umma_bf16(buf, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), idesc_s | ((cols >> 3) << 17),
                     k ? 1u : 0u);
         tc_commit(&empty[s]);
         tc_commit(s_full);
         return true;
       };
-      bool go = mbar_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
+      bool go = mbar_park(q_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
-        if (j + 1 < kt.n && !scores(j + 1)) {
+        if (C::kBufs == 2 && j + 1 < kt.n && !scores(j + 1)) {
           go = false;
           break;
         }
         const int it = 2 * j + 1, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
-        if (!mbar_wait(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull) ||
-            !mbar_wait(p_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
+        if (!mbar_park(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull) ||
+            !mbar_park(p_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
           go = false;
           break;
         }
         tc_fence_after();
         for (int k = 0; k < cols / 16; ++k)  // O += P V
-          umma_bf16_ts(tmem + C::kO, tmem + C::kP + k * 8, desc_mn(sr + s * C::kSlot, KT, k), idesc_o,
+          umma_bf16_ts(tmem + C::kO, tmem + (j % C::kBufs) * 64 + k * 8, desc_mn(sr + s * C::kSlot, KT, k), idesc_o,
                        (j | k) ? 1u : 0u);
         tc_commit(&empty[s]);
         tc_commit(pv_done);
+        if (C::kBufs == 1 && j + 1 < kt.n && !scores(j + 1)) go = false;
       }
       if (!go) *abort_flag = 1;
     }
@@ -353,46 +395,40 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
     const float c = p.scale * kLog2e;
     const int w0 = i0 + q4 * 32, w1 = w0 + 31;  // this warp's queries
-    float m = -INFINITY, l = 0.f;               // m in the scaled base-2 domain
+    float m = -INFINITY;                        // in the scaled base-2 domain
+    float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;
     for (int j = 0; j < kt.n; ++j) {
       int j0, cols;
       key_tile<KT>(kt, j, &j0, &cols);
+      const uint32_t buf = tmem + lanes + (j % C::kBufs) * 64;
+      const bool whole = j >= kt.n_sink && cols == KT && j0 + cols <= L && j0 > w1 - p.window &&
+                         j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
       if (!(ok = warp_wait(s_full, j & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
       tc_fence_after();
-      float s[KT];
+      const Sight si = whole ? words(~0ull) : sight_of(p, kt, L, i, j, j0);
+      auto half_row = [&](int half, float (&s)[32]) {  // 32 scores, -inf where out of sight
+        load_row32(buf + half * 32, s);
+        tmem_ld_wait();
+        if (!whole) {
 #pragma unroll
-      for (int ch = 0; ch < KT / 32; ++ch)
-        if (ch * 32 < cols) load_row32(tmem + lanes + ch * 32, s + ch * 32);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(s_empty);
-      // columns in sight
-      const bool whole = j >= kt.n_sink && (cols & 31) == 0 && j0 + cols <= L && j0 > w1 - p.window &&
-                         j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
-      float mx = -INFINITY;
-      if (whole) {
+          for (int e = 0; e < 32; ++e) s[e] = (si.w[half] & (1u << e)) ? s[e] : -INFINITY;
+        }
+      };
+      // Twice through the scores, the second time for the weights: TMEM gives them
+      // again for less than the registers that would keep them cost in resident warps.
+      float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-        for (int ch = 0; ch < KT / 32; ++ch)
-          if (ch * 32 < cols) {
+      for (int half = 0; half < 2; ++half)
+        if (half * 32 < cols) {
+          float s[32];
+          half_row(half, s);
 #pragma unroll
-            for (int e = 0; e < 32; ++e) mx = fmaxf(mx, s[ch * 32 + e]);
-          }
-      } else {
-        const Sight si = sight_of(p, kt, L, i, j, j0);
+          for (int e = 0; e < 32; e += 8)
 #pragma unroll
-        for (int ch = 0; ch < KT / 32; ++ch)
-          if (ch * 32 < cols) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const int col = ch * 32 + e;
-              s[col] = in_sight(si, col) ? s[col] : -INFINITY;
-              mx = fmaxf(mx, s[col]);
-            }
-          }
-      }
-      mx *= c;
+            for (int u = 0; u < 4; ++u) t4[u] = fmaxf(fmaxf(t4[u], s[e + u]), s[e + u + 4]);
+        }
+      const float mx = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * c;
       float f = 1.f;
       bool raise = false;
       if (m == -INFINITY) {
@@ -400,42 +436,43 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       } else if (mx > m + 8.f) {
         f = ex2(m - mx);
         m = mx;
-        l *= f;
+        l2 = mul2(l2, make_float2(f, f));
         raise = true;
       }
       const float base = m == -INFINITY ? 0.f : m;
+      const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
       uint32_t pk[KT / 2];
-      float sum = 0.f;
 #pragma unroll
-      for (int ch = 0; ch < KT / 32; ++ch)
-        if (ch * 32 < cols) {
+      for (int half = 0; half < 2; ++half)
+        if (half * 32 < cols) {
+          float s[32];
+          half_row(half, s);
 #pragma unroll
           for (int e = 0; e < 32; e += 2) {
-            const float a0 = ex2(fmaf(s[ch * 32 + e], c, -base)), a1 = ex2(fmaf(s[ch * 32 + e + 1], c, -base));
-            sum += a0 + a1;
-            pk[ch * 16 + e / 2] = pack_f2(a0, a1);
+            float2 w = fma2(make_float2(s[e], s[e + 1]), c2, b2);
+            w.x = ex2(w.x);
+            w.y = ex2(w.y);
+            l2 = add2(l2, w);
+            pk[half * 16 + e / 2] = pack_f2(w.x, w.y);
           }
         }
-      l += sum;
-      // the weights of the tile before have been used
-      if (j > 0) {
+      if (j > 0 && __any_sync(0xffffffffu, raise)) {
         if (!(ok = warp_wait(pv_done, (j - 1) & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
         tc_fence_after();
-        if (__any_sync(0xffffffffu, raise)) {
+#pragma unroll 1
+        for (int ch = 0; ch < DP / 16; ++ch) {
+          uint32_t o[16];
+          tmem_ld_32x32b_x16(tmem + C::kO + lanes + ch * 16, o);
+          tmem_ld_wait();
 #pragma unroll
-          for (int ch = 0; ch < DP / 32; ++ch) {
-            uint32_t o[32];
-            tmem_ld_32x32b_x32(tmem + C::kO + lanes + ch * 32, o);
-            tmem_ld_wait();
-#pragma unroll
-            for (int e = 0; e < 32; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
-            tmem_st_32x32b_x32(tmem + C::kO + lanes + ch * 32, o);
-          }
+          for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * f);
+          tmem_st_32x32b_x16(tmem + C::kO + lanes + ch * 16, o);
         }
       }
-#pragma unroll
-      for (int ch = 0; ch < KT / 32; ++ch)
-        if (ch * 32 < cols) tmem_st_32x32b_x16(tmem + C::kP + lanes + ch * 16, pk + ch * 16);
+      if (cols > 32)
+        tmem_st_32x32b_x32(buf, pk);
+      else
+        tmem_st_32x32b_x16(buf, pk);
       if (j0 + cols > L) {
         const int it = 2 * j + 1, sl = it % C::kSlots;
         if (!(ok = warp_wait(&full[sl], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull))) break;
@@ -451,6 +488,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     if (!ok) {
       *abort_flag = 1;
     } else {
+      const float l = l2.x + l2.y;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       // every product has read the queries: their tile is the staging tile now
       stage_row<DP>(smem, tmem + C::kO + lanes, kt.n > 0, inv, row);
@@ -466,7 +504,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 256);
+    tmem_dealloc(tmem, C::kCols);
   }
 }
 
@@ -543,7 +581,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         key_tile<KT>(kt, j, &j0, &cols);
         for (int kv = 0; kv < 2; ++kv, ++it) {
           const int s = it % C::kSlots;
-          if (!mbar_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+          if (!mbar_park(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
             *abort_flag = 1;
             go = false;
             break;
@@ -554,9 +592,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
             tma_load_4d(ring + s * C::kSlot + a * KT * kAtom, kv ? &maps.v : &maps.k, &full[s], a * 64, j0, hk, b);
         }
       }
-      mbar_wait(q_full, 0, err, kErrTimeoutDrain);
+      mbar_park(q_full, 0, err, kErrTimeoutDrain);
       for (int i = max(0, it - C::kSlots); i < it; ++i)
-        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
+        mbar_park(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
     if (lane == 0 && kt.n > 0) {
@@ -568,12 +606,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         const uint32_t id = idesc_s | ((cols >> 3) << 17);
         const int ik = 2 * j, iv = ik + 1, s = ik % C::kSlots, sv = iv % C::kSlots;
         // S lies over dS at D = 128: then the product that reads dS has to be over, not only the reading of S
-        if (j > 0 && !mbar_wait(C::kAlias ? dq_done : s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
-        if (!mbar_wait(&full[s], (ik / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (j > 0 && !mbar_park(C::kAlias ? dq_done : s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
+        if (!mbar_park(&full[s], (ik / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
         for (int k = 0; k < kd; ++k)
           umma_bf16(tmem, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), id, k ? 1u : 0u);
-        if (!mbar_wait(&full[sv], (iv / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (!mbar_park(&full[sv], (iv / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
         for (int k = 0; k < kd; ++k)
           umma_bf16(tmem + C::kDp, desc_k(sg, 128, k), desc_k(sr + sv * C::kSlot, KT, k), id, k ? 1u : 0u);
@@ -581,7 +619,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         tc_commit(s_full);
         return true;
       };
-      bool go = mbar_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
+      bool go = mbar_park(q_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
         if (!C::kAlias && j + 1 < kt.n && !scores(j + 1)) {
           go = false;
@@ -590,7 +628,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
         const int s = (2 * j) % C::kSlots;
-        if (!mbar_wait(ds_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
+        if (!mbar_park(ds_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
           go = false;
           break;
         }
@@ -628,15 +666,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       }
       p.delta[srow] = delta;
     }
+    const float2 c2 = make_float2(c, c), lse2 = make_float2(-lse, -lse), delta2 = make_float2(-delta, -delta);
     bool ok = true;
     for (int j = 0; j < kt.n; ++j) {
       int j0, cols;
       key_tile<KT>(kt, j, &j0, &cols);
       if (!(ok = warp_wait(s_full, j & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
       tc_fence_after();
-      const bool whole = j >= kt.n_sink && (cols & 31) == 0 && j0 + cols <= L && j0 > w1 - p.window &&
+      const bool whole = j >= kt.n_sink && cols == KT && j0 + cols <= L && j0 > w1 - p.window &&
                          j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
-      const Sight si = sight_of(p, kt, L, i, j, j0);
       uint32_t ds[KT / 2];
 #pragma unroll
       for (int ch = 0; ch < KT / 32; ++ch)
@@ -646,10 +684,18 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           load_row32(tmem + C::kDp + lanes + ch * 32, dp);
           tmem_ld_wait();
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = ex2(fmaf(s[e], c, -lse)) * (dp[e] - delta);
+          for (int e = 0; e < 32; e += 2) {
+            float2 w = fma2(make_float2(s[e], s[e + 1]), c2, lse2);
+            w.x = ex2(w.x);
+            w.y = ex2(w.y);
+            w = mul2(w, add2(make_float2(dp[e], dp[e + 1]), delta2));
+            s[e] = w.x;
+            s[e + 1] = w.y;
+          }
           if (!whole) {
+            const uint32_t si = sight_of(p, kt, L, i, j, j0).w[ch];
 #pragma unroll
-            for (int e = 0; e < 32; ++e) s[e] = in_sight(si, ch * 32 + e) ? s[e] : 0.f;
+            for (int e = 0; e < 32; ++e) s[e] = (si & (1u << e)) ? s[e] : 0.f;
           }
 #pragma unroll
           for (int e = 0; e < 32; e += 2) ds[ch * 16 + e / 2] = pack_f2(s[e], s[e + 1]);
@@ -814,7 +860,7 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
         query_tile(t, &h, &i0, &end);
         for (int qg = 0; qg < 2; ++qg, ++it) {
           const int s = it % C::kSlots;
-          if (!mbar_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+          if (!mbar_park(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
             *abort_flag = 1;
             go = false;
             break;
@@ -825,9 +871,9 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
             tma_load_4d(ring + s * C::kSlot + a * QT * kAtom, qg ? &maps.g : &maps.q, &full[s], a * 64, i0, h, b);
         }
       }
-      mbar_wait(k_full, 0, err, kErrTimeoutDrain);
+      mbar_park(k_full, 0, err, kErrTimeoutDrain);
       for (int i = max(0, it - C::kSlots); i < it; ++i)
-        mbar_wait(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
+        mbar_park(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
     if (lane == 0 && n > 0) {
@@ -835,27 +881,27 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       const uint32_t sk = smem_u32(smem), sv = sk + C::kK, sr = smem_u32(ring);
       // S^T = K Q^T and dP^T = V dO^T, once the products that read P and dS from this buffer are over
       auto scores = [&](int t) {
-        if (t >= C::kBufs && !mbar_wait(d_done, (t - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
+        if (t >= C::kBufs && !mbar_park(d_done, (t - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
         const uint32_t buf = tmem + (t % C::kBufs) * 128;
         const int iq = 2 * t, ig = iq + 1, s = iq % C::kSlots, sg = ig % C::kSlots;
-        if (!mbar_wait(&full[s], (iq / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (!mbar_park(&full[s], (iq / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
         for (int k = 0; k < kd; ++k)
           umma_bf16(buf, desc_k(sk, 128, k), desc_k(sr + s * C::kSlot, QT, k), idesc_s, k ? 1u : 0u);
-        if (!mbar_wait(&full[sg], (ig / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (!mbar_park(&full[sg], (ig / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
         for (int k = 0; k < kd; ++k)
           umma_bf16(buf + 64, desc_k(sv, 128, k), desc_k(sr + sg * C::kSlot, QT, k), idesc_s, k ? 1u : 0u);
         tc_commit(s_full);
         return true;
       };
-      bool go = mbar_wait(k_full, 0, err, kErrTimeoutFull) && scores(0);
+      bool go = mbar_park(k_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int t = 0; t < n && go; ++t) {
         if (C::kBufs == 2 && t + 1 < n && !scores(t + 1)) {
           go = false;
           break;
         }
-        if (!mbar_wait(ds_full, t & 1, err, kErrTimeoutFull) || *abort_flag) {
+        if (!mbar_park(ds_full, t & 1, err, kErrTimeoutFull) || *abort_flag) {
           go = false;
           break;
         }
@@ -887,12 +933,13 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
     const bool idle = extra && w0 >= p.sinks;
     const bool sink = j < p.sinks, valid = j < L;
     const bool part_rows = sp.extra > 0 && tile < sp.tiles;
-    auto load_stat = [&](int t) {  // this thread's value of iteration t's lse (threads 0-63) or delta
+    const float2 c2 = make_float2(c, c);
+    auto load_stat = [&](int t) {  // this thread's value of iteration t's -lse (threads 0-63) or -delta
       int h, i0, end;
       query_tile(t, &h, &i0, &end);
       const int i = i0 + (tid & 63);
       const long long at = (static_cast<long long>(b) * p.H + h) * p.S + i;
-      return tid < 64 ? (i < end ? p.lse[at] : INFINITY) : (i < end ? p.delta[at] : 0.f);
+      return tid < 64 ? (i < end ? -p.lse[at] : -INFINITY) : (i < end ? -p.delta[at] : 0.f);
     };
     float next = n > 0 ? load_stat(0) : 0.f;
     bool ok = true;
@@ -920,6 +967,7 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
         }
         const bool whole = !extra && w1 < L && i0 >= (p.causal ? w1 : w1 - (p.window - 1)) &&
                            i0 + QT <= w0 + p.window;
+        const Sight seen = words(bits_below(qb) & ~bits_below(qa));
         uint32_t pk[QT / 2], dk[QT / 2];
 #pragma unroll
         for (int ch = 0; ch < QT / 32; ++ch) {
@@ -931,17 +979,22 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
           for (int e = 0; e < 32; e += 4) {
             const float4 ls = *reinterpret_cast<const float4*>(st + ch * 32 + e);
             const float4 de = *reinterpret_cast<const float4*>(st + QT + ch * 32 + e);
-            const float lv[4] = {ls.x, ls.y, ls.z, ls.w}, dv[4] = {de.x, de.y, de.z, de.w};
+            const float2 lv[2] = {make_float2(ls.x, ls.y), make_float2(ls.z, ls.w)};
+            const float2 dv[2] = {make_float2(de.x, de.y), make_float2(de.z, de.w)};
 #pragma unroll
-            for (int u = 0; u < 4; ++u) {
-              s[e + u] = ex2(fmaf(s[e + u], c, -lv[u]));
-              dp[e + u] = s[e + u] * (dp[e + u] - dv[u]);
+            for (int u = 0; u < 2; ++u) {
+              float2 w = fma2(make_float2(s[e + 2 * u], s[e + 2 * u + 1]), c2, lv[u]);
+              w.x = ex2(w.x);
+              w.y = ex2(w.y);
+              const float2 g = mul2(w, add2(make_float2(dp[e + 2 * u], dp[e + 2 * u + 1]), dv[u]));
+              s[e + 2 * u] = w.x, s[e + 2 * u + 1] = w.y;
+              dp[e + 2 * u] = g.x, dp[e + 2 * u + 1] = g.y;
             }
           }
           if (!whole) {
 #pragma unroll
             for (int e = 0; e < 32; ++e) {
-              const bool on = ch * 32 + e >= qa && ch * 32 + e < qb;
+              const bool on = seen.w[ch] & (1u << e);
               s[e] = on ? s[e] : 0.f;
               dp[e] = on ? dp[e] : 0.f;
             }
