@@ -357,38 +357,44 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           mbar_park(&full_bar[i % kPairStages], (i / kPairStages) & 1, p.err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0 && rank == 0) {
-      int it = 0, n = 0;
-      for (int t = first; t < n_tiles && !*abort_flag; t += step) {
+    if (rank == 0) {
+      // The whole warp keeps step, one lane issues: addresses stay in uniform registers.
+      const bool issuer = elect_lane();
+      const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t a0 = desc_lo(smem_u32(smem), A_MN ? kOperand / 2 : 16);
+      const uint32_t b0 = desc_lo(smem_u32(smem) + kOperand, B_MN ? kOperand / 2 : 16);
+      int s = 0, n = 0;
+      uint32_t phase = 0;
+      bool go = true;
+      for (int t = first; t < n_tiles && go; t += step) {
         const PairTile c = pair_tile<MODE>(p, t);
         if (c.nkb == 0) continue;
         const int acc = n & 1;
-        if (!mbar_park(&acc_empty[acc], ((n >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty)) {
-          *abort_flag = 1;
-          break;
-        }
+        go = mbar_park(&acc_empty[acc], ((n >> 1) & 1) ^ 1, p.err, kErrTimeoutEmpty);
         tc_fence_after();
-        for (int i = 0; i < c.nkb; ++i, ++it) {
-          const int s = it % kPairStages;
-          if (!mbar_park(&full_bar[s], (it / kPairStages) & 1, p.err, kErrTimeoutFull)) {
-            *abort_flag = 1;
-            break;
-          }
+        for (int i = 0; i < c.nkb && go; ++i) {
+          go = mbar_park(&full_bar[s], phase, p.err, kErrTimeoutFull);
           tc_fence_after();
-          const uint32_t sa = smem_u32(smem + s * kPairStage), sb = sa + kOperand;
+          if (go && issuer) {
+            const uint32_t ad = a0 + s * (kPairStage >> 4), bd = b0 + s * (kPairStage >> 4);
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            const uint64_t ad = A_MN ? make_sw128_desc(sa + k * 2048, kOperand / 2, 1024)
-                                     : make_sw128_desc(sa + k * 32, 16, 1024);
-            const uint64_t bd = B_MN ? make_sw128_desc(sb + k * 2048, kOperand / 2, 1024)
-                                     : make_sw128_desc(sb + k * 32, 16, 1024);
-            pair_umma_bf16(tmem + acc * 256, ad, bd, kIdesc, (i | k) ? 1u : 0u);
+            for (int k = 0; k < 4; ++k)
+              pair_umma_ss(d0 + acc * 256, ad + (A_MN ? step_mn(k) : step_k(128, k)),
+                           bd + (B_MN ? step_mn(k) : step_k(128, k)), kIdesc, (i | k) ? 1u : 0u);
+            pair_commit(&empty_bar[s]);
           }
-          pair_commit(&empty_bar[s]);
+          __syncwarp();
+          if (++s == kPairStages) {
+            s = 0;
+            phase ^= 1;
+          }
         }
-        pair_commit(&acc_full[acc]);  // also after a timeout: the epilogue does not wait for nothing
+        go = __all_sync(0xffffffffu, go && !*abort_flag);
+        if (issuer) pair_commit(&acc_full[acc]);  // also after a timeout: the epilogue does not wait for nothing
+        __syncwarp();
         ++n;
       }
+      if (!go) *abort_flag = 1;
     }
   } else {
     const int q = warp & 3, half = (warp - 2) >> 2;

@@ -81,14 +81,53 @@ __device__ __forceinline__ void pair_commit(uint64_t* bar) {
       : "memory");
 }
 
-__device__ __forceinline__ void pair_umma_bf16(uint32_t tmem_d, uint64_t adesc, uint64_t bdesc, uint32_t idesc,
-                                               uint32_t accumulate) {
+// Matrix descriptors (128-byte swizzle, rows of 128 bytes in groups of eight,
+// 1024 bytes apart) as their two words.  The upper one is a constant and the
+// lower one moves by an addition from step to step: the issuing warp has a few
+// dozen cycles for an instruction, less than it takes to build a descriptor anew.
+constexpr uint32_t kDescHi = (1024u >> 4) | (1u << 14) | (2u << 29);
+
+// lead: bytes between 64-value chunks of an MN-major operand (K-major: ignored).
+__device__ __forceinline__ uint32_t desc_lo(uint32_t smem_addr, uint32_t lead = 16) {
+  return ((smem_addr >> 4) & 0x3FFFu) | ((lead >> 4) << 16);
+}
+// Steps of 16 along the reduction: within a K-major row (four to a 64-value
+// chunk, `rows` rows each), or 16 rows down an MN-major tile.
+__device__ __forceinline__ constexpr uint32_t step_k(int rows, int k) { return (k >> 2) * rows * 8 + (k & 3) * 2; }
+__device__ __forceinline__ constexpr uint32_t step_mn(int k) { return k * 128; }
+
+#define TGCM_UMMA(NAME, GROUP)                                                                                     \
+  __device__ __forceinline__ void NAME(uint32_t tmem_d, uint32_t a_lo, uint32_t b_lo, uint32_t idesc,              \
+                                       uint32_t accumulate) {                                                      \
+    asm volatile(                                                                                                  \
+        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\t"                                                              \
+        "mov.b64 da, {%1, %5};\n\tmov.b64 db, {%2, %5};\n\t"                                                       \
+        "setp.ne.b32 p, %4, 0;\n\t"                                                                                \
+        "tcgen05.mma.cta_group::" #GROUP ".kind::f16 [%0], da, db, %3, p;\n\t}" ::"r"(tmem_d),                     \
+        "r"(a_lo), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi)                                            \
+        : "memory");                                                                                               \
+  }
+TGCM_UMMA(umma_ss, 1)        // one CTA
+TGCM_UMMA(pair_umma_ss, 2)   // both CTAs of a pair
+#undef TGCM_UMMA
+
+// A from TMEM (one CTA).
+__device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32_t b_lo, uint32_t idesc,
+                                        uint32_t accumulate) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\t"
+      "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\t"
+      "mov.b64 db, {%2, %5};\n\t"
       "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "l"(adesc), "l"(bdesc), "r"(idesc), "r"(accumulate)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %3, p;\n\t}" ::"r"(tmem_d),
+      "r"(tmem_a), "r"(b_lo), "r"(idesc), "r"(accumulate), "r"(kDescHi)
       : "memory");
+}
+
+// One lane of a converged warp, the same one every time.
+__device__ __forceinline__ bool elect_lane() {
+  uint32_t is;
+  asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(is));
+  return is != 0;
 }
 
 // 32 lanes x 32 columns of 32 bits, one row to a thread.

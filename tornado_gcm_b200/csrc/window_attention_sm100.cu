@@ -68,17 +68,6 @@ __device__ __forceinline__ void tma_load_4d(void* dst, const CUtensorMap* map, u
       : "memory");
 }
 
-// D(tmem) (+)= A(tmem) * B(smem desc), bf16.
-__device__ __forceinline__ void umma_bf16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t bdesc, uint32_t idesc,
-                                             uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\t"
-      "setp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-      "r"(tmem_a), "l"(bdesc), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-
 __device__ __forceinline__ void tmem_st_32x32b_x32(uint32_t taddr, const uint32_t* r) {
   asm volatile(
       "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
@@ -148,15 +137,6 @@ __device__ __forceinline__ void load_row32(uint32_t taddr, float* s) {
   tmem_ld_32x32b_x32(taddr, r);
 #pragma unroll
   for (int i = 0; i < 32; ++i) s[i] = __uint_as_float(r[i]);
-}
-
-// K-major operand (rows x 64-value atoms) and the same tile read the other way
-// round (MN-major: the rows are the reduction).  `rows`: of the whole tile.
-__device__ __forceinline__ uint64_t desc_k(uint32_t tile, int rows, int k16) {
-  return make_sw128_desc(tile + (k16 >> 2) * rows * kAtom + (k16 & 3) * 32, 16, 1024);
-}
-__device__ __forceinline__ uint64_t desc_mn(uint32_t tile, int rows, int k16) {
-  return make_sw128_desc(tile + k16 * 16 * kAtom, rows * kAtom, 1024);
 }
 
 // Bounded wait of a whole warp: false in all lanes when one gave up.
@@ -347,46 +327,52 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
         mbar_park(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0 && kt.n > 0) {
+    if (kt.n > 0) {
+      // The whole warp keeps step, one lane issues: addresses stay in uniform registers.
+      const bool issuer = elect_lane();
       const uint32_t idesc_s = make_idesc(1, 0, 0, 128, 0), idesc_o = make_idesc(1, 0, 1, 128, 16 * kd);
-      const uint32_t sq = smem_u32(smem), sr = smem_u32(ring);
+      const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q0 = desc_lo(smem_u32(smem)), k0 = desc_lo(smem_u32(ring)), v0 = desc_lo(smem_u32(ring), KT * kAtom);
       // S = Q K^T, once the product that read the weights of this buffer is over
       auto scores = [&](int j) {
         const int it = 2 * j, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
-        if (!mbar_park(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
-        if (j >= C::kBufs && !mbar_park(pv_done, (j - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
+        if (!warp_wait(&full[s], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
+        if (j >= C::kBufs && !warp_wait(pv_done, (j - C::kBufs) & 1, abort_flag, err, kErrTimeoutEmpty)) return false;
         tc_fence_after();
-        const uint32_t buf = tmem + (j % C::kBufs) * 64;
-        for (int k = 0; k < kd; ++k)
-          umma_bf16(buf, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), idesc_s | ((cols >> 3) << 17),
-                    k ? 1u : 0u);
-        tc_commit(&empty[s]);
-        tc_commit(s_full);
+        if (issuer) {
+          const uint32_t buf = d0 + (j % C::kBufs) * 64, id = idesc_s | ((cols >> 3) << 17);
+          const uint32_t ks = k0 + s * (C::kSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < kd) umma_ss(buf, q0 + step_k(128, k), ks + step_k(KT, k), id, k ? 1u : 0u);
+          tc_commit(&empty[s]);
+          tc_commit(s_full);
+        }
+        __syncwarp();
         return true;
       };
-      bool go = mbar_park(q_full, 0, err, kErrTimeoutFull) && scores(0);
+      bool go = warp_wait(q_full, 0, abort_flag, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
-        if (C::kBufs == 2 && j + 1 < kt.n && !scores(j + 1)) {
-          go = false;
-          break;
-        }
+        if (C::kBufs == 2 && j + 1 < kt.n && !(go = scores(j + 1))) break;
         const int it = 2 * j + 1, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
-        if (!mbar_park(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull) ||
-            !mbar_park(p_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
-          go = false;
-          break;
-        }
+        go = warp_wait(&full[s], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull) &&
+             warp_wait(p_full, j & 1, abort_flag, err, kErrTimeoutFull);
+        if (!go) break;
         tc_fence_after();
-        for (int k = 0; k < cols / 16; ++k)  // O += P V
-          umma_bf16_ts(tmem + C::kO, tmem + (j % C::kBufs) * 64 + k * 8, desc_mn(sr + s * C::kSlot, KT, k), idesc_o,
-                       (j | k) ? 1u : 0u);
-        tc_commit(&empty[s]);
-        tc_commit(pv_done);
-        if (C::kBufs == 1 && j + 1 < kt.n && !scores(j + 1)) go = false;
+        if (issuer) {
+          const uint32_t vs = v0 + s * (C::kSlot >> 4), pa = d0 + (j % C::kBufs) * 64;
+#pragma unroll
+          for (int k = 0; k < KT / 16; ++k)  // O += P V
+            if (k * 16 < cols) umma_ts(d0 + C::kO, pa + k * 8, vs + step_mn(k), idesc_o, (j | k) ? 1u : 0u);
+          tc_commit(&empty[s]);
+          tc_commit(pv_done);
+        }
+        __syncwarp();
+        if (C::kBufs == 1 && j + 1 < kt.n) go = scores(j + 1);
       }
       if (!go) *abort_flag = 1;
     }
@@ -597,48 +583,55 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         mbar_park(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0 && kt.n > 0) {
+    if (kt.n > 0) {
+      const bool issuer = elect_lane();
       const uint32_t idesc_s = make_idesc(1, 0, 0, 128, 0), idesc_q = make_idesc(1, 0, 1, 128, 16 * kd);
-      const uint32_t sq = smem_u32(smem), sg = sq + C::kQ, sr = smem_u32(ring);
+      const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t q0 = desc_lo(smem_u32(smem)), g0 = desc_lo(smem_u32(smem) + C::kQ);
+      const uint32_t k0 = desc_lo(smem_u32(ring)), t0 = desc_lo(smem_u32(ring), KT * kAtom);
       auto scores = [&](int j) {  // S = Q K^T, dP = dO V^T
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
         const uint32_t id = idesc_s | ((cols >> 3) << 17);
         const int ik = 2 * j, iv = ik + 1, s = ik % C::kSlots, sv = iv % C::kSlots;
         // S lies over dS at D = 128: then the product that reads dS has to be over, not only the reading of S
-        if (j > 0 && !mbar_park(C::kAlias ? dq_done : s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
-        if (!mbar_park(&full[s], (ik / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (j > 0 &&
+            !warp_wait(C::kAlias ? dq_done : s_empty, (j - 1) & 1, abort_flag, err, kErrTimeoutEmpty)) return false;
+        if (!warp_wait(&full[s], (ik / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
+        if (!warp_wait(&full[sv], (iv / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
         tc_fence_after();
-        for (int k = 0; k < kd; ++k)
-          umma_bf16(tmem, desc_k(sq, 128, k), desc_k(sr + s * C::kSlot, KT, k), id, k ? 1u : 0u);
-        if (!mbar_park(&full[sv], (iv / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
-        tc_fence_after();
-        for (int k = 0; k < kd; ++k)
-          umma_bf16(tmem + C::kDp, desc_k(sg, 128, k), desc_k(sr + sv * C::kSlot, KT, k), id, k ? 1u : 0u);
-        tc_commit(&empty[sv]);
-        tc_commit(s_full);
+        if (issuer) {
+          const uint32_t ks = k0 + s * (C::kSlot >> 4), vs = k0 + sv * (C::kSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < kd) umma_ss(d0, q0 + step_k(128, k), ks + step_k(KT, k), id, k ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < kd) umma_ss(d0 + C::kDp, g0 + step_k(128, k), vs + step_k(KT, k), id, k ? 1u : 0u);
+          tc_commit(&empty[sv]);
+          tc_commit(s_full);
+        }
+        __syncwarp();
         return true;
       };
-      bool go = mbar_park(q_full, 0, err, kErrTimeoutFull) && scores(0);
+      bool go = warp_wait(q_full, 0, abort_flag, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
-        if (!C::kAlias && j + 1 < kt.n && !scores(j + 1)) {
-          go = false;
-          break;
-        }
+        if (!C::kAlias && j + 1 < kt.n && !(go = scores(j + 1))) break;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
         const int s = (2 * j) % C::kSlots;
-        if (!mbar_park(ds_full, j & 1, err, kErrTimeoutFull) || *abort_flag) {
-          go = false;
-          break;
-        }
+        if (!(go = warp_wait(ds_full, j & 1, abort_flag, err, kErrTimeoutFull))) break;
         tc_fence_after();
-        for (int k = 0; k < cols / 16; ++k)  // dQ += dS K
-          umma_bf16_ts(tmem + C::kDq, tmem + C::kDs + k * 8, desc_mn(sr + s * C::kSlot, KT, k), idesc_q,
-                       (j | k) ? 1u : 0u);
-        tc_commit(&empty[s]);
-        tc_commit(dq_done);
-        if (C::kAlias && j + 1 < kt.n && !scores(j + 1)) go = false;
+        if (issuer) {
+          const uint32_t ks = t0 + s * (C::kSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < KT / 16; ++k)  // dQ += dS K
+            if (k * 16 < cols) umma_ts(d0 + C::kDq, d0 + C::kDs + k * 8, ks + step_mn(k), idesc_q, (j | k) ? 1u : 0u);
+          tc_commit(&empty[s]);
+          tc_commit(dq_done);
+        }
+        __syncwarp();
+        if (C::kAlias && j + 1 < kt.n) go = scores(j + 1);
       }
       if (!go) *abort_flag = 1;
     }
@@ -876,50 +869,55 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
         mbar_park(&full[i % C::kSlots], (i / C::kSlots) & 1, err, kErrTimeoutDrain);
     }
   } else if (warp == 1) {
-    if (lane == 0 && n > 0) {
+    if (n > 0) {
+      const bool issuer = elect_lane();
       const uint32_t idesc_s = make_idesc(1, 0, 0, 128, QT), idesc_d = make_idesc(1, 0, 1, 128, 16 * kd);
-      const uint32_t sk = smem_u32(smem), sv = sk + C::kK, sr = smem_u32(ring);
+      const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
+      const uint32_t k0 = desc_lo(smem_u32(smem)), v0 = desc_lo(smem_u32(smem) + C::kK);
+      const uint32_t q0 = desc_lo(smem_u32(ring)), t0 = desc_lo(smem_u32(ring), QT * kAtom);
       // S^T = K Q^T and dP^T = V dO^T, once the products that read P and dS from this buffer are over
       auto scores = [&](int t) {
-        if (t >= C::kBufs && !mbar_park(d_done, (t - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
-        const uint32_t buf = tmem + (t % C::kBufs) * 128;
         const int iq = 2 * t, ig = iq + 1, s = iq % C::kSlots, sg = ig % C::kSlots;
-        if (!mbar_park(&full[s], (iq / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (t >= C::kBufs && !warp_wait(d_done, (t - C::kBufs) & 1, abort_flag, err, kErrTimeoutEmpty)) return false;
+        if (!warp_wait(&full[s], (iq / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
+        if (!warp_wait(&full[sg], (ig / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
         tc_fence_after();
-        for (int k = 0; k < kd; ++k)
-          umma_bf16(buf, desc_k(sk, 128, k), desc_k(sr + s * C::kSlot, QT, k), idesc_s, k ? 1u : 0u);
-        if (!mbar_park(&full[sg], (ig / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
-        tc_fence_after();
-        for (int k = 0; k < kd; ++k)
-          umma_bf16(buf + 64, desc_k(sv, 128, k), desc_k(sr + sg * C::kSlot, QT, k), idesc_s, k ? 1u : 0u);
-        tc_commit(s_full);
+        if (issuer) {
+          const uint32_t buf = d0 + (t % C::kBufs) * 128;
+          const uint32_t qs = q0 + s * (C::kSlot >> 4), gs = q0 + sg * (C::kSlot >> 4);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < kd) umma_ss(buf, k0 + step_k(128, k), qs + step_k(QT, k), idesc_s, k ? 1u : 0u);
+#pragma unroll
+          for (int k = 0; k < DP / 16; ++k)
+            if (k < kd) umma_ss(buf + 64, v0 + step_k(128, k), gs + step_k(QT, k), idesc_s, k ? 1u : 0u);
+          tc_commit(s_full);
+        }
+        __syncwarp();
         return true;
       };
-      bool go = mbar_park(k_full, 0, err, kErrTimeoutFull) && scores(0);
+      bool go = warp_wait(k_full, 0, abort_flag, err, kErrTimeoutFull) && scores(0);
       for (int t = 0; t < n && go; ++t) {
-        if (C::kBufs == 2 && t + 1 < n && !scores(t + 1)) {
-          go = false;
-          break;
-        }
-        if (!mbar_park(ds_full, t & 1, err, kErrTimeoutFull) || *abort_flag) {
-          go = false;
-          break;
-        }
+        if (C::kBufs == 2 && t + 1 < n && !(go = scores(t + 1))) break;
+        if (!(go = warp_wait(ds_full, t & 1, abort_flag, err, kErrTimeoutFull))) break;
         tc_fence_after();
-        const uint32_t buf = tmem + (t % C::kBufs) * 128;
         const int s = (2 * t) % C::kSlots, sg = (2 * t + 1) % C::kSlots;
+        if (issuer) {
+          const uint32_t buf = d0 + (t % C::kBufs) * 128;
+          const uint32_t qs = t0 + s * (C::kSlot >> 4), gs = t0 + sg * (C::kSlot >> 4);
 #pragma unroll
-        for (int k = 0; k < QT / 16; ++k)  // dV += P^T dO
-          umma_bf16_ts(tmem + C::kDv, buf + k * 8, desc_mn(sr + sg * C::kSlot, QT, k), idesc_d, (t | k) ? 1u : 0u);
-        tc_commit(&empty[sg]);
+          for (int k = 0; k < QT / 16; ++k)  // dV += P^T dO
+            umma_ts(d0 + C::kDv, buf + k * 8, gs + step_mn(k), idesc_d, (t | k) ? 1u : 0u);
+          tc_commit(&empty[sg]);
 #pragma unroll
-        for (int k = 0; k < QT / 16; ++k)  // dK += dS^T Q
-          umma_bf16_ts(tmem + C::kDk, buf + 64 + k * 8, desc_mn(sr + s * C::kSlot, QT, k), idesc_d,
-                       (t | k) ? 1u : 0u);
-        tc_commit(&empty[s]);
-        tc_commit(d_done);
-        if (t + 1 == n) tc_commit(all_done);
-        if (C::kBufs == 1 && t + 1 < n && !scores(t + 1)) go = false;
+          for (int k = 0; k < QT / 16; ++k)  // dK += dS^T Q
+            umma_ts(d0 + C::kDk, buf + 64 + k * 8, qs + step_mn(k), idesc_d, (t | k) ? 1u : 0u);
+          tc_commit(&empty[s]);
+          tc_commit(d_done);
+          if (t + 1 == n) tc_commit(all_done);
+        }
+        __syncwarp();
+        if (C::kBufs == 1 && t + 1 < n) go = scores(t + 1);
       }
       if (!go) *abort_flag = 1;
     }
