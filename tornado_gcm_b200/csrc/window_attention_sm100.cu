@@ -47,10 +47,6 @@
 namespace tgcm {
 namespace {
 
-#ifndef TGCM_FB
-#define TGCM_FB 1
-#define TGCM_FP 3
-#endif
 constexpr int kAttnThreads = 192;
 constexpr int kAtom = 128;  // bytes of a swizzled row: 64 bf16
 
@@ -127,6 +123,25 @@ __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
   return d;
 }
 
+// 2^t of two values on the FMA pipe: t = n + f with |f| <= 1/2 (n by adding and
+// taking away 1.5 * 2^23), a cubic for 2^f (least largest relative error on the
+// interval, 7.5e-5: a twentieth of a bf16 weight's rounding), n into the
+// exponent.  t below -126 gives 2^-126.
+__device__ __forceinline__ float2 ex2_poly2(float2 t) {
+  t.x = fmaxf(t.x, -126.f);
+  t.y = fmaxf(t.y, -126.f);
+  const float2 shift = make_float2(12582912.f, 12582912.f), back = make_float2(-12582912.f, -12582912.f);
+  const float2 z = add2(t, shift);
+  const float2 n = add2(z, back);
+  const float2 f = fma2(n, make_float2(-1.f, -1.f), t);
+  float2 v = fma2(f, make_float2(0.05517166853f, 0.05517166853f), make_float2(0.24261112511f, 0.24261112511f));
+  v = fma2(v, f, make_float2(0.69326096773f, 0.69326096773f));
+  v = fma2(v, f, make_float2(0.99992805719f, 0.99992805719f));
+  v.x = __int_as_float(__float_as_int(v.x) + (__float_as_int(z.x) << 23));
+  v.y = __int_as_float(__float_as_int(v.y) + (__float_as_int(z.y) << 23));
+  return v;
+}
+
 __device__ __forceinline__ uint32_t pack_f2(float a, float b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
   return *reinterpret_cast<const uint32_t*>(&h);
@@ -140,9 +155,8 @@ __device__ __forceinline__ void load_row32(uint32_t taddr, float* s) {
 }
 
 // Bounded wait of a whole warp: false in all lanes when one gave up.
-__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, volatile int* abort_flag, int* err, int code) {
-  const bool ok = mbar_park(bar, parity, err, code);
-  return !__any_sync(0xffffffffu, !ok || *abort_flag);
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t parity, int* err, int code) {
+  return __all_sync(0xffffffffu, mbar_park(bar, parity, err, code));
 }
 
 // One row of D <= 64 * A values in bf16 from this thread to the staging tile
@@ -245,18 +259,16 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int rows, int first, i
 template <int DP>
 struct FwdCfg {
   static constexpr int KT = 64;
-  static constexpr int kBufs = DP == 64 ? TGCM_FB : 2;  // score tiles in flight
-  static constexpr int kPerSm = DP == 64 ? TGCM_FP : 2;
+  static constexpr int kBufs = 2;   // score tiles in flight
   static constexpr int kSlots = 4;
   static constexpr int kSlot = KT * DP * 2;
   static constexpr int kQ = 128 * DP * 2;
   static constexpr int kSmem = kQ + kSlots * kSlot + 256 + 1024;
   static constexpr uint32_t kO = kBufs * 64;                // TMEM columns: the scores first, P over them
-  static constexpr uint32_t kCols = kO + DP <= 128 ? 128 : 256;
 };
 
 template <int DP>
-__global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
+__global__ void __launch_bounds__(kAttnThreads, 2)
     win_fwd_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, int* err) {
   using C = FwdCfg<DP>;
   constexpr int KT = C::KT;
@@ -266,10 +278,13 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kSlot);
   uint64_t* empty = full + C::kSlots;
   uint64_t* q_full = empty + C::kSlots;
+  // Of each buffer its own: with one barrier for both, the scores (or weights) of
+  // tile j + 1 could complete a second phase before anyone had looked at tile j's.
   uint64_t* s_full = q_full + 1;
-  uint64_t* p_full = s_full + 1;
-  uint64_t* pv_done = p_full + 1;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(pv_done + 1);
+  uint64_t* p_full = s_full + C::kBufs;
+  uint64_t* pv_done = p_full + C::kBufs;  // of a tile
+  uint64_t* all_done = pv_done + 1;  // of the last one
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -284,14 +299,17 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
       mbar_init(&empty[s], 1);
     }
     mbar_init(q_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(p_full, 4);
+    for (int i = 0; i < C::kBufs; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&p_full[i], 4);
+    }
     mbar_init(pv_done, 1);
+    mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
   if (warp == 1) {
-    tmem_alloc(tmem_slot, C::kCols);
+    tmem_alloc(tmem_slot, 256);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -338,8 +356,8 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
         const int it = 2 * j, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
-        if (!warp_wait(&full[s], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
-        if (j >= C::kBufs && !warp_wait(pv_done, (j - C::kBufs) & 1, abort_flag, err, kErrTimeoutEmpty)) return false;
+        if (!warp_wait(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (j >= C::kBufs && !warp_wait(pv_done, (j - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
         tc_fence_after();
         if (issuer) {
           const uint32_t buf = d0 + (j % C::kBufs) * 64, id = idesc_s | ((cols >> 3) << 17);
@@ -348,19 +366,19 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
           for (int k = 0; k < DP / 16; ++k)
             if (k < kd) umma_ss(buf, q0 + step_k(128, k), ks + step_k(KT, k), id, k ? 1u : 0u);
           tc_commit(&empty[s]);
-          tc_commit(s_full);
+          tc_commit(&s_full[j % C::kBufs]);
         }
         __syncwarp();
         return true;
       };
-      bool go = warp_wait(q_full, 0, abort_flag, err, kErrTimeoutFull) && scores(0);
+      bool go = warp_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
         if (C::kBufs == 2 && j + 1 < kt.n && !(go = scores(j + 1))) break;
         const int it = 2 * j + 1, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
-        go = warp_wait(&full[s], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull) &&
-             warp_wait(p_full, j & 1, abort_flag, err, kErrTimeoutFull);
+        go = warp_wait(&full[s], (it / C::kSlots) & 1, err, kErrTimeoutFull) &&
+             warp_wait(&p_full[j % C::kBufs], (j / C::kBufs) & 1, err, kErrTimeoutFull);
         if (!go) break;
         tc_fence_after();
         if (issuer) {
@@ -370,6 +388,7 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
             if (k * 16 < cols) umma_ts(d0 + C::kO, pa + k * 8, vs + step_mn(k), idesc_o, (j | k) ? 1u : 0u);
           tc_commit(&empty[s]);
           tc_commit(pv_done);
+          if (j + 1 == kt.n) tc_commit(all_done);
         }
         __syncwarp();
         if (C::kBufs == 1 && j + 1 < kt.n) go = scores(j + 1);
@@ -384,36 +403,31 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
     float m = -INFINITY;                        // in the scaled base-2 domain
     float2 l2 = make_float2(0.f, 0.f);
     bool ok = true;
+    // tiles that all of this warp's queries see whole
+    const int from = kt.n_sink + max(0, w1 - p.window + 1 - kt.lo + KT - 1) / KT;
+    const int room = min(L, p.causal ? w0 + 1 : w0 + p.window) - kt.lo;
+    const int to = room < KT ? 0 : kt.n_sink + room / KT;
     for (int j = 0; j < kt.n; ++j) {
       int j0, cols;
       key_tile<KT>(kt, j, &j0, &cols);
       const uint32_t buf = tmem + lanes + (j % C::kBufs) * 64;
-      const bool whole = j >= kt.n_sink && cols == KT && j0 + cols <= L && j0 > w1 - p.window &&
-                         j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
-      if (!(ok = warp_wait(s_full, j & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+      const bool whole = j >= from && j < to;
+      if (!(ok = warp_wait(&s_full[j % C::kBufs], (j / C::kBufs) & 1, err, kErrTimeoutTmemFull))) break;
       tc_fence_after();
-      const Sight si = whole ? words(~0ull) : sight_of(p, kt, L, i, j, j0);
-      auto half_row = [&](int half, float (&s)[32]) {  // 32 scores, -inf where out of sight
-        load_row32(buf + half * 32, s);
-        tmem_ld_wait();
-        if (!whole) {
+      float s[KT];
+      load_row32(buf, s);
+      load_row32(buf + 32, s + 32);  // a narrow tile's columns behind its end are out of sight
+      tmem_ld_wait();
+      if (!whole) {
+        const Sight si = sight_of(p, kt, L, i, j, j0);
 #pragma unroll
-          for (int e = 0; e < 32; ++e) s[e] = (si.w[half] & (1u << e)) ? s[e] : -INFINITY;
-        }
-      };
-      // Twice through the scores, the second time for the weights: TMEM gives them
-      // again for less than the registers that would keep them cost in resident warps.
+        for (int e = 0; e < KT; ++e) s[e] = (si.w[e >> 5] & (1u << (e & 31))) ? s[e] : -INFINITY;
+      }
       float t4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        if (half * 32 < cols) {
-          float s[32];
-          half_row(half, s);
+      for (int e = 0; e < KT; e += 8)
 #pragma unroll
-          for (int e = 0; e < 32; e += 8)
-#pragma unroll
-            for (int u = 0; u < 4; ++u) t4[u] = fmaxf(fmaxf(t4[u], s[e + u]), s[e + u + 4]);
-        }
+        for (int u = 0; u < 4; ++u) t4[u] = fmaxf(fmaxf(t4[u], s[e + u]), s[e + u + 4]);
       const float mx = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * c;
       float f = 1.f;
       bool raise = false;
@@ -428,22 +442,38 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
       const float base = m == -INFINITY ? 0.f : m;
       const float2 c2 = make_float2(c, c), b2 = make_float2(-base, -base);
       uint32_t pk[KT / 2];
+      if (whole) {
+        // Three of eight pairs of exponentials on the FMA pipe: the special-function
+        // unit's 4 a cycle and scheduler are what the others wait for.
 #pragma unroll
-      for (int half = 0; half < 2; ++half)
-        if (half * 32 < cols) {
-          float s[32];
-          half_row(half, s);
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float2 w = fma2(make_float2(s[e], s[e + 1]), c2, b2);
+        for (int e = 0; e < KT; e += 2) {
+          float2 w = fma2(make_float2(s[e], s[e + 1]), c2, b2);
+          if ((e / 2) % 8 == 1 || (e / 2) % 8 == 4 || (e / 2) % 8 == 6) {
+            w = ex2_poly2(w);
+          } else {
             w.x = ex2(w.x);
             w.y = ex2(w.y);
-            l2 = add2(l2, w);
-            pk[half * 16 + e / 2] = pack_f2(w.x, w.y);
           }
+          l2 = add2(l2, w);
+          pk[e / 2] = pack_f2(w.x, w.y);
         }
+      } else {
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          if (half * 32 < cols) {
+#pragma unroll
+            for (int e = half * 32; e < half * 32 + 32; e += 2) {
+              float2 w = fma2(make_float2(s[e], s[e + 1]), c2, b2);
+              w.x = ex2(w.x);
+              w.y = ex2(w.y);
+              l2 = add2(l2, w);
+              pk[e / 2] = pack_f2(w.x, w.y);
+            }
+          }
+      }
       if (j > 0 && __any_sync(0xffffffffu, raise)) {
-        if (!(ok = warp_wait(pv_done, (j - 1) & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+        // S_j was made after the product of tile j - 2: only that of j - 1 can be under way
+        if (!(ok = warp_wait(pv_done, (j - 1) & 1, err, kErrTimeoutTmemFull))) break;
         tc_fence_after();
 #pragma unroll 1
         for (int ch = 0; ch < DP / 16; ++ch) {
@@ -461,15 +491,16 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
         tmem_st_32x32b_x16(buf, pk);
       if (j0 + cols > L) {
         const int it = 2 * j + 1, sl = it % C::kSlots;
-        if (!(ok = warp_wait(&full[sl], (it / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull))) break;
+        if (!(ok = warp_wait(&full[sl], (it / C::kSlots) & 1, err, kErrTimeoutFull))) break;
         clear_rows<DP>(ring + sl * C::kSlot, KT, max(0, L - j0), cols, threadIdx.x - 64);
       }
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(p_full);
+      if (lane == 0) mbar_arrive(&p_full[j % C::kBufs]);
     }
-    if (ok && kt.n > 0) ok = warp_wait(pv_done, (kt.n - 1) & 1, abort_flag, err, kErrTimeoutTmemFull);
+    // not on pv_done: the tile before the last may still be under way, and its phase looks like the last one's
+    if (ok && kt.n > 0) ok = warp_wait(all_done, 0, err, kErrTimeoutTmemFull);
     tc_fence_after();
     if (!ok) {
       *abort_flag = 1;
@@ -490,7 +521,7 @@ __global__ void __launch_bounds__(kAttnThreads, FwdCfg<DP>::kPerSm)
   __syncthreads();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, C::kCols);
+    tmem_dealloc(tmem, 256);
   }
 }
 
@@ -596,9 +627,9 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         const int ik = 2 * j, iv = ik + 1, s = ik % C::kSlots, sv = iv % C::kSlots;
         // S lies over dS at D = 128: then the product that reads dS has to be over, not only the reading of S
         if (j > 0 &&
-            !warp_wait(C::kAlias ? dq_done : s_empty, (j - 1) & 1, abort_flag, err, kErrTimeoutEmpty)) return false;
-        if (!warp_wait(&full[s], (ik / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
-        if (!warp_wait(&full[sv], (iv / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
+            !warp_wait(C::kAlias ? dq_done : s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
+        if (!warp_wait(&full[s], (ik / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (!warp_wait(&full[sv], (iv / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
         if (issuer) {
           const uint32_t ks = k0 + s * (C::kSlot >> 4), vs = k0 + sv * (C::kSlot >> 4);
@@ -614,13 +645,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         __syncwarp();
         return true;
       };
-      bool go = warp_wait(q_full, 0, abort_flag, err, kErrTimeoutFull) && scores(0);
+      bool go = warp_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
         if (!C::kAlias && j + 1 < kt.n && !(go = scores(j + 1))) break;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
         const int s = (2 * j) % C::kSlots;
-        if (!(go = warp_wait(ds_full, j & 1, abort_flag, err, kErrTimeoutFull))) break;
+        if (!(go = warp_wait(ds_full, j & 1, err, kErrTimeoutFull))) break;
         tc_fence_after();
         if (issuer) {
           const uint32_t ks = t0 + s * (C::kSlot >> 4);
@@ -664,7 +695,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     for (int j = 0; j < kt.n; ++j) {
       int j0, cols;
       key_tile<KT>(kt, j, &j0, &cols);
-      if (!(ok = warp_wait(s_full, j & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+      if (!(ok = warp_wait(s_full, j & 1, err, kErrTimeoutTmemFull))) break;
       tc_fence_after();
       const bool whole = j >= kt.n_sink && cols == KT && j0 + cols <= L && j0 > w1 - p.window &&
                          j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
@@ -698,7 +729,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         __syncwarp();
         if (lane == 0) mbar_arrive(s_empty);
         if (j > 0) {  // the product before has read dS
-          if (!(ok = warp_wait(dq_done, (j - 1) & 1, abort_flag, err, kErrTimeoutTmemFull))) break;
+          if (!(ok = warp_wait(dq_done, (j - 1) & 1, err, kErrTimeoutTmemFull))) break;
           tc_fence_after();
         }
       }
@@ -712,7 +743,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
-    if (ok && kt.n > 0) ok = warp_wait(dq_done, (kt.n - 1) & 1, abort_flag, err, kErrTimeoutTmemFull);
+    if (ok && kt.n > 0) ok = warp_wait(dq_done, (kt.n - 1) & 1, err, kErrTimeoutTmemFull);
     tc_fence_after();
     if (!ok) {
       *abort_flag = 1;
@@ -765,9 +796,9 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
   uint64_t* full = reinterpret_cast<uint64_t*>(stat + 4 * QT);
   uint64_t* empty = full + C::kSlots;
   uint64_t* k_full = empty + C::kSlots;
-  uint64_t* s_full = k_full + 1;   // S and dP
-  uint64_t* ds_full = s_full + 1;  // P and dS
-  uint64_t* d_done = ds_full + 1;   // dV and dK of an iteration
+  uint64_t* s_full = k_full + 1;             // S and dP; of each buffer its own, as in the forward
+  uint64_t* ds_full = s_full + C::kBufs;     // P and dS
+  uint64_t* d_done = ds_full + C::kBufs;     // dV and dK of an iteration
   uint64_t* all_done = d_done + 1;  // of the last one
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
@@ -820,8 +851,10 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       mbar_init(&empty[s], 1);
     }
     mbar_init(k_full, 1);
-    mbar_init(s_full, 1);
-    mbar_init(ds_full, 4);
+    for (int i = 0; i < C::kBufs; ++i) {
+      mbar_init(&s_full[i], 1);
+      mbar_init(&ds_full[i], 4);
+    }
     mbar_init(d_done, 1);
     mbar_init(all_done, 1);
     *abort_flag = 0;
@@ -878,9 +911,9 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       // S^T = K Q^T and dP^T = V dO^T, once the products that read P and dS from this buffer are over
       auto scores = [&](int t) {
         const int iq = 2 * t, ig = iq + 1, s = iq % C::kSlots, sg = ig % C::kSlots;
-        if (t >= C::kBufs && !warp_wait(d_done, (t - C::kBufs) & 1, abort_flag, err, kErrTimeoutEmpty)) return false;
-        if (!warp_wait(&full[s], (iq / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
-        if (!warp_wait(&full[sg], (ig / C::kSlots) & 1, abort_flag, err, kErrTimeoutFull)) return false;
+        if (t >= C::kBufs && !warp_wait(d_done, (t - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
+        if (!warp_wait(&full[s], (iq / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
+        if (!warp_wait(&full[sg], (ig / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
         if (issuer) {
           const uint32_t buf = d0 + (t % C::kBufs) * 128;
@@ -891,15 +924,15 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
 #pragma unroll
           for (int k = 0; k < DP / 16; ++k)
             if (k < kd) umma_ss(buf + 64, v0 + step_k(128, k), gs + step_k(QT, k), idesc_s, k ? 1u : 0u);
-          tc_commit(s_full);
+          tc_commit(&s_full[t % C::kBufs]);
         }
         __syncwarp();
         return true;
       };
-      bool go = warp_wait(k_full, 0, abort_flag, err, kErrTimeoutFull) && scores(0);
+      bool go = warp_wait(k_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int t = 0; t < n && go; ++t) {
         if (C::kBufs == 2 && t + 1 < n && !(go = scores(t + 1))) break;
-        if (!(go = warp_wait(ds_full, t & 1, abort_flag, err, kErrTimeoutFull))) break;
+        if (!(go = warp_wait(&ds_full[t % C::kBufs], (t / C::kBufs) & 1, err, kErrTimeoutFull))) break;
         tc_fence_after();
         const int s = (2 * t) % C::kSlots, sg = (2 * t + 1) % C::kSlots;
         if (issuer) {
@@ -949,7 +982,7 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       asm volatile("bar.sync 1, 128;" ::: "memory");  // also: everyone is done with the buffer of t - 1
       if (t + 1 < n) next = load_stat(t + 1);
       // after a wait that gave up the loop goes on empty: the other warps count on this one at the barrier
-      if (ok) ok = warp_wait(s_full, t & 1, abort_flag, err, kErrTimeoutTmemFull);
+      if (ok) ok = warp_wait(&s_full[t % C::kBufs], (t / C::kBufs) & 1, err, kErrTimeoutTmemFull);
       if (!ok) continue;
       tc_fence_after();
       if (!idle) {
@@ -1009,9 +1042,9 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(ds_full);
+      if (lane == 0) mbar_arrive(&ds_full[t % C::kBufs]);
     }
-    if (ok && n > 0) ok = warp_wait(all_done, 0, abort_flag, err, kErrTimeoutTmemFull);
+    if (ok && n > 0) ok = warp_wait(all_done, 0, err, kErrTimeoutTmemFull);
     tc_fence_after();
     if (!ok) {
       *abort_flag = 1;
