@@ -32,6 +32,7 @@
 #include <c10/cuda/CUDAGuard.h>
 
 #include <algorithm>
+#include <array>
 #include <string>
 
 #include "common.cuh"
@@ -42,6 +43,10 @@ namespace {
 constexpr int kRotThreads = 256;
 constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kRotMaxDim = 256;
+constexpr int kRotBatch = 2;  // heads that a lane group asks for at once
+// Resident blocks of an SM: more of them spill (8192 x 2 tokens, 16 + 4 heads of 64: forward 28 us with 3, 36 us
+// with 4; adjoint 47 us with 2, 54 us with 3).
+constexpr int kRotFwdBlocks = 3, kRotBwdBlocks = 2;
 
 enum NormKind : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };
 
@@ -56,6 +61,7 @@ struct HeadSet {
   const float* b;
   float* dparam;           // adjoint: [blocks][2][D] partial sums of dw, db (or null)
   int H;
+  int block0, blocks;      // the blocks that work on this set
 };
 
 struct RotParams {
@@ -163,23 +169,25 @@ __device__ __forceinline__ void turn(float (&v)[V], const float (&c)[V], const f
 }
 
 // Vector kernel.  BWD: the adjoint.  A block's warps take tokens of one set
-// (blockIdx.y), strided by the grid.
+// (blockIdx.x), strided by the set's blocks.
 template <typename T, int LPR, bool BWD>
-__global__ void __launch_bounds__(kRotThreads) rot_vec_kernel(const __grid_constant__ RotParams p) {
+__global__ void __launch_bounds__(kRotThreads, BWD ? kRotBwdBlocks : kRotFwdBlocks) rot_vec_kernel(const __grid_constant__ RotParams p) {
   constexpr int V = HVec<T>::n;
   constexpr int ROWS = 32 / LPR;
-  const HeadSet& hs = p.set[blockIdx.y];
+  constexpr int kBatch = kRotBatch;
+  __shared__ __align__(16) float sw[LPR * V], sb[LPR * V];  // scale and shift: registers are warps here
+  const HeadSet& hs = p.set[blockIdx.x >= p.set[1].block0];
+  const int block = blockIdx.x - hs.block0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int l = lane % LPR, sub = lane / LPR;
   const int d0 = l * V;
   const bool live = d0 < p.D;
   const float inv_d = 1.f / static_cast<float>(p.D);
-  float w[V], bias[V];
-#pragma unroll
-  for (int e = 0; e < V; ++e) {
-    w[e] = (live && hs.w) ? hs.w[d0 + e] : 1.f;
-    bias[e] = (live && hs.b) ? hs.b[d0 + e] : 0.f;
+  for (int d = threadIdx.x; d < LPR * V; d += kRotThreads) {
+    sw[d] = (d < p.D && hs.w) ? hs.w[d] : 1.f;
+    sb[d] = (d < p.D && hs.b) ? hs.b[d] : 0.f;
   }
+  __syncthreads();
   float dw[V], db[V];
 #pragma unroll
   for (int e = 0; e < V; ++e) dw[e] = db[e] = 0.f;
@@ -189,14 +197,37 @@ __global__ void __launch_bounds__(kRotThreads) rot_vec_kernel(const __grid_const
   const bool first = live && d0 < half, second = live && d0 >= half && d0 < p.R;
   const int partner = p.interleaved ? lane : (first ? lane + hl : (second ? lane - hl : lane));
   const int H = hs.H;
-  const long long step = static_cast<long long>(gridDim.x) * kRotWarps;
-  for (long long t = static_cast<long long>(blockIdx.x) * kRotWarps + warp; t < p.tokens; t += step) {
-    const int b = static_cast<int>(t / p.S), s = static_cast<int>(t - static_cast<long long>(b) * p.S);
+  const int step = hs.blocks * kRotWarps, tokens = static_cast<int>(p.tokens);
+  int t = block * kRotWarps + warp;
+  int b = t / p.S, s = t - b * p.S;
+  int at = p.R && t < tokens ? table_row(p, b, s) : 0;  // asked for one token ahead
+  for (; t < tokens; t += step) {
+    const T* xt = static_cast<const T*>(hs.x) + b * hs.sb + s * hs.ss + d0;
+    const T* gt = BWD ? static_cast<const T*>(hs.dy) + b * hs.gb + s * hs.gs + d0 : nullptr;
+    T* yt = static_cast<T*>(hs.y) + static_cast<long long>(t) * H * p.D + d0;
+    // kBatch heads of every lane group are asked for at once, the first ones before the table's row
+    uint4 xu[kBatch], gu[kBatch];
+    auto fetch = [&](int h0) {
+#pragma unroll
+      for (int u = 0; u < kBatch; ++u) {
+        const int h = h0 + u * ROWS + sub;
+        const bool on = live && h < H;
+        xu[u] = make_uint4(0, 0, 0, 0);
+        if (on && (!BWD || p.norm != kNormNone)) xu[u] = __ldg(reinterpret_cast<const uint4*>(xt + h * hs.sh));
+        if (BWD) {
+          gu[u] = make_uint4(0, 0, 0, 0);
+          if (on) gu[u] = __ldg(reinterpret_cast<const uint4*>(gt + h * hs.gh));
+        }
+      }
+    };
+    fetch(0);
+    const int b_next = (t + step) / p.S, s_next = t + step - b_next * p.S;
+    const int at_next = p.R && t + step < tokens ? table_row(p, b_next, s_next) : 0;
     float c[V], sn[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) c[e] = 1.f, sn[e] = 0.f;
     if (live && d0 < p.R) {
-      const float2* row = p.table + static_cast<long long>(table_row(p, b, s)) * half;
+      const float2* row = p.table + static_cast<long long>(at) * half;
       const float dir = BWD ? -1.f : 1.f;
       if (p.interleaved) {
 #pragma unroll
@@ -207,71 +238,71 @@ __global__ void __launch_bounds__(kRotThreads) rot_vec_kernel(const __grid_const
             sn[e] = dir * cs.y;
           }
       } else {
-        const int i0 = first ? d0 : d0 - half;
+        // half is a multiple of V here, so the row and its pieces lie on 16-byte boundaries
+        const float4* cs4 = reinterpret_cast<const float4*>(row + (first ? d0 : d0 - half));
         const float sign = first ? -dir : dir;
 #pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const float2 cs = __ldg(row + i0 + e);
-          c[e] = cs.x;
-          sn[e] = sign * cs.y;
+        for (int e = 0; e < V; e += 2) {
+          const float4 cs = __ldg(cs4 + e / 2);
+          c[e] = cs.x, c[e + 1] = cs.z;
+          sn[e] = sign * cs.y, sn[e + 1] = sign * cs.w;
         }
       }
     }
-    const T* xt = static_cast<const T*>(hs.x) + b * hs.sb + s * hs.ss + d0;
-    const T* gt = BWD ? static_cast<const T*>(hs.dy) + b * hs.gb + s * hs.gs + d0 : nullptr;
-    T* yt = static_cast<T*>(hs.y) + t * H * p.D + d0;
-#pragma unroll 2
-    for (int h0 = 0; h0 < H; h0 += ROWS) {
-      const int h = h0 + sub;
-      const bool on = live && h < H;
-      uint4 xu = make_uint4(0, 0, 0, 0), gu = make_uint4(0, 0, 0, 0);
-      if (on && (!BWD || p.norm != kNormNone)) xu = __ldg(reinterpret_cast<const uint4*>(xt + h * hs.sh));
-      if (BWD && on) gu = __ldg(reinterpret_cast<const uint4*>(gt + h * hs.gh));
-      float x[V];
-      unpack16<T>(xu, x);
-      float r = 1.f;
-      if (p.norm == kNormLayer) {
-        float m = 0.f;
+    for (int h0 = 0; h0 < H; h0 += ROWS * kBatch) {
+      if (h0 > 0) fetch(h0);
 #pragma unroll
-        for (int e = 0; e < V; ++e) m += x[e];
-        m = row_sum<LPR>(m) * inv_d;
+      for (int u = 0; u < kBatch; ++u) {
+        if (h0 + u * ROWS >= H) break;
+        const int h = h0 + u * ROWS + sub;
+        const bool on = live && h < H;
+        float x[V];
+        unpack16<T>(xu[u], x);
+        float r = 1.f;
+        if (p.norm == kNormLayer) {
+          float m = 0.f;
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = live ? x[e] - m : 0.f;  // absent lanes stay out of the variance
-      }
-      if (p.norm != kNormNone) {
-        float q = 0.f;
+          for (int e = 0; e < V; ++e) m += x[e];
+          m = row_sum<LPR>(m) * inv_d;
 #pragma unroll
-        for (int e = 0; e < V; ++e) q = fmaf(x[e], x[e], q);
-        r = rsqrtf(row_sum<LPR>(q) * inv_d + p.eps);
-      }
-      if (!BWD) {
-#pragma unroll
-        for (int e = 0; e < V; ++e) x[e] = fmaf(x[e] * r, w[e], bias[e]);
-        turn<V>(x, c, sn, p.interleaved, partner);
-        if (on) *reinterpret_cast<uint4*>(yt + h * p.D) = pack16<T>(x);
-      } else {
-        float g[V];
-        unpack16<T>(gu, g);
-        turn<V>(g, c, sn, p.interleaved, partner);
+          for (int e = 0; e < V; ++e) x[e] = live ? x[e] - m : 0.f;  // absent lanes stay out of the variance
+        }
         if (p.norm != kNormNone) {
-          float m1 = 0.f, m2 = 0.f;
+          float q = 0.f;
 #pragma unroll
-          for (int e = 0; e < V; ++e) {
-            x[e] *= r;
-            dw[e] = fmaf(g[e], x[e], dw[e]);
-            db[e] += g[e];
-            g[e] *= w[e];
-            m1 += g[e];
-            m2 = fmaf(g[e], x[e], m2);
-          }
-          m2 = row_sum<LPR>(m2) * inv_d;
-          m1 = p.norm == kNormLayer ? row_sum<LPR>(m1) * inv_d : 0.f;
-#pragma unroll
-          for (int e = 0; e < V; ++e) g[e] = r * (g[e] - m1 - x[e] * m2);
+          for (int e = 0; e < V; ++e) q = fmaf(x[e], x[e], q);
+          r = rsqrtf(row_sum<LPR>(q) * inv_d + p.eps);
         }
-        if (on) *reinterpret_cast<uint4*>(yt + h * p.D) = pack16<T>(g);
+        if (!BWD) {
+#pragma unroll
+          for (int e = 0; e < V; ++e) x[e] = fmaf(x[e] * r, sw[d0 + e], sb[d0 + e]);
+          turn<V>(x, c, sn, p.interleaved, partner);
+          if (on) *reinterpret_cast<uint4*>(yt + h * p.D) = pack16<T>(x);
+        } else {
+          float g[V];
+          unpack16<T>(gu[u], g);
+          turn<V>(g, c, sn, p.interleaved, partner);
+          if (p.norm != kNormNone) {
+            float m1 = 0.f, m2 = 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) {
+              x[e] *= r;
+              dw[e] = fmaf(g[e], x[e], dw[e]);
+              db[e] += g[e];
+              g[e] *= sw[d0 + e];
+              m1 += g[e];
+              m2 = fmaf(g[e], x[e], m2);
+            }
+            m2 = row_sum<LPR>(m2) * inv_d;
+            m1 = p.norm == kNormLayer ? row_sum<LPR>(m1) * inv_d : 0.f;
+#pragma unroll
+            for (int e = 0; e < V; ++e) g[e] = r * (g[e] - m1 - x[e] * m2);
+          }
+          if (on) *reinterpret_cast<uint4*>(yt + h * p.D) = pack16<T>(g);
+        }
       }
     }
+    b = b_next, s = s_next, at = at_next;
   }
   if (BWD && hs.dparam != nullptr) {  // the block's sums: rows of a warp, then the warps, in order
     __shared__ float part[kRotWarps][2][LPR * V];
@@ -292,7 +323,7 @@ __global__ void __launch_bounds__(kRotThreads) rot_vec_kernel(const __grid_const
       const int k = i / p.D, d = i - k * p.D;
       float a = 0.f;
       for (int q = 0; q < kRotWarps; ++q) a += part[q][k][d];
-      hs.dparam[(static_cast<long long>(blockIdx.x) * 2 + k) * p.D + d] = a;
+      hs.dparam[(static_cast<long long>(block) * 2 + k) * p.D + d] = a;
     }
   }
 }
@@ -303,7 +334,8 @@ __global__ void __launch_bounds__(kRotThreads) rot_row_kernel(const __grid_const
   constexpr int E = kRotMaxDim / 32;
   __shared__ float rowbuf[kRotWarps][kRotMaxDim];
   __shared__ float part[kRotWarps][2][kRotMaxDim];
-  const HeadSet& hs = p.set[blockIdx.y];
+  const HeadSet& hs = p.set[blockIdx.x >= p.set[1].block0];
+  const int block = blockIdx.x - hs.block0;
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   float* buf = rowbuf[warp];
   const int D = p.D, half = p.R / 2;
@@ -312,8 +344,8 @@ __global__ void __launch_bounds__(kRotThreads) rot_row_kernel(const __grid_const
 #pragma unroll
   for (int j = 0; j < E; ++j) dw[j] = db[j] = 0.f;
   const long long rows = p.tokens * hs.H;
-  for (long long row = static_cast<long long>(blockIdx.x) * kRotWarps + warp; row < rows;
-       row += static_cast<long long>(gridDim.x) * kRotWarps) {
+  for (long long row = static_cast<long long>(block) * kRotWarps + warp; row < rows;
+       row += static_cast<long long>(hs.blocks) * kRotWarps) {
     const long long t = row / hs.H;
     const int h = static_cast<int>(row - t * hs.H);
     const int b = static_cast<int>(t / p.S), s = static_cast<int>(t - static_cast<long long>(b) * p.S);
@@ -398,48 +430,61 @@ __global__ void __launch_bounds__(kRotThreads) rot_row_kernel(const __grid_const
       const int k = i / D, d = i - k * D;
       float a = 0.f;
       for (int q = 0; q < kRotWarps; ++q) a += part[q][k][d];
-      hs.dparam[(static_cast<long long>(blockIdx.x) * 2 + k) * D + d] = a;
+      hs.dparam[(static_cast<long long>(block) * 2 + k) * D + d] = a;
     }
   }
 }
 
-// out[i] = sum over the blocks' partials; one block of 8 warps per 32 columns
-// of (set, dw/db, D), the blocks split over the warps and added in order.
-__global__ void __launch_bounds__(256) rot_param_kernel(const float* __restrict__ part, float* __restrict__ out,
-                                                       int blocks, int cols) {
+struct ParamGrads {
+  float* out[2][2];      // q, k: dw, db, or null
+  const float* part[2];
+  int blocks[2];
+};
+
+// Sums of the blocks' partials, in order: one block of 8 warps for 32 columns of
+// (set, dw or db), the blocks dealt to the warps in turn.
+__global__ void __launch_bounds__(256) rot_param_kernel(const ParamGrads g, int D) {
   __shared__ float acc[8][32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int c = blockIdx.x * 32 + lane;
-  const float* src = part + static_cast<long long>(blockIdx.y) * blocks * cols;
+  const int set = blockIdx.z, k = blockIdx.y, d = blockIdx.x * 32 + lane;
+  float* out = g.out[set][k];
+  if (out == nullptr) return;
+  const float* src = g.part[set] + k * D + d;
+  const int blocks = g.blocks[set];
   float a = 0.f;
-  if (c < cols)
-    for (int b = warp; b < blocks; b += 8) a += src[static_cast<long long>(b) * cols + c];
+  if (d < D) {
+#pragma unroll 8
+    for (int b = warp; b < blocks; b += 8) a += src[static_cast<long long>(b) * 2 * D];
+  }
   acc[warp][lane] = a;
   __syncthreads();
-  if (warp == 0 && c < cols) {
+  if (warp == 0 && d < D) {
     float t = 0.f;
     for (int w = 0; w < 8; ++w) t += acc[w][lane];
-    out[static_cast<long long>(blockIdx.y) * cols + c] = t;
+    out[d] = t;
   }
 }
 
+// Lanes to a row in the vector kernel.
+int row_lanes(int D, int vec) {
+  int l = 2;
+  while (l < 32 && l * vec < D) l *= 2;
+  return l;
+}
+
 template <typename T, bool BWD>
-void launch_rot(const RotParams& p, bool vec, int blocks, cudaStream_t st) {
-  const dim3 grid(blocks, 2);
+void launch_rot(const RotParams& p, bool vec, cudaStream_t st) {
+  const int grid = p.set[0].blocks + p.set[1].blocks;
   if (!vec) {
     rot_row_kernel<T, BWD><<<grid, kRotThreads, 0, st>>>(p);
   } else {
-    const int lanes = (p.D + HVec<T>::n - 1) / HVec<T>::n;
-    if (lanes <= 2)
-      rot_vec_kernel<T, 2, BWD><<<grid, kRotThreads, 0, st>>>(p);
-    else if (lanes <= 4)
-      rot_vec_kernel<T, 4, BWD><<<grid, kRotThreads, 0, st>>>(p);
-    else if (lanes <= 8)
-      rot_vec_kernel<T, 8, BWD><<<grid, kRotThreads, 0, st>>>(p);
-    else if (lanes <= 16)
-      rot_vec_kernel<T, 16, BWD><<<grid, kRotThreads, 0, st>>>(p);
-    else
-      rot_vec_kernel<T, 32, BWD><<<grid, kRotThreads, 0, st>>>(p);
+    switch (row_lanes(p.D, HVec<T>::n)) {
+      case 2: rot_vec_kernel<T, 2, BWD><<<grid, kRotThreads, 0, st>>>(p); break;
+      case 4: rot_vec_kernel<T, 4, BWD><<<grid, kRotThreads, 0, st>>>(p); break;
+      case 8: rot_vec_kernel<T, 8, BWD><<<grid, kRotThreads, 0, st>>>(p); break;
+      case 16: rot_vec_kernel<T, 16, BWD><<<grid, kRotThreads, 0, st>>>(p); break;
+      default: rot_vec_kernel<T, 32, BWD><<<grid, kRotThreads, 0, st>>>(p); break;
+    }
   }
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
@@ -488,6 +533,7 @@ Prepared prepare(const at::Tensor& q, const at::Tensor& k, const c10::optional<a
   TORCH_CHECK(D >= 1 && D <= kRotMaxDim, "qk_norm_rotary: head_dim 1 to 256 expected, got " + std::to_string(D));
   TORCH_CHECK(q.size(1) < (1ll << 31) && q.size(2) < (1 << 20) && k.size(2) < (1 << 20),
               "qk_norm_rotary: sequence or head count too large");
+  TORCH_CHECK(q.size(0) * q.size(1) < (1ll << 31) - (1 << 20), "qk_norm_rotary: 2^31 tokens or more");
   Prepared r{};
   RotParams& p = r.p;
   p.S = static_cast<int>(q.size(1));
@@ -538,15 +584,26 @@ Prepared prepare(const at::Tensor& q, const at::Tensor& k, const c10::optional<a
     p.set[i].b = bs[i];
     r.vec = r.vec && aligned16(x);
   }
-  r.vec = r.vec && D % V == 0 && (interleaved || (p.R / 2) % V == 0) && D / V <= 32;
+  r.vec = r.vec && reinterpret_cast<uintptr_t>(p.table) % 16 == 0 && D % V == 0 && (interleaved || (p.R / 2) % V == 0) && D / V <= 32;
   return r;
 }
 
-// Blocks for each set: a warp takes at least one token (or, in the row kernel,
-// one row); at most eight blocks to an SM in all.
-int rot_blocks(const Prepared& r) {
-  const long long units = r.vec ? r.p.tokens : r.p.tokens * std::max(r.p.set[0].H, r.p.set[1].H);
-  return static_cast<int>(std::max<long long>(1, std::min<long long>((units + kRotWarps - 1) / kRotWarps, 148 * 4)));
+// The SMs' resident blocks shared out by what a token of the set takes (a trip to
+// memory for each batch of heads); a warp takes at least one token (in the row
+// kernel one row).
+void share_blocks(Prepared& r, bool bwd, int lane_groups) {
+  const int resident = at::cuda::getCurrentDeviceProperties()->multiProcessorCount * (r.vec ? (bwd ? kRotBwdBlocks : kRotFwdBlocks) : 8);
+  int trips[2];
+  for (int i = 0; i < 2; ++i)
+    trips[i] = r.vec ? (r.p.set[i].H + lane_groups * kRotBatch - 1) / (lane_groups * kRotBatch) : r.p.set[i].H;
+  for (int i = 0; i < 2; ++i) {
+    HeadSet& s = r.p.set[i];
+    const long long units = r.vec ? r.p.tokens : r.p.tokens * s.H;
+    const long long share = static_cast<long long>(resident) * trips[i] / std::max(1, trips[0] + trips[1]);
+    s.blocks = static_cast<int>(std::max<long long>(1, std::min((units + kRotWarps - 1) / kRotWarps, share)));
+  }
+  r.p.set[0].block0 = 0;
+  r.p.set[1].block0 = r.p.set[0].blocks;
 }
 
 }  // namespace
@@ -564,20 +621,21 @@ std::vector<at::Tensor> qk_norm_rotary_fwd(const at::Tensor& q, const at::Tensor
   if (r.p.tokens == 0) return {yq, yk};
   r.p.set[0].y = yq.data_ptr();
   r.p.set[1].y = yk.data_ptr();
+  share_blocks(r, false, 32 / row_lanes(r.p.D, 16 / static_cast<int>(q.element_size())));
   auto st = at::cuda::getCurrentCUDAStream();
   if (q.scalar_type() == at::kBFloat16)
-    launch_rot<__nv_bfloat16, false>(r.p, r.vec, rot_blocks(r), st);
+    launch_rot<__nv_bfloat16, false>(r.p, r.vec, st);
   else
-    launch_rot<float, false>(r.p, r.vec, rot_blocks(r), st);
+    launch_rot<float, false>(r.p, r.vec, st);
   return {yq, yk};
 }
 
-// Returns dq, dk and, with `params`, a (2, 2, D) tensor: dw and db of q, then of k.
+// Returns dq, dk, dq_weight, dk_weight, dq_bias, dk_bias; the last four are undefined unless asked for.
 std::vector<at::Tensor> qk_norm_rotary_bwd(const at::Tensor& dyq, const at::Tensor& dyk, const at::Tensor& q,
                                            const at::Tensor& k, const c10::optional<at::Tensor>& table,
                                            const c10::optional<at::Tensor>& positions,
                                            const c10::optional<at::Tensor>& qw, const c10::optional<at::Tensor>& kw,
-                                           int64_t norm, bool interleaved, double eps, bool params,
+                                           int64_t norm, bool interleaved, double eps, std::array<bool, 4> need,
                                            const c10::optional<at::Tensor>& err) {
   auto r = prepare(q, k, table, positions, qw, kw, c10::nullopt, c10::nullopt, norm, interleaved, eps, err);
   c10::cuda::CUDAGuard guard(q.device());
@@ -592,32 +650,45 @@ std::vector<at::Tensor> qk_norm_rotary_bwd(const at::Tensor& dyq, const at::Tens
     r.p.set[i].gh = gs[i]->stride(2);
     r.vec = r.vec && aligned16(*gs[i]);
   }
-  auto dq = out_empty(q.sizes(), q.options()), dk = out_empty(k.sizes(), k.options());
   const int64_t D = q.size(3);
-  auto dp = params ? out_empty({2, 2, D}, q.options().dtype(at::kFloat)) : at::Tensor();
-  if (r.p.tokens == 0) {
-    if (params) dp.zero_();
-    return params ? std::vector<at::Tensor>{dq, dk, dp} : std::vector<at::Tensor>{dq, dk};
+  std::vector<at::Tensor> out(6);
+  out[0] = out_empty(q.sizes(), q.options());
+  out[1] = out_empty(k.sizes(), k.options());
+  ParamGrads pg{};
+  bool params = false;
+  for (int i = 0; i < 4; ++i) {
+    if (!need[i]) continue;
+    params = true;
+    out[2 + i] = out_empty({D}, q.options().dtype(at::kFloat));
+    pg.out[i & 1][i >> 1] = out[2 + i].data_ptr<float>();
   }
-  r.p.set[0].y = dq.data_ptr();
-  r.p.set[1].y = dk.data_ptr();
-  const int blocks = rot_blocks(r);
+  if (r.p.tokens == 0) {
+    for (int i = 2; i < 6; ++i)
+      if (out[i].defined()) out[i].zero_();
+    return out;
+  }
+  r.p.set[0].y = out[0].data_ptr();
+  r.p.set[1].y = out[1].data_ptr();
+  share_blocks(r, true, 32 / row_lanes(r.p.D, 16 / static_cast<int>(q.element_size())));
   at::Tensor part;
   if (params) {
-    part = out_empty({2, blocks, 2, D}, q.options().dtype(at::kFloat));
-    r.p.set[0].dparam = part.data_ptr<float>();
-    r.p.set[1].dparam = part.data_ptr<float>() + static_cast<int64_t>(blocks) * 2 * D;
+    part = out_empty({r.p.set[0].blocks + r.p.set[1].blocks, 2, D}, q.options().dtype(at::kFloat));
+    for (int i = 0; i < 2; ++i) {
+      r.p.set[i].dparam = part.data_ptr<float>() + static_cast<int64_t>(r.p.set[i].block0) * 2 * D;
+      pg.part[i] = r.p.set[i].dparam;
+      pg.blocks[i] = r.p.set[i].blocks;
+    }
   }
   auto st = at::cuda::getCurrentCUDAStream();
   if (q.scalar_type() == at::kBFloat16)
-    launch_rot<__nv_bfloat16, true>(r.p, r.vec, blocks, st);
+    launch_rot<__nv_bfloat16, true>(r.p, r.vec, st);
   else
-    launch_rot<float, true>(r.p, r.vec, blocks, st);
-  if (!params) return {dq, dk};
-  rot_param_kernel<<<dim3(static_cast<unsigned>((2 * D + 31) / 32), 2), 256, 0, st>>>(
-      part.data_ptr<float>(), dp.data_ptr<float>(), blocks, static_cast<int>(2 * D));
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
-  return {dq, dk, dp};
+    launch_rot<float, true>(r.p, r.vec, st);
+  if (params) {
+    rot_param_kernel<<<dim3(static_cast<unsigned>((D + 31) / 32), 2, 2), 256, 0, st>>>(pg, static_cast<int>(D));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
+  return out;
 }
 
 }  // namespace tgcm

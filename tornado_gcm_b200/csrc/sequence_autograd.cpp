@@ -72,10 +72,11 @@ struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
     const bool qw = d["qw"].toBool(), kw = d["kw"].toBool(), qb = d["qb"].toBool(), kb = d["kb"].toBool();
     auto r = qk_norm_rotary_bwd(rows_like(g[0], s[0]), rows_like(g[1], s[1]), s[0], s[1], opt(s[2]), opt(s[3]),
                                 opt(s[4]), opt(s[5]), d["norm"].toInt(), d["inter"].toBool(), d["eps"].toDouble(),
-                                qw || kw || qb || kb, d["err"].toOptional<at::Tensor>());
-    auto at = [&](int i, int j, bool on) { return on ? r[2][i][j] : at::Tensor(); };
-    return {r[0],         r[1],         at::Tensor(), at::Tensor(), at(0, 0, qw), at(1, 0, kw),
-            at(0, 1, qb), at(1, 1, kb), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+                                {qw, kw, qb, kb}, d["err"].toOptional<at::Tensor>());
+    variable_list out(12);
+    out[0] = r[0], out[1] = r[1];
+    for (int i = 0; i < 4; ++i) out[4 + i] = r[2 + i];
+    return out;
   }
 };
 

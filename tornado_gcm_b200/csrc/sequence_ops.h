@@ -3,6 +3,7 @@
 
 #include <ATen/ATen.h>
 
+#include <array>
 #include <vector>
 
 namespace tgcm {
@@ -20,11 +21,11 @@ std::vector<at::Tensor> qk_norm_rotary_fwd(const at::Tensor& q, const at::Tensor
                                            const OptTensor& positions, const OptTensor& qw, const OptTensor& kw,
                                            const OptTensor& qb, const OptTensor& kb, int64_t norm, bool interleaved,
                                            double eps, const OptTensor& err);
-// dq, dk and, with `params`, (2, 2, D): dw and db of q, then of k
+// dq, dk, dq_weight, dk_weight, dq_bias, dk_bias; of the last four those that `need` names
 std::vector<at::Tensor> qk_norm_rotary_bwd(const at::Tensor& dyq, const at::Tensor& dyk, const at::Tensor& q,
                                            const at::Tensor& k, const OptTensor& table, const OptTensor& positions,
                                            const OptTensor& qw, const OptTensor& kw, int64_t norm, bool interleaved,
-                                           double eps, bool params, const OptTensor& err);
+                                           double eps, std::array<bool, 4> need, const OptTensor& err);
 
 // o, lse
 std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
