@@ -78,46 +78,69 @@ struct PairParams {
   int* err;
 };
 
-// act(z) and act'(z).  __expf and the fast division are good to a few units of
-// 1e-7 relative: far below the rounding of the bf16 result.
+// 1 / (1 + 2^t) of two values: the sigmoid of -t ln 2.  Two special-function
+// instructions each, exact to a few units of 1e-7: far below the rounding of
+// the bf16 result.  2^t = inf gives 0.
+__device__ __forceinline__ float2 sigmoid2(float2 t) {
+  const float2 d = add2(make_float2(ex2(t.x), ex2(t.y)), make_float2(1.f, 1.f));
+  return make_float2(rcp(d.x), rcp(d.y));
+}
+__device__ __forceinline__ float2 all2(float v) { return make_float2(v, v); }
+
+// gelu_tanh(z) = z sigmoid(2u) with 2u = c1 z (1 + 0.044715 z^2), c1 = 2 sqrt(2 / pi)
+constexpr float kGeluC1 = 1.5957691216057308f, kGeluC3 = 0.044715f;
+constexpr float kLog2E = 1.4426950408889634f;
+
+// act(z) of a pair of pre-activations
 template <int ACT>
-__device__ __forceinline__ float act_val(float z) {
-  if constexpr (ACT == kActRelu) return fmaxf(z, 0.f);
-  else if constexpr (ACT == kActGelu) return gelu_erf_f(z);
-  else if constexpr (ACT == kActGeluTanh) {  // z sigmoid(2u) = z (1 + tanh u) / 2
-    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z, z * z, z);
-    return __fdividef(z, 1.f + __expf(-u2));
-  } else if constexpr (ACT == kActSilu) return __fdividef(z, 1.f + __expf(-z));
-  else if constexpr (ACT == kActTanh) return tanhf(z);
-  else return z;
+__device__ __forceinline__ float2 act_val2(float2 z) {
+  if constexpr (ACT == kActGeluTanh) {
+    const float2 k = fma2(mul2(z, z), all2(-kGeluC1 * kGeluC3 * kLog2E), all2(-kGeluC1 * kLog2E));
+    return mul2(z, sigmoid2(mul2(k, z)));
+  } else if constexpr (ACT == kActSilu) {
+    return mul2(z, sigmoid2(mul2(z, all2(-kLog2E))));
+  } else if constexpr (ACT == kActRelu) {
+    return make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f));
+  } else if constexpr (ACT == kActGelu) {
+    return make_float2(gelu_erf_f(z.x), gelu_erf_f(z.y));
+  } else if constexpr (ACT == kActTanh) {
+    return make_float2(tanhf(z.x), tanhf(z.y));
+  } else {
+    return z;
+  }
 }
 
+// act(z) and act'(z)
 template <int ACT>
-__device__ __forceinline__ void act_both(float z, float* a, float* da) {
-  if constexpr (ACT == kActRelu) {
-    *a = fmaxf(z, 0.f);
-    *da = z > 0.f ? 1.f : 0.f;
+__device__ __forceinline__ void act_both2(float2 z, float2* a, float2* da) {
+  if constexpr (ACT == kActGeluTanh || ACT == kActSilu) {
+    float2 s, slope;  // slope: the derivative of the sigmoid's argument
+    if constexpr (ACT == kActGeluTanh) {
+      const float2 z2 = mul2(z, z);
+      const float2 k = fma2(z2, all2(-kGeluC1 * kGeluC3 * kLog2E), all2(-kGeluC1 * kLog2E));
+      s = sigmoid2(mul2(k, z));
+      slope = fma2(z2, all2(3.f * kGeluC1 * kGeluC3), all2(kGeluC1));
+    } else {
+      s = sigmoid2(mul2(z, all2(-kLog2E)));
+    }
+    *a = mul2(z, s);
+    float2 t = mul2(*a, fma2(s, all2(-1.f), all2(1.f)));  // z s (1 - s)
+    *da = ACT == kActGeluTanh ? fma2(t, slope, s) : add2(t, s);
+  } else if constexpr (ACT == kActRelu) {
+    *a = make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f));
+    *da = make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
   } else if constexpr (ACT == kActGelu) {
-    const float c = 0.5f * (1.f + erff(z * 0.7071067811865476f));
-    *a = z * c;
-    *da = fmaf(z * 0.3989422804014327f, __expf(-0.5f * z * z), c);
-  } else if constexpr (ACT == kActGeluTanh) {
-    const float z2 = z * z;
-    const float u2 = 1.5957691216057308f * fmaf(0.044715f * z, z2, z);
-    const float s = __fdividef(1.f, 1.f + __expf(-u2));
-    *a = z * s;
-    *da = s + z * s * (1.f - s) * 1.5957691216057308f * fmaf(3.f * 0.044715f, z2, 1.f);
-  } else if constexpr (ACT == kActSilu) {
-    const float s = __fdividef(1.f, 1.f + __expf(-z));
-    *a = z * s;
-    *da = s * fmaf(z, 1.f - s, 1.f);
+    const float2 c = make_float2(0.5f * (1.f + erff(z.x * 0.7071067811865476f)),
+                                 0.5f * (1.f + erff(z.y * 0.7071067811865476f)));
+    const float2 q = mul2(mul2(z, z), all2(-0.5f * kLog2E));
+    *a = mul2(z, c);
+    *da = fma2(mul2(z, all2(0.3989422804014327f)), make_float2(ex2(q.x), ex2(q.y)), c);
   } else if constexpr (ACT == kActTanh) {
-    const float t = tanhf(z);
-    *a = t;
-    *da = 1.f - t * t;
+    *a = make_float2(tanhf(z.x), tanhf(z.y));
+    *da = fma2(mul2(*a, all2(-1.f)), *a, all2(1.f));
   } else {
     *a = z;
-    *da = 1.f;
+    *da = all2(1.f);
   }
 }
 
@@ -125,12 +148,23 @@ __device__ __forceinline__ void act_both(float z, float* a, float* da) {
 #define TGCM_GATED_ACTS(CASE) \
   CASE(kActRelu) CASE(kActGelu) CASE(kActGeluTanh) CASE(kActSilu) CASE(kActTanh) CASE(kActNone)
 
+__device__ __forceinline__ float2 pair_at(const uint32_t (&v)[32], int j) {
+  return make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
+}
+__device__ __forceinline__ void pair_to(uint32_t (&v)[32], int j, float2 x) {
+  v[j] = __float_as_uint(x.x);
+  v[j + 1] = __float_as_uint(x.y);
+}
+__device__ __forceinline__ float2 bf2(uint32_t w) {
+  return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
+}
+
 __device__ __forceinline__ void gate32(int act, uint32_t (&g)[32], const uint32_t (&u)[32]) {
   switch (act) {
-#define TGCM_CASE(A)                                                                               \
-  case A:                                                                                          \
-    _Pragma("unroll") for (int j = 0; j < 32; ++j) g[j] =                                          \
-        __float_as_uint(act_val<A>(__uint_as_float(g[j])) * __uint_as_float(u[j]));                \
+#define TGCM_CASE(A)                                                                                  \
+  case A:                                                                                             \
+    _Pragma("unroll") for (int j = 0; j < 32; j += 2)                                                 \
+        pair_to(g, j, mul2(act_val2<A>(pair_at(g, j)), pair_at(u, j)));                               \
     break;
     TGCM_GATED_ACTS(TGCM_CASE)
 #undef TGCM_CASE
@@ -140,19 +174,38 @@ __device__ __forceinline__ void gate32(int act, uint32_t (&g)[32], const uint32_
 // (zg, zu, dh) -> (dg, du)
 __device__ __forceinline__ void dgate32(int act, uint32_t (&g)[32], uint32_t (&u)[32], const uint32_t (&dh)[16]) {
   switch (act) {
-#define TGCM_CASE(A)                                                                               \
-  case A:                                                                                          \
-    _Pragma("unroll") for (int j = 0; j < 32; ++j) {                                               \
-      const uint32_t w = dh[j >> 1];                                                               \
-      const float d = __uint_as_float((j & 1) ? (w & 0xffff0000u) : (w << 16));                    \
-      float a, da;                                                                                 \
-      act_both<A>(__uint_as_float(g[j]), &a, &da);                                                 \
-      g[j] = __float_as_uint(d * __uint_as_float(u[j]) * da);                                      \
-      u[j] = __float_as_uint(d * a);                                                               \
-    }                                                                                              \
+#define TGCM_CASE(A)                                                                                  \
+  case A:                                                                                             \
+    _Pragma("unroll") for (int j = 0; j < 32; j += 2) {                                               \
+      const float2 d = bf2(dh[j >> 1]);                                                               \
+      float2 a, da;                                                                                   \
+      act_both2<A>(pair_at(g, j), &a, &da);                                                           \
+      pair_to(g, j, mul2(mul2(d, pair_at(u, j)), da));                                                \
+      pair_to(u, j, mul2(d, a));                                                                      \
+    }                                                                                                 \
     break;
     TGCM_GATED_ACTS(TGCM_CASE)
 #undef TGCM_CASE
+  }
+}
+
+// z += bias for the 32 columns from col; whole 16-byte pieces of the vector, the
+// same for every lane, where they lie inside it.
+__device__ __forceinline__ void add_bias32(uint32_t (&z)[32], const __nv_bfloat16* bias, int col, int n, int lane) {
+  if (col + 32 <= n && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
+    const uint4* b = reinterpret_cast<const uint4*>(bias + col);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const uint4 w = __ldg(b + i);
+      pair_to(z, 8 * i, add2(pair_at(z, 8 * i), bf2(w.x)));
+      pair_to(z, 8 * i + 2, add2(pair_at(z, 8 * i + 2), bf2(w.y)));
+      pair_to(z, 8 * i + 4, add2(pair_at(z, 8 * i + 4), bf2(w.z)));
+      pair_to(z, 8 * i + 6, add2(pair_at(z, 8 * i + 6), bf2(w.w)));
+    }
+  } else {
+    const float b = col + lane < n ? __bfloat162float(bias[col + lane]) : 0.f;
+#pragma unroll
+    for (int j = 0; j < 32; ++j) z[j] = __float_as_uint(__uint_as_float(z[j]) + __shfl_sync(0xffffffffu, b, j));
   }
 }
 
@@ -428,14 +481,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           tmem_ld_32x32b_x32(ta + 128 + colw + ch * 32, u);
           tmem_ld_wait();
           if (p.bias_g != nullptr) {
-            const int col = col0 + ch * 32 + lane;
-            const float bg = col < p.N ? __bfloat162float(p.bias_g[col]) : 0.f;
-            const float bu = col < p.N ? __bfloat162float(p.bias_u[col]) : 0.f;
-#pragma unroll
-            for (int j = 0; j < 32; ++j) {
-              g[j] = __float_as_uint(__uint_as_float(g[j]) + __shfl_sync(0xffffffffu, bg, j));
-              u[j] = __float_as_uint(__uint_as_float(u[j]) + __shfl_sync(0xffffffffu, bu, j));
-            }
+            add_bias32(g, p.bias_g, col0 + ch * 32, p.N, lane);
+            add_bias32(u, p.bias_u, col0 + ch * 32, p.N, lane);
           }
           if constexpr (MODE == kFwd) {
             gate32(p.act, g, u);
@@ -630,7 +677,7 @@ __global__ void __launch_bounds__(256) skinny_kernel(const __nv_bfloat16* __rest
   float a = zg;
   switch (act) {
 #define TGCM_CASE(A) \
-  case A: a = act_val<A>(zg); break;
+  case A: a = act_val2<A>(make_float2(zg, 0.f)).x; break;
     TGCM_GATED_ACTS(TGCM_CASE)
 #undef TGCM_CASE
   }
