@@ -28,7 +28,7 @@
 // its own TMEM, double buffered so that the epilogue of one tile runs under the
 // products of the next.  Each SM then reads 128 + 128 operand rows for 256 x
 // 128 outputs: half the shared-memory traffic of one CTA alone.  Warp roles
-// (320 threads): warp 0 TMA, warp 1 MMA, warps 2-9 epilogue.  Waits are bounded.
+// (576 threads): warp 0 TMA, warp 1 MMA, warps 2-17 epilogue.  Waits are bounded.
 //
 // A few tokens (T <= 8) take skinny_kernel instead: bound by reading the
 // weights once, a warp to each hidden value, both weight rows in flight.
@@ -47,12 +47,13 @@
 namespace tgcm {
 namespace {
 
-constexpr int kPairThreads = 320;
+constexpr int kEpilogueWarps = 16;              // four to a scheduler: one warp's epilogue is mostly latency
+constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;
 constexpr int kPairStages = 6;
 constexpr int kOperand = 128 * 128;             // bytes: 128 rows of 64 bf16
 constexpr int kPairStage = 2 * kOperand;
-constexpr int kWarpStage = 32 * 128;            // bytes: one epilogue warp's 32 x 64 bf16 tile
-constexpr int kPairSmem = kPairStages * kPairStage + 8 * kWarpStage + 256 + 1024;
+constexpr int kWarpStage = 32 * 64;             // bytes: one epilogue warp's 32 x 32 bf16 tile
+constexpr int kPairSmem = kPairStages * kPairStage + kEpilogueWarps * kWarpStage + 256 + 1024;
 constexpr int kSkinnyTokens = 8;
 
 enum PairMode : int { kFwd = 0, kDact = 1, kDx = 2, kDw = 3 };
@@ -144,14 +145,14 @@ __device__ __forceinline__ void act_both2(float2 z, float2* a, float2* da) {
   }
 }
 
-// One switch for 32 values, so the epilogue is compiled once, not once an activation.
+// One switch for 16 values, so the epilogue is compiled once, not once an activation.
 #define TGCM_GATED_ACTS(CASE) \
   CASE(kActRelu) CASE(kActGelu) CASE(kActGeluTanh) CASE(kActSilu) CASE(kActTanh) CASE(kActNone)
 
-__device__ __forceinline__ float2 pair_at(const uint32_t (&v)[32], int j) {
+__device__ __forceinline__ float2 pair_at(const uint32_t (&v)[16], int j) {
   return make_float2(__uint_as_float(v[j]), __uint_as_float(v[j + 1]));
 }
-__device__ __forceinline__ void pair_to(uint32_t (&v)[32], int j, float2 x) {
+__device__ __forceinline__ void pair_to(uint32_t (&v)[16], int j, float2 x) {
   v[j] = __float_as_uint(x.x);
   v[j + 1] = __float_as_uint(x.y);
 }
@@ -159,11 +160,11 @@ __device__ __forceinline__ float2 bf2(uint32_t w) {
   return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u));
 }
 
-__device__ __forceinline__ void gate32(int act, uint32_t (&g)[32], const uint32_t (&u)[32]) {
+__device__ __forceinline__ void gate16(int act, uint32_t (&g)[16], const uint32_t (&u)[16]) {
   switch (act) {
 #define TGCM_CASE(A)                                                                                  \
   case A:                                                                                             \
-    _Pragma("unroll") for (int j = 0; j < 32; j += 2)                                                 \
+    _Pragma("unroll") for (int j = 0; j < 16; j += 2)                                                 \
         pair_to(g, j, mul2(act_val2<A>(pair_at(g, j)), pair_at(u, j)));                               \
     break;
     TGCM_GATED_ACTS(TGCM_CASE)
@@ -172,11 +173,11 @@ __device__ __forceinline__ void gate32(int act, uint32_t (&g)[32], const uint32_
 }
 
 // (zg, zu, dh) -> (dg, du)
-__device__ __forceinline__ void dgate32(int act, uint32_t (&g)[32], uint32_t (&u)[32], const uint32_t (&dh)[16]) {
+__device__ __forceinline__ void dgate16(int act, uint32_t (&g)[16], uint32_t (&u)[16], const uint32_t (&dh)[8]) {
   switch (act) {
 #define TGCM_CASE(A)                                                                                  \
   case A:                                                                                             \
-    _Pragma("unroll") for (int j = 0; j < 32; j += 2) {                                               \
+    _Pragma("unroll") for (int j = 0; j < 16; j += 2) {                                               \
       const float2 d = bf2(dh[j >> 1]);                                                               \
       float2 a, da;                                                                                   \
       act_both2<A>(pair_at(g, j), &a, &da);                                                           \
@@ -189,46 +190,26 @@ __device__ __forceinline__ void dgate32(int act, uint32_t (&g)[32], uint32_t (&u
   }
 }
 
-// z += bias for the 32 columns from col; whole 16-byte pieces of the vector, the
-// same for every lane, where they lie inside it.
-__device__ __forceinline__ void add_bias32(uint32_t (&z)[32], const __nv_bfloat16* bias, int col, int n, int lane) {
-  if (col + 32 <= n && (reinterpret_cast<uintptr_t>(bias) & 15) == 0) {
-    const uint4* b = reinterpret_cast<const uint4*>(bias + col);
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const uint4 w = __ldg(b + i);
-      pair_to(z, 8 * i, add2(pair_at(z, 8 * i), bf2(w.x)));
-      pair_to(z, 8 * i + 2, add2(pair_at(z, 8 * i + 2), bf2(w.y)));
-      pair_to(z, 8 * i + 4, add2(pair_at(z, 8 * i + 4), bf2(w.z)));
-      pair_to(z, 8 * i + 6, add2(pair_at(z, 8 * i + 6), bf2(w.w)));
-    }
-  } else {
-    const float b = col + lane < n ? __bfloat162float(bias[col + lane]) : 0.f;
-#pragma unroll
-    for (int j = 0; j < 32; ++j) z[j] = __float_as_uint(__uint_as_float(z[j]) + __shfl_sync(0xffffffffu, b, j));
-  }
-}
-
 __device__ __forceinline__ uint32_t pack2(uint32_t a, uint32_t b) {
   const __nv_bfloat162 h = __floats2bfloat162_rn(__uint_as_float(a), __uint_as_float(b));
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// Epilogue tiles are 32 rows of eight 16-byte pieces; piece c of row r sits at
-// c ^ (r & 7), so a lane writing its own row and eight lanes reading one row
+// Epilogue tiles are 32 rows of four 16-byte pieces; piece c of row r sits at
+// c ^ (r / 2 & 3), so a lane writing its own row and four lanes reading one row
 // both spread over all banks.
 __device__ __forceinline__ uint4* piece(uint8_t* stage, int row, int c) {
-  return reinterpret_cast<uint4*>(stage + row * 128 + ((c ^ (row & 7)) << 4));
+  return reinterpret_cast<uint4*>(stage + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
 
-// 32 x 64 bf16 tile to global memory, clipped to nrows x ncols.
+// 32 x 32 bf16 tile to global memory, clipped to nrows x ncols.
 __device__ __forceinline__ void tile_out(uint8_t* stage, __nv_bfloat16* g, long long ld, int nrows, int ncols,
                                          int lane) {
   const bool vec = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  const int c = lane & 7;
+  const int c = lane & 3;
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int row = it * 4 + (lane >> 3);
+  for (int it = 0; it < 4; ++it) {
+    const int row = it * 8 + (lane >> 2);
     if (row >= nrows || c * 8 >= ncols) continue;
     const uint4 v = *piece(stage, row, c);
     __nv_bfloat16* dst = g + row * ld + c * 8;
@@ -246,46 +227,46 @@ __device__ __forceinline__ void tile_out(uint8_t* stage, __nv_bfloat16* g, long 
 __device__ __forceinline__ void tile_in(uint8_t* stage, const __nv_bfloat16* g, long long ld, int nrows, int ncols,
                                         int lane) {
   const bool vec = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  const int c = lane & 7;
-  uint4 v[8];
+  const int c = lane & 3;
+  uint4 v[4];
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int row = it * 4 + (lane >> 3);
+  for (int it = 0; it < 4; ++it) {
+    const int row = it * 8 + (lane >> 2);
     v[it] = make_uint4(0, 0, 0, 0);
     if (row >= nrows || c * 8 >= ncols) continue;
     const __nv_bfloat16* src = g + row * ld + c * 8;
     if (vec && c * 8 + 8 <= ncols) {
       v[it] = __ldg(reinterpret_cast<const uint4*>(src));
     } else {
-      alignas(16) __nv_bfloat16 e[8];
+      __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&v[it]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) e[k] = c * 8 + k < ncols ? src[k] : __float2bfloat16(0.f);
-      v[it] = *reinterpret_cast<uint4*>(e);
+      for (int k = 0; k < 8; ++k)
+        if (c * 8 + k < ncols) e[k] = src[k];
     }
   }
 #pragma unroll
-  for (int it = 0; it < 8; ++it) *piece(stage, it * 4 + (lane >> 3), c) = v[it];
+  for (int it = 0; it < 4; ++it) *piece(stage, it * 8 + (lane >> 2), c) = v[it];
 }
 
-// 32 x 32 fp32 tile (same 128-byte rows) to global memory.
+// 32 x 16 fp32 tile (the same 64-byte rows) to global memory.
 __device__ __forceinline__ void tile_out_f32(uint8_t* stage, float* g, long long ld, int nrows, int ncols, int lane) {
-  const int c = lane & 7;  // part_ld is a multiple of 4
+  const int c = lane & 3;  // part_ld is a multiple of 4
 #pragma unroll
-  for (int it = 0; it < 8; ++it) {
-    const int row = it * 4 + (lane >> 3);
+  for (int it = 0; it < 4; ++it) {
+    const int row = it * 8 + (lane >> 2);
     if (row >= nrows || c * 4 >= ncols) continue;
     *reinterpret_cast<uint4*>(g + row * ld + c * 4) = *piece(stage, row, c);
   }
 }
 
-// Column sums of a 32 x 32 block held one row to a lane: after the halving
-// steps lane j has the sum of column j.
-__device__ __forceinline__ float column_sums(const uint32_t (&v)[32], int lane) {
-  float a[32];
+// Column sums of a 32 x 16 block held one row to a lane: after the halving
+// steps lanes j and j + 16 have the sum of column j.
+__device__ __forceinline__ float column_sums(const uint32_t (&v)[16], int lane) {
+  float a[16];
 #pragma unroll
-  for (int j = 0; j < 32; ++j) a[j] = __uint_as_float(v[j]);
+  for (int j = 0; j < 16; ++j) a[j] = __uint_as_float(v[j]);
 #pragma unroll
-  for (int n = 16; n >= 1; n >>= 1) {
+  for (int n = 8; n >= 1; n >>= 1) {
     const bool up = lane & n;
 #pragma unroll
     for (int j = 0; j < n; ++j) {
@@ -293,7 +274,12 @@ __device__ __forceinline__ float column_sums(const uint32_t (&v)[32], int lane) 
       a[j] = keep + __shfl_xor_sync(0xffffffffu, give, n);
     }
   }
-  return a[0];
+  return a[0] + __shfl_xor_sync(0xffffffffu, a[0], 16);
+}
+
+__device__ __forceinline__ uint4 pack8(const uint32_t (&v)[16], int j) {
+  return make_uint4(pack2(v[j], v[j + 1]), pack2(v[j + 2], v[j + 3]), pack2(v[j + 4], v[j + 5]),
+                    pack2(v[j + 6], v[j + 7]));
 }
 
 struct PairTile {
@@ -338,7 +324,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* staging = smem + kPairStages * kPairStage;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + 8 * kWarpStage);  // the leader's are used
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + kEpilogueWarps * kWarpStage);  // the leader's are used
   uint64_t* empty_bar = full_bar + kPairStages;
   uint64_t* acc_full = empty_bar + kPairStages;   // [2]
   uint64_t* acc_empty = acc_full + 2;             // [2], the leader's are used
@@ -357,7 +343,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&acc_full[i], 1);
-      mbar_init(&acc_empty[i], 16);  // eight epilogue warps of each CTA
+      mbar_init(&acc_empty[i], 2 * kEpilogueWarps);  // of both CTAs
     }
     *abort_flag = 0;
     fence_barrier_init();
@@ -450,16 +436,22 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       if (!go) *abort_flag = 1;
     }
   } else {
-    const int q = warp & 3, half = (warp - 2) >> 2;
+    const int q = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes, quarter of the tile's columns
     uint8_t* stage = staging + (warp - 2) * kWarpStage;
     int n = 0;
     for (int t = first; t < n_tiles; t += step) {
       const PairTile c = pair_tile<MODE>(p, t);
       const int row0 = c.tm * 256 + rank * 128 + q * 32;
       const int nrows = min(32, p.M - row0);
-      const int colw = half * (kTileN / 2);            // this warp's columns of the tile
+      const int colw = part * (kTileN / 4);            // this warp's columns of the tile
       const int col0 = c.tn * kTileN + colw;
-      if (MODE == kDact) {
+      uint32_t bias = 0;  // of column col0 + lane: the gate's in the lower half, the other's in the upper
+      if constexpr (MODE == kFwd || MODE == kDact) {
+        if (p.bias_g != nullptr && col0 + lane < p.N)
+          bias = static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p.bias_g) + col0 + lane)) |
+                 static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p.bias_u) + col0 + lane)) << 16;
+      }
+      if constexpr (MODE == kDact) {
         __syncwarp();
         tile_in(stage, p.dh + static_cast<long long>(row0) * p.dh_ld + col0, p.dh_ld, nrows, p.N - col0, lane);
         __syncwarp();
@@ -473,44 +465,42 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
       }
       const uint32_t ta = tmem + acc * 256 + (static_cast<uint32_t>(q * 32) << 16);
       if constexpr (MODE == kFwd || MODE == kDact) {
-        uint32_t keep[2][16];  // kDact: du, packed
+        uint32_t keep[16];  // kDact: du, packed
 #pragma unroll
         for (int ch = 0; ch < 2; ++ch) {
-          uint32_t g[32], u[32];
-          tmem_ld_32x32b_x32(ta + colw + ch * 32, g);
-          tmem_ld_32x32b_x32(ta + 128 + colw + ch * 32, u);
+          uint32_t g[16], u[16];
+          tmem_ld_32x32b_x16(ta + colw + ch * 16, g);
+          tmem_ld_32x32b_x16(ta + 128 + colw + ch * 16, u);
           tmem_ld_wait();
           if (p.bias_g != nullptr) {
-            add_bias32(g, p.bias_g, col0 + ch * 32, p.N, lane);
-            add_bias32(u, p.bias_u, col0 + ch * 32, p.N, lane);
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+              const float2 b = bf2(__shfl_sync(0xffffffffu, bias, ch * 16 + j));
+              g[j] = __float_as_uint(__uint_as_float(g[j]) + b.x);
+              u[j] = __float_as_uint(__uint_as_float(u[j]) + b.y);
+            }
           }
           if constexpr (MODE == kFwd) {
-            gate32(p.act, g, u);
+            gate16(p.act, g, u);
           } else {
-            uint32_t dh[16];
+            uint32_t dh[8];
 #pragma unroll
-            for (int v = 0; v < 4; ++v) {
-              const uint4 w = *piece(stage, lane, ch * 4 + v);
+            for (int v = 0; v < 2; ++v) {
+              const uint4 w = *piece(stage, lane, ch * 2 + v);
               dh[4 * v] = w.x, dh[4 * v + 1] = w.y, dh[4 * v + 2] = w.z, dh[4 * v + 3] = w.w;
             }
-            dgate32(p.act, g, u, dh);
+            dgate16(p.act, g, u, dh);
             if (p.bias_part != nullptr) {
               const float sg = column_sums(g, lane), su = column_sums(u, lane);
-              const int col = col0 + ch * 32 + lane;
-              if (col < p.N) {
-                float* bp = p.bias_part + static_cast<long long>(row0 >> 5) * 2 * p.N + col;
-                bp[0] = sg;
-                bp[p.N] = su;
-              }
+              const int col = col0 + ch * 16 + (lane & 15);
+              if (col < p.N)  // the lower half of the warp has the gate's sums to write, the upper the other's
+                p.bias_part[(static_cast<long long>(row0 >> 5) * 2 + (lane >> 4)) * p.N + col] = lane < 16 ? sg : su;
             }
 #pragma unroll
-            for (int v = 0; v < 16; ++v) keep[ch][v] = pack2(u[2 * v], u[2 * v + 1]);
+            for (int v = 0; v < 8; ++v) keep[ch * 8 + v] = pack2(u[2 * v], u[2 * v + 1]);
           }
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            *piece(stage, lane, ch * 4 + v) =
-                make_uint4(pack2(g[8 * v], g[8 * v + 1]), pack2(g[8 * v + 2], g[8 * v + 3]),
-                           pack2(g[8 * v + 4], g[8 * v + 5]), pack2(g[8 * v + 6], g[8 * v + 7]));
+          *piece(stage, lane, ch * 2) = pack8(g, 0);
+          *piece(stage, lane, ch * 2 + 1) = pack8(g, 8);
         }
         tc_fence_before();
         __syncwarp();
@@ -519,9 +509,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if constexpr (MODE == kDact) {
 #pragma unroll
-          for (int v = 0; v < 8; ++v)
-            *piece(stage, lane, v) = make_uint4(keep[v >> 2][4 * (v & 3)], keep[v >> 2][4 * (v & 3) + 1],
-                                                keep[v >> 2][4 * (v & 3) + 2], keep[v >> 2][4 * (v & 3) + 3]);
+          for (int v = 0; v < 4; ++v)
+            *piece(stage, lane, v) = make_uint4(keep[4 * v], keep[4 * v + 1], keep[4 * v + 2], keep[4 * v + 3]);
           __syncwarp();
           tile_out(stage, p.out[1] + static_cast<long long>(row0) * p.ld + col0, p.ld, nrows, p.N - col0, lane);
         }
@@ -531,39 +520,36 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           float* dst = p.part + (static_cast<long long>(c.split * 2 + c.which) * p.M + row0) * p.part_ld;
 #pragma unroll 1
           for (int ch = 0; ch < 4; ++ch) {
-            uint32_t v[32];
-            tmem_ld_32x32b_x32(ta + colw + ch * 32, v);
+            uint32_t v[16];
+            tmem_ld_32x32b_x16(ta + colw + ch * 16, v);
             tmem_ld_wait();
             if (c.nkb == 0) {
 #pragma unroll
-              for (int j = 0; j < 32; ++j) v[j] = 0u;
+              for (int j = 0; j < 16; ++j) v[j] = 0u;
             }
             __syncwarp();
 #pragma unroll
-            for (int j = 0; j < 8; ++j)
+            for (int j = 0; j < 4; ++j)
               *piece(stage, lane, j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
             __syncwarp();
-            const int col = col0 + ch * 32;
+            const int col = col0 + ch * 16;
             tile_out_f32(stage, dst + col, p.part_ld, nrows, static_cast<int>(p.part_ld) - col, lane);
           }
         } else {
           __nv_bfloat16* dst = p.out[c.which] + static_cast<long long>(row0) * p.ld;
 #pragma unroll 1
           for (int c2 = 0; c2 < 2; ++c2) {
+            uint32_t v[16], w[16];
+            tmem_ld_32x32b_x16(ta + colw + c2 * 32, v);
+            tmem_ld_32x32b_x16(ta + colw + c2 * 32 + 16, w);
+            tmem_ld_wait();
             __syncwarp();
-#pragma unroll
-            for (int ch = 0; ch < 2; ++ch) {
-              uint32_t v[32];
-              tmem_ld_32x32b_x32(ta + colw + c2 * 64 + ch * 32, v);
-              tmem_ld_wait();
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                *piece(stage, lane, ch * 4 + j) =
-                    make_uint4(pack2(v[8 * j], v[8 * j + 1]), pack2(v[8 * j + 2], v[8 * j + 3]),
-                               pack2(v[8 * j + 4], v[8 * j + 5]), pack2(v[8 * j + 6], v[8 * j + 7]));
-            }
+            *piece(stage, lane, 0) = pack8(v, 0);
+            *piece(stage, lane, 1) = pack8(v, 8);
+            *piece(stage, lane, 2) = pack8(w, 0);
+            *piece(stage, lane, 3) = pack8(w, 8);
             __syncwarp();
-            const int col = col0 + c2 * 64;
+            const int col = col0 + c2 * 32;
             tile_out(stage, dst + col, p.ld, nrows, p.N - col, lane);
           }
         }
@@ -610,8 +596,10 @@ __global__ void __launch_bounds__(256) join_bias_kernel(const float* __restrict_
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int c = blockIdx.x * 32 + lane;
   float a = 0.f;
-  if (c < 2 * F)
+  if (c < 2 * F) {
+#pragma unroll 8
     for (int g = warp; g < groups; g += 8) a += part[static_cast<long long>(g) * 2 * F + c];
+  }
   acc[warp][lane] = a;
   __syncthreads();
   if (warp == 0 && c < 2 * F) {
@@ -905,15 +893,18 @@ std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_i
     PairParams p{};
     p.M = static_cast<int>(F), p.N = static_cast<int>(K0);
     p.tiles_m = ceil_div(F, 256), p.tiles_n = ceil_div(K0, 256), p.kb = ceil_div(T, 64);
-    // Parts of the reduction: the fewest steps of the slowest pair, counting a part's write and
-    // its share of the joining kernel as eight steps; at least eight steps to a part.
+    // Parts of the reduction, by their estimated time: the slowest pair's steps of 0.27 us (512 cycles of
+    // products), and for more than one part 3 us and the parts' way to memory and back at 5 TB/s.  At F = 1000,
+    // K = 384, T = 8192 four parts take 23 us against 43 us for one; at 4096, 1024, 16384 the parts' 268 MB would
+    // cost more than the idle pairs of one part's second wave.
     const int pairs = resident_pairs();
     const int64_t tiles = 2ll * p.tiles_m * p.tiles_n;
-    int64_t best = -1;
+    const double bytes = 2.0 * F * K0 * 8;
+    double best = 0;
     p.splits = 1;
     for (int s = 1; s <= 32 && (s == 1 || p.kb / s >= 8); ++s) {
-      const int64_t cost = ((tiles * s + pairs - 1) / pairs) * (ceil_div(p.kb, s) + (s > 1 ? 8 : 0));
-      if (best < 0 || cost < best) best = cost, p.splits = s;
+      const double cost = 0.27 * ((tiles * s + pairs - 1) / pairs) * ceil_div(p.kb, s) + (s > 1 ? 3 + s * bytes / 5e6 : 0);
+      if (s == 1 || cost < best) best = cost, p.splits = s;
     }
     p.out[0] = bf16_ptr(dwg), p.out[1] = bf16_ptr(dwu);
     p.ld = K0;
