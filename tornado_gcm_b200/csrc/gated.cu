@@ -894,9 +894,9 @@ std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_i
     p.M = static_cast<int>(F), p.N = static_cast<int>(K0);
     p.tiles_m = ceil_div(F, 256), p.tiles_n = ceil_div(K0, 256), p.kb = ceil_div(T, 64);
     // Parts of the reduction, by their estimated time: the slowest pair's steps of 0.27 us (512 cycles of
-    // products), and for more than one part 3 us and the parts' way to memory and back at 5 TB/s.  At F = 1000,
-    // K = 384, T = 8192 four parts take 23 us against 43 us for one; at 4096, 1024, 16384 the parts' 268 MB would
-    // cost more than the idle pairs of one part's second wave.
+    // products), and for more than one part 3 us and the parts' way to memory and back at 5 TB/s.  F = 1000,
+    // K = 384, T = 8192 gets four parts (20 us and 3 us to join them); 4096, 1024, 16384 one (204 us; four parts
+    // took 186 us and 27 us to join).
     const int pairs = resident_pairs();
     const int64_t tiles = 2ll * p.tiles_m * p.tiles_n;
     const double bytes = 2.0 * F * K0 * 8;

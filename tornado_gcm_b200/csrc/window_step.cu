@@ -8,12 +8,13 @@
 // of the slots does not matter to a softmax.
 //
 // Bound by reading the cache once: 2 D values for each slot and key head
-// against 4 D FLOP per query head.  A group of LPK lanes covers a slot's row
-// with one 16-byte vector each, so a warp reads 32 / LPK rows of K and of V
-// per load, kUnroll of them in flight; the query heads that share the key
-// head (up to kHeads) are all scored against the row while it is in
-// registers.  Each lane group keeps its own running maximum, sum and output
-// (fp32), rescaled once for kUnroll rows.  The slots of a sequence are split
+// against 4 D FLOP per query head; the query heads that share a key head are
+// scored together while its rows are on the SM.  bf16 rows go through warp matrix
+// instructions (step_mma_kernel); fp32 ones, and head sizes off 16, through
+// step_kernel: a group of LPK lanes covers a slot's row with one 16-byte vector
+// each, a warp reads 32 / LPK rows of K and of V per load, kUnroll of them in
+// flight, and each lane group keeps its own running maximum, sum and output,
+// rescaled once for kUnroll rows.  The slots of a sequence are split
 // over a cluster of up to 8 blocks, because batch x key heads alone leave SMs
 // idle; the blocks leave their statistics in shared memory and each combines
 // its part of the outputs through distributed shared memory: one launch, no
@@ -94,6 +95,261 @@ __device__ __forceinline__ float ld_peer(const float* p, uint32_t rank) {
   return v;
 }
 
+// Outputs of the cluster's blocks joined: statistics and unnormalised outputs of
+// every block lie in its shared memory, each block finishes its share of them.
+template <typename T>
+__device__ __forceinline__ void join_cluster(const StepParams& p, int b, int h0, int heads, uint32_t rank, int splits,
+                                             const float* blk_m, const float* blk_l, const float* blk_o, int o_ld) {
+  cluster_sync();
+  for (int i = rank * kStepThreads + threadIdx.x; i < heads * p.D; i += splits * kStepThreads) {
+    const int g = i / p.D, d = i - g * p.D;
+    float mb = -INFINITY;
+    for (int r = 0; r < splits; ++r) mb = fmaxf(mb, ld_peer(blk_m + g, r));
+    const float base = mb == -INFINITY ? 0.f : mb;
+    float a = 0.f, t = 0.f;
+    for (int r = 0; r < splits; ++r) {
+      const float f = exp2f(ld_peer(blk_m + g, r) - base);
+      t = fmaf(ld_peer(blk_l + g, r), f, t);
+      a = fmaf(ld_peer(blk_o + g * o_ld + d, r), f, a);
+    }
+    const float out = t == 0.f ? 0.f : a / t;
+    T* o = static_cast<T*>(p.o) + (static_cast<long long>(b) * p.H + h0 + g) * p.D + d;
+    if constexpr (std::is_same<T, float>::value)
+      *o = out;
+    else
+      *o = __float2bfloat16(out);
+  }
+  cluster_sync();  // nobody leaves while its shared memory is read
+}
+
+// What a block works on.
+struct StepShare {
+  int hk, hb, b, h0, heads, slot, s0, s1;
+};
+__device__ __forceinline__ StepShare step_share(const StepParams& p, uint32_t rank, int splits) {
+  StepShare w;
+  w.hk = blockIdx.y / p.head_blocks, w.hb = blockIdx.y % p.head_blocks, w.b = blockIdx.z;
+  const int group = p.H / p.Hk;
+  w.h0 = w.hk * group + w.hb * p.heads_per_block;
+  w.heads = min(p.heads_per_block, (w.hk + 1) * group - w.h0);
+  const int at = p.lengths[w.b];
+  const int seen = at < 0 ? 0 : (at < p.cap ? at + 1 : p.cap);
+  const int window = p.cap - p.sinks;
+  w.slot = at < 0 ? -1 : (at < p.cap ? at : p.sinks + (at - p.sinks) % window);
+  const int per = (seen + splits - 1) / splits;
+  w.s0 = min(seen, static_cast<int>(rank) * per), w.s1 = min(seen, w.s0 + per);
+  return w;
+}
+
+// The new token goes to its slot.  Whoever meets that slot reads the inputs
+// instead, so this write races with no read.
+template <typename T>
+__device__ __forceinline__ void put_token(const StepParams& p, const StepShare& w, const T* kn, const T* vn, T* kc,
+                                          T* vc) {
+  if (w.hb == 0 && w.slot >= w.s0 && w.slot < w.s1)
+    for (int d = threadIdx.x; d < p.D; d += kStepThreads) {
+      kc[w.slot * p.kc_ss + d] = kn[d];
+      vc[w.slot * p.vc_ss + d] = vn[d];
+    }
+}
+
+// ── bf16, D a multiple of 16: warp matrix instructions ─────────────────────
+// A warp takes 16 slots at a time: S (16 heads x 16 slots) = q K^T and
+// O (16 heads x D) += P V, up to 8 of the 16 head rows in use.  One token's few
+// query heads cannot fill a tcgen05 tile (128 rows), and the kernel is bound by
+// the cache's bytes; the warp instructions take a fifth of the issue slots that
+// fp32 arithmetic on the same rows took (256 sequences of up to 1464 slots,
+// 16 + 4 heads of 64: 113 us before).  Slots arrive by 16-byte asynchronous copies
+// into the warp's own ring, kStages groups deep; rows are padded by 16 bytes so
+// that the eight rows of a matrix load lie in different banks.  P enters the
+// second product as two bf16 terms (value and remainder): its rounding would
+// otherwise be as large as the output's own.
+constexpr int kStages = 4;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
+  const int n = on ? 16 : 0;  // 0: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(n) : "memory");
+}
+__device__ __forceinline__ void ldm_x4(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+__device__ __forceinline__ void ldm_x4_t(uint32_t (&r)[4], uint32_t addr) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+// C (16 x 8) += A (16 x 16) B (16 x 8); rows 8-15 of A are zero.
+__device__ __forceinline__ void mma_8rows(float (&c)[4], uint32_t a0, uint32_t a2, uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %5}, {%7, %8}, {%0, %1, %2, "
+      "%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a0), "r"(0u), "r"(a2), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t pack_pair(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <int ND>
+struct MmaStep {
+  static constexpr int kRow = ND * 32 + 16;            // bytes of a padded row
+  static constexpr int kGroup = 2 * 16 * kRow;         // K and V of 16 slots
+  static constexpr int kWarp = kStages * kGroup;
+  static constexpr int kOut = (kStepWarps + 1) * 8 * ND * 16 * 4;  // outputs of the warps and of the block, over the rings
+  static constexpr int kSmem = kStepWarps * kWarp > kOut ? kStepWarps * kWarp : kOut;
+};
+
+template <int ND>
+__global__ void __launch_bounds__(kStepThreads) step_mma_kernel(const __grid_constant__ StepParams p) {
+  using C = MmaStep<ND>;
+  using T = __nv_bfloat16;
+  constexpr int D = ND * 16;
+  extern __shared__ __align__(16) uint8_t ring[];
+  __shared__ float sm_m[kStepWarps][8], sm_l[kStepWarps][8], blk_m[8], blk_l[8];
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int g = lane >> 2, t = lane & 3;
+  const uint32_t rank = cluster_rank();
+  const int splits = gridDim.x;
+  const StepShare w = step_share(p, rank, splits);
+  const T* kn = static_cast<const T*>(p.k) + w.b * p.k_sb + w.hk * p.k_sh;
+  const T* vn = static_cast<const T*>(p.v) + w.b * p.v_sb + w.hk * p.v_sh;
+  T* kc = static_cast<T*>(p.kc) + w.b * p.kc_sb + w.hk * p.kc_sh;
+  T* vc = static_cast<T*>(p.vc) + w.b * p.vc_sb + w.hk * p.vc_sh;
+  put_token<T>(p, w, kn, vn, kc, vc);
+
+  const uint32_t my = smem_u32(ring) + warp * C::kWarp;
+  const int groups = w.s1 > w.s0 + warp * 16 ? (w.s1 - w.s0 - warp * 16 + kStepWarps * 16 - 1) / (kStepWarps * 16) : 0;
+  auto fetch = [&](int i) {  // group i of this warp; an empty commit behind the last one keeps the count
+    if (i < groups) {
+      const int j0 = w.s0 + (warp + i * kStepWarps) * 16;
+      const uint32_t dst = my + (i % kStages) * C::kGroup;
+#pragma unroll
+      for (int e = lane; e < 16 * 2 * ND; e += 32) {
+        const int r = e / (2 * ND), c = e % (2 * ND), j = j0 + r;
+        const bool on = j < w.s1;
+        const int js = on ? j : w.s0;
+        const T* ks = js == w.slot ? kn : kc + js * p.kc_ss;
+        const T* vs = js == w.slot ? vn : vc + js * p.vc_ss;
+        cp_async16(dst + r * C::kRow + c * 16, ks + c * 8, on);
+        cp_async16(dst + 16 * C::kRow + r * C::kRow + c * 16, vs + c * 8, on);
+      }
+    }
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) fetch(i);
+
+  uint32_t qa[ND][2];
+  {
+    const T* qr = static_cast<const T*>(p.q) + w.b * p.q_sb + (w.h0 + (g < w.heads ? g : 0)) * p.q_sh;
+#pragma unroll
+    for (int s = 0; s < ND; ++s)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        qa[s][u] = g < w.heads ? *reinterpret_cast<const uint32_t*>(qr + s * 16 + u * 8 + 2 * t) : 0u;
+  }
+  const float sc = p.scale * kLog2e;
+  float o[2 * ND][4];
+#pragma unroll
+  for (int i = 0; i < 2 * ND; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+  float m = -INFINITY, l = 0.f;  // of head g; l of this lane's slots
+  // Lane's row and column of a matrix load: K's four matrices are (slots 0-7, d 0-7), (0-7, 8-15), (8-15, 0-7),
+  // (8-15, 8-15); V's, transposed on the way, (slots 0-7, d 0-7), (8-15, 0-7), (0-7, 8-15), (8-15, 8-15).
+  const uint32_t k_at = ((lane & 7) + ((lane >> 4) << 3)) * C::kRow + ((lane >> 3) & 1) * 16;
+  const uint32_t v_at = 16 * C::kRow + ((lane & 7) + (((lane >> 3) & 1) << 3)) * C::kRow + (lane >> 4) * 16;
+
+  for (int i = 0; i < groups; ++i) {
+    asm volatile("cp.async.wait_group %0;" ::"n"(kStages - 2) : "memory");
+    __syncwarp();  // group i of every lane has landed, and group i - 1 has been read by all
+    fetch(i + kStages - 1);
+    const uint32_t at = my + (i % kStages) * C::kGroup;
+    float s0[4] = {0.f, 0.f, 0.f, 0.f}, s1[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < ND; ++s) {
+      uint32_t k[4];
+      ldm_x4(k, at + k_at + s * 32);
+      mma_8rows(s0, qa[s][0], qa[s][1], k[0], k[1]);
+      mma_8rows(s1, qa[s][0], qa[s][1], k[2], k[3]);
+    }
+    const int j = w.s0 + (warp + i * kStepWarps) * 16 + 2 * t;
+    float z[4] = {s0[0] * sc, s0[1] * sc, s1[0] * sc, s1[1] * sc};
+    if (j + 10 > w.s1) {  // the last group
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j + (e >> 1) * 8 + (e & 1) >= w.s1) z[e] = -INFINITY;
+    }
+    float mx = fmaxf(fmaxf(z[0], z[1]), fmaxf(z[2], z[3]));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
+    mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
+    if (__any_sync(0xffffffffu, mx > m)) {
+      const float mn = fmaxf(m, mx);
+      const float f = mn == -INFINITY ? 1.f : exp2f(m - mn);
+      m = mn;
+      l *= f;
+#pragma unroll
+      for (int n = 0; n < 2 * ND; ++n) {
+        o[n][0] *= f;
+        o[n][1] *= f;
+      }
+    }
+    const float base = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) z[e] = exp2f(z[e] - base);
+    l += (z[0] + z[1]) + (z[2] + z[3]);
+    const uint32_t p0 = pack_pair(z[0], z[1]), p2 = pack_pair(z[2], z[3]);
+    const uint32_t r0 = pack_pair(z[0] - __uint_as_float(p0 << 16), z[1] - __uint_as_float(p0 & 0xffff0000u));
+    const uint32_t r2 = pack_pair(z[2] - __uint_as_float(p2 << 16), z[3] - __uint_as_float(p2 & 0xffff0000u));
+#pragma unroll
+    for (int s = 0; s < ND; ++s) {
+      uint32_t v[4];
+      ldm_x4_t(v, at + v_at + s * 32);
+      mma_8rows(o[2 * s], p0, p2, v[0], v[1]);
+      mma_8rows(o[2 * s], r0, r2, v[0], v[1]);
+      mma_8rows(o[2 * s + 1], p0, p2, v[2], v[3]);
+      mma_8rows(o[2 * s + 1], r0, r2, v[2], v[3]);
+    }
+  }
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  l += __shfl_xor_sync(0xffffffffu, l, 1);
+  l += __shfl_xor_sync(0xffffffffu, l, 2);
+  if (t == 0) {
+    sm_m[warp][g] = m;
+    sm_l[warp][g] = l;
+  }
+  __syncthreads();  // statistics are there, and the rings are free
+  float mb = -INFINITY;
+#pragma unroll
+  for (int v = 0; v < kStepWarps; ++v) mb = fmaxf(mb, sm_m[v][g]);
+  const float base = mb == -INFINITY ? 0.f : mb;
+  const float f = exp2f(m - base);
+  float* outs = reinterpret_cast<float*>(ring);  // [warp][head][D], then the block's [head][D]
+#pragma unroll
+  for (int n = 0; n < 2 * ND; ++n)
+    *reinterpret_cast<float2*>(outs + (warp * 8 + g) * D + n * 8 + 2 * t) = make_float2(o[n][0] * f, o[n][1] * f);
+  if (warp == 0 && t == 0) {
+    float lb = 0.f;
+#pragma unroll
+    for (int v = 0; v < kStepWarps; ++v) lb += sm_l[v][g] * exp2f(sm_m[v][g] - base);
+    blk_m[g] = mb;
+    blk_l[g] = lb;
+  }
+  __syncthreads();
+  float* blk_o = outs + kStepWarps * 8 * D;
+  for (int i = threadIdx.x; i < 8 * D; i += kStepThreads) {
+    float a = 0.f;
+#pragma unroll
+    for (int v = 0; v < kStepWarps; ++v) a += outs[v * 8 * D + i];
+    blk_o[i] = a;
+  }
+  join_cluster<T>(p, w.b, w.h0, w.heads, rank, splits, blk_m, blk_l, blk_o, D);
+}
+
+// ── any type and head size: fp32 arithmetic ────────────────────────────────
 template <typename T, int LPK, int G>
 __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constant__ StepParams p) {
   constexpr int V = 16 / sizeof(T);
@@ -110,28 +366,13 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
   const bool live = d0 < p.D;
   const uint32_t rank = cluster_rank();
   const int splits = gridDim.x;              // the cluster spans the grid's x
-  const int hk = blockIdx.y / p.head_blocks, hb = blockIdx.y % p.head_blocks, b = blockIdx.z;
-  const int group = p.H / p.Hk;
-  const int h0 = hk * group + hb * p.heads_per_block;
-  const int heads = min(p.heads_per_block, (hk + 1) * group - h0);
-  const int at = p.lengths[b];
-  const int seen = at < 0 ? 0 : (at < p.cap ? at + 1 : p.cap);
-  const int window = p.cap - p.sinks;
-  const int slot = at < 0 ? -1 : (at < p.cap ? at : p.sinks + (at - p.sinks) % window);
-  const int per = (seen + splits - 1) / splits;
-  const int s0 = min(seen, static_cast<int>(rank) * per), s1 = min(seen, s0 + per);
-
+  const StepShare w = step_share(p, rank, splits);
+  const int hk = w.hk, b = w.b, h0 = w.h0, heads = w.heads, slot = w.slot, s0 = w.s0, s1 = w.s1;
   const T* kn = static_cast<const T*>(p.k) + b * p.k_sb + hk * p.k_sh;
   const T* vn = static_cast<const T*>(p.v) + b * p.v_sb + hk * p.v_sh;
   T* kc = static_cast<T*>(p.kc) + b * p.kc_sb + hk * p.kc_sh;
   T* vc = static_cast<T*>(p.vc) + b * p.vc_sb + hk * p.vc_sh;
-  // The new token is read from the inputs by whoever meets its slot, so the
-  // write below races with no read.
-  if (hb == 0 && slot >= s0 && slot < s1)
-    for (int d = threadIdx.x; d < p.D; d += kStepThreads) {
-      kc[slot * p.kc_ss + d] = kn[d];
-      vc[slot * p.vc_ss + d] = vn[d];
-    }
+  put_token<T>(p, w, kn, vn, kc, vc);
 
   float q[G][V], acc[G][V], m[G], z[G];
 #pragma unroll
@@ -235,34 +476,15 @@ __global__ void __launch_bounds__(kStepThreads) step_kernel(const __grid_constan
     for (int w = 0; w < kStepWarps; ++w) a += sm_acc[w][g][d];
     blk_o[g][d] = a;
   }
-  cluster_sync();
-  // cluster: outputs i = rank, rank + splits, ... of this block's heads
-  for (int i = rank * kStepThreads + threadIdx.x; i < heads * p.D; i += splits * kStepThreads) {
-    const int g = i / p.D, d = i - g * p.D;
-    float mb = -INFINITY;
-    for (int r = 0; r < splits; ++r) mb = fmaxf(mb, ld_peer(&blk_m[g], r));
-    const float base = mb == -INFINITY ? 0.f : mb;
-    float a = 0.f, t = 0.f;
-    for (int r = 0; r < splits; ++r) {
-      const float f = exp2f(ld_peer(&blk_m[g], r) - base);
-      t = fmaf(ld_peer(&blk_l[g], r), f, t);
-      a = fmaf(ld_peer(&blk_o[g][d], r), f, a);
-    }
-    const float out = t == 0.f ? 0.f : a / t;
-    T* o = static_cast<T*>(p.o) + (static_cast<long long>(b) * p.H + h0 + g) * p.D + d;
-    if constexpr (std::is_same<T, float>::value)
-      *o = out;
-    else
-      *o = __float2bfloat16(out);
-  }
-  cluster_sync();  // nobody leaves while its shared memory is read
+  join_cluster<T>(p, b, h0, heads, rank, splits, blk_m, blk_l, &blk_o[0][0], DP);
 }
 
-template <typename T, int LPK, int G>
-void launch_step(const StepParams& p, int splits, int B, cudaStream_t st) {
+template <typename K>
+void launch_cluster(K kern, const StepParams& p, int splits, int B, size_t smem, cudaStream_t st) {
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(splits, p.Hk * p.head_blocks, B);
   cfg.blockDim = dim3(kStepThreads);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -271,7 +493,25 @@ void launch_step(const StepParams& p, int splits, int B, cudaStream_t st) {
   attr[0].val.clusterDim.z = 1;
   cfg.attrs = attr;
   cfg.numAttrs = 1;
-  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, step_kernel<T, LPK, G>, p));
+  C10_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kern, p));
+}
+
+template <typename T, int LPK, int G>
+void launch_step(const StepParams& p, int splits, int B, cudaStream_t st) {
+  launch_cluster(step_kernel<T, LPK, G>, p, splits, B, 0, st);
+}
+
+template <int ND>
+void launch_mma(const StepParams& p, int splits, int B, cudaStream_t st) {
+  static bool set[64] = {false};
+  int dev = 0;
+  C10_CUDA_CHECK(cudaGetDevice(&dev));
+  if (dev >= 64 || !set[dev]) {
+    C10_CUDA_CHECK(cudaFuncSetAttribute(step_mma_kernel<ND>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                        MmaStep<ND>::kSmem));
+    if (dev < 64) set[dev] = true;
+  }
+  launch_cluster(step_mma_kernel<ND>, p, splits, B, MmaStep<ND>::kSmem, st);
 }
 
 template <typename T, int LPK>
@@ -350,19 +590,35 @@ at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const
   p.cap = static_cast<int>(cap), p.sinks = static_cast<int>(sinks);
   p.scale = static_cast<float>(scale);
   const int64_t group = H / Hk;
-  p.heads_per_block = group >= 4 ? 4 : static_cast<int>(group == 3 ? 4 : group);
-  p.head_blocks = static_cast<int>((group + p.heads_per_block - 1) / p.heads_per_block);
   p.vec = D % (16 / q.element_size()) == 0 && rows16(q) && rows16(k) && rows16(v) && rows16(k_cache) && rows16(v_cache);
-  // Enough blocks for two waves of resident blocks, none with less than 32 slots.
+  // Rows of whole 32-byte steps of bf16 go to the matrix instructions, the rest to fp32 arithmetic.
+  const bool mma = q.scalar_type() == at::kBFloat16 && p.vec && D % 16 == 0;
+  const int64_t most = mma ? 8 : 4;
+  p.heads_per_block = static_cast<int>(mma ? std::min(group, most) : (group >= 3 ? 4 : group));
+  p.head_blocks = static_cast<int>((group + p.heads_per_block - 1) / p.heads_per_block);
+  // Enough blocks to fill the SMs a few times over, none with less than 32 slots (64 for the matrix kernel:
+  // 16 to a warp).
   const int64_t units = B * Hk * p.head_blocks;
   int splits = 1;
-  while (splits < kMaxSplits && units * splits < 148 * 8 && cap / (2 * splits) >= 32) splits *= 2;
+  while (splits < kMaxSplits && units * splits < 148 * 8 && cap / (2 * splits) >= (mma ? 64 : 32)) splits *= 2;
   auto st = at::cuda::getCurrentCUDAStream();
   TORCH_CHECK(p.Hk * static_cast<int64_t>(p.head_blocks) <= 65535, "window_attention_step: too many heads");
-  if (q.scalar_type() == at::kBFloat16)
-    by_lanes<__nv_bfloat16>(p, splits, static_cast<int>(B), st);
+  const int nb = static_cast<int>(B);
+  if (mma)
+    switch (D / 16) {
+      case 1: launch_mma<1>(p, splits, nb, st); break;
+      case 2: launch_mma<2>(p, splits, nb, st); break;
+      case 3: launch_mma<3>(p, splits, nb, st); break;
+      case 4: launch_mma<4>(p, splits, nb, st); break;
+      case 5: launch_mma<5>(p, splits, nb, st); break;
+      case 6: launch_mma<6>(p, splits, nb, st); break;
+      case 7: launch_mma<7>(p, splits, nb, st); break;
+      default: launch_mma<8>(p, splits, nb, st); break;
+    }
+  else if (q.scalar_type() == at::kBFloat16)
+    by_lanes<__nv_bfloat16>(p, splits, nb, st);
   else
-    by_lanes<float>(p, splits, static_cast<int>(B), st);
+    by_lanes<float>(p, splits, nb, st);
   return o;
 }
 
