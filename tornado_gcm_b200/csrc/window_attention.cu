@@ -42,6 +42,7 @@ namespace {
 
 constexpr int kRows = 32;                // rows of a block
 constexpr int kTile = 32;                // staged rows of the other side
+constexpr int kStep = 4;                 // of them in work at once
 constexpr int kWinThreads = 4 * kRows;
 
 template <typename T>
@@ -87,20 +88,26 @@ __device__ __forceinline__ void stage_rows(float* s, const T* g, long long strid
   }
 }
 
-template <int N>
-__device__ __forceinline__ float dot_share(const float (&a)[N], const float* row, int part) {
-  float s = 0.f;
+// Products with kStep staged rows at once: one row's chain of FMAs and shuffles
+// is latency from end to end.
+template <int N, int DP>
+__device__ __forceinline__ void dot_rows(const float (&a)[N], const float* rows, int part, float (&s)[kStep]) {
 #pragma unroll
-  for (int i = 0; i < N; i += 4) {
-    const float4 b = *reinterpret_cast<const float4*>(row + 4 * (part + i));
-    s = fmaf(a[i], b.x, s);
-    s = fmaf(a[i + 1], b.y, s);
-    s = fmaf(a[i + 2], b.z, s);
-    s = fmaf(a[i + 3], b.w, s);
-  }
-  s += __shfl_xor_sync(0xffffffffu, s, 1);
-  s += __shfl_xor_sync(0xffffffffu, s, 2);
-  return s;
+  for (int u = 0; u < kStep; ++u) s[u] = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; i += 4)
+#pragma unroll
+    for (int u = 0; u < kStep; ++u) {
+      const float4 b = *reinterpret_cast<const float4*>(rows + u * DP + 4 * (part + i));
+      s[u] = fmaf(a[i], b.x, s[u]);
+      s[u] = fmaf(a[i + 1], b.y, s[u]);
+      s[u] = fmaf(a[i + 2], b.z, s[u]);
+      s[u] = fmaf(a[i + 3], b.w, s[u]);
+    }
+#pragma unroll
+  for (int u = 0; u < kStep; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], 1);
+#pragma unroll
+  for (int u = 0; u < kStep; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], 2);
 }
 template <int N>
 __device__ __forceinline__ void axpy_share(float (&a)[N], float f, const float* row, int part) {
@@ -152,10 +159,15 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(const WinParams p)
       stage_rows<T, DP>(vs, vb, p.v_ss, j0, end, p.D);
       __syncthreads();
       const int n = min(kTile, end - j0);
-      for (int t = 0; t < n; ++t) {
-        const float z = dot_share<N>(q, ks + t * DP, part);
-        if (!win_sees(p, L, i, j0 + t)) continue;  // the four threads of a row agree
-        const float mn = fmaxf(m, z);
+      for (int t = 0; t < n; t += kStep) {
+        float z[kStep];
+        dot_rows<N, DP>(q, ks + t * DP, part, z);
+        float mn = m;
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {  // the four threads of a row agree
+          z[u] = t + u < n && win_sees(p, L, i, j0 + t + u) ? z[u] : -INFINITY;
+          mn = fmaxf(mn, z[u]);
+        }
         if (mn > m) {
           const float c = exp2f(m - mn);  // 0 for the row's first key
           l *= c;
@@ -163,11 +175,14 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(const WinParams p)
           for (int e = 0; e < N; ++e) acc[e] *= c;
           m = mn;
         }
-        const float w = z == -INFINITY ? 0.f : exp2f(z - m);  // m may be -inf still
-        l += w;
-        axpy_share<N>(acc, w, vs + t * DP, part);
+#pragma unroll
+        for (int u = 0; u < kStep; ++u) {
+          if (z[u] == -INFINITY) continue;  // also: a value behind the end may be NaN
+          const float w = exp2f(z[u] - m);
+          l += w;
+          axpy_share<N>(acc, w, vs + (t + u) * DP, part);
+        }
       }
-      __syncwarp();
     }
   }
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
@@ -217,13 +232,15 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(const WinParams p) 
       stage_rows<T, DP>(vs, vb, p.v_ss, j0, end, p.D);
       __syncthreads();
       const int n = min(kTile, end - j0);
-      for (int t = 0; t < n; ++t) {
-        const float z = dot_share<N>(q, ks + t * DP, part);
-        const float dp = dot_share<N>(g, vs + t * DP, part);
-        if (!win_sees(p, L, i, j0 + t)) continue;
-        axpy_share<N>(acc, exp2f(z - lse) * (dp - delta), ks + t * DP, part);
+      for (int t = 0; t < n; t += kStep) {
+        float z[kStep], dp[kStep];
+        dot_rows<N, DP>(q, ks + t * DP, part, z);
+        dot_rows<N, DP>(g, vs + t * DP, part, dp);
+#pragma unroll
+        for (int u = 0; u < kStep; ++u)
+          if (t + u < n && win_sees(p, L, i, j0 + t + u))
+            axpy_share<N>(acc, exp2f(z[u] - lse) * (dp[u] - delta), ks + (t + u) * DP, part);
       }
-      __syncwarp();
     }
   }
   store_share<T, N>(static_cast<T*>(p.dq) + orow, p.D, part, on, acc, p.scale);
@@ -269,15 +286,18 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(const WinParams p)
         ds[threadIdx.x] = p.delta[srow + i0 + threadIdx.x];
       }
       __syncthreads();
-      for (int t = 0; t < n; ++t) {
-        const float z = dot_share<N>(k, qs + t * DP, part);
-        const float dp = dot_share<N>(v, gs + t * DP, part);
-        if (!win_sees(p, L, i0 + t, j)) continue;
-        const float w = exp2f(z - ls[t]);
-        axpy_share<N>(dv, w, gs + t * DP, part);
-        axpy_share<N>(dk, w * (dp - ds[t]), qs + t * DP, part);
+      for (int t = 0; t < n; t += kStep) {
+        float z[kStep], dp[kStep];
+        dot_rows<N, DP>(k, qs + t * DP, part, z);
+        dot_rows<N, DP>(v, gs + t * DP, part, dp);
+#pragma unroll
+        for (int u = 0; u < kStep; ++u)
+          if (t + u < n && win_sees(p, L, i0 + t + u, j)) {
+            const float w = exp2f(z[u] - ls[t + u]);
+            axpy_share<N>(dv, w, gs + (t + u) * DP, part);
+            axpy_share<N>(dk, w * (dp[u] - ds[t + u]), qs + (t + u) * DP, part);
+          }
       }
-      __syncwarp();
     }
   }
   const bool in = j < p.S;

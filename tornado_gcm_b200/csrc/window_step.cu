@@ -160,11 +160,12 @@ __device__ __forceinline__ void put_token(const StepParams& p, const StepShare& 
 // the cache's bytes; the warp instructions take a fifth of the issue slots that
 // fp32 arithmetic on the same rows took (256 sequences of up to 1464 slots,
 // 16 + 4 heads of 64: 113 us before).  Slots arrive by 16-byte asynchronous copies
-// into the warp's own ring, kStages groups deep; rows are padded by 16 bytes so
+// into the warp's own ring of kStages groups (two: more blocks to an SM do better than
+// deeper rings, 59 us against 62 with three and 71 with four); rows are padded by 16 bytes so
 // that the eight rows of a matrix load lie in different banks.  P enters the
 // second product as two bf16 terms (value and remainder): its rounding would
 // otherwise be as large as the output's own.
-constexpr int kStages = 4;
+constexpr int kStages = 2;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
   const int n = on ? 16 : 0;  // 0: zeros
@@ -596,8 +597,8 @@ at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const
   const int64_t most = mma ? 8 : 4;
   p.heads_per_block = static_cast<int>(mma ? std::min(group, most) : (group >= 3 ? 4 : group));
   p.head_blocks = static_cast<int>((group + p.heads_per_block - 1) / p.heads_per_block);
-  // Enough blocks to fill the SMs a few times over, none with less than 32 slots (64 for the matrix kernel:
-  // 16 to a warp).
+  // Enough blocks to fill the SMs with the last of them short, none with less than 32 slots (64 for the matrix
+  // kernel: 16 to a warp).  1024 units of up to 1464 slots: 64 us whole, 59 us in halves, more in quarters.
   const int64_t units = B * Hk * p.head_blocks;
   int splits = 1;
   while (splits < kMaxSplits && units * splits < 148 * 8 && cap / (2 * splits) >= (mma ? 64 : 32)) splits *= 2;

@@ -30,7 +30,6 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
         return torch.zeros(())
     if not grads[0].is_cuda:
         return _plain_norm(grads)
-    grads = [g if g.is_contiguous() else g.contiguous() for g in grads]
     return _ext.require("gradient norm").grad_norm.default(grads)
 
 
@@ -41,38 +40,28 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
     ``out`` has one dense tensor for each gradient, of its shape; bf16 gradients may have fp32 outputs and
     the other way round.  A norm that is infinite or NaN scales as the formula says (to zero or NaN).
     """
-    grads = list(grads)
-    if out is None:
-        grads = [g for g in grads if g is not None]
-        out = grads
-    if any(g is None for g in grads):
-        raise ValueError("clip_grad_norm: with `out` every gradient must be there")
-    out = list(out)
-    if len(out) != len(grads):
-        raise ValueError(f"clip_grad_norm: {len(out)} outputs for {len(grads)} gradients")
     if not float(max_norm) >= 0.0:
         raise ValueError(f"clip_grad_norm: max_norm must not be negative, got {max_norm}")
+    if out is None:
+        grads = out_list = [g for g in grads if g is not None]
+    else:
+        grads, out_list = list(grads), list(out)
+        if len(out_list) != len(grads):
+            raise ValueError(f"clip_grad_norm: {len(out_list)} outputs for {len(grads)} gradients")
+        if any(g is None for g in grads):
+            raise ValueError("clip_grad_norm: with `out` every gradient must be there")
     if not grads:
         return torch.zeros(())
+    if grads[0].is_cuda:
+        # the operator changes its arguments in place below autograd's sight, as an optimizer does
+        return _ext.require("gradient clipping").clip_grad_norm.default(grads, [] if out is None else out_list,
+                                                                        float(max_norm))
     with torch.no_grad():
-        if not grads[0].is_cuda:
-            for g, o in zip(grads, out):
-                if g.shape != o.shape:
-                    raise ValueError("clip_grad_norm: an output has another shape than its gradient")
-            norm = _plain_norm(grads)
-            coef = torch.clamp(float(max_norm) / (norm + 1e-6), max=1.0)
-            for g, o in zip(grads, out):
-                o.copy_(g * coef.to(g.dtype) if g.dtype == torch.float64 else g.float() * coef)
-            return norm
-        ops = _ext.require("gradient clipping")
-        dense = [g.is_contiguous() and o.is_contiguous() for g, o in zip(grads, out)]
-        if all(dense):
-            return ops.clip_grad_norm.default(grads, out, float(max_norm))
-        # strided gradients or outputs pass through contiguous copies
-        g2 = [g.contiguous() for g in grads]
-        o2 = [o if d else torch.empty_like(g, dtype=o.dtype) for g, o, d in zip(g2, out, dense)]
-        norm = ops.clip_grad_norm.default(g2, o2, float(max_norm))
-        for o, t, d in zip(out, o2, dense):
-            if not d:
-                o.copy_(t)
+        for g, o in zip(grads, out_list):
+            if g.shape != o.shape:
+                raise ValueError("clip_grad_norm: an output has another shape than its gradient")
+        norm = _plain_norm(grads)
+        coef = torch.clamp(float(max_norm) / (norm + 1e-6), max=1.0)
+        for g, o in zip(grads, out_list):
+            o.copy_(g * coef.to(g.dtype) if g.dtype == torch.float64 else g.float() * coef)
         return norm
