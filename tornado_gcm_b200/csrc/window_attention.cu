@@ -78,13 +78,27 @@ __device__ __forceinline__ void store_share(T* row, int D, int part, bool on, co
   }
 }
 
-// Rows [j0, j0 + kTile) below `end` into shared memory, zero elsewhere.
+// Rows [j0, j0 + kTile) below `end` of two tensors into shared memory, zero
+// elsewhere; all of a thread's loads are under way before the first is stored.
 template <typename T, int DP>
-__device__ __forceinline__ void stage_rows(float* s, const T* g, long long stride, int j0, int end, int D) {
-  for (int e = threadIdx.x; e < kTile * DP; e += kWinThreads) {
-    const int r = e / DP, d = e % DP;
-    const int j = j0 + r;
-    s[e] = (j < end && d < D) ? ldw(g + j * stride + d) : 0.f;
+__device__ __forceinline__ void stage_rows(float* sa, const T* a, long long a_stride, float* sb, const T* b,
+                                           long long b_stride, int j0, int end, int D, int thread) {
+  constexpr int kEach = kTile * DP / kWinThreads, kOnce = kEach < 16 ? kEach : 16;
+#pragma unroll
+  for (int e0 = 0; e0 < kEach; e0 += kOnce) {
+    float va[kOnce], vb[kOnce];
+#pragma unroll
+    for (int e = 0; e < kOnce; ++e) {
+      const int at = (e0 + e) * kWinThreads + thread, j = j0 + at / DP, d = at % DP;
+      const bool on = j < end && d < D;
+      va[e] = on ? ldw(a + j * a_stride + d) : 0.f;
+      vb[e] = on ? ldw(b + j * b_stride + d) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < kOnce; ++e) {
+      sa[(e0 + e) * kWinThreads + thread] = va[e];
+      sb[(e0 + e) * kWinThreads + thread] = vb[e];
+    }
   }
 }
 
@@ -121,20 +135,61 @@ __device__ __forceinline__ void axpy_share(float (&a)[N], float f, const float* 
   }
 }
 
-// Keys in sight of some query of [i0, i0 + n): sinks [0, *se) and window [*lo, *hi).
-__device__ __forceinline__ void key_ranges(const WinParams& p, int L, int i0, int n, int* se, int* lo, int* hi) {
-  const int last = min(i0 + n, p.S) - 1;
-  *lo = max(0, i0 - (p.window - 1));
-  *hi = min(L, p.causal ? last + 1 : max(last + p.window, p.sinks));
-  *se = min(min(p.sinks, *lo), L);
+// Threads of a block beside its rows: kGroups groups of 128 take the staged tiles
+// in turn and join their sums at the end, in order.  (One group alone leaves most
+// of a short sequence's time to the latency of tile after tile, and the keys of a
+// sink meet every query of the sequence.)
+template <int DP>
+struct RowShape {
+  static constexpr int kGroups = DP <= 32 ? 4 : 2;
+  static constexpr int kTileBytes = 2 * kTile * DP * 4 + 2 * kTile * 4;
+  static constexpr int kSmem = kGroups * kTileBytes;
+};
+
+__device__ __forceinline__ void group_sync(int gid) { asm volatile("bar.sync %0, 128;" ::"r"(gid + 1) : "memory"); }
+
+// Adds up the groups' values of one array in group 0; every thread of the block calls it.
+template <int N, int GROUPS>
+__device__ __forceinline__ void join_groups(float (&acc)[N], float* smem, int gid, int thread) {
+  __syncthreads();
+  if (gid > 0) {
+#pragma unroll
+    for (int e = 0; e < N; ++e) smem[((gid - 1) * N + e) * kWinThreads + thread] = acc[e];
+  }
+  __syncthreads();
+  if (gid == 0) {
+#pragma unroll
+    for (int o = 1; o < GROUPS; ++o)
+#pragma unroll
+      for (int e = 0; e < N; ++e) acc[e] += smem[((o - 1) * N + e) * kWinThreads + thread];
+  }
 }
 
+// Keys in sight of some query of [i0, i0 + kRows): the sinks below the window's
+// first key, [0, sinks), then [lo, hi), in tiles.
+struct KeyRun {
+  int sinks, lo, hi, sink_tiles, tiles;
+  __device__ __forceinline__ KeyRun(const WinParams& p, int L, int i0) {
+    const int last = min(i0 + kRows, p.S) - 1;
+    lo = max(0, i0 - (p.window - 1));
+    hi = min(L, p.causal ? last + 1 : max(last + p.window, p.sinks));
+    sinks = min(min(p.sinks, lo), L);
+    sink_tiles = (sinks + kTile - 1) / kTile;
+    tiles = sink_tiles + (hi > lo ? (hi - lo + kTile - 1) / kTile : 0);
+  }
+  __device__ __forceinline__ int first(int t) const { return t < sink_tiles ? t * kTile : lo + (t - sink_tiles) * kTile; }
+  __device__ __forceinline__ int end(int t) const { return t < sink_tiles ? sinks : hi; }
+};
+
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(const WinParams p) {
+__global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_fwd_kernel(const WinParams p) {
+  using C = RowShape<DP>;
   constexpr int N = DP / 4;
-  __shared__ __align__(16) float ks[kTile * DP];
-  __shared__ __align__(16) float vs[kTile * DP];
-  const int part = threadIdx.x & 3, r = threadIdx.x >> 2;
+  extern __shared__ __align__(16) float row_smem[];
+  const int gid = threadIdx.x / kWinThreads, thread = threadIdx.x % kWinThreads;
+  float* ks = row_smem + gid * (C::kTileBytes / 4);
+  float* vs = ks + kTile * DP;
+  const int part = thread & 3, r = thread >> 2;
   const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
   const int i0 = blockIdx.x * kRows, i = i0 + r;
   const bool on = i < p.S;
@@ -149,56 +204,69 @@ __global__ void __launch_bounds__(kWinThreads) win_fwd_kernel(const WinParams p)
     acc[e] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
-  int se, lo, hi;
-  key_ranges(p, L, i0, kRows, &se, &lo, &hi);
-  for (int phase = 0; phase < 2; ++phase) {
-    const int end = phase ? hi : se;
-    for (int j0 = phase ? lo : 0; j0 < end; j0 += kTile) {
-      __syncthreads();
-      stage_rows<T, DP>(ks, kb, p.k_ss, j0, end, p.D);
-      stage_rows<T, DP>(vs, vb, p.v_ss, j0, end, p.D);
-      __syncthreads();
-      const int n = min(kTile, end - j0);
-      for (int t = 0; t < n; t += kStep) {
-        float z[kStep];
-        dot_rows<N, DP>(q, ks + t * DP, part, z);
-        float mn = m;
+  const KeyRun run(p, L, i0);
+  for (int it = gid; it < run.tiles; it += C::kGroups) {
+    const int j0 = run.first(it), end = run.end(it), n = min(kTile, end - j0);
+    group_sync(gid);
+    stage_rows<T, DP>(ks, kb, p.k_ss, vs, vb, p.v_ss, j0, end, p.D, thread);
+    group_sync(gid);
+    for (int t = 0; t < n; t += kStep) {
+      float z[kStep];
+      dot_rows<N, DP>(q, ks + t * DP, part, z);
+      float mn = m;
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) {  // the four threads of a row agree
-          z[u] = t + u < n && win_sees(p, L, i, j0 + t + u) ? z[u] : -INFINITY;
-          mn = fmaxf(mn, z[u]);
-        }
-        if (mn > m) {
-          const float c = exp2f(m - mn);  // 0 for the row's first key
-          l *= c;
+      for (int u = 0; u < kStep; ++u) {  // the four threads of a row agree
+        z[u] = t + u < n && win_sees(p, L, i, j0 + t + u) ? z[u] : -INFINITY;
+        mn = fmaxf(mn, z[u]);
+      }
+      if (mn > m) {
+        const float c = exp2f(m - mn);  // 0 for the row's first key
+        l *= c;
 #pragma unroll
-          for (int e = 0; e < N; ++e) acc[e] *= c;
-          m = mn;
-        }
+        for (int e = 0; e < N; ++e) acc[e] *= c;
+        m = mn;
+      }
 #pragma unroll
-        for (int u = 0; u < kStep; ++u) {
-          if (z[u] == -INFINITY) continue;  // also: a value behind the end may be NaN
-          const float w = exp2f(z[u] - m);
-          l += w;
-          axpy_share<N>(acc, w, vs + (t + u) * DP, part);
-        }
+      for (int u = 0; u < kStep; ++u) {
+        if (z[u] == -INFINITY) continue;  // also: a value behind the end may be NaN
+        const float w = exp2f(z[u] - m);
+        l += w;
+        axpy_share<N>(acc, w, vs + (t + u) * DP, part);
       }
     }
   }
+  // the groups' sums on one scale
+  __syncthreads();
+  row_smem[threadIdx.x] = m;
+  __syncthreads();
+  float mb = m;
+#pragma unroll
+  for (int o = 0; o < C::kGroups; ++o) mb = fmaxf(mb, row_smem[o * kWinThreads + thread]);
+  const float f = m == -INFINITY ? 0.f : exp2f(m - mb);
+  float ls[1] = {l * f};
+#pragma unroll
+  for (int e = 0; e < N; ++e) acc[e] *= f;
+  join_groups<1, C::kGroups>(ls, row_smem, gid, thread);
+  join_groups<N, C::kGroups>(acc, row_smem, gid, thread);
+  if (gid > 0) return;
+  l = ls[0];
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
   store_share<T, N>(static_cast<T*>(p.o) + ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D, p.D, part, on, acc,
                     inv);
   if (on && part == 0)
-    p.lse[(static_cast<long long>(b) * p.H + h) * p.S + i] = l == 0.f ? INFINITY : m + log2f(l);
+    p.lse[(static_cast<long long>(b) * p.H + h) * p.S + i] = l == 0.f ? INFINITY : mb + log2f(l);
 }
 
 // dq and delta; rows are queries.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWinThreads) win_dq_kernel(const WinParams p) {
+__global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dq_kernel(const WinParams p) {
+  using C = RowShape<DP>;
   constexpr int N = DP / 4;
-  __shared__ __align__(16) float ks[kTile * DP];
-  __shared__ __align__(16) float vs[kTile * DP];
-  const int part = threadIdx.x & 3, r = threadIdx.x >> 2;
+  extern __shared__ __align__(16) float row_smem[];
+  const int gid = threadIdx.x / kWinThreads, thread = threadIdx.x % kWinThreads;
+  float* ks = row_smem + gid * (C::kTileBytes / 4);
+  float* vs = ks + kTile * DP;
+  const int part = thread & 3, r = thread >> 2;
   const int h = blockIdx.y, b = blockIdx.z, hk = h / (p.H / p.Hk);
   const int i0 = blockIdx.x * kRows, i = i0 + r;
   const bool on = i < p.S;
@@ -221,39 +289,38 @@ __global__ void __launch_bounds__(kWinThreads) win_dq_kernel(const WinParams p) 
   delta += __shfl_xor_sync(0xffffffffu, delta, 1);
   delta += __shfl_xor_sync(0xffffffffu, delta, 2);
   const float lse = on ? p.lse[srow] : INFINITY;
-  if (on && part == 0) p.delta[srow] = delta;
-  int se, lo, hi;
-  key_ranges(p, L, i0, kRows, &se, &lo, &hi);
-  for (int phase = 0; phase < 2; ++phase) {
-    const int end = phase ? hi : se;
-    for (int j0 = phase ? lo : 0; j0 < end; j0 += kTile) {
-      __syncthreads();
-      stage_rows<T, DP>(ks, kb, p.k_ss, j0, end, p.D);
-      stage_rows<T, DP>(vs, vb, p.v_ss, j0, end, p.D);
-      __syncthreads();
-      const int n = min(kTile, end - j0);
-      for (int t = 0; t < n; t += kStep) {
-        float z[kStep], dp[kStep];
-        dot_rows<N, DP>(q, ks + t * DP, part, z);
-        dot_rows<N, DP>(g, vs + t * DP, part, dp);
+  if (on && part == 0 && gid == 0) p.delta[srow] = delta;
+  const KeyRun run(p, L, i0);
+  for (int it = gid; it < run.tiles; it += C::kGroups) {
+    const int j0 = run.first(it), end = run.end(it), n = min(kTile, end - j0);
+    group_sync(gid);
+    stage_rows<T, DP>(ks, kb, p.k_ss, vs, vb, p.v_ss, j0, end, p.D, thread);
+    group_sync(gid);
+    for (int t = 0; t < n; t += kStep) {
+      float z[kStep], dp[kStep];
+      dot_rows<N, DP>(q, ks + t * DP, part, z);
+      dot_rows<N, DP>(g, vs + t * DP, part, dp);
 #pragma unroll
-        for (int u = 0; u < kStep; ++u)
-          if (t + u < n && win_sees(p, L, i, j0 + t + u))
-            axpy_share<N>(acc, exp2f(z[u] - lse) * (dp[u] - delta), ks + (t + u) * DP, part);
-      }
+      for (int u = 0; u < kStep; ++u)
+        if (t + u < n && win_sees(p, L, i, j0 + t + u))
+          axpy_share<N>(acc, exp2f(z[u] - lse) * (dp[u] - delta), ks + (t + u) * DP, part);
     }
   }
+  join_groups<N, C::kGroups>(acc, row_smem, gid, thread);
+  if (gid > 0) return;
   store_share<T, N>(static_cast<T*>(p.dq) + orow, p.D, part, on, acc, p.scale);
 }
 
 // dk and dv; rows are keys, the staged side the queries of each head that shares them.
 template <typename T, int DP>
-__global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(const WinParams p) {
+__global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dkv_kernel(const WinParams p) {
+  using C = RowShape<DP>;
   constexpr int N = DP / 4;
-  __shared__ __align__(16) float qs[kTile * DP];
-  __shared__ __align__(16) float gs[kTile * DP];
-  __shared__ float ls[kTile], ds[kTile];
-  const int part = threadIdx.x & 3, r = threadIdx.x >> 2;
+  extern __shared__ __align__(16) float row_smem[];
+  const int gid = threadIdx.x / kWinThreads, thread = threadIdx.x % kWinThreads;
+  float* qs = row_smem + gid * (C::kTileBytes / 4);
+  float *gs = qs + kTile * DP, *ls = gs + kTile * DP, *ds = ls + kTile;
+  const int part = thread & 3, r = thread >> 2;
   const int hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hk;
   const int j0 = blockIdx.x * kRows, j = j0 + r;
   const int L = win_length(p, b);
@@ -272,38 +339,48 @@ __global__ void __launch_bounds__(kWinThreads) win_dkv_kernel(const WinParams p)
                          : (sink ? p.S
                                  : static_cast<int>(min(static_cast<long long>(p.S),
                                                         static_cast<long long>(j0) + kRows - 1 + p.window)));
-  for (int h = hk * group; h < (hk + 1) * group; ++h) {
+  const int tiles = hi > lo ? (hi - lo + kTile - 1) / kTile : 0;
+  for (int it = gid; it < tiles * group; it += C::kGroups) {
+    const int h = hk * group + it / tiles, i0 = lo + (it % tiles) * kTile;
     const T* qb = static_cast<const T*>(p.q) + b * p.q_sb + h * p.q_sh;
     const T* gb = static_cast<const T*>(p.dout) + b * p.g_sb + h * p.g_sh;
     const long long srow = (static_cast<long long>(b) * p.H + h) * p.S;
-    for (int i0 = lo; i0 < hi; i0 += kTile) {
-      __syncthreads();
-      stage_rows<T, DP>(qs, qb, p.q_ss, i0, hi, p.D);
-      stage_rows<T, DP>(gs, gb, p.g_ss, i0, hi, p.D);
-      const int n = min(kTile, hi - i0);
-      if (static_cast<int>(threadIdx.x) < n) {
-        ls[threadIdx.x] = p.lse[srow + i0 + threadIdx.x];
-        ds[threadIdx.x] = p.delta[srow + i0 + threadIdx.x];
-      }
-      __syncthreads();
-      for (int t = 0; t < n; t += kStep) {
-        float z[kStep], dp[kStep];
-        dot_rows<N, DP>(k, qs + t * DP, part, z);
-        dot_rows<N, DP>(v, gs + t * DP, part, dp);
+    const int n = min(kTile, hi - i0);
+    group_sync(gid);
+    stage_rows<T, DP>(qs, qb, p.q_ss, gs, gb, p.g_ss, i0, hi, p.D, thread);
+    if (thread < n) {
+      ls[thread] = p.lse[srow + i0 + thread];
+      ds[thread] = p.delta[srow + i0 + thread];
+    }
+    group_sync(gid);
+    for (int t = 0; t < n; t += kStep) {
+      float z[kStep], dp[kStep];
+      dot_rows<N, DP>(k, qs + t * DP, part, z);
+      dot_rows<N, DP>(v, gs + t * DP, part, dp);
 #pragma unroll
-        for (int u = 0; u < kStep; ++u)
-          if (t + u < n && win_sees(p, L, i0 + t + u, j)) {
-            const float w = exp2f(z[u] - ls[t + u]);
-            axpy_share<N>(dv, w, gs + (t + u) * DP, part);
-            axpy_share<N>(dk, w * (dp[u] - ds[t + u]), qs + (t + u) * DP, part);
-          }
-      }
+      for (int u = 0; u < kStep; ++u)
+        if (t + u < n && win_sees(p, L, i0 + t + u, j)) {
+          const float w = exp2f(z[u] - ls[t + u]);
+          axpy_share<N>(dv, w, gs + (t + u) * DP, part);
+          axpy_share<N>(dk, w * (dp[u] - ds[t + u]), qs + (t + u) * DP, part);
+        }
     }
   }
+  join_groups<N, C::kGroups>(dk, row_smem, gid, thread);
+  join_groups<N, C::kGroups>(dv, row_smem, gid, thread);
+  if (gid > 0) return;
   const bool in = j < p.S;
   const long long row = ((static_cast<long long>(b) * p.S + j) * p.Hk + hk) * p.D;
   store_share<T, N>(static_cast<T*>(p.dk) + row, p.D, part, in, dk, p.scale);
   store_share<T, N>(static_cast<T*>(p.dv) + row, p.D, part, in, dv, 1.f);
+}
+
+template <int DP, typename K>
+void launch_rows(K kern, const WinParams& p, int heads, cudaStream_t st) {
+  using C = RowShape<DP>;
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, C::kSmem));
+  kern<<<dim3((p.S + kRows - 1) / kRows, heads, p.B), C::kGroups * kWinThreads, C::kSmem, st>>>(p);
+  C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
 template <typename F>
@@ -316,10 +393,6 @@ void by_dim(int D, F&& f) {
     f(std::integral_constant<int, 64>());
   else
     f(std::integral_constant<int, 128>());
-}
-
-dim3 row_grid(const WinParams& p, int heads) {
-  return dim3((p.S + kRows - 1) / kRows, heads, p.B);
 }
 
 void check_qkv(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks) {
@@ -397,11 +470,10 @@ std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tens
   by_dim(p.D, [&](auto dc) {
     constexpr int DP = decltype(dc)::value;
     if (bf16)
-      win_fwd_kernel<__nv_bfloat16, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
+      launch_rows<DP>(win_fwd_kernel<__nv_bfloat16, DP>, p, p.H, st);
     else
-      win_fwd_kernel<float, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
+      launch_rows<DP>(win_fwd_kernel<float, DP>, p, p.H, st);
   });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {o, lse};
 }
 
@@ -440,14 +512,13 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
   by_dim(p.D, [&](auto dc) {
     constexpr int DP = decltype(dc)::value;
     if (bf16) {
-      win_dq_kernel<__nv_bfloat16, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
-      win_dkv_kernel<__nv_bfloat16, DP><<<row_grid(p, p.Hk), kWinThreads, 0, st>>>(p);
+      launch_rows<DP>(win_dq_kernel<__nv_bfloat16, DP>, p, p.H, st);
+      launch_rows<DP>(win_dkv_kernel<__nv_bfloat16, DP>, p, p.Hk, st);
     } else {
-      win_dq_kernel<float, DP><<<row_grid(p, p.H), kWinThreads, 0, st>>>(p);
-      win_dkv_kernel<float, DP><<<row_grid(p, p.Hk), kWinThreads, 0, st>>>(p);
+      launch_rows<DP>(win_dq_kernel<float, DP>, p, p.H, st);
+      launch_rows<DP>(win_dkv_kernel<float, DP>, p, p.Hk, st);
     }
   });
-  C10_CUDA_KERNEL_LAUNCH_CHECK();
   return {dq, dk, dv};
 }
 
