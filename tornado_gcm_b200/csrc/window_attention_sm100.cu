@@ -1141,7 +1141,16 @@ void bwd(const WinParams& p, cudaStream_t st, int* err) {
     sp.tiles = sink_tiles;
     sp.rows = std::min(p.sinks, 128);
     sp.extra = static_cast<int>(std::max(1ll, (p.S - 127ll - p.window + own - 1) / own));
-    sp.extra = std::min(sp.extra, std::max(1, 512 / sink_tiles));  // enough to fill the SMs; bounds the parts
+    // Not one more than the last round of resident CTAs has room for, unless that is less than half of them: 12
+    // extra CTAs for each of 8 heads on top of 512 start a third round (225 us), 10 fit into the second
+    // (190 us).
+    const long long heads = static_cast<long long>(p.B) * p.Hk;
+    const long long resident = static_cast<long long>(at::cuda::getCurrentDeviceProperties()->multiProcessorCount) *
+                               C::kPerSm;
+    const long long own_ctas = heads * k_tiles, rounds = (own_ctas + resident - 1) / resident;
+    const long long room = (rounds * resident - own_ctas) / (heads * sink_tiles);
+    if (room < sp.extra && 2 * room >= sp.extra) sp.extra = static_cast<int>(room);
+    sp.extra = std::min(sp.extra, std::max(1, 512 / sink_tiles));  // bounds the parts
     part = out_empty({p.B, p.Hk, sp.tiles, 1 + sp.extra, 2, sp.rows, p.D},
                      at::TensorOptions().dtype(at::kFloat).device(at::kCUDA, at::cuda::current_device()));
     sp.part = part.data_ptr<float>();
