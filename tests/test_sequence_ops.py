@@ -596,3 +596,84 @@ def test_clip_grad_norm_refusals_and_graph():
     graph.replay()
     torch.cuda.synchronize()
     assert abs(float(n) - want) <= 1e-6 * want and abs(_norm64(g) - 3.0) <= 1e-5
+
+
+# ── the operators together ─────────────────────────────────────────────────
+@pytest.mark.parametrize("D,window,sinks,causal", [(128, 640, 16, False), (64, 512, 4, True), (96, 300, 0, True)])
+def test_window_attention_many_blocks_against_fp32_kernels(D, window, sinks, causal):
+    """Thousands of blocks, several rounds of the GPU: the tensor-core kernels against the CUDA-core ones in fp32
+    (which the tests above hold to fp64), on the same bf16 values."""
+    from tornado_gcm_b200.ops.window_attention import window_attention
+
+    B, S, H, Hk = 2, 8192, 8, 2
+    q, k, v = (_randn(B, S, h, D, seed=i, dtype=torch.bfloat16) for i, h in enumerate((H, Hk, Hk)))
+    do = _randn(B, S, H, D, seed=5, dtype=torch.bfloat16)
+    L = torch.tensor([S, 3000], dtype=torch.int32, device=DEV)
+    res = []
+    for dt in (torch.bfloat16, torch.float32):
+        ts = [t.to(dt).requires_grad_() for t in (q, k, v)]
+        o = window_attention(*ts, window=window, sinks=sinks, causal=causal, lengths=L)
+        res.append([o, *torch.autograd.grad(o, ts, do.to(dt))])
+    for name, a, b in zip(("o", "dq", "dk", "dv"), *res):
+        _close(a, b, TOL[torch.bfloat16], name)
+    _ext.check_error_flag(DEV)
+
+
+def test_sequence_model_on_the_gpu_follows_the_cpu():
+    """One training pass and a cached forecast against the fp32 CPU forms of the same weights: BF16 products in two
+    blocks, so a few times the rounding of one."""
+    from tornado_gcm_b200.models import sequence
+
+    torch.manual_seed(0)
+    cpu = sequence.SequenceEmulator(20, 3, statics=3, d_model=128, num_heads=2, kv_heads=1, num_layers=2, d_ff=200,
+                                    window=40, max_positions=512)
+    torch.nn.init.normal_(cpu.head.weight, std=0.05)
+    gpu = sequence.SequenceEmulator(20, 3, statics=3, d_model=128, num_heads=2, kv_heads=1, num_layers=2, d_ff=200,
+                                    window=40, max_positions=512).to(DEV)
+    gpu.load_state_dict(cpu.state_dict())
+    states, static = sequence.synthetic_columns(3, 150, 20, 3)
+    L = torch.tensor([150, 80, 0], dtype=torch.int32)
+    a = cpu.loss(states, static, L)
+    b = gpu.loss(states.to(DEV), static.to(DEV), L.to(DEV))
+    a.backward()
+    b.backward()
+    assert abs(float(a) - float(b)) <= 1e-2 * float(a)
+    for (n, p), r in zip(gpu.named_parameters(), cpu.parameters()):
+        _close(p.grad.cpu(), r.grad, 5e-2, n)
+    f = gpu.forecast(states[:, :100].to(DEV), static.to(DEV), steps=60)
+    with torch.no_grad():
+        whole = gpu(torch.cat([states[:, :100].to(DEV), f[:, :-1]], 1), static.to(DEV))[:, 99:]
+    _close(f, whole, 1e-2)
+    _ext.check_error_flag(DEV)
+
+
+def test_sequence_example_on_the_gpu():
+    from tornado_gcm_b200.models import sequence
+
+    r = sequence.main(["--steps", "31", "--batch", "4", "--length", "300", "--features", "12", "--window", "64",
+                       "--layers", "2", "--width", "128", "--forecast", "20"])
+    assert r["losses"][-1] < 0.5 * r["losses"][0] and r["gap"] < 1e-2
+
+
+def test_trainer_with_native_clipping():
+    """The hybrid trainer's step with either clipping: the same loss and, after it, the same weights."""
+    from tornado_gcm_b200.training.trainer import GCMTrainer
+
+    class Net(torch.nn.Module):
+        def __init__(self):
+            super().__init__()
+            self.lin = torch.nn.Linear(6, 5)
+
+        def loss(self, data0, targets, forcings):
+            return 100.0 * (self.lin(data0["x"]) - targets[0]["x"]).square().mean()
+
+    torch.manual_seed(0)
+    nets = [Net().to(DEV) for _ in range(2)]
+    nets[1].load_state_dict(nets[0].state_dict())
+    data, tgt = {"x": torch.randn(32, 6)}, [{"x": torch.randn(32, 5)}]
+    trs = [GCMTrainer(n, lr=1e-2, max_grad_norm=0.5, graph=True, native_clip=native) for n, native in zip(nets, (False, True))]
+    for _ in range(4):
+        losses = [float(t.train_step(data, tgt, {})) for t in trs]
+        assert abs(losses[0] - losses[1]) <= 1e-5 * losses[0]
+    for a, b in zip(nets[0].parameters(), nets[1].parameters()):
+        _close(a, b, 1e-5)

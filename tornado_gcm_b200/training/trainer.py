@@ -219,7 +219,8 @@ class GCMTrainer:
 
     def __init__(self, gcm: nn.Module, lr: float = 1e-4, weight_decay: float = 0.0, max_grad_norm: float = 1.0,
                  ema_num_steps: int = 1999, graph: bool = False, betas=(0.9, 0.95), eps: float = 1e-6,
-                 data_parallel: bool = False, grad_average: bool = True, check_errors_every: int = 0):
+                 data_parallel: bool = False, grad_average: bool = True, check_errors_every: int = 0,
+                 native_clip: bool = False):
         """``data_parallel``: replicated weights, gradients reduced over the ranks after
         backward — averaged (data parallelism: each rank's loss is a full loss of its own
         samples) or summed with ``grad_average=False`` (a model sharded over the ranks:
@@ -230,7 +231,10 @@ class GCMTrainer:
         ``check_errors_every``: every that many steps, read the device error flag that the
         kernels set when a bounded wait expires or a table index is out of range, and raise
         (one host synchronisation; 0 leaves the check to the caller, see
-        :meth:`check_device_errors`)."""
+        :meth:`check_device_errors`).
+        ``native_clip``: clip with :func:`tornado_gcm_b200.ops.gradnorm.clip_grad_norm` (two
+        launches for all parameters, fp64 sum) instead of ``torch.nn.utils.clip_grad_norm_``;
+        the sharded optimizer clips its own chunk either way."""
         self.gcm = gcm
         params = [p for p in gcm.parameters() if p.requires_grad]
         self.dp = None
@@ -271,6 +275,7 @@ class GCMTrainer:
                                                fused=dev.type == "cuda", capturable=graph and dev.type == "cuda")
         self.params = params
         self.max_grad_norm = max_grad_norm
+        self.native_clip = bool(native_clip)
         self.ema = _Ema(gcm, ema_num_steps)
         self.use_graph = graph and dev.type == "cuda"
         self._graph = None
@@ -314,7 +319,12 @@ class GCMTrainer:
         else:
             if self.dp is not None:
                 self.dp.reduce()
-            torch.nn.utils.clip_grad_norm_(self.params, self.max_grad_norm, foreach=True)
+            if self.native_clip:
+                from tornado_gcm_b200.ops.gradnorm import clip_grad_norm
+
+                clip_grad_norm([p.grad for p in self.params], self.max_grad_norm)
+            else:
+                torch.nn.utils.clip_grad_norm_(self.params, self.max_grad_norm, foreach=True)
             self.optimizer.step()
         self.ema.update()
         return loss.detach()
