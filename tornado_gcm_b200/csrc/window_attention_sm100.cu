@@ -16,10 +16,10 @@
 // products run under the other's exponentials.  Only at D = 128 do dk and dv
 // need all of TMEM; that kernel keeps two score tiles in flight instead.
 //   D <= 64:  forward 128-key tiles (S 128, P 64, O 64 columns),
-//             dq 64-key tiles (S 64, dP 64, dS 32, dQ 64),
-//             dk/dv 64-query tiles (S, dP, dV, dK 64 each; P and dS over S and dP)
+//             dq 64-key tiles (S, dP, dQ 64 each),
+//             dk/dv 64-query tiles (S, dP, dV, dK 64 each)
 //   D <= 128: forward 64-key tiles (S 64, P 32, O 128),
-//             dq 64-key tiles (S, under dS, 64, dP 64, dQ 128),
+//             dq 64-key tiles (S 64, dP 64, dQ 128),
 //             dk/dv 64-query tiles (2 x (S, dP 64), dV, dK 128)
 // A head narrower than its tile is filled with zeros by TMA; products run over
 // the columns that are there, rounded up to 16.
@@ -491,12 +491,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 template <int DP>
 struct DqCfg {
   static constexpr int KT = 64;
-  static constexpr bool kAlias = DP == 128;  // dS over S: no room for its own columns
   static constexpr int kSlots = DP == 64 ? 4 : 2;
+  // With one pair of slots the next tile's keys arrive only after the product that reads this tile's.
+  static constexpr bool kEarly = kSlots == 4;
   static constexpr int kSlot = KT * DP * 2;
   static constexpr int kQ = 128 * DP * 2;
-  static constexpr int kSmem = 2 * kQ + kSlots * kSlot + 256 + 1024;
-  static constexpr uint32_t kDp = 64, kDs = kAlias ? 0 : 192, kDq = 128;
+  static constexpr int kDs = 128 * KT * 2;                // dS as the A operand of dQ += dS K
+  static constexpr int kSmem = 2 * kQ + kDs + kSlots * kSlot + 256;
+  static constexpr uint32_t kDp = 64, kDq = 128;          // TMEM columns: S at 0
 };
 
 template <int DP>
@@ -504,9 +506,13 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     win_dq_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, int* err) {
   using C = DqCfg<DP>;
   constexpr int KT = C::KT;
-  extern __shared__ __align__(1024) uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + 2 * C::kQ;  // queries, dO, then the ring
+  extern __shared__ __align__(1024) uint8_t smem[];  // no slack to align it in: two CTAs fill the SM at D = 128
+  if (smem_u32(smem) & 1023u) {
+    record_error(err, kErrBounds);
+    return;
+  }
+  uint8_t* ds_tile = smem + 2 * C::kQ;  // queries, dO, dS, then the ring
+  uint8_t* ring = ds_tile + C::kDs;
   uint64_t* full = reinterpret_cast<uint64_t*>(ring + C::kSlots * C::kSlot);
   uint64_t* empty = full + C::kSlots;
   uint64_t* q_full = empty + C::kSlots;
@@ -581,15 +587,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const uint32_t idesc_s = make_idesc(1, 0, 0, 128, 0), idesc_q = make_idesc(1, 0, 1, 128, 16 * kd);
       const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t q0 = desc_lo(smem_u32(smem)), g0 = desc_lo(smem_u32(smem) + C::kQ);
+      const uint32_t a0 = desc_lo(smem_u32(ds_tile));
       const uint32_t k0 = desc_lo(smem_u32(ring)), t0 = desc_lo(smem_u32(ring), KT * kAtom);
       auto scores = [&](int j) {  // S = Q K^T, dP = dO V^T
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
         const uint32_t id = idesc_s | ((cols >> 3) << 17);
         const int ik = 2 * j, iv = ik + 1, s = ik % C::kSlots, sv = iv % C::kSlots;
-        // S lies over dS at D = 128: then the product that reads dS has to be over, not only the reading of S
-        if (j > 0 &&
-            !warp_wait(C::kAlias ? dq_done : s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
+        if (j > 0 && !warp_wait(s_empty, (j - 1) & 1, err, kErrTimeoutEmpty)) return false;
         if (!warp_wait(&full[s], (ik / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         if (!warp_wait(&full[sv], (iv / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
@@ -609,7 +614,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       };
       bool go = warp_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
-        if (!C::kAlias && j + 1 < kt.n && !(go = scores(j + 1))) break;
+        if (C::kEarly && j + 1 < kt.n && !(go = scores(j + 1))) break;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
         const int s = (2 * j) % C::kSlots;
@@ -619,12 +624,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           const uint32_t ks = t0 + s * (C::kSlot >> 4);
 #pragma unroll
           for (int k = 0; k < KT / 16; ++k)  // dQ += dS K
-            if (k * 16 < cols) umma_ts(d0 + C::kDq, d0 + C::kDs + k * 8, ks + step_mn(k), idesc_q, (j | k) ? 1u : 0u);
+            if (k * 16 < cols) umma_ss(d0 + C::kDq, a0 + step_k(128, k), ks + step_mn(k), idesc_q, (j | k) ? 1u : 0u);
           tc_commit(&empty[s]);
           tc_commit(dq_done);
         }
         __syncwarp();
-        if (C::kAlias && j + 1 < kt.n) go = scores(j + 1);
+        if (!C::kEarly && j + 1 < kt.n) go = scores(j + 1);
       }
       if (!go) *abort_flag = 1;
     }
@@ -653,55 +658,52 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       p.delta[srow] = delta;
     }
     const float2 c2 = make_float2(c, c), lse2 = make_float2(-lse, -lse), delta2 = make_float2(-delta, -delta);
+    // tiles that all of this warp's queries see whole
+    const int from = kt.n_sink + max(0, w1 - p.window + 1 - kt.lo + KT - 1) / KT;
+    const int room = min(L, p.causal ? w0 + 1 : w0 + p.window) - kt.lo;
+    const int to = room < KT ? 0 : kt.n_sink + room / KT;
     bool ok = true;
     for (int j = 0; j < kt.n; ++j) {
       int j0, cols;
       key_tile<KT>(kt, j, &j0, &cols);
       if (!(ok = warp_wait(s_full, j & 1, err, kErrTimeoutTmemFull))) break;
       tc_fence_after();
-      const bool whole = j >= kt.n_sink && cols == KT && j0 + cols <= L && j0 > w1 - p.window &&
-                         j0 + cols - 1 < (p.causal ? w0 + 1 : w0 + p.window);
-      uint32_t ds[KT / 2];
+      // The whole row at once, so that the next tile's scores are made under this one's arithmetic.
+      float s[KT], dp[KT];
 #pragma unroll
-      for (int ch = 0; ch < KT / 32; ++ch)
-        if (ch * 32 < cols) {
-          float s[32], dp[32];
-          load_row32(tmem + lanes + ch * 32, s);
-          load_row32(tmem + C::kDp + lanes + ch * 32, dp);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            float2 w = fma2(make_float2(s[e], s[e + 1]), c2, lse2);
-            w.x = ex2(w.x);
-            w.y = ex2(w.y);
-            w = mul2(w, add2(make_float2(dp[e], dp[e + 1]), delta2));
-            s[e] = w.x;
-            s[e + 1] = w.y;
-          }
-          if (!whole) {
-            const uint32_t si = sight_of(p, kt, L, i, j, j0).w[ch];
-#pragma unroll
-            for (int e = 0; e < 32; ++e) s[e] = (si & (1u << e)) ? s[e] : 0.f;
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) ds[ch * 16 + e / 2] = pack_f2(s[e], s[e + 1]);
-        }
+      for (int half = 0; half < 2; ++half) {  // a narrow tile's columns behind its end are out of sight
+        load_row32(tmem + lanes + half * 32, s + half * 32);
+        load_row32(tmem + C::kDp + lanes + half * 32, dp + half * 32);
+      }
+      tmem_ld_wait();
       tc_fence_before();
-      if (!C::kAlias) {
-        __syncwarp();
-        if (lane == 0) mbar_arrive(s_empty);
-        if (j > 0) {  // the product before has read dS
-          if (!(ok = warp_wait(dq_done, (j - 1) & 1, err, kErrTimeoutTmemFull))) break;
-          tc_fence_after();
-        }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(s_empty);
+#pragma unroll
+      for (int e = 0; e < KT; e += 2) {
+        float2 w = fma2(make_float2(s[e], s[e + 1]), c2, lse2);
+        w.x = ex2(w.x);
+        w.y = ex2(w.y);
+        w = mul2(w, add2(make_float2(dp[e], dp[e + 1]), delta2));
+        s[e] = w.x;
+        s[e + 1] = w.y;
+      }
+      if (j < from || j >= to) {
+        const Sight si = sight_of(p, kt, L, i, j, j0);
+#pragma unroll
+        for (int e = 0; e < KT; ++e) s[e] = (si.w[e >> 5] & (1u << (e & 31))) ? s[e] : 0.f;
+      }
+      if (j > 0) {  // the product before has read dS
+        if (!(ok = warp_wait(dq_done, (j - 1) & 1, err, kErrTimeoutTmemFull))) break;
       }
 #pragma unroll
-      for (int ch = 0; ch < KT / 32; ++ch)
-        if (ch * 32 < cols) tmem_st_32x32b_x16(tmem + C::kDs + lanes + ch * 16, ds + ch * 16);
+      for (int c8 = 0; c8 < KT / 8; ++c8)
+        *stage_piece(ds_tile, 0, row, c8) =
+            make_uint4(pack_f2(s[8 * c8], s[8 * c8 + 1]), pack_f2(s[8 * c8 + 2], s[8 * c8 + 3]),
+                       pack_f2(s[8 * c8 + 4], s[8 * c8 + 5]), pack_f2(s[8 * c8 + 6], s[8 * c8 + 7]));
       if (j0 + cols > L)  // K has arrived: S was made from it
         clear_rows<DP>(ring + ((2 * j) % C::kSlots) * C::kSlot, KT, max(0, L - j0), cols, threadIdx.x - 64);
-      tmem_st_wait();
-      tc_fence_before();
+      fence_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(ds_full);
     }
@@ -729,11 +731,12 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 template <int DP>
 struct DkvCfg {
   static constexpr int QT = 64;
-  static constexpr int kBufs = DP == 64 ? 1 : 2;  // score tiles in flight
+  static constexpr int kBufs = DP == 64 ? 1 : 2;  // score tiles in TMEM
   static constexpr int kSlots = 4;
   static constexpr int kSlot = QT * DP * 2;
   static constexpr int kK = 128 * DP * 2;
-  static constexpr int kSmem = 2 * kK + kSlots * kSlot + 2 * 2 * QT * 4 + 256 + 1024;
+  static constexpr int kP = 128 * QT * 2;             // P^T, and dS^T, as A operands of dV += P^T dO, dK += dS^T Q
+  static constexpr int kSmem = 2 * kK + 2 * kP + kSlots * kSlot + 2 * 2 * QT * 4 + 256 + 1024;
   static constexpr uint32_t kCols = DP == 64 ? 256 : 512;
   static constexpr uint32_t kDv = kBufs * 128, kDk = kDv + DP;  // S at 0, dP at 64 of each buffer
   static constexpr int kPerSm = DP == 64 ? 2 : 1;
@@ -753,16 +756,18 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
   constexpr int QT = C::QT;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* ring = smem + 2 * C::kK;  // keys, values, then the ring
-  float* stat = reinterpret_cast<float*>(ring + C::kSlots * C::kSlot);  // [2][lse, delta][QT]
+  uint8_t* p_tile = smem + 2 * C::kK;  // keys, values, P, dS, then the ring
+  uint8_t* ds_tile = p_tile + C::kP;
+  uint8_t* ring = ds_tile + C::kP;
+  float* stat = reinterpret_cast<float*>(ring + C::kSlots * C::kSlot);  // [2][-lse, -delta][QT], one for each dO slot
   uint64_t* full = reinterpret_cast<uint64_t*>(stat + 4 * QT);
   uint64_t* empty = full + C::kSlots;
   uint64_t* k_full = empty + C::kSlots;
   uint64_t* s_full = k_full + 1;             // S and dP; of each buffer its own, as in the forward
-  uint64_t* ds_full = s_full + C::kBufs;     // P and dS
-  uint64_t* d_done = ds_full + C::kBufs;     // dV and dK of an iteration
-  uint64_t* all_done = d_done + 1;  // of the last one
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(all_done + 1);
+  uint64_t* s_empty = s_full + C::kBufs;
+  uint64_t* ds_full = s_empty + C::kBufs;    // P and dS
+  uint64_t* d_done = ds_full + 1;            // dV and dK of an iteration
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(d_done + 1);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -791,10 +796,14 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
     n = span * group;
   }
   if (j0 >= L) n = 0;
-  // head and first query of iteration it, and where its queries end
-  auto query_tile = [&](int it, int* h, int* i0, int* end) {
-    const int u = first + it, t = u % span;
-    *h = hk * group + u / span;
+  // The iterations in order: head, first query, and where that run of queries ends.
+  struct Walk {
+    int h, t;
+  };
+  Walk walk{hk * group + (span > 0 ? first / span : 0), span > 0 ? first % span : 0};
+  auto next_tile = [&](int* h, int* i0, int* end) {
+    *h = walk.h;
+    const int t = walk.t;
     if (!extra) {
       *i0 = lo + t * QT;
       *end = hi;
@@ -805,20 +814,24 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       *i0 = hi + (t - before) * QT;
       *end = p.S;
     }
+    if (++walk.t == span) {
+      walk.t = 0;
+      ++walk.h;
+    }
   };
 
   if (threadIdx.x == 0) {
     for (int s = 0; s < C::kSlots; ++s) {
-      mbar_init(&full[s], 1);
+      mbar_init(&full[s], (s & 1) ? 33 : 1);  // dO's slots also wait for their rows' lse and delta
       mbar_init(&empty[s], 1);
     }
     mbar_init(k_full, 1);
     for (int i = 0; i < C::kBufs; ++i) {
       mbar_init(&s_full[i], 1);
-      mbar_init(&ds_full[i], 4);
+      mbar_init(&s_empty[i], 4);
     }
+    mbar_init(ds_full, 4);
     mbar_init(d_done, 1);
-    mbar_init(all_done, 1);
     *abort_flag = 0;
     fence_barrier_init();
   }
@@ -832,31 +845,52 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0 && n > 0) {
-      mbar_arrive_expect_tx(k_full, 2 * C::kK);
+    if (n > 0) {
+      if (lane == 0) {
+        mbar_arrive_expect_tx(k_full, 2 * C::kK);
 #pragma unroll
-      for (int a = 0; a < DP / 64; ++a)
+        for (int a = 0; a < DP / 64; ++a)
 #pragma unroll
-        for (int r = 0; r < 2; ++r) {  // the keys' map has boxes of 64 rows
-          tma_load_4d(smem + (a * 128 + r * 64) * kAtom, &maps.k, k_full, a * 64, j0 + r * 64, hk, b);
-          tma_load_4d(smem + C::kK + (a * 128 + r * 64) * kAtom, &maps.v, k_full, a * 64, j0 + r * 64, hk, b);
-        }
+          for (int r = 0; r < 2; ++r) {  // the keys' map has boxes of 64 rows
+            tma_load_4d(smem + (a * 128 + r * 64) * kAtom, &maps.k, k_full, a * 64, j0 + r * 64, hk, b);
+            tma_load_4d(smem + C::kK + (a * 128 + r * 64) * kAtom, &maps.v, k_full, a * 64, j0 + r * 64, hk, b);
+          }
+      }
       int it = 0;
       bool go = true;
       for (int t = 0; t < n && go; ++t) {
         int h, i0, end;
-        query_tile(t, &h, &i0, &end);
+        next_tile(&h, &i0, &end);
+        // -lse and -delta of the tile's queries, two of each to a lane; -inf makes a weight of zero
+        const float* ls = p.lse + (static_cast<long long>(b) * p.H + h) * p.S;
+        const float* de = p.delta + (static_cast<long long>(b) * p.H + h) * p.S;
+        float v[4];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+          const int i = i0 + lane + 32 * u;
+          v[u] = i < end ? -ls[i] : -INFINITY;
+          v[2 + u] = i < end ? -de[i] : 0.f;
+        }
         for (int qg = 0; qg < 2; ++qg, ++it) {
           const int s = it % C::kSlots;
-          if (!mbar_park(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) || *abort_flag) {
+          go = warp_wait(&empty[s], ((it / C::kSlots) & 1) ^ 1, err, kErrTimeoutEmpty) && !*abort_flag;
+          go = __all_sync(0xffffffffu, go);
+          if (!go) {
             *abort_flag = 1;
-            go = false;
             break;
           }
-          mbar_arrive_expect_tx(&full[s], C::kSlot);
+          if (qg) {
+            float* st = stat + (t & 1) * 2 * QT;
+            st[lane] = v[0], st[lane + 32] = v[1], st[QT + lane] = v[2], st[QT + lane + 32] = v[3];
+            mbar_arrive(&full[s]);
+          }
+          if (lane == 0) {
+            mbar_arrive_expect_tx(&full[s], C::kSlot);
 #pragma unroll
-          for (int a = 0; a < DP / 64; ++a)
-            tma_load_4d(ring + s * C::kSlot + a * QT * kAtom, qg ? &maps.g : &maps.q, &full[s], a * 64, i0, h, b);
+            for (int a = 0; a < DP / 64; ++a)
+              tma_load_4d(ring + s * C::kSlot + a * QT * kAtom, qg ? &maps.g : &maps.q, &full[s], a * 64, i0, h, b);
+          }
+          __syncwarp();
         }
       }
       mbar_park(k_full, 0, err, kErrTimeoutDrain);
@@ -870,10 +904,12 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       const uint32_t d0 = __shfl_sync(0xffffffffu, tmem, 0);
       const uint32_t k0 = desc_lo(smem_u32(smem)), v0 = desc_lo(smem_u32(smem) + C::kK);
       const uint32_t q0 = desc_lo(smem_u32(ring)), t0 = desc_lo(smem_u32(ring), QT * kAtom);
-      // S^T = K Q^T and dP^T = V dO^T, once the products that read P and dS from this buffer are over
+      const uint32_t p0 = desc_lo(smem_u32(p_tile)), ds0 = desc_lo(smem_u32(ds_tile));
+      // S^T = K Q^T and dP^T = V dO^T, once the buffer has been read
       auto scores = [&](int t) {
         const int iq = 2 * t, ig = iq + 1, s = iq % C::kSlots, sg = ig % C::kSlots;
-        if (t >= C::kBufs && !warp_wait(d_done, (t - C::kBufs) & 1, err, kErrTimeoutEmpty)) return false;
+        if (t >= C::kBufs &&
+            !warp_wait(&s_empty[t % C::kBufs], (t / C::kBufs - 1) & 1, err, kErrTimeoutEmpty)) return false;
         if (!warp_wait(&full[s], (iq / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         if (!warp_wait(&full[sg], (ig / C::kSlots) & 1, err, kErrTimeoutFull)) return false;
         tc_fence_after();
@@ -893,26 +929,23 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
       };
       bool go = warp_wait(k_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int t = 0; t < n && go; ++t) {
-        if (C::kBufs == 2 && t + 1 < n && !(go = scores(t + 1))) break;
-        if (!(go = warp_wait(&ds_full[t % C::kBufs], (t / C::kBufs) & 1, err, kErrTimeoutFull))) break;
+        if (t + 1 < n && !(go = scores(t + 1))) break;
+        if (!(go = warp_wait(ds_full, t & 1, err, kErrTimeoutFull))) break;
         tc_fence_after();
         const int s = (2 * t) % C::kSlots, sg = (2 * t + 1) % C::kSlots;
         if (issuer) {
-          const uint32_t buf = d0 + (t % C::kBufs) * 128;
           const uint32_t qs = t0 + s * (C::kSlot >> 4), gs = t0 + sg * (C::kSlot >> 4);
 #pragma unroll
           for (int k = 0; k < QT / 16; ++k)  // dV += P^T dO
-            umma_ts(d0 + C::kDv, buf + k * 8, gs + step_mn(k), idesc_d, (t | k) ? 1u : 0u);
+            umma_ss(d0 + C::kDv, p0 + step_k(128, k), gs + step_mn(k), idesc_d, (t | k) ? 1u : 0u);
           tc_commit(&empty[sg]);
 #pragma unroll
           for (int k = 0; k < QT / 16; ++k)  // dK += dS^T Q
-            umma_ts(d0 + C::kDk, buf + 64 + k * 8, qs + step_mn(k), idesc_d, (t | k) ? 1u : 0u);
+            umma_ss(d0 + C::kDk, ds0 + step_k(128, k), qs + step_mn(k), idesc_d, (t | k) ? 1u : 0u);
           tc_commit(&empty[s]);
           tc_commit(d_done);
-          if (t + 1 == n) tc_commit(all_done);
         }
         __syncwarp();
-        if (C::kBufs == 1 && t + 1 < n) go = scores(t + 1);
       }
       if (!go) *abort_flag = 1;
     }
@@ -920,93 +953,89 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
     const int q4 = warp & 3, row = q4 * 32 + lane, j = j0 + row;
     const uint32_t lanes = static_cast<uint32_t>(q4 * 32) << 16;
     const float c = p.scale * kLog2e;
-    const int tid = threadIdx.x - 64;
     const int w0 = j0 + q4 * 32, w1 = w0 + 31;
     // an extra CTA's rows behind the sinks are nobody's: their warps only keep step
     const bool idle = extra && w0 >= p.sinks;
     const bool sink = j < p.sinks, valid = j < L;
     const bool part_rows = sp.extra > 0 && tile < sp.tiles;
     const float2 c2 = make_float2(c, c);
-    auto load_stat = [&](int t) {  // this thread's value of iteration t's -lse (threads 0-63) or -delta
-      int h, i0, end;
-      query_tile(t, &h, &i0, &end);
-      const int i = i0 + (tid & 63);
-      const long long at = (static_cast<long long>(b) * p.H + h) * p.S + i;
-      return tid < 64 ? (i < end ? -p.lse[at] : -INFINITY) : (i < end ? -p.delta[at] : 0.f);
-    };
-    float next = n > 0 ? load_stat(0) : 0.f;
     bool ok = true;
     for (int t = 0; t < n; ++t) {
       int h, i0, end;
-      query_tile(t, &h, &i0, &end);
-      float* st = stat + (t & 1) * 2 * QT;
-      st[tid] = next;
-      asm volatile("bar.sync 1, 128;" ::: "memory");  // also: everyone is done with the buffer of t - 1
-      if (t + 1 < n) next = load_stat(t + 1);
-      // after a wait that gave up the loop goes on empty: the other warps count on this one at the barrier
-      if (ok) ok = warp_wait(&s_full[t % C::kBufs], (t / C::kBufs) & 1, err, kErrTimeoutTmemFull);
-      if (!ok) continue;
+      next_tile(&h, &i0, &end);
+      const float* st = stat + (t & 1) * 2 * QT;
+      const int ig = 2 * t + 1;
+      ok = warp_wait(&s_full[t % C::kBufs], (t / C::kBufs) & 1, err, kErrTimeoutTmemFull) &&
+           warp_wait(&full[ig % C::kSlots], (ig / C::kSlots) & 1, err, kErrTimeoutFull);
+      if (!ok) break;
       tc_fence_after();
+      const uint32_t buf = tmem + lanes + (t % C::kBufs) * 128;
+      // The whole row at once, so that the next tile's scores are made under this one's arithmetic.
+      float s[QT], dp[QT];
       if (!idle) {
-        const uint32_t buf = tmem + lanes + (t % C::kBufs) * 128;
-        // queries [qa, qb) of the tile see this thread's key
-        int qa, qb;
-        if (extra) {
-          qa = 0;
-          qb = sink && valid ? QT : 0;
-        } else {
-          qa = (p.causal ? j : (sink ? i0 : j - (p.window - 1))) - i0;
-          qb = valid ? (sink ? QT : j + p.window - i0) : 0;
+#pragma unroll
+        for (int ch = 0; ch < 2; ++ch) {
+          load_row32(buf + ch * 32, s + ch * 32);
+          load_row32(buf + 64 + ch * 32, dp + ch * 32);
         }
-        const bool whole = !extra && w1 < L && i0 >= (p.causal ? w1 : w1 - (p.window - 1)) &&
-                           i0 + QT <= w0 + p.window;
-        const Sight seen = words(bits_below(qb) & ~bits_below(qa));
-        uint32_t pk[QT / 2], dk[QT / 2];
-#pragma unroll
-        for (int ch = 0; ch < QT / 32; ++ch) {
-          float s[32], dp[32];
-          load_row32(buf + ch * 32, s);
-          load_row32(buf + 64 + ch * 32, dp);
-          tmem_ld_wait();
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            const float4 ls = *reinterpret_cast<const float4*>(st + ch * 32 + e);
-            const float4 de = *reinterpret_cast<const float4*>(st + QT + ch * 32 + e);
-            const float2 lv[2] = {make_float2(ls.x, ls.y), make_float2(ls.z, ls.w)};
-            const float2 dv[2] = {make_float2(de.x, de.y), make_float2(de.z, de.w)};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-              float2 w = fma2(make_float2(s[e + 2 * u], s[e + 2 * u + 1]), c2, lv[u]);
-              w.x = ex2(w.x);
-              w.y = ex2(w.y);
-              const float2 g = mul2(w, add2(make_float2(dp[e + 2 * u], dp[e + 2 * u + 1]), dv[u]));
-              s[e + 2 * u] = w.x, s[e + 2 * u + 1] = w.y;
-              dp[e + 2 * u] = g.x, dp[e + 2 * u + 1] = g.y;
-            }
-          }
-          if (!whole) {
-#pragma unroll
-            for (int e = 0; e < 32; ++e) {
-              const bool on = seen.w[ch] & (1u << e);
-              s[e] = on ? s[e] : 0.f;
-              dp[e] = on ? dp[e] : 0.f;
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 32; e += 2) {
-            pk[ch * 16 + e / 2] = pack_f2(s[e], s[e + 1]);
-            dk[ch * 16 + e / 2] = pack_f2(dp[e], dp[e + 1]);
-          }
-        }
-        tmem_st_32x32b_x32(buf, pk);
-        tmem_st_32x32b_x32(buf + 64, dk);
-        tmem_st_wait();
+        tmem_ld_wait();
       }
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive(&ds_full[t % C::kBufs]);
+      if (lane == 0) mbar_arrive(&s_empty[t % C::kBufs]);
+      // the products before have read P and dS
+      if (t > 0 && !(ok = warp_wait(d_done, (t - 1) & 1, err, kErrTimeoutTmemFull))) break;
+      if (!idle) {
+#pragma unroll
+        for (int e = 0; e < QT; e += 4) {
+          const float4 ls = *reinterpret_cast<const float4*>(st + e);
+          const float4 de = *reinterpret_cast<const float4*>(st + QT + e);
+          const float2 lv[2] = {make_float2(ls.x, ls.y), make_float2(ls.z, ls.w)};
+          const float2 dv[2] = {make_float2(de.x, de.y), make_float2(de.z, de.w)};
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            float2 w = fma2(make_float2(s[e + 2 * u], s[e + 2 * u + 1]), c2, lv[u]);
+            w.x = ex2(w.x);
+            w.y = ex2(w.y);
+            const float2 g = mul2(w, add2(make_float2(dp[e + 2 * u], dp[e + 2 * u + 1]), dv[u]));
+            s[e + 2 * u] = w.x, s[e + 2 * u + 1] = w.y;
+            dp[e + 2 * u] = g.x, dp[e + 2 * u + 1] = g.y;
+          }
+        }
+        const bool whole = !extra && w1 < L && i0 >= (p.causal ? w1 : w1 - (p.window - 1)) &&
+                           i0 + QT <= w0 + p.window;
+        if (!whole) {
+          // queries [qa, qb) of the tile see this thread's key
+          int qa, qb;
+          if (extra) {
+            qa = 0;
+            qb = sink && valid ? QT : 0;
+          } else {
+            qa = (p.causal ? j : (sink ? i0 : j - (p.window - 1))) - i0;
+            qb = valid ? (sink ? QT : j + p.window - i0) : 0;
+          }
+          const Sight seen = words(bits_below(qb) & ~bits_below(qa));
+#pragma unroll
+          for (int e = 0; e < QT; ++e) {
+            const bool on = seen.w[e >> 5] & (1u << (e & 31));
+            s[e] = on ? s[e] : 0.f;
+            dp[e] = on ? dp[e] : 0.f;
+          }
+        }
+#pragma unroll
+        for (int c8 = 0; c8 < QT / 8; ++c8) {
+          const int e = 8 * c8;
+          *stage_piece(p_tile, 0, row, c8) = make_uint4(pack_f2(s[e], s[e + 1]), pack_f2(s[e + 2], s[e + 3]),
+                                                        pack_f2(s[e + 4], s[e + 5]), pack_f2(s[e + 6], s[e + 7]));
+          *stage_piece(ds_tile, 0, row, c8) = make_uint4(pack_f2(dp[e], dp[e + 1]), pack_f2(dp[e + 2], dp[e + 3]),
+                                                         pack_f2(dp[e + 4], dp[e + 5]), pack_f2(dp[e + 6], dp[e + 7]));
+        }
+        fence_async_smem();
+      }
+      __syncwarp();
+      if (lane == 0) mbar_arrive(ds_full);
     }
-    if (ok && n > 0) ok = warp_wait(all_done, 0, err, kErrTimeoutTmemFull);
+    if (ok && n > 0) ok = warp_wait(d_done, (n - 1) & 1, err, kErrTimeoutTmemFull);
     tc_fence_after();
     if (!ok) {
       *abort_flag = 1;
