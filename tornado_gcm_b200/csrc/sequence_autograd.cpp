@@ -5,6 +5,8 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
+#include <cstring>
+
 #include "sequence_ops.h"
 
 namespace tgcm {
@@ -25,25 +27,39 @@ at::Tensor rows_like(const at::Tensor& g, const at::Tensor& like) {
   return r.size(-1) == 1 || r.stride(-1) == 1 ? r : r.contiguous();
 }
 
+// What a node keeps beside its tensors: the numbers in one entry (an entry for each would cost
+// more than a kernel's launch), and the error flag (not a saved variable: it is cleared between passes).
+int64_t bits_of(double x) {
+  int64_t b;
+  std::memcpy(&b, &x, sizeof(b));
+  return b;
+}
+double double_of(int64_t b) {
+  double x;
+  std::memcpy(&x, &b, sizeof(x));
+  return x;
+}
+void keep(AutogradContext* ctx, std::vector<int64_t> v, const OptTensor& err) {
+  ctx->saved_data["cfg"] = std::move(v);
+  ctx->saved_data["err"] = err;
+}
+OptTensor flag_of(AutogradContext* ctx) { return ctx->saved_data["err"].toOptional<at::Tensor>(); }
+std::vector<int64_t> kept(AutogradContext* ctx) { return ctx->saved_data["cfg"].toIntVector(); }
+
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                             const OptTensor& bg, const OptTensor& bu, int64_t act, const OptTensor& err) {
     ctx->save_for_backward({x, wg, wu, undef_or(bg), undef_or(bu)});
-    ctx->saved_data["act"] = act;
-    ctx->saved_data["err"] = err;
-    ctx->saved_data["x"] = wants(x);
-    ctx->saved_data["w"] = wants(wg) || wants(wu);
-    ctx->saved_data["b"] = wants(bg) || wants(bu);
+    keep(ctx, {act, wants(x), wants(wg) || wants(wu), wants(bg) || wants(bu)}, err);
     return gated_fwd(x, wg, wu, bg, bu, act, err);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     if (!g[0].defined()) return variable_list(7);
-    auto& d = ctx->saved_data;
+    const auto c = kept(ctx);
     const at::Tensor dh = g[0].scalar_type() == at::kBFloat16 ? g[0] : g[0].to(at::kBFloat16);
     auto r = gated_bwd(dh.size(1) == 1 || dh.stride(1) == 1 ? dh : dh.contiguous(), s[0], s[1], s[2], opt(s[3]),
-                       opt(s[4]), d["act"].toInt(), d["x"].toBool(), d["w"].toBool(), d["b"].toBool(),
-                       d["err"].toOptional<at::Tensor>());
+                       opt(s[4]), c[0], c[1], c[2], c[3], flag_of(ctx));
     return {r[0], r[1], r[2], s[3].defined() ? r[3] : at::Tensor(), s[4].defined() ? r[4] : at::Tensor(),
             at::Tensor(), at::Tensor()};
   }
@@ -55,24 +71,15 @@ struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
                                const OptTensor& qb, const OptTensor& kb, int64_t norm, bool interleaved, double eps,
                                const OptTensor& err) {
     ctx->save_for_backward({q, k, undef_or(table), undef_or(positions), undef_or(qw), undef_or(kw)});
-    auto& d = ctx->saved_data;
-    d["norm"] = norm;
-    d["inter"] = interleaved;
-    d["eps"] = eps;
-    d["err"] = err;
-    d["qw"] = wants(qw);
-    d["kw"] = wants(kw);
-    d["qb"] = wants(qb);
-    d["kb"] = wants(kb);
+    keep(ctx, {norm, interleaved, bits_of(eps), wants(qw), wants(kw), wants(qb), wants(kb)}, err);
     return qk_norm_rotary_fwd(q, k, table, positions, qw, kw, qb, kb, norm, interleaved, eps, err);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
-    auto& d = ctx->saved_data;
-    const bool qw = d["qw"].toBool(), kw = d["kw"].toBool(), qb = d["qb"].toBool(), kb = d["kb"].toBool();
+    const auto c = kept(ctx);
     auto r = qk_norm_rotary_bwd(rows_like(g[0], s[0]), rows_like(g[1], s[1]), s[0], s[1], opt(s[2]), opt(s[3]),
-                                opt(s[4]), opt(s[5]), d["norm"].toInt(), d["inter"].toBool(), d["eps"].toDouble(),
-                                {qw, kw, qb, kb}, d["err"].toOptional<at::Tensor>());
+                                opt(s[4]), opt(s[5]), c[0], c[1], double_of(c[2]),
+                                {c[3] != 0, c[4] != 0, c[5] != 0, c[6] != 0}, flag_of(ctx));
     variable_list out(12);
     out[0] = r[0], out[1] = r[1];
     for (int i = 0; i < 4; ++i) out[4 + i] = r[2 + i];
@@ -86,21 +93,15 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
                             const OptTensor& err) {
     auto r = window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, err);
     ctx->save_for_backward({q, k, v, r[0], r[1], undef_or(lengths)});
-    auto& d = ctx->saved_data;
-    d["window"] = window;
-    d["sinks"] = sinks;
-    d["causal"] = causal;
-    d["scale"] = scale;
-    d["err"] = err;
+    keep(ctx, {window, sinks, causal, bits_of(scale)}, err);
     return r[0];
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
     if (!g[0].defined()) return variable_list(9);
-    auto& d = ctx->saved_data;
-    auto r = window_attention_bwd(rows_like(g[0], s[3]), s[0], s[1], s[2], s[3], s[4], d["window"].toInt(),
-                                  d["sinks"].toInt(), d["causal"].toBool(), opt(s[5]), d["scale"].toDouble(),
-                                  d["err"].toOptional<at::Tensor>());
+    const auto c = kept(ctx);
+    auto r = window_attention_bwd(rows_like(g[0], s[3]), s[0], s[1], s[2], s[3], s[4], c[0], c[1], c[2], opt(s[5]),
+                                  double_of(c[3]), flag_of(ctx));
     variable_list out(9);
     for (int i = 0; i < 3; ++i) out[i] = r[i];
     return out;
@@ -113,10 +114,27 @@ at::Tensor gated_linear(const at::Tensor& x, const at::Tensor& wg, const at::Ten
 }
 at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const OptTensor& bg,
                                  const OptTensor& bu, int64_t act, const OptTensor& err) {
-  if (at::GradMode::is_enabled() && (wants(x) || wants(wg) || wants(wu) || wants(bg) || wants(bu)))
-    return GatedLinear::apply(x, wg, wu, bg, bu, act, err);
-  at::AutoDispatchBelowADInplaceOrView below;
-  return gated_fwd(x, wg, wu, bg, bu, act, err);
+  TORCH_CHECK_VALUE(x.dim() >= 1 && wg.dim() == 2 && wg.sizes() == wu.sizes() && x.size(-1) == wg.size(1),
+                    "gated_linear: x (..., features) and two weights (hidden, features) expected");
+  TORCH_CHECK_VALUE(bg.has_value() == bu.has_value(), "gated_linear: both biases or none");
+  // Other types are rounded to bf16 here, above autograd, so that gradients come back in the caller's type.
+  auto bf = [](const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? t : t.to(at::kBFloat16); };
+  auto bf_opt = [&](const OptTensor& t) { return t.has_value() ? OptTensor(bf(*t)) : t; };
+  const bool flat = x.dim() == 2;
+  const at::Tensor x2 = flat ? bf(x) : bf(x).reshape({-1, x.size(-1)});
+  const at::Tensor wg2 = bf(wg), wu2 = bf(wu);
+  const OptTensor bg2 = bf_opt(bg), bu2 = bf_opt(bu);
+  at::Tensor h;
+  if (at::GradMode::is_enabled() && (wants(x2) || wants(wg2) || wants(wu2) || wants(bg2) || wants(bu2))) {
+    h = GatedLinear::apply(x2, wg2, wu2, bg2, bu2, act, err);
+  } else {
+    at::AutoDispatchBelowADInplaceOrView below;
+    h = gated_fwd(x2, wg2, wu2, bg2, bu2, act, err);
+  }
+  if (flat) return h;
+  auto sizes = x.sizes().vec();
+  sizes.back() = h.size(1);
+  return h.reshape(sizes);
 }
 
 std::tuple<at::Tensor, at::Tensor> qk_norm_rotary(const at::Tensor& q, const at::Tensor& k, const OptTensor& table,

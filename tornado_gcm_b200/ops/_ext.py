@@ -12,6 +12,8 @@ import os
 
 import torch
 
+from tornado_gcm_b200.ops import accounting as _COUNTING
+
 _LOADED = None
 _ERROR = None
 
@@ -41,11 +43,22 @@ def require(what: str = "kernel"):
         raise RuntimeError(
             f"tornado_gcm_b200 CUDA extension required for {what} but not loaded "
             f"(found {found}; error: {_ERROR}). Build it with `python setup.py build_ext --inplace`.")
-    from tornado_gcm_b200.ops import accounting
-
-    if accounting.active() is not None:
-        return accounting.CountingOps(torch.ops.tgcm)
+    if _COUNTING.active() is not None:
+        return _COUNTING.CountingOps(torch.ops.tgcm)
     return torch.ops.tgcm
+
+
+_OPS: dict = {}
+
+
+def op(name: str):
+    """The single overload of the operator ``name``, for calls where the host's time counts; counted like the others."""
+    if _COUNTING.active() is not None:
+        return getattr(require(name), name)
+    fn = _OPS.get(name)
+    if fn is None:
+        fn = _OPS[name] = getattr(require(name), name).default
+    return fn
 
 
 _POISON = os.environ.get("TGCM_POISON", "0") not in ("", "0")

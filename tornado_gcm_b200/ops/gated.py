@@ -26,21 +26,17 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
 
     On the GPU the result is BF16 and so is the arithmetic's input; on the CPU it has ``x``'s type.
     """
-    if activation not in ACT_CODES:
+    act = ACT_CODES.get(activation)
+    if act is None:
         raise ValueError(f"gated_linear: activation must be one of {sorted(ACT_CODES)}, got {activation!r}")
+    if x.is_cuda:
+        return _ext.op("gated_linear")(x, w_gate, w_up, b_gate, b_up, act, _ext.error_flag(x.device))
     if w_gate.ndim != 2 or w_gate.shape != w_up.shape or x.shape[-1] != w_gate.shape[1]:
         raise ValueError(f"gated_linear: weights (hidden, features) that match x expected, got x {tuple(x.shape)}, "
                          f"{tuple(w_gate.shape)} and {tuple(w_up.shape)}")
     if (b_gate is None) != (b_up is None):
         raise ValueError("gated_linear: both biases or none")
-    if not x.is_cuda:
-        from tornado_gcm_b200.neural.standard_layers import apply_activation
+    from tornado_gcm_b200.neural.standard_layers import apply_activation
 
-        lin = torch.nn.functional.linear
-        return apply_activation(activation, lin(x, w_gate, b_gate)) * lin(x, w_up, b_up)
-    bf = torch.bfloat16
-    args = [t if t is None or t.dtype == bf else t.to(bf) for t in (x, w_gate, w_up, b_gate, b_up)]
-    if x.ndim != 2:
-        args[0] = args[0].reshape(-1, x.shape[-1])
-    h = _ext.require("gated linear layer").gated_linear.default(*args, ACT_CODES[activation], _ext.error_flag(x.device))
-    return h if x.ndim == 2 else h.reshape(*x.shape[:-1], h.shape[-1])
+    lin = torch.nn.functional.linear
+    return apply_activation(activation, lin(x, w_gate, b_gate)) * lin(x, w_up, b_up)

@@ -30,7 +30,7 @@ def grad_norm(grads: Iterable[torch.Tensor]) -> torch.Tensor:
         return torch.zeros(())
     if not grads[0].is_cuda:
         return _plain_norm(grads)
-    return _ext.require("gradient norm").grad_norm.default(grads)
+    return _ext.op("grad_norm")(grads)
 
 
 def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
@@ -54,8 +54,7 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
         return torch.zeros(())
     if grads[0].is_cuda:
         # the operator changes its arguments in place below autograd's sight, as an optimizer does
-        return _ext.require("gradient clipping").clip_grad_norm.default(grads, [] if out is None else out_list,
-                                                                        float(max_norm))
+        return _ext.op("clip_grad_norm")(grads, [] if out is None else out_list, float(max_norm))
     with torch.no_grad():
         for g, o in zip(grads, out_list):
             if g.shape != o.shape:

@@ -103,6 +103,6 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tenso
         q = q.contiguous()
     if k.stride(-1) != 1:
         k = k.contiguous()
-    return _ext.require("head norm and rotation").qk_norm_rotary.default(
+    return _ext.op("qk_norm_rotary")(
         q, k, table, positions, q_weight, k_weight, q_bias, k_bias, NORM_CODES[norm], bool(interleaved), float(eps),
         _ext.error_flag(q.device))

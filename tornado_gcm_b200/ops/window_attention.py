@@ -68,7 +68,7 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
             raise ValueError("window_attention: q (B, S, H, D) and k, v (B, S, Hk, D) with Hk dividing H expected")
         return _torch_form(q, k, v, window, sinks, causal, lengths, scale)
     q, k, v = (t if t.stride(-1) == 1 else t.contiguous() for t in (q, k, v))
-    return _ext.require("window attention").window_attention.default(
+    return _ext.op("window_attention")(
         q, k, v, int(window), int(sinks), bool(causal), lengths, scale, _ext.error_flag(q.device))
 
 
@@ -90,8 +90,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     """
     scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
     if q.is_cuda:
-        return _ext.require("window attention step").window_attention_step.default(
-            q, k, v, k_cache, v_cache, lengths, int(sinks), scale)
+        return _ext.op("window_attention_step")(q, k, v, k_cache, v_cache, lengths, int(sinks), scale)
     cap = k_cache.shape[1]
     if not 0 <= sinks < cap:
         raise ValueError("window_attention_step: sinks must lie between 0 and the cache's slots")
