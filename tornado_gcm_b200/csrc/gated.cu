@@ -202,50 +202,71 @@ __device__ __forceinline__ uint4* piece(uint8_t* stage, int row, int c) {
   return reinterpret_cast<uint4*>(stage + row * 64 + ((c ^ ((row >> 1) & 3)) << 4));
 }
 
-// 32 x 32 bf16 tile to global memory, clipped to nrows x ncols.
+// 32 x 32 bf16 tile to global memory, clipped to nrows x ncols: four lanes to a row's 64
+// bytes, or, where rows do not start on 16-byte boundaries, one value to a lane and
+// a row to an instruction.
 __device__ __forceinline__ void tile_out(uint8_t* stage, __nv_bfloat16* g, long long ld, int nrows, int ncols,
                                          int lane) {
-  const bool vec = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  const int c = lane & 3;
+  if ((ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+    const int c = lane & 3;
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int row = it * 8 + (lane >> 2);
-    if (row >= nrows || c * 8 >= ncols) continue;
-    const uint4 v = *piece(stage, row, c);
-    __nv_bfloat16* dst = g + row * ld + c * 8;
-    if (vec && c * 8 + 8 <= ncols) {
-      *reinterpret_cast<uint4*>(dst) = v;
-    } else {
-      const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&v);
+    for (int it = 0; it < 4; ++it) {
+      const int row = it * 8 + (lane >> 2);
+      if (row >= nrows || c * 8 >= ncols) continue;
+      const uint4 v = *piece(stage, row, c);
+      __nv_bfloat16* dst = g + row * ld + c * 8;
+      if (c * 8 + 8 <= ncols) {
+        *reinterpret_cast<uint4*>(dst) = v;
+      } else {
+        const __nv_bfloat16* e = reinterpret_cast<const __nv_bfloat16*>(&v);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c * 8 + k < ncols) dst[k] = e[k];
+        for (int k = 0; k < 8; ++k)
+          if (c * 8 + k < ncols) dst[k] = e[k];
+      }
     }
+  } else if (lane < ncols) {
+#pragma unroll 8
+    for (int row = 0; row < 32; ++row)
+      if (row < nrows)
+        g[row * ld + lane] = reinterpret_cast<const __nv_bfloat16*>(piece(stage, row, lane >> 3))[lane & 7];
   }
 }
 
 __device__ __forceinline__ void tile_in(uint8_t* stage, const __nv_bfloat16* g, long long ld, int nrows, int ncols,
                                         int lane) {
-  const bool vec = (ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0;
-  const int c = lane & 3;
-  uint4 v[4];
+  if ((ld & 7) == 0 && (reinterpret_cast<uintptr_t>(g) & 15) == 0) {
+    const int c = lane & 3;
+    uint4 v[4];
 #pragma unroll
-  for (int it = 0; it < 4; ++it) {
-    const int row = it * 8 + (lane >> 2);
-    v[it] = make_uint4(0, 0, 0, 0);
-    if (row >= nrows || c * 8 >= ncols) continue;
-    const __nv_bfloat16* src = g + row * ld + c * 8;
-    if (vec && c * 8 + 8 <= ncols) {
-      v[it] = __ldg(reinterpret_cast<const uint4*>(src));
-    } else {
-      __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&v[it]);
+    for (int it = 0; it < 4; ++it) {
+      const int row = it * 8 + (lane >> 2);
+      v[it] = make_uint4(0, 0, 0, 0);
+      if (row >= nrows || c * 8 >= ncols) continue;
+      const __nv_bfloat16* src = g + row * ld + c * 8;
+      if (c * 8 + 8 <= ncols) {
+        v[it] = __ldg(reinterpret_cast<const uint4*>(src));
+      } else {
+        __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&v[it]);
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        if (c * 8 + k < ncols) e[k] = src[k];
+        for (int k = 0; k < 8; ++k)
+          if (c * 8 + k < ncols) e[k] = src[k];
+      }
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it) *piece(stage, it * 8 + (lane >> 2), c) = v[it];
+  } else {
+    const unsigned short* src = reinterpret_cast<const unsigned short*>(g);
+#pragma unroll
+    for (int r0 = 0; r0 < 32; r0 += 16) {
+      unsigned short v[16];
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        v[r] = r0 + r < nrows && lane < ncols ? __ldg(src + (r0 + r) * ld + lane) : static_cast<unsigned short>(0);
+#pragma unroll
+      for (int r = 0; r < 16; ++r)
+        reinterpret_cast<unsigned short*>(piece(stage, r0 + r, lane >> 3))[lane & 7] = v[r];
     }
   }
-#pragma unroll
-  for (int it = 0; it < 4; ++it) *piece(stage, it * 8 + (lane >> 2), c) = v[it];
 }
 
 // 32 x 16 fp32 tile (the same 64-byte rows) to global memory.
@@ -672,6 +693,23 @@ __global__ void __launch_bounds__(256) skinny_kernel(const __nv_bfloat16* __rest
   h[static_cast<long long>(lane) * F + f] = __float2bfloat16(a * zu);
 }
 
+// Rows of `from` values (any strides) to rows of `to` values behind one another, zeros behind the end: TMA's
+// 16-byte rows for matrices that have none.
+__global__ void __launch_bounds__(256) pad_rows_kernel(const __nv_bfloat16* __restrict__ in, long long row_stride,
+                                                      long long col_stride, __nv_bfloat16* __restrict__ out, int rows,
+                                                      int from, int to) {
+  for (long long i = static_cast<long long>(blockIdx.x) * 256 + threadIdx.x; i < static_cast<long long>(rows) * to / 8;
+       i += static_cast<long long>(gridDim.x) * 256) {
+    const int r = static_cast<int>(i / (to / 8)), c = static_cast<int>(i - static_cast<long long>(r) * (to / 8)) * 8;
+    uint4 v = make_uint4(0, 0, 0, 0);
+    __nv_bfloat16* e = reinterpret_cast<__nv_bfloat16*>(&v);
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (c + k < from) e[k] = in[r * row_stride + (c + k) * col_stride];
+    reinterpret_cast<uint4*>(out)[i] = v;
+  }
+}
+
 // Rows of 64 (K-major operands: 128 of them; MN-major ones: 64 steps of the reduction).
 CUtensorMap matrix_map(const at::Tensor& t, uint32_t box_rows) {
   const uint64_t dims[2] = {static_cast<uint64_t>(t.size(1)), static_cast<uint64_t>(t.size(0))};
@@ -734,9 +772,15 @@ bool tma_ok(const at::Tensor& t) {
 at::Tensor tma_rows(const at::Tensor& t) {
   if (tma_ok(t)) return t;
   const int64_t w = (t.size(1) + 7) / 8 * 8;
-  auto c = at::empty({t.size(0), w}, t.options());
-  if (w != t.size(1)) c.narrow(1, t.size(1), w - t.size(1)).zero_();
-  c.narrow(1, 0, t.size(1)).copy_(t);
+  auto c = out_empty({t.size(0), w}, t.options());
+  const int64_t blocks = std::min<int64_t>((t.size(0) * w / 8 + 255) / 256, 148 * 8);
+  if (blocks > 0) {
+    pad_rows_kernel<<<static_cast<unsigned>(blocks), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
+        reinterpret_cast<const __nv_bfloat16*>(t.data_ptr()), t.stride(0), t.stride(1),
+        reinterpret_cast<__nv_bfloat16*>(c.data_ptr()), static_cast<int>(t.size(0)), static_cast<int>(t.size(1)),
+        static_cast<int>(w));
+    C10_CUDA_KERNEL_LAUNCH_CHECK();
+  }
   return c;
 }
 
@@ -766,6 +810,13 @@ const __nv_bfloat16* bf16_or_null(const c10::optional<at::Tensor>& t) {
 __nv_bfloat16* bf16_ptr(const at::Tensor& t) { return reinterpret_cast<__nv_bfloat16*>(t.data_ptr()); }
 
 }  // namespace
+
+at::Tensor gated_rows(const at::Tensor& t) {
+  TORCH_CHECK(t.is_cuda() && t.dim() == 2 && t.scalar_type() == at::kBFloat16,
+              "gated_linear: bf16 CUDA matrices of one device expected");
+  c10::cuda::CUDAGuard guard(t.device());
+  return tma_rows(t);
+}
 
 at::Tensor gated_fwd(const at::Tensor& x_in, const at::Tensor& wg_in, const at::Tensor& wu_in,
                      const c10::optional<at::Tensor>& bg, const c10::optional<at::Tensor>& bu, int64_t act,
@@ -813,13 +864,15 @@ at::Tensor gated_fwd(const at::Tensor& x_in, const at::Tensor& wg_in, const at::
   return h;
 }
 
-// dx, dWg, dWu, dbg, dbu; the ones not asked for are undefined.
+// dx, dWg, dWu, dbg, dbu; the ones not asked for are undefined.  x and the weights may be padded (gated_rows): the
+// first `features` columns count.
 std::vector<at::Tensor> gated_bwd(const at::Tensor& dh_in, const at::Tensor& x_in, const at::Tensor& wg_in,
                                   const at::Tensor& wu_in, const c10::optional<at::Tensor>& bg,
-                                  const c10::optional<at::Tensor>& bu, int64_t act, bool need_x, bool need_w,
+                                  const c10::optional<at::Tensor>& bu, int64_t act, int64_t features, bool need_x, bool need_w,
                                   bool need_b, const c10::optional<at::Tensor>& err) {
   check_gated(x_in, wg_in, wu_in, bg, bu, act);
-  const int64_t T = x_in.size(0), F = wg_in.size(0), K0 = x_in.size(1);
+  const int64_t T = x_in.size(0), F = wg_in.size(0), K0 = features;
+  TORCH_CHECK(K0 >= 1 && K0 <= x_in.size(1), "gated_linear backward: features beyond x's rows");
   TORCH_CHECK(dh_in.dim() == 2 && dh_in.size(0) == T && dh_in.size(1) == F && dh_in.device() == x_in.device() &&
                   dh_in.scalar_type() == at::kBFloat16 && (F == 1 || dh_in.stride(1) == 1),
               "gated_linear backward: the gradient must be bf16 (tokens, hidden) with contiguous rows");

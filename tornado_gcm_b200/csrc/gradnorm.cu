@@ -210,7 +210,18 @@ __device__ __forceinline__ void scale_chunk(const Ti* in, To* out, int n, float 
     for (; i < nv; i += kNormThreads) put(i, vi[i]);
     done = nv * V;
   }
-  for (int j = done + threadIdx.x; j < n; j += kNormThreads) out[j] = scaled<To, C>(to_f(in[j]), coef);
+  // What is left, or all of it where the two sides are not aligned to each other (views of a flat buffer behind
+  // a tensor of odd size): single values, every warp access still one run of memory.
+  constexpr int S = 16;
+  int j = done + threadIdx.x;
+  for (; j + (S - 1) * kNormThreads < n; j += S * kNormThreads) {
+    Ti a[S];
+#pragma unroll
+    for (int u = 0; u < S; ++u) a[u] = in[j + u * kNormThreads];
+#pragma unroll
+    for (int u = 0; u < S; ++u) out[j + u * kNormThreads] = scaled<To, C>(to_f(a[u]), coef);
+  }
+  for (; j < n; j += kNormThreads) out[j] = scaled<To, C>(to_f(in[j]), coef);
 }
 
 // Pass 2.  Block 0 of the last launch writes the norm; with `in_place` and a

@@ -49,9 +49,11 @@ std::vector<int64_t> kept(AutogradContext* ctx) { return ctx->saved_data["cfg"].
 struct GatedLinear : torch::autograd::Function<GatedLinear> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu,
                             const OptTensor& bg, const OptTensor& bu, int64_t act, const OptTensor& err) {
-    ctx->save_for_backward({x, wg, wu, undef_or(bg), undef_or(bu)});
-    keep(ctx, {act, wants(x), wants(wg) || wants(wu), wants(bg) || wants(bu)}, err);
-    return gated_fwd(x, wg, wu, bg, bu, act, err);
+    // rows that had to be padded are padded once for both passes
+    const at::Tensor xr = gated_rows(x), wgr = gated_rows(wg), wur = gated_rows(wu);
+    ctx->save_for_backward({xr, wgr, wur, undef_or(bg), undef_or(bu)});
+    keep(ctx, {act, x.size(1), wants(x), wants(wg) || wants(wu), wants(bg) || wants(bu)}, err);
+    return gated_fwd(xr, wgr, wur, bg, bu, act, err);
   }
   static variable_list backward(AutogradContext* ctx, variable_list g) {
     const auto s = ctx->get_saved_variables();
@@ -59,7 +61,7 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     const auto c = kept(ctx);
     const at::Tensor dh = g[0].scalar_type() == at::kBFloat16 ? g[0] : g[0].to(at::kBFloat16);
     auto r = gated_bwd(dh.size(1) == 1 || dh.stride(1) == 1 ? dh : dh.contiguous(), s[0], s[1], s[2], opt(s[3]),
-                       opt(s[4]), c[0], c[1], c[2], c[3], flag_of(ctx));
+                       opt(s[4]), c[0], c[1], c[2], c[3], c[4], flag_of(ctx));
     return {r[0], r[1], r[2], s[3].defined() ? r[3] : at::Tensor(), s[4].defined() ? r[4] : at::Tensor(),
             at::Tensor(), at::Tensor()};
   }

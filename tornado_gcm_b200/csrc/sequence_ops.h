@@ -10,12 +10,14 @@ namespace tgcm {
 
 using OptTensor = c10::optional<at::Tensor>;
 
+// t itself where its rows can be read as they are, else a copy with rows padded by zeros to 16 bytes
+at::Tensor gated_rows(const at::Tensor& t);
 at::Tensor gated_fwd(const at::Tensor& x, const at::Tensor& wg, const at::Tensor& wu, const OptTensor& bg,
                      const OptTensor& bu, int64_t act, const OptTensor& err);
-// dx, dWg, dWu, dbg, dbu; the ones not asked for are undefined
+// dx, dWg, dWu, dbg, dbu; the ones not asked for are undefined.  x and the weights as gated_rows left them
 std::vector<at::Tensor> gated_bwd(const at::Tensor& dh, const at::Tensor& x, const at::Tensor& wg,
                                   const at::Tensor& wu, const OptTensor& bg, const OptTensor& bu, int64_t act,
-                                  bool need_x, bool need_w, bool need_b, const OptTensor& err);
+                                  int64_t features, bool need_x, bool need_w, bool need_b, const OptTensor& err);
 
 std::vector<at::Tensor> qk_norm_rotary_fwd(const at::Tensor& q, const at::Tensor& k, const OptTensor& table,
                                            const OptTensor& positions, const OptTensor& qw, const OptTensor& kw,

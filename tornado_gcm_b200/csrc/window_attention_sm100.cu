@@ -6,19 +6,25 @@
 // other side that are in sight of them: a run of tiles through the window,
 // and the sinks.  Warp 0 feeds a ring of shared-memory slots by TMA, one
 // thread of warp 1 issues tcgen05.mma, warps 2-5 own one row to a thread and
-// do the softmax arithmetic on accumulators read from TMEM; the weights (or
-// their gradients) go back to TMEM as bf16, where they are the A operand of the
-// next product.  Nothing of the size of the score matrix leaves the SM.
+// do the softmax arithmetic on accumulators read from TMEM; the weights and
+// their gradients are the A operand of the next product as bf16, from TMEM
+// (forward) or shared memory (backward, where TMEM is full).  Nothing of the
+// size of the score matrix leaves the SM.
 //
-// What bounds them: 128 x 128 scores are 16 384 exponentials, 1024 cycles of
-// the SM's 16 a cycle, against 512 cycles of products at D = 64; so two CTAs
-// share an SM (tiles sized for half of its TMEM and shared memory) and one's
-// products run under the other's exponentials.  Only at D = 128 do dk and dv
-// need all of TMEM; that kernel keeps two score tiles in flight instead.
-//   D <= 64:  forward 128-key tiles (S 128, P 64, O 64 columns),
+// What bounds them: 128 x 64 scores are 8192 exponentials, 512 cycles of the
+// SM's 16 a cycle, against 256 cycles of products at D = 64, but a tile's way
+// through wait, accumulator read, maximum, exponentials and write-back takes one
+// CTA 1400 cycles (2950 in dk/dv).  So two CTAs share an SM (tiles sized for half of
+// its TMEM and shared memory), and the next tile's scores are made while this
+// one's are worked on.  Only at D = 128 do dk and dv need all of TMEM.
+// Measured on 2 x 8192 tokens, 16 + 4 heads of 64, window 512, 4 sinks: forward 97
+// us, dq 130 us, dk/dv 182 us.  Eight softmax warps instead of four, smaller TMEM
+// shares for three or four CTAs, and weights kept in TMEM in the backward were
+// each tried and took as long or longer.
+//   D <= 64:  forward 64-key tiles (2 x S, under P, 64, O 64 columns),
 //             dq 64-key tiles (S, dP, dQ 64 each),
 //             dk/dv 64-query tiles (S, dP, dV, dK 64 each)
-//   D <= 128: forward 64-key tiles (S 64, P 32, O 128),
+//   D <= 128: forward 64-key tiles (2 x S, under P, 64, O 128),
 //             dq 64-key tiles (S 64, dP 64, dQ 128),
 //             dk/dv 64-query tiles (2 x (S, dP 64), dV, dK 128)
 // A head narrower than its tile is filled with zeros by TMA; products run over
@@ -679,19 +685,37 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive(s_empty);
+      const bool whole = j >= from && j < to;
+      if (kt.n == 1) {
+        // The row's few keys are all here: delta from the weights themselves.  From O it would carry O's rounding
+        // to bf16, which is as large as dS's own when a row has two or three keys.
+        const Sight si = whole ? words(~0ull) : sight_of(p, kt, L, i, j, j0);
+        delta = 0.f;
 #pragma unroll
-      for (int e = 0; e < KT; e += 2) {
-        float2 w = fma2(make_float2(s[e], s[e + 1]), c2, lse2);
-        w.x = ex2(w.x);
-        w.y = ex2(w.y);
-        w = mul2(w, add2(make_float2(dp[e], dp[e + 1]), delta2));
-        s[e] = w.x;
-        s[e + 1] = w.y;
-      }
-      if (j < from || j >= to) {
-        const Sight si = sight_of(p, kt, L, i, j, j0);
+        for (int e = 0; e < KT; ++e) {
+          const bool on = si.w[e >> 5] & (1u << (e & 31));
+          s[e] = on ? ex2(fmaf(s[e], c, -lse)) : 0.f;
+          dp[e] = on ? dp[e] : 0.f;
+          delta = fmaf(s[e], dp[e], delta);
+        }
+        if (i < p.S) p.delta[srow] = delta;
 #pragma unroll
-        for (int e = 0; e < KT; ++e) s[e] = (si.w[e >> 5] & (1u << (e & 31))) ? s[e] : 0.f;
+        for (int e = 0; e < KT; ++e) s[e] *= dp[e] - delta;
+      } else {
+#pragma unroll
+        for (int e = 0; e < KT; e += 2) {
+          float2 w = fma2(make_float2(s[e], s[e + 1]), c2, lse2);
+          w.x = ex2(w.x);
+          w.y = ex2(w.y);
+          w = mul2(w, add2(make_float2(dp[e], dp[e + 1]), delta2));
+          s[e] = w.x;
+          s[e + 1] = w.y;
+        }
+        if (!whole) {
+          const Sight si = sight_of(p, kt, L, i, j, j0);
+#pragma unroll
+          for (int e = 0; e < KT; ++e) s[e] = (si.w[e >> 5] & (1u << (e & 31))) ? s[e] : 0.f;
+        }
       }
       if (j > 0) {  // the product before has read dS
         if (!(ok = warp_wait(dq_done, (j - 1) & 1, err, kErrTimeoutTmemFull))) break;

@@ -10,7 +10,7 @@
 // Bound by reading the cache once: 2 D values for each slot and key head
 // against 4 D FLOP per query head; the query heads that share a key head are
 // scored together while its rows are on the SM.  bf16 rows go through warp matrix
-// instructions (step_mma_kernel); fp32 ones, and head sizes off 16, through
+// instructions (step_mma_kernel); fp32 ones, and head sizes off 8, through
 // step_kernel: a group of LPK lanes covers a slot's row with one 16-byte vector
 // each, a warp reads 32 / LPK rows of K and of V per load, kUnroll of them in
 // flight, and each lane group keeps its own running maximum, sum and output,
@@ -153,7 +153,7 @@ __device__ __forceinline__ void put_token(const StepParams& p, const StepShare& 
     }
 }
 
-// ── bf16, D a multiple of 16: warp matrix instructions ─────────────────────
+// ── bf16, D a multiple of 8: warp matrix instructions ──────────────────────
 // A warp takes 16 slots at a time: S (16 heads x 16 slots) = q K^T and
 // O (16 heads x D) += P V, up to 8 of the 16 head rows in use.  One token's few
 // query heads cannot fill a tcgen05 tile (128 rows), and the kernel is bound by
@@ -164,7 +164,7 @@ __device__ __forceinline__ void put_token(const StepParams& p, const StepShare& 
 // deeper rings, 59 us against 62 with three and 71 with four); rows are padded by 16 bytes so
 // that the eight rows of a matrix load lie in different banks.  P enters the
 // second product as two bf16 terms (value and remainder): its rounding would
-// otherwise be as large as the output's own.
+// otherwise be as large as the output's own.  Heads are filled up to 16 with zeros.
 constexpr int kStages = 2;
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool on) {
@@ -232,12 +232,13 @@ __global__ void __launch_bounds__(kStepThreads) step_mma_kernel(const __grid_con
 #pragma unroll
       for (int e = lane; e < 16 * 2 * ND; e += 32) {
         const int r = e / (2 * ND), c = e % (2 * ND), j = j0 + r;
-        const bool on = j < w.s1;
+        const bool on = j < w.s1 && c * 8 < p.D;
         const int js = on ? j : w.s0;
         const T* ks = js == w.slot ? kn : kc + js * p.kc_ss;
         const T* vs = js == w.slot ? vn : vc + js * p.vc_ss;
-        cp_async16(dst + r * C::kRow + c * 16, ks + c * 8, on);
-        cp_async16(dst + 16 * C::kRow + r * C::kRow + c * 16, vs + c * 8, on);
+        const int d = on ? c * 8 : 0;
+        cp_async16(dst + r * C::kRow + c * 16, ks + d, on);
+        cp_async16(dst + 16 * C::kRow + r * C::kRow + c * 16, vs + d, on);
       }
     }
     asm volatile("cp.async.commit_group;" ::: "memory");
@@ -252,7 +253,8 @@ __global__ void __launch_bounds__(kStepThreads) step_mma_kernel(const __grid_con
     for (int s = 0; s < ND; ++s)
 #pragma unroll
       for (int u = 0; u < 2; ++u)
-        qa[s][u] = g < w.heads ? *reinterpret_cast<const uint32_t*>(qr + s * 16 + u * 8 + 2 * t) : 0u;
+        qa[s][u] = g < w.heads && s * 16 + u * 8 < p.D
+                       ? *reinterpret_cast<const uint32_t*>(qr + s * 16 + u * 8 + 2 * t) : 0u;
   }
   const float sc = p.scale * kLog2e;
   float o[2 * ND][4];
@@ -592,8 +594,8 @@ at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const
   p.scale = static_cast<float>(scale);
   const int64_t group = H / Hk;
   p.vec = D % (16 / q.element_size()) == 0 && rows16(q) && rows16(k) && rows16(v) && rows16(k_cache) && rows16(v_cache);
-  // Rows of whole 32-byte steps of bf16 go to the matrix instructions, the rest to fp32 arithmetic.
-  const bool mma = q.scalar_type() == at::kBFloat16 && p.vec && D % 16 == 0;
+  // Rows of whole 16-byte pieces of bf16 go to the matrix instructions, the rest to fp32 arithmetic.
+  const bool mma = q.scalar_type() == at::kBFloat16 && p.vec;
   const int64_t most = mma ? 8 : 4;
   p.heads_per_block = static_cast<int>(mma ? std::min(group, most) : (group >= 3 ? 4 : group));
   p.head_blocks = static_cast<int>((group + p.heads_per_block - 1) / p.heads_per_block);
@@ -606,7 +608,7 @@ at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const
   TORCH_CHECK(p.Hk * static_cast<int64_t>(p.head_blocks) <= 65535, "window_attention_step: too many heads");
   const int nb = static_cast<int>(B);
   if (mma)
-    switch (D / 16) {
+    switch ((D + 15) / 16) {
       case 1: launch_mma<1>(p, splits, nb, st); break;
       case 2: launch_mma<2>(p, splits, nb, st); break;
       case 3: launch_mma<3>(p, splits, nb, st); break;
