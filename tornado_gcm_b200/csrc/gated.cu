@@ -49,11 +49,16 @@ namespace {
 
 constexpr int kEpilogueWarps = 16;              // four to a scheduler: one warp's epilogue is mostly latency
 constexpr int kPairThreads = 64 + 32 * kEpilogueWarps;
-constexpr int kPairStages = 6;
 constexpr int kOperand = 128 * 128;             // bytes: 128 rows of 64 bf16
 constexpr int kPairStage = 2 * kOperand;
 constexpr int kWarpStage = 32 * 64;             // bytes: one epilogue warp's 32 x 32 bf16 tile
-constexpr int kPairSmem = kPairStages * kPairStage + kEpilogueWarps * kWarpStage + 256 + 1024;
+// Ring stages: kDact gives one up for the tiles of dh, which are on their way while the tile before is worked on.
+template <int MODE>
+struct PairCfg {
+  static constexpr int kStages = MODE == 1 ? 5 : 6;
+  static constexpr int kStaging = (MODE == 1 ? 2 : 1) * kEpilogueWarps * kWarpStage;
+  static constexpr int kSmem = kStages * kPairStage + kStaging + 256 + 1024;
+};
 constexpr int kSkinnyTokens = 8;
 
 enum PairMode : int { kFwd = 0, kDact = 1, kDx = 2, kDw = 3 };
@@ -269,6 +274,23 @@ __device__ __forceinline__ void tile_in(uint8_t* stage, const __nv_bfloat16* g, 
   }
 }
 
+// The same by asynchronous copies; false where rows do not start on 16-byte boundaries.
+__device__ __forceinline__ bool tile_in_async(uint8_t* stage, const __nv_bfloat16* g, long long ld, int nrows,
+                                              int ncols, int lane) {
+  if ((ld & 7) != 0 || (reinterpret_cast<uintptr_t>(g) & 15) != 0) return false;
+  const int c = lane & 3;
+#pragma unroll
+  for (int it = 0; it < 4; ++it) {
+    const int row = it * 8 + (lane >> 2);
+    const int have = row < nrows ? max(0, min(8, ncols - c * 8)) * 2 : 0;  // bytes; the rest is zeros
+    const __nv_bfloat16* src = have > 0 ? g + row * ld + c * 8 : g;
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem_u32(piece(stage, row, c))),
+                 "l"(src), "r"(have)
+                 : "memory");
+  }
+  return true;
+}
+
 // 32 x 16 fp32 tile (the same 64-byte rows) to global memory.
 __device__ __forceinline__ void tile_out_f32(uint8_t* stage, float* g, long long ld, int nrows, int ncols, int lane) {
   const int c = lane & 3;  // part_ld is a multiple of 4
@@ -344,8 +366,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
 
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  constexpr int kPairStages = PairCfg<MODE>::kStages;
   uint8_t* staging = smem + kPairStages * kPairStage;
-  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + kEpilogueWarps * kWarpStage);  // the leader's are used
+  uint64_t* full_bar = reinterpret_cast<uint64_t*>(staging + PairCfg<MODE>::kStaging);  // the leader's are used
   uint64_t* empty_bar = full_bar + kPairStages;
   uint64_t* acc_full = empty_bar + kPairStages;   // [2]
   uint64_t* acc_empty = acc_full + 2;             // [2], the leader's are used
@@ -459,6 +482,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
   } else {
     const int q = warp & 3, part = (warp - 2) >> 2;  // TMEM lanes, quarter of the tile's columns
     uint8_t* stage = staging + (warp - 2) * kWarpStage;
+    // kDact: dh of the tile to come, asked for as soon as this tile's du has left its place
+    uint8_t* dh_stage = staging + (kEpilogueWarps + warp - 2) * kWarpStage;
+    auto fetch_dh = [&](int t) {
+      if (t < n_tiles) {
+        const PairTile c = pair_tile<MODE>(p, t);
+        const int row0 = c.tm * 256 + rank * 128 + q * 32, col0 = c.tn * kTileN + part * (kTileN / 4);
+        const int nrows = min(32, p.M - row0), ncols = p.N - col0;
+        if (nrows > 0 && ncols > 0) {
+          const __nv_bfloat16* src = p.dh + static_cast<long long>(row0) * p.dh_ld + col0;
+          if (!tile_in_async(dh_stage, src, p.dh_ld, nrows, ncols, lane))
+            tile_in(dh_stage, src, p.dh_ld, nrows, ncols, lane);
+        } else {
+#pragma unroll
+          for (int v = 0; v < 4; ++v) *piece(dh_stage, lane, v) = make_uint4(0, 0, 0, 0);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    if constexpr (MODE == kDact) fetch_dh(first);
     int n = 0;
     for (int t = first; t < n_tiles; t += step) {
       const PairTile c = pair_tile<MODE>(p, t);
@@ -472,11 +514,6 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
           bias = static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p.bias_g) + col0 + lane)) |
                  static_cast<uint32_t>(__ldg(reinterpret_cast<const unsigned short*>(p.bias_u) + col0 + lane)) << 16;
       }
-      if constexpr (MODE == kDact) {
-        __syncwarp();
-        tile_in(stage, p.dh + static_cast<long long>(row0) * p.dh_ld + col0, p.dh_ld, nrows, p.N - col0, lane);
-        __syncwarp();
-      }
       const int acc = n & 1;
       if (c.nkb > 0) {
         const bool have = mbar_park(&acc_full[acc], (n >> 1) & 1, p.err, kErrTimeoutTmemFull);
@@ -484,10 +521,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         tc_fence_after();
         ++n;
       }
+      if constexpr (MODE == kDact) {
+        asm volatile("cp.async.wait_group 0;" ::: "memory");
+        __syncwarp();  // every lane's part of dh has landed, and the staging tile has been read
+      }
       const uint32_t ta = tmem + acc * 256 + (static_cast<uint32_t>(q * 32) << 16);
       if constexpr (MODE == kFwd || MODE == kDact) {
-        uint32_t keep[16];  // kDact: du, packed
-#pragma unroll
+        // One body for both chunks: unrolled, the recompute's instructions outgrow their cache (8192 tokens,
+        // 384 x 1000: 34.7 us with two bodies, 31.5 with one).
+#pragma unroll 1
         for (int ch = 0; ch < 2; ++ch) {
           uint32_t g[16], u[16];
           tmem_ld_32x32b_x16(ta + colw + ch * 16, g);
@@ -507,7 +549,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
             uint32_t dh[8];
 #pragma unroll
             for (int v = 0; v < 2; ++v) {
-              const uint4 w = *piece(stage, lane, ch * 2 + v);
+              const uint4 w = *piece(dh_stage, lane, ch * 2 + v);
               dh[4 * v] = w.x, dh[4 * v + 1] = w.y, dh[4 * v + 2] = w.z, dh[4 * v + 3] = w.w;
             }
             dgate16(p.act, g, u, dh);
@@ -517,8 +559,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
               if (col < p.N)  // the lower half of the warp has the gate's sums to write, the upper the other's
                 p.bias_part[(static_cast<long long>(row0 >> 5) * 2 + (lane >> 4)) * p.N + col] = lane < 16 ? sg : su;
             }
-#pragma unroll
-            for (int v = 0; v < 8; ++v) keep[ch * 8 + v] = pack2(u[2 * v], u[2 * v + 1]);
+            *piece(dh_stage, lane, ch * 2) = pack8(u, 0);  // du takes dh's place
+            *piece(dh_stage, lane, ch * 2 + 1) = pack8(u, 8);
           }
           *piece(stage, lane, ch * 2) = pack8(g, 0);
           *piece(stage, lane, ch * 2 + 1) = pack8(g, 8);
@@ -527,14 +569,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         __syncwarp();
         if (lane == 0) arrive_cluster(leader_addr(&acc_empty[acc]));
         tile_out(stage, p.out[0] + static_cast<long long>(row0) * p.ld + col0, p.ld, nrows, p.N - col0, lane);
-        __syncwarp();
         if constexpr (MODE == kDact) {
-#pragma unroll
-          for (int v = 0; v < 4; ++v)
-            *piece(stage, lane, v) = make_uint4(keep[4 * v], keep[4 * v + 1], keep[4 * v + 2], keep[4 * v + 3]);
+          tile_out(dh_stage, p.out[1] + static_cast<long long>(row0) * p.ld + col0, p.ld, nrows, p.N - col0, lane);
           __syncwarp();
-          tile_out(stage, p.out[1] + static_cast<long long>(row0) * p.ld + col0, p.ld, nrows, p.N - col0, lane);
+          fetch_dh(t + step);
         }
+        __syncwarp();
       } else {
         const bool parts = MODE == kDw && p.splits > 1;
         if (parts) {
@@ -579,6 +619,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kPairThreads, 1)
         if (lane == 0 && c.nkb > 0) arrive_cluster(leader_addr(&acc_empty[acc]));
       }
     }
+    if constexpr (MODE == kDact) asm volatile("cp.async.wait_group 0;" ::: "memory");
   }
 
   tc_fence_before();
@@ -726,12 +767,12 @@ int resident_pairs() {
   C10_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev < 64 && pairs[dev] > 0) return pairs[dev];
   auto kern = pair_gemm_kernel<kFwd>;
-  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+  C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<kFwd>::kSmem));
   const int sms = at::cuda::getCurrentDeviceProperties()->multiProcessorCount;
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3(sms / 2 * 2);
   cfg.blockDim = dim3(kPairThreads);
-  cfg.dynamicSmemBytes = kPairSmem;
+  cfg.dynamicSmemBytes = PairCfg<kFwd>::kSmem;
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -753,10 +794,10 @@ void launch_pair(const PairMaps& maps, const PairParams& p, int tiles, cudaStrea
   int dev = 0;
   C10_CUDA_CHECK(cudaGetDevice(&dev));
   if (dev >= 64 || !set[dev]) {
-    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, kPairSmem));
+    C10_CUDA_CHECK(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, PairCfg<MODE>::kSmem));
     if (dev < 64) set[dev] = true;
   }
-  kern<<<2 * std::max(1, std::min(tiles, resident_pairs())), kPairThreads, kPairSmem, st>>>(maps, p);
+  kern<<<2 * std::max(1, std::min(tiles, resident_pairs())), kPairThreads, PairCfg<MODE>::kSmem, st>>>(maps, p);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
