@@ -172,6 +172,14 @@ __device__ __forceinline__ void umma_ts(uint32_t tmem_d, uint32_t tmem_a, uint32
       : "memory");
 }
 
+// Start of a kernel's work: waits until the kernel before it in the stream has ended and its
+// writes are seen, then lets the next one's blocks come in beside this one's.  Before this
+// call a block touches nothing but its own shared memory, tensor memory and parameters.
+__device__ __forceinline__ void after_previous() {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // One lane of a converged warp, the same one every time.
 __device__ __forceinline__ bool elect_lane() {
   uint32_t is;
