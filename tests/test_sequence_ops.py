@@ -389,6 +389,52 @@ def test_window_attention_on_another_stream_and_in_a_graph():
     assert torch.equal(captured, window_attention(q, k, v, window=99, sinks=1))
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [64, 72, 128, 30])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("bad", [float("nan"), float("inf")])
+def test_window_attention_passes_on_what_is_not_finite(dtype, D, causal, bad):
+    """One key holds NaN, or an infinity in one component: the queries that get a NaN or plus infinity for a score
+    give NaN, all others what they would give anyway.  The key stands at another place of its tile in every batch."""
+    from tornado_gcm_b200.ops.window_attention import window_attention
+
+    B, S, H, W = 64, 200, 1, 90
+    q, k, v = (_randn(B, S, H, D, seed=i, dtype=dtype) for i in range(3))
+    b = torch.arange(B, device=DEV)
+    k[b, 64 + b, 0, 3] = 0.0
+    sound = window_attention(q, k, v, window=W, causal=causal)
+    k[b, 64 + b, 0, 3] = bad
+    got = window_attention(q, k, v, window=W, causal=causal)
+    i, j = torch.arange(S, device=DEV)[None], (64 + b)[:, None]
+    see = ((i - j) < W) & (i >= j) if causal else (i - j).abs() < W
+    hit = see if bad != bad else see & (q[:, :, 0, 3] > 0)
+    assert torch.equal(got.isnan().all(-1)[..., 0], hit)
+    assert torch.equal(got.isnan().any(-1)[..., 0], hit)
+    apart = ~see[..., None, None].expand_as(got)
+    assert torch.equal(got[apart], sound[apart])
+    qg, kg, vg = (t.clone().requires_grad_() for t in (q, k, v))
+    dq, _, dv = torch.autograd.grad(window_attention(qg, kg, vg, window=W, causal=causal), [qg, kg, vg],
+                                    torch.ones_like(q))
+    assert dq[hit].isnan().all()
+    seen = torch.stack([torch.zeros(S, dtype=torch.bool, device=DEV)] * B)
+    for n in range(S):  # keys that a query with NaN for a result sees
+        far = ((i - n) < W) & (i >= n) if causal else (i - n).abs() < W
+        seen[:, n] = (hit & far).any(-1)
+    assert dv[seen].isnan().all()
+
+
+@pytest.mark.parametrize("scale", [0.0, -0.125, float("inf"), float("nan"), 1e-60])
+def test_window_attention_scale_refusals(scale):
+    from tornado_gcm_b200.ops.window_attention import window_attention, window_attention_step
+
+    q = torch.zeros(1, 4, 1, 64, device=DEV)
+    with pytest.raises((RuntimeError, ValueError), match="scale must be positive and finite"):
+        window_attention(q, q, q, window=2, scale=scale)
+    n = torch.zeros(1, dtype=torch.int32, device=DEV)
+    with pytest.raises((RuntimeError, ValueError), match="scale must be positive and finite"):
+        window_attention_step(q[:, 0], q[:, 0], q[:, 0], q.clone(), q.clone(), n, scale=scale)
+
+
 def test_window_attention_refusals():
     from tornado_gcm_b200.ops.window_attention import window_attention
 

@@ -435,6 +435,7 @@ WinParams params_of(const at::Tensor& q, const at::Tensor& k, const at::Tensor& 
   p.sinks = static_cast<int>(std::min<int64_t>(sinks, p.S));
   p.causal = causal;
   p.scale = static_cast<float>(scale);
+  TORCH_CHECK(p.scale > 0.f && p.scale < INFINITY, "window_attention: the scale must be positive and finite");
   if (lengths.has_value() && lengths->defined()) {
     TORCH_CHECK(lengths->device() == q.device() && lengths->scalar_type() == at::kInt && lengths->is_contiguous() &&
                     lengths->dim() == 1 && lengths->size(0) == q.size(0),

@@ -91,10 +91,17 @@ __device__ __forceinline__ void tmem_st_32x32b_x16(uint32_t taddr, const uint32_
 __device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void fence_async_smem() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+// Largest of three, NaN if one is.
+__device__ __forceinline__ float max_nan(float a, float b, float c) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+
 // 2^t of two values on the FMA pipe: t = n + f with |f| <= 1/2 (n by adding and
 // taking away 1.5 * 2^23), a cubic for 2^f (least largest relative error on the
 // interval, 7.5e-5: a twentieth of a bf16 weight's rounding), n into the
-// exponent.  t below -126 gives 2^-126.
+// exponent.  t below -126 gives 2^-126, and so does NaN.
 __device__ __forceinline__ float2 ex2_poly2(float2 t) {
   t.x = fmaxf(t.x, -126.f);
   t.y = fmaxf(t.y, -126.f);
@@ -395,13 +402,14 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
 #pragma unroll
       for (int e = 0; e < KT; e += 8)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) t4[u] = fmaxf(fmaxf(t4[u], s[e + u]), s[e + u + 4]);
-      const float mx = fmaxf(fmaxf(t4[0], t4[1]), fmaxf(t4[2], t4[3])) * c;
+        for (int u = 0; u < 4; ++u) t4[u] = max_nan(t4[u], s[e + u], s[e + u + 4]);
+      float mx = max_nan(max_nan(t4[0], t4[1], t4[2]), t4[3], t4[3]) * c;
+      mx = mx < INFINITY ? mx : NAN;  // a score that is NaN or infinite makes the row NaN, as its softmax is
       float f = 1.f;
       bool raise = false;
       if (m == -INFINITY) {
         m = mx;
-      } else if (mx > m + 8.f) {
+      } else if (!(mx <= m + 8.f)) {
         f = ex2(m - mx);
         m = mx;
         l2 = mul2(l2, make_float2(f, f));

@@ -575,6 +575,8 @@ at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const
   TORCH_CHECK(lengths.device() == q.device() && lengths.scalar_type() == at::kInt && lengths.is_contiguous() &&
                   lengths.dim() == 1 && lengths.size(0) == B,
               "window_attention_step: lengths must be a contiguous int32 vector of one value for each sequence");
+  TORCH_CHECK(static_cast<float>(scale) > 0.f && static_cast<float>(scale) < INFINITY,
+              "window_attention_step: the scale must be positive and finite");
   TORCH_CHECK(B <= 65535 && H <= 65535, "window_attention_step: batch and heads up to 65535");
   c10::cuda::CUDAGuard guard(q.device());
   auto o = out_empty({B, H, D}, q.options());

@@ -49,6 +49,15 @@ def _torch_form(q, k, v, window, sinks, causal, lengths, scale):
     return (p @ vh).transpose(1, 2).to(q.dtype)
 
 
+def _scale(q: torch.Tensor, scale: Optional[float], name: str) -> float:
+    if scale is None:
+        return q.shape[-1] ** -0.5
+    scale = float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError(f"{name}: the scale must be positive and finite, got {scale}")
+    return scale
+
+
 def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, window: int, sinks: int = 0,
                      causal: bool = True, lengths: Optional[torch.Tensor] = None,
                      scale: Optional[float] = None) -> torch.Tensor:
@@ -56,13 +65,14 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
 
     bf16 or fp32, ``D`` up to 128, any strides with a contiguous last axis.  ``lengths``: int32 ``(B,)``, the number
     of valid keys of every sequence (what lies behind may hold anything, NaN included); a query that sees no key
-    gives zeros and no gradient.  ``scale`` defaults to ``D ** -0.5``.
+    gives zeros and no gradient, one that sees a score of NaN or plus infinity gives NaN.  ``scale`` (positive)
+    defaults to ``D ** -0.5``.
     """
     if window < 1:
         raise ValueError(f"window_attention: the window must hold at least the token itself, got {window}")
     if sinks < 0:
         raise ValueError(f"window_attention: sinks must not be negative, got {sinks}")
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = _scale(q, scale, "window_attention")
     if not q.is_cuda:
         if q.ndim != 4 or k.shape != v.shape or q.shape[2] % k.shape[2]:
             raise ValueError("window_attention: q (B, S, H, D) and k, v (B, S, Hk, D) with Hk dividing H expected")
@@ -88,7 +98,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     writes the same slots).  A negative length marks a sequence that takes no part: zeros, its cache untouched.
     The result equals the last row of :func:`window_attention` with ``causal`` over the whole history.
     """
-    scale = q.shape[-1] ** -0.5 if scale is None else float(scale)
+    scale = _scale(q, scale, "window_attention_step")
     if q.is_cuda:
         return _ext.op("window_attention_step")(q, k, v, k_cache, v_cache, lengths, int(sinks), scale)
     cap = k_cache.shape[1]
