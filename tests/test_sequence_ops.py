@@ -423,6 +423,31 @@ def test_window_attention_passes_on_what_is_not_finite(dtype, D, causal, bad):
     assert dv[seen].isnan().all()
 
 
+@pytest.mark.parametrize("dtype,D", [(torch.bfloat16, 64), (torch.bfloat16, 128), (torch.bfloat16, 30),
+                                     (torch.float32, 32)])
+@pytest.mark.parametrize("S,window,sinks,causal,length", [
+    (300, 1, 0, True, None), (300, 1, 0, False, None), (300, 7, 0, True, 1), (300, 400, 1, False, 1),
+    (700, 3, 1, True, 1), (1, 5, 2, True, None), (40, 1, 0, False, None)])
+def test_window_attention_one_key_has_no_score_gradient(dtype, D, S, window, sinks, causal, length):
+    """Where every query sees one key or none its weight is 1 whatever the score: dq and dk are zeros, dv sums dO."""
+    from tornado_gcm_b200.ops.window_attention import window_attention
+
+    B, H, Hk = 2, 4, 2
+    q, k, v, g = (_randn(B, S, h, D, seed=i, dtype=dtype).requires_grad_() for i, h in enumerate((H, Hk, Hk, H)))
+    n = None if length is None else torch.full((B,), length, dtype=torch.int32, device=DEV)
+    o = window_attention(q, k, v, window=window, sinks=sinks, causal=causal, lengths=n)
+    dq, dk, dv = torch.autograd.grad(o, [q, k, v], g)
+    assert not dq.any() and not dk.any()
+    i, j = torch.arange(S, device=DEV)[:, None], torch.arange(S, device=DEV)[None]
+    see = (j < (S if length is None else length)) & (((i - j).abs() < window) | (j < sinks))
+    if causal:
+        see &= i >= j
+    assert (see.sum(1) <= 1).all()
+    want = torch.einsum("ij,bihd->bjhd", see.double(), g.detach().double().view(B, S, Hk, H // Hk, D).sum(3))
+    # weights of 1 within an ulp or two of fp32; one rounding of the result
+    _close(dv, want, 4e-3 if dtype == torch.bfloat16 else 2e-6, "dv")
+
+
 @pytest.mark.parametrize("scale", [0.0, -0.125, float("inf"), float("nan"), 1e-60])
 def test_window_attention_scale_refusals(scale):
     from tornado_gcm_b200.ops.window_attention import window_attention, window_attention_step

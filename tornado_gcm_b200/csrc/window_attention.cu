@@ -142,7 +142,7 @@ __device__ __forceinline__ void axpy_share(float (&a)[N], float f, const float* 
 template <int DP>
 struct RowShape {
   static constexpr int kGroups = DP <= 32 ? 4 : 2;
-  static constexpr int kTileBytes = 2 * kTile * DP * 4 + 2 * kTile * 4;
+  static constexpr int kTileBytes = 2 * kTile * DP * 4 + 3 * kTile * 4;
   static constexpr int kSmem = kGroups * kTileBytes;
 };
 
@@ -289,6 +289,7 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dq_ker
   delta += __shfl_xor_sync(0xffffffffu, delta, 1);
   delta += __shfl_xor_sync(0xffffffffu, delta, 2);
   const float lse = on ? p.lse[srow] : INFINITY;
+  const float gate = win_alone(p, L, i) ? 0.f : 1.f;
   if (on && part == 0 && gid == 0) p.delta[srow] = delta;
   const KeyRun run(p, L, i0);
   for (int it = gid; it < run.tiles; it += C::kGroups) {
@@ -303,7 +304,7 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dq_ker
 #pragma unroll
       for (int u = 0; u < kStep; ++u)
         if (t + u < n && win_sees(p, L, i, j0 + t + u))
-          axpy_share<N>(acc, exp2f(z[u] - lse) * (dp[u] - delta), ks + (t + u) * DP, part);
+          axpy_share<N>(acc, exp2f(z[u] - lse) * (dp[u] - delta) * gate, ks + (t + u) * DP, part);
     }
   }
   join_groups<N, C::kGroups>(acc, row_smem, gid, thread);
@@ -319,7 +320,7 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dkv_ke
   extern __shared__ __align__(16) float row_smem[];
   const int gid = threadIdx.x / kWinThreads, thread = threadIdx.x % kWinThreads;
   float* qs = row_smem + gid * (C::kTileBytes / 4);
-  float *gs = qs + kTile * DP, *ls = gs + kTile * DP, *ds = ls + kTile;
+  float *gs = qs + kTile * DP, *ls = gs + kTile * DP, *ds = ls + kTile, *gate = ds + kTile;
   const int part = thread & 3, r = thread >> 2;
   const int hk = blockIdx.y, b = blockIdx.z, group = p.H / p.Hk;
   const int j0 = blockIdx.x * kRows, j = j0 + r;
@@ -351,6 +352,7 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dkv_ke
     if (thread < n) {
       ls[thread] = p.lse[srow + i0 + thread];
       ds[thread] = p.delta[srow + i0 + thread];
+      gate[thread] = win_alone(p, L, i0 + thread) ? 0.f : 1.f;
     }
     group_sync(gid);
     for (int t = 0; t < n; t += kStep) {
@@ -362,7 +364,7 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dkv_ke
         if (t + u < n && win_sees(p, L, i0 + t + u, j)) {
           const float w = exp2f(z[u] - ls[t + u]);
           axpy_share<N>(dv, w, gs + (t + u) * DP, part);
-          axpy_share<N>(dk, w * (dp[u] - ds[t + u]), qs + (t + u) * DP, part);
+          axpy_share<N>(dk, w * (dp[u] - ds[t + u]) * gate[t + u], qs + (t + u) * DP, part);
         }
     }
   }

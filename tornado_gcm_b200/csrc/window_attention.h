@@ -41,6 +41,14 @@ __device__ __forceinline__ bool win_sees(const WinParams& p, int L, int i, int j
   const int far = i - j;
   return j < L && !(p.causal && far < 0) && (j < p.sinks || (far < p.window && -far < p.window));
 }
+
+// Whether query i sees exactly one key.  Its weight is 1 whatever its score, so its ds is zero; from dP - delta,
+// sums of the same values in two orders, it would be what their roundings differ by.
+__device__ __forceinline__ bool win_alone(const WinParams& p, int L, int i) {
+  const int lo = max(0, i - (p.window - 1)), hi = min(L, p.causal ? i + 1 : i + p.window);
+  const int sinks = min(min(p.sinks, L), p.causal ? i + 1 : L);
+  return sinks + max(0, hi - max(lo, sinks)) == 1;
+}
 #endif
 
 }  // namespace tgcm

@@ -672,6 +672,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       p.delta[srow] = delta;
     }
     const float2 c2 = make_float2(c, c), lse2 = make_float2(-lse, -lse), delta2 = make_float2(-delta, -delta);
+    const bool alone = win_alone(p, L, i);  // never a row that sees a tile whole
     // tiles that all of this warp's queries see whole
     const int from = kt.n_sink + max(0, w1 - p.window + 1 - kt.lo + KT - 1) / KT;
     const int room = min(L, p.causal ? w0 + 1 : w0 + p.window) - kt.lo;
@@ -708,7 +709,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         }
         if (i < p.S) p.delta[srow] = delta;
 #pragma unroll
-        for (int e = 0; e < KT; ++e) s[e] *= dp[e] - delta;
+        for (int e = 0; e < KT; ++e) s[e] *= alone ? 0.f : dp[e] - delta;
       } else {
 #pragma unroll
         for (int e = 0; e < KT; e += 2) {
@@ -723,6 +724,10 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           const Sight si = sight_of(p, kt, L, i, j, j0);
 #pragma unroll
           for (int e = 0; e < KT; ++e) s[e] = (si.w[e >> 5] & (1u << (e & 31))) ? s[e] : 0.f;
+          if (alone) {
+#pragma unroll
+            for (int e = 0; e < KT; ++e) s[e] *= 0.f;
+          }
         }
       }
       if (j > 0) {  // the product before has read dS
@@ -1047,6 +1052,15 @@ __global__ void __launch_bounds__(kAttnThreads, DkvCfg<DP>::kPerSm)
             qb = valid ? (sink ? QT : j + p.window - i0) : 0;
           }
           const Sight seen = words(bits_below(qb) & ~bits_below(qa));
+          // queries whose only key this is: the first one, ones behind the last key, or all of a window of one
+          if (i0 == 0 || i0 + QT > L || p.window == 1) {
+            Sight alone;
+            alone.w[0] = __ballot_sync(0xffffffffu, win_alone(p, L, i0 + lane));
+            alone.w[1] = __ballot_sync(0xffffffffu, win_alone(p, L, i0 + 32 + lane));
+#pragma unroll
+            for (int e = 0; e < QT; ++e)
+              if (alone.w[e >> 5] & (1u << (e & 31))) dp[e] *= 0.f;
+          }
 #pragma unroll
           for (int e = 0; e < QT; ++e) {
             const bool on = seen.w[e >> 5] & (1u << (e & 31));
