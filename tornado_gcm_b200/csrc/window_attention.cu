@@ -83,7 +83,7 @@ __device__ __forceinline__ void store_share(T* row, int D, int part, bool on, co
 template <typename T, int DP>
 __device__ __forceinline__ void stage_rows(float* sa, const T* a, long long a_stride, float* sb, const T* b,
                                            long long b_stride, int j0, int end, int D, int thread) {
-  constexpr int kEach = kTile * DP / kWinThreads, kOnce = kEach < 16 ? kEach : 16;
+  constexpr int kEach = kTile * DP / kWinThreads, kOnce = kEach <= 16 ? kEach : kEach / 2;
 #pragma unroll
   for (int e0 = 0; e0 < kEach; e0 += kOnce) {
     float va[kOnce], vb[kOnce];
@@ -393,6 +393,8 @@ void by_dim(int D, F&& f) {
     f(std::integral_constant<int, 32>());
   else if (D <= 64)
     f(std::integral_constant<int, 64>());
+  else if (D <= 96)
+    f(std::integral_constant<int, 96>());
   else
     f(std::integral_constant<int, 128>());
 }

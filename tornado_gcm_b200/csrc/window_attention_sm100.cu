@@ -18,7 +18,7 @@
 // its TMEM and shared memory), and the next tile's scores are made while this
 // one's are worked on.  Only at D = 128 do dk and dv need all of TMEM.
 // Measured on 2 x 8192 tokens, 16 + 4 heads of 64, window 512, 4 sinks: forward 97
-// us, dq 130 us, dk/dv 182 us.  Eight softmax warps instead of four, smaller TMEM
+// us, dq 131 us, dk/dv 183 us.  Eight softmax warps instead of four, smaller TMEM
 // shares for three or four CTAs, and weights kept in TMEM in the backward were
 // each tried and took as long or longer.
 //   D <= 64:  forward 64-key tiles (2 x S, under P, 64, O 64 columns),
