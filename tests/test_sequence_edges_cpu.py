@@ -1,0 +1,82 @@
+"""The sequence operators' CPU forms and the model at their edges: ragged histories, given positions, long forecasts,
+padding, values that are not finite, refusals (no GPU)."""
+
+import math
+
+import pytest
+import torch
+
+from tornado_gcm_b200.models import sequence
+from tornado_gcm_b200.neural.sequence_layers import SequenceTransformer
+from tornado_gcm_b200.ops.rotary import qk_norm_rotary, rotary_table
+from tornado_gcm_b200.ops.window_attention import fill_window_cache, window_attention, window_attention_step
+
+
+def _randn(*shape, seed=0, dtype=torch.float32):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed), dtype=torch.float64).to(dtype)
+
+
+def _body(max_positions=64, window=5, **kw):
+    torch.manual_seed(0)
+    return SequenceTransformer(32, 2, 2, 48, window, kv_heads=1, sinks=2, max_positions=max_positions, **kw)
+
+
+def _emulator(max_positions=64):
+    torch.manual_seed(0)
+    m = sequence.SequenceEmulator(5, 3, statics=2, d_model=32, num_heads=2, num_layers=1, d_ff=40, window=6,
+                                  max_positions=max_positions)
+    torch.nn.init.normal_(m.head.weight, std=0.1)
+    return m
+
+
+@pytest.mark.parametrize("S", [1, 2, 5, 7, 8, 20])
+@pytest.mark.parametrize("window,sinks", [(5, 2), (1, 0), (4, 3)])
+def test_fill_window_cache_of_ragged_histories(S, window, sinks):
+    """What single steps of the valid tokens leave, in every slot; NaN behind the end, and slots never written keep."""
+    lengths = [S, S - 1, S // 2, min(sinks, S), 0, -1, S + 3]
+    B, cap = len(lengths), window + sinks
+    k, v = _randn(B, S, 1, 6, seed=1), _randn(B, S, 1, 6, seed=2)
+    for b, n in enumerate(lengths):
+        k[b, max(n, 0):], v[b, max(n, 0):] = math.nan, math.nan
+    got = [torch.full((B, cap, 1, 6), 7.0) for _ in range(2)]
+    want = [t.clone() for t in got]
+    fill_window_cache(k, v, *got, sinks=sinks, lengths=torch.tensor(lengths, dtype=torch.int32))
+    for b, n in enumerate(lengths):
+        for t in range(min(max(n, 0), S)):
+            slot = t if t < cap else sinks + (t - sinks) % window
+            want[0][b, slot], want[1][b, slot] = k[b, t], v[b, t]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+    with pytest.raises(ValueError):
+        fill_window_cache(k, v, *got, sinks=sinks, lengths=torch.tensor([1, 2], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("S", [6, 12, 30])  # the cache holds seven tokens
+def test_steps_behind_a_ragged_history(S):
+    m = _body()
+    x = _randn(4, S + 9, 32, seed=3)
+    L = [S, S - 4, 1, 0]
+    padded = x[:, :S].clone()
+    for b, n in enumerate(L):
+        padded[b, n:] = 5.0
+    with torch.no_grad():
+        cache = m.new_cache(4)
+        m(padded, torch.tensor(L, dtype=torch.int32), cache=cache)
+        assert cache.lengths.tolist() == L
+        got = torch.stack([m.step(x[:, S + t], cache) for t in range(9)], 1)
+        for b, n in enumerate(L):
+            whole = m(torch.cat([x[b:b + 1, :n], x[b:b + 1, S:]], 1))[:, n:]
+            assert torch.allclose(got[b:b + 1], whole, atol=1e-5), b
+
+
+def test_emulator_takes_a_ragged_history_into_a_cache():
+    m = _emulator()
+    states, static = sequence.synthetic_columns(3, 16, 5, 3)
+    lengths = torch.tensor([12, 4, -1], dtype=torch.int32)
+    with torch.no_grad():
+        cache = m.body.new_cache(3)
+        m(states[:, :12], static, lengths, cache=cache)
+        assert cache.lengths.tolist() == [14, 6, -1]
+        got = states[:, 12] + m.head(m.body.step(m.embed(states[:, 12]), cache))
+        for b, n in enumerate([12, 4]):
+            whole = m(torch.cat([states[b:b + 1, :n], states[b:b + 1, 12:13]], 1), static[b:b + 1])[:, -1]
+            assert torch.allclose(got[b:b + 1], whole, atol=1e-5)

@@ -47,9 +47,10 @@ class SequenceEmulator(nn.Module):
     def forward(self, states: torch.Tensor, static: Optional[torch.Tensor] = None,
                 lengths: Optional[torch.Tensor] = None, cache: Optional[WindowCache] = None) -> torch.Tensor:
         """``states (B, T, features)`` and ``static (B, static_features)`` to the next state of every step.
-        ``lengths`` int32 ``(B,)``: valid states of each sequence; ``cache`` takes the history in."""
+        ``lengths`` int32 ``(B,)``: valid states of each sequence (negative: it takes no part); ``cache`` takes the
+        valid history in."""
         if lengths is not None:
-            lengths = lengths + self.statics
+            lengths = torch.where(lengths < 0, lengths, lengths + self.statics)
         h = self.body(self._tokens(states, static), lengths, cache=cache)
         return states + self.head(h[:, self.statics:])
 

@@ -82,10 +82,10 @@ class WindowSelfAttention(nn.Module):
     def forward(self, x: torch.Tensor, lengths: Optional[torch.Tensor] = None,
                 positions: Optional[torch.Tensor] = None, cache: Optional[tuple] = None) -> torch.Tensor:
         """``x (B, S, d_model)``; ``lengths`` int32 ``(B,)``: valid tokens; ``cache``: a pair that takes the keys and
-        values of this whole history."""
+        values of this whole history's valid tokens."""
         q, k, v = self._heads(x, positions)
         if cache is not None:
-            fill_window_cache(k, v, *cache, sinks=self.sinks)
+            fill_window_cache(k, v, *cache, sinks=self.sinks, lengths=lengths)
         o = window_attention(q, k, v, window=self.window, sinks=self.sinks, causal=self.causal, lengths=lengths)
         return _linear(o.flatten(-2), self.out)
 
@@ -146,10 +146,15 @@ class SequenceTransformer(nn.Module):
         self.final_ln = nn.LayerNorm(d_model)
 
     def forward(self, x: torch.Tensor, lengths=None, positions=None, cache: Optional[WindowCache] = None) -> torch.Tensor:
+        """``cache`` takes the history in; with ``lengths`` each sequence's valid tokens only, so that its steps go on
+        behind them (a negative length: the sequence takes no part)."""
         for i, layer in enumerate(self.layers):
             x = layer(x, lengths, positions, None if cache is None else (cache.k[i], cache.v[i]))
         if cache is not None:
-            cache.lengths.fill_(x.shape[1])
+            if lengths is None:
+                cache.lengths.fill_(x.shape[1])
+            else:
+                cache.lengths.copy_(lengths.clamp(max=x.shape[1]))
         return self.final_ln(x)
 
     def step(self, x: torch.Tensor, cache: WindowCache) -> torch.Tensor:

@@ -119,13 +119,33 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
 
 
 def fill_window_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, *,
-                      sinks: int = 0) -> None:
-    """Puts a whole history ``k, v (B, S, Hk, D)`` in the caches, as that many steps would have left them."""
+                      sinks: int = 0, lengths: Optional[torch.Tensor] = None) -> None:
+    """Puts a whole history ``k, v (B, S, Hk, D)`` in the caches, as that many steps would have left them.
+
+    ``lengths (B,)``: valid tokens of every sequence (what lies behind is not stored); a negative one leaves the
+    sequence's cache as it is.
+    """
     S, cap = k.shape[1], k_cache.shape[1]
     if not 0 <= sinks < cap:
         raise ValueError("fill_window_cache: sinks must lie between 0 and the cache's slots")
-    keep = torch.arange(S, device=k.device)
-    if S > cap:
-        keep = torch.cat([keep[:sinks], keep[S - (cap - sinks):]])
-    slot = window_slot(keep, cap, sinks)
-    k_cache[:, slot], v_cache[:, slot] = k[:, keep].to(k_cache.dtype), v[:, keep].to(v_cache.dtype)
+    if lengths is None:
+        keep = torch.arange(S, device=k.device)
+        if S > cap:
+            keep = torch.cat([keep[:sinks], keep[S - (cap - sinks):]])
+        slot = window_slot(keep, cap, sinks)
+        k_cache[:, slot], v_cache[:, slot] = k[:, keep].to(k_cache.dtype), v[:, keep].to(v_cache.dtype)
+        return
+    if lengths.shape != (k.shape[0],):
+        raise ValueError(f"fill_window_cache: one length for each of {k.shape[0]} sequences expected, got {tuple(lengths.shape)}")
+    if S == 0:
+        return
+    # The token that each slot holds behind `lengths` steps: itself among the sinks, behind them the latest one of
+    # its residue; negative, or beyond the length, where the slot has not been written yet.
+    last = lengths.to(k.device).long().clamp(max=S)[:, None] - 1
+    slot = torch.arange(cap, device=k.device)
+    held = last - (last - slot) % (cap - sinks)
+    token = torch.where(slot < sinks, slot, torch.where(held >= sinks, held, -1))
+    on = ((token >= 0) & (token <= last))[:, :, None, None]
+    at = token.clamp(min=0, max=S - 1)[:, :, None, None].expand(-1, -1, *k.shape[2:])
+    for cache, t in ((k_cache, k), (v_cache, v)):
+        cache.copy_(torch.where(on, t.gather(1, at).to(cache.dtype), cache))
