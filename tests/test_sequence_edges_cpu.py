@@ -80,3 +80,36 @@ def test_emulator_takes_a_ragged_history_into_a_cache():
         for b, n in enumerate([12, 4]):
             whole = m(torch.cat([states[b:b + 1, :n], states[b:b + 1, 12:13]], 1), static[b:b + 1])[:, -1]
             assert torch.allclose(got[b:b + 1], whole, atol=1e-5)
+
+
+def test_steps_behind_a_history_at_given_positions():
+    m = _body()
+    x = _randn(2, 20, 32, seed=3)
+    for pos in (torch.arange(20) + 17, torch.stack([torch.arange(20) + 3, torch.arange(20) + 40])):
+        with torch.no_grad():
+            whole = m(x, None, pos)
+            cache = m.new_cache(2)
+            m(x[:, :12], None, pos[..., :12], cache=cache)
+            got = torch.stack([m.step(x[:, t], cache) for t in range(12, 20)], 1)
+        assert torch.allclose(got, whole[:, 12:], atol=1e-5)
+    # ragged: each sequence goes on behind its own last valid position, one without tokens at its first position
+    pos = torch.stack([torch.arange(20) + 3, torch.arange(20) + 40])
+    cache = m.new_cache(2)
+    with torch.no_grad():
+        m(x[:, :12], torch.tensor([5, 0], dtype=torch.int32), pos[:, :12], cache=cache)
+        got = m.step(x[:, 12], cache)
+        for b, n in enumerate((5, 0)):
+            rows = torch.cat([x[b:b + 1, :n], x[b:b + 1, 12:13]], 1)
+            assert torch.allclose(got[b:b + 1], m(rows, None, pos[b, :n + 1])[:, -1], atol=1e-5)
+    # positions that do not follow on are given to the step
+    pos = torch.arange(20) * 3
+    cache = m.new_cache(2)
+    with torch.no_grad():
+        whole = m(x, None, pos)
+        m(x[:, :12], None, pos[:12], cache=cache)
+        got = torch.stack([m.step(x[:, t], cache, positions=pos[t].expand(2)) for t in range(12, 20)], 1)
+    assert torch.allclose(got, whole[:, 12:], atol=1e-5)
+    # a history without positions makes the cache count tokens again
+    with torch.no_grad():
+        m(x[:, :12], cache=cache)
+        assert torch.allclose(m.step(x[:, 12], cache), m(x[:, :13])[:, -1], atol=1e-5)

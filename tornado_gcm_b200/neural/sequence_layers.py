@@ -35,11 +35,13 @@ def _zone(x: torch.Tensor) -> torch.Tensor:
 @dataclasses.dataclass
 class WindowCache:
     """Keys and values of the tokens in sight, one pair of ``(B, sinks + window, heads, head_dim)`` for each block,
-    and the number of tokens that every sequence has seen (int32 ``(B,)``; negative: it takes no part)."""
+    the number of tokens that every sequence has seen (int32 ``(B,)``; negative: it takes no part), and the position
+    of its next token (``(B,)``) where that is another number than its count."""
 
     k: list
     v: list
     lengths: torch.Tensor
+    positions: Optional[torch.Tensor] = None
 
 
 class WindowSelfAttention(nn.Module):
@@ -89,11 +91,13 @@ class WindowSelfAttention(nn.Module):
         o = window_attention(q, k, v, window=self.window, sinks=self.sinks, causal=self.causal, lengths=lengths)
         return _linear(o.flatten(-2), self.out)
 
-    def step(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
-        """One token ``x (B, d_model)`` behind ``lengths`` earlier ones."""
+    def step(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
+             positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token ``x (B, d_model)`` behind ``lengths`` earlier ones, at ``positions (B,)`` or, without, at
+        ``lengths``."""
         if not self.causal:
             raise ValueError("a two-sided window has no one-token form")
-        positions = None if self.table is None else lengths.clamp(min=0)[:, None]
+        positions = None if self.table is None else (lengths.clamp(min=0) if positions is None else positions)[:, None]
         q, k, v = (t[:, 0] for t in self._heads(x[:, None], positions))
         return _linear(window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks=self.sinks).flatten(-2), self.out)
 
@@ -132,8 +136,8 @@ class SequenceBlock(nn.Module):
         x = x + self.attn(_zone(self.ln1(x)), lengths, positions, cache)
         return x + self.ffn(_zone(self.ln2(x)))
 
-    def step(self, x: torch.Tensor, k_cache, v_cache, lengths) -> torch.Tensor:
-        x = x + self.attn.step(_zone(self.ln1(x)), k_cache, v_cache, lengths)
+    def step(self, x: torch.Tensor, k_cache, v_cache, lengths, positions=None) -> torch.Tensor:
+        x = x + self.attn.step(_zone(self.ln1(x)), k_cache, v_cache, lengths, positions)
         return x + self.ffn(_zone(self.ln2(x)))
 
 
@@ -147,7 +151,8 @@ class SequenceTransformer(nn.Module):
 
     def forward(self, x: torch.Tensor, lengths=None, positions=None, cache: Optional[WindowCache] = None) -> torch.Tensor:
         """``cache`` takes the history in; with ``lengths`` each sequence's valid tokens only, so that its steps go on
-        behind them (a negative length: the sequence takes no part)."""
+        behind them (a negative length: the sequence takes no part).  ``positions``, ``(S,)`` or ``(B, S)``: those of
+        the tokens; steps go on behind the last valid one (a sequence without tokens: at the first)."""
         for i, layer in enumerate(self.layers):
             x = layer(x, lengths, positions, None if cache is None else (cache.k[i], cache.v[i]))
         if cache is not None:
@@ -155,12 +160,22 @@ class SequenceTransformer(nn.Module):
                 cache.lengths.fill_(x.shape[1])
             else:
                 cache.lengths.copy_(lengths.clamp(max=x.shape[1]))
+            cache.positions = None
+            if positions is not None and x.shape[1]:
+                at = positions.expand(x.shape[:2])
+                last = at.gather(1, (cache.lengths.long() - 1).clamp(min=0)[:, None])[:, 0]
+                cache.positions = last + (cache.lengths > 0)
         return self.final_ln(x)
 
-    def step(self, x: torch.Tensor, cache: WindowCache) -> torch.Tensor:
-        """One token ``(B, d_model)`` of every sequence; the cache takes it in."""
+    def step(self, x: torch.Tensor, cache: WindowCache, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """One token ``(B, d_model)`` of every sequence; the cache takes it in.  ``positions (B,)``: where these tokens
+        stand, if not right behind the last ones; later steps go on behind them."""
+        if positions is not None:
+            cache.positions = positions.clone()
         for i, layer in enumerate(self.layers):
-            x = layer.step(x, cache.k[i], cache.v[i], cache.lengths)
+            x = layer.step(x, cache.k[i], cache.v[i], cache.lengths, cache.positions)
+        if cache.positions is not None:
+            cache.positions += cache.lengths >= 0
         cache.lengths += cache.lengths >= 0
         return self.final_ln(x)
 
