@@ -113,3 +113,56 @@ def test_steps_behind_a_history_at_given_positions():
     with torch.no_grad():
         m(x[:, :12], cache=cache)
         assert torch.allclose(m.step(x[:, 12], cache), m(x[:, :13])[:, -1], atol=1e-5)
+
+
+def test_forecast_past_the_table_of_positions():
+    states, static = sequence.synthetic_columns(2, 20, 5, 3)
+    want = _emulator(256).forecast(states, static, steps=60)
+    for rows in (4, 22, 40):  # short of the history, of the first step, of the last
+        m = _emulator(rows)
+        assert torch.equal(m.forecast(states, static, steps=60), want)
+        assert torch.equal(m.forecast(states, static, steps=60), want)
+    for steps in (0, -3):
+        with pytest.raises(ValueError):
+            _emulator().forecast(states, static, steps=steps)
+
+
+def test_steps_past_the_table_of_positions_are_refused_until_it_grows():
+    m = _body(max_positions=14)
+    big = _body(max_positions=64)
+    x = _randn(2, 30, 32, seed=3)
+    cache = m.new_cache(2)
+    with torch.no_grad():
+        m(x[:, :12], cache=cache)
+        for t in (12, 13):
+            m.step(x[:, t], cache)
+        before = [t.clone() for t in cache.k], cache.lengths.clone()
+        with pytest.raises(IndexError, match="reserve"):
+            m.step(x[:, 14], cache)
+        assert all(torch.equal(a, b) for a, b in zip(cache.k, before[0])) and torch.equal(cache.lengths, before[1])
+        m.reserve(30)
+        got = torch.stack([m.step(x[:, t], cache) for t in range(14, 30)], 1)
+        assert torch.allclose(got, big(x)[:, 14:], atol=1e-5)
+        cache = m.new_cache(2)
+        m(x[:, :3], None, torch.tensor([20, 25, 29]), cache=cache)
+        with pytest.raises(IndexError, match="reserve"):
+            m.step(x[:, 3], cache)
+    table = m.layers[0].attn.table.clone()
+    m.reserve(10)
+    assert torch.equal(m.layers[0].attn.table, table)
+    scaled = _body(max_positions=8, rotary_scaling="base", rotary_factor=4.0)
+    scaled.reserve(50)
+    assert torch.equal(scaled.layers[1].attn.table[:50], rotary_table(50, 16, scaling="base", factor=4.0))
+
+
+def test_train_step_reads_the_error_flag_when_asked(monkeypatch):
+    asked = []
+    monkeypatch.setattr(sequence._ext, "check_error_flag", lambda device: asked.append(torch.device(device).type))
+    m = _emulator()
+    states, static = sequence.synthetic_columns(2, 10, 5, 3)
+    opt = torch.optim.SGD(m.parameters(), lr=1e-3)
+    sequence.train_step(m, opt, states, static)
+    assert not asked
+    sequence.train_step(m, opt, states, static, check_errors=True)
+    m.forecast(states, static, steps=2)
+    assert asked == ["cpu", "cpu"]

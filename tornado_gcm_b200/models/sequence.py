@@ -21,6 +21,7 @@ import torch
 import torch.nn as nn
 
 from tornado_gcm_b200.neural.sequence_layers import SequenceTransformer, WindowCache
+from tornado_gcm_b200.ops import _ext
 from tornado_gcm_b200.ops.gradnorm import clip_grad_norm
 
 
@@ -66,25 +67,35 @@ class SequenceEmulator(nn.Module):
 
     @torch.no_grad()
     def forecast(self, states: torch.Tensor, static: Optional[torch.Tensor] = None, *, steps: int) -> torch.Tensor:
-        """``(B, steps, features)``: the states that follow ``states (B, T, features)``, one cached step at a time."""
+        """``(B, steps, features)``: the states that follow ``states (B, T, features)``, one cached step at a time.
+        The tables of rotations grow to the forecast's length; what a kernel reported on the way is raised at the end."""
+        if steps < 1:
+            raise ValueError(f"forecast: at least one step expected, got {steps}")
+        self.body.reserve(self.statics + states.shape[1] + steps - 1)
         cache = self.body.new_cache(states.shape[0], states.device)
         state = self(states, static, cache=cache)[:, -1]
         out = [state]
         for _ in range(steps - 1):
             state = state + self.head(self.body.step(self.embed(state), cache))
             out.append(state)
+        _ext.check_error_flag(states.device)
         return torch.stack(out, 1)
 
 
 def train_step(model: SequenceEmulator, optimizer: torch.optim.Optimizer, states: torch.Tensor,
                static: Optional[torch.Tensor] = None, lengths: Optional[torch.Tensor] = None,
-               max_grad_norm: float = 1.0) -> tuple[torch.Tensor, torch.Tensor]:
-    """One optimizer step; the loss and the gradients' norm before clipping, both 0-d device tensors."""
+               max_grad_norm: float = 1.0, check_errors: bool = False) -> tuple[torch.Tensor, torch.Tensor]:
+    """One optimizer step; the loss and the gradients' norm before clipping, both 0-d device tensors.
+
+    ``check_errors``: read the device error flag afterwards (one host synchronisation) and raise if a kernel's bounded
+    wait ran out or a table's index was out of range since it was last read."""
     optimizer.zero_grad(set_to_none=True)
     loss = model.loss(states, static, lengths)
     loss.backward()
     norm = clip_grad_norm([p.grad for p in model.parameters()], max_grad_norm)
     optimizer.step()
+    if check_errors:
+        _ext.check_error_flag(states.device)
     return loss.detach(), norm
 
 
@@ -121,8 +132,9 @@ def main(argv=None) -> dict:
     losses = []
     start = time.perf_counter()
     for i in range(a.steps):
-        loss, norm = train_step(model, opt, states, static)
-        if i % 10 == 0 or i == a.steps - 1:
+        shown = i % 10 == 0 or i == a.steps - 1
+        loss, norm = train_step(model, opt, states, static, check_errors=shown)
+        if shown:
             losses.append(float(loss))
             print(f"step {i}: loss {losses[-1]:.3e}, gradient norm {float(norm):.3e}, "
                   f"{(time.perf_counter() - start) / (i + 1) * 1e3:.1f} ms a step")

@@ -35,13 +35,15 @@ def _zone(x: torch.Tensor) -> torch.Tensor:
 @dataclasses.dataclass
 class WindowCache:
     """Keys and values of the tokens in sight, one pair of ``(B, sinks + window, heads, head_dim)`` for each block,
-    the number of tokens that every sequence has seen (int32 ``(B,)``; negative: it takes no part), and the position
-    of its next token (``(B,)``) where that is another number than its count."""
+    the number of tokens that every sequence has seen (int32 ``(B,)``; negative: it takes no part), the position of
+    its next token (``(B,)``) where that is another number than its count, and the host's bound on positions: the next
+    token of every sequence stands at ``reach`` or before it."""
 
     k: list
     v: list
     lengths: torch.Tensor
     positions: Optional[torch.Tensor] = None
+    reach: int = 0
 
 
 class WindowSelfAttention(nn.Module):
@@ -70,8 +72,16 @@ class WindowSelfAttention(nn.Module):
         else:
             self.q_bias = self.k_bias = None
         rotary_dim = self.head_dim // 2 * 2 if rotary_dim is None else rotary_dim
-        table = rotary_table(max_positions, rotary_dim, scaling=rotary_scaling, factor=rotary_factor) if rotary_dim else None
-        self.register_buffer("table", table, persistent=False)
+        self.rotary = dict(rotary_dim=rotary_dim, scaling=rotary_scaling, factor=rotary_factor)
+        self.register_buffer("table", rotary_table(max_positions, **self.rotary) if rotary_dim else None, persistent=False)
+        self._outgrown = []
+
+    def reserve(self, positions: int) -> None:
+        """Makes the table of rotations hold at least ``positions`` positions.  A CUDA graph captured before keeps the
+        table that it was captured with."""
+        if self.table is not None and positions > self.table.shape[0]:
+            self._outgrown.append(self.table)  # captured graphs read it still
+            self.table = rotary_table(max(positions, 2 * self.table.shape[0]), **self.rotary, device=self.table.device)
 
     def _heads(self, x: torch.Tensor, positions: Optional[torch.Tensor]):
         """``x (B, S, d_model)`` to rotated q and k and plain v, all ``(B, S, heads, head_dim)`` without copies of v."""
@@ -160,8 +170,9 @@ class SequenceTransformer(nn.Module):
                 cache.lengths.fill_(x.shape[1])
             else:
                 cache.lengths.copy_(lengths.clamp(max=x.shape[1]))
-            cache.positions = None
+            cache.positions, cache.reach = None, x.shape[1]
             if positions is not None and x.shape[1]:
+                cache.reach = int(positions.max()) + 1
                 at = positions.expand(x.shape[:2])
                 last = at.gather(1, (cache.lengths.long() - 1).clamp(min=0)[:, None])[:, 0]
                 cache.positions = last + (cache.lengths > 0)
@@ -169,15 +180,33 @@ class SequenceTransformer(nn.Module):
 
     def step(self, x: torch.Tensor, cache: WindowCache, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One token ``(B, d_model)`` of every sequence; the cache takes it in.  ``positions (B,)``: where these tokens
-        stand, if not right behind the last ones; later steps go on behind them."""
+        stand, if not right behind the last ones; later steps go on behind them.
+
+        A token behind the table of rotations (``max_positions``; see :meth:`reserve`) is refused where the host can
+        tell: positions given to a step, or steps replayed from a CUDA graph, are only seen by the kernel, which
+        reports them through the device error flag (:func:`tornado_gcm_b200.ops._ext.check_error_flag`).
+        """
         if positions is not None:
             cache.positions = positions.clone()
+        elif (rows := self.positions()) is not None and cache.reach >= rows:
+            raise IndexError(f"a token at position {cache.reach} of a table of {rows}: reserve() more positions first")
         for i, layer in enumerate(self.layers):
             x = layer.step(x, cache.k[i], cache.v[i], cache.lengths, cache.positions)
         if cache.positions is not None:
             cache.positions += cache.lengths >= 0
         cache.lengths += cache.lengths >= 0
+        cache.reach += 1
         return self.final_ln(x)
+
+    def positions(self) -> Optional[int]:
+        """Positions that the tables of rotations hold; ``None`` without rotation."""
+        tables = [layer.attn.table for layer in self.layers if layer.attn.table is not None]
+        return min(t.shape[0] for t in tables) if tables else None
+
+    def reserve(self, positions: int) -> None:
+        """Makes every block's table of rotations hold at least ``positions`` positions."""
+        for layer in self.layers:
+            layer.attn.reserve(positions)
 
     def new_cache(self, batch: int, device=None) -> WindowCache:
         """An empty cache for ``batch`` sequences."""
