@@ -1,0 +1,89 @@
+"""The sequence operators on the GPU where they are easily wrong: narrow windows and sharp scores, scores of minus
+infinity, values that are not finite where they should not matter, derivatives that the operators do not have,
+shared memory, capture in a graph, other streams and broadcast gradients.
+
+Tolerances are those of ``test_sequence_ops.py``; where a third rounding to bf16 comes in the 2-norm of the error is
+held to sqrt(3) * 1.7e-3 = 3e-3.
+"""
+
+import math
+
+import pytest
+import torch
+
+from tests.test_sequence_ops import DEV, TOL, _attn64, _close, _gated_inputs, _qk64, _randn, _see
+from tornado_gcm_b200.ops import _ext
+
+pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(), reason="needs CUDA")]
+
+BF = torch.bfloat16
+
+
+# ── derivatives ────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_window_step_has_no_gradient_and_says_so(dtype):
+    from tornado_gcm_b200.ops.window_attention import window_attention_step
+
+    n = torch.zeros(2, dtype=torch.int32, device=DEV)
+    base = [_randn(2, h, 32, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2))] + [
+        torch.zeros(2, 6, 2, 32, dtype=dtype, device=DEV) for _ in range(2)]
+    want = window_attention_step(*base, n)
+    for i in range(5):
+        ts = [t.clone().requires_grad_() if j == i else t.clone() for j, t in enumerate(base)]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            window_attention_step(*ts, n)
+        with torch.no_grad():
+            assert torch.equal(window_attention_step(*ts, n), want)
+
+
+# ── the model's caches ─────────────────────────────────────────────────────
+def _body():
+    from tornado_gcm_b200.neural.sequence_layers import SequenceTransformer
+
+    torch.manual_seed(0)
+    return SequenceTransformer(128, 2, 2, 96, 40, kv_heads=1, sinks=3, max_positions=256).to(DEV)
+
+
+def test_steps_behind_a_ragged_history():
+    m = _body()
+    x = _randn(4, 106, 128, seed=1)
+    L = [100, 57, 2, 0]
+    padded = x[:, :100].clone()
+    for b, n in enumerate(L):
+        padded[b, n:] = math.nan
+    with torch.no_grad():
+        cache = m.new_cache(4)
+        m(padded, torch.tensor(L, dtype=torch.int32, device=DEV), cache=cache)
+        got = torch.stack([m.step(x[:, 100 + t], cache) for t in range(6)], 1)
+        for b, n in enumerate(L):
+            whole = m(torch.cat([x[b:b + 1, :n], x[b:b + 1, 100:]], 1))[:, n:]
+            _close(got[b:b + 1], whole, 1e-2)
+    assert cache.lengths.tolist() == [n + 6 for n in L]
+    _ext.check_error_flag(DEV)
+
+
+def test_steps_behind_a_history_at_given_positions():
+    m = _body()
+    x = _randn(2, 30, 128, seed=1)
+    pos = torch.stack([torch.arange(30) + 20, torch.arange(30) + 101]).to(DEV)
+    with torch.no_grad():
+        whole = m(x, None, pos)
+        cache = m.new_cache(2)
+        m(x[:, :24], None, pos[:, :24], cache=cache)
+        got = torch.stack([m.step(x[:, 24 + t], cache) for t in range(6)], 1)
+    _close(got, whole[:, 24:], 1e-2)
+
+
+def test_forecast_past_the_table_of_positions():
+    from tornado_gcm_b200.models import sequence
+
+    res = []
+    for rows in (20, 256):
+        torch.manual_seed(0)
+        m = sequence.SequenceEmulator(9, 3, statics=2, d_model=128, num_heads=2, num_layers=1, d_ff=80, window=12,
+                                      max_positions=rows).to(DEV)
+        torch.nn.init.normal_(m.head.weight, std=0.1)
+        states, static = sequence.synthetic_columns(2, 16, 9, 3, device=DEV)
+        res.append(m.forecast(states, static, steps=40))
+    assert torch.equal(*res)
+    _ext.check_error_flag(DEV)

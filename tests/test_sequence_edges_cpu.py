@@ -166,3 +166,24 @@ def test_train_step_reads_the_error_flag_when_asked(monkeypatch):
     sequence.train_step(m, opt, states, static, check_errors=True)
     m.forecast(states, static, steps=2)
     assert asked == ["cpu", "cpu"]
+
+
+def test_the_step_has_no_gradient_and_says_so():
+    base = [_randn(2, 2, 8, seed=i) for i in range(3)] + [torch.zeros(2, 6, 2, 8) for _ in range(2)]
+    n = torch.zeros(2, dtype=torch.int32)
+    for i in range(5):
+        ts = [t.clone().requires_grad_() if j == i else t.clone() for j, t in enumerate(base)]
+        with pytest.raises(RuntimeError, match="no gradient"):
+            window_attention_step(*ts, n)
+        with torch.no_grad():
+            window_attention_step(*ts, n)
+    # the layers' steps are outside autograd as a whole, not in part
+    m = _body()
+    x = _randn(2, 9, 32, seed=3).requires_grad_()
+    cache = m.new_cache(2)
+    m(x[:, :8], cache=cache)
+    assert not any(t.requires_grad for t in cache.k + cache.v)
+    assert not m.step(x[:, 8], cache).requires_grad
+    layer = m.layers[0]
+    assert not layer.step(x[:, 8], cache.k[0], cache.v[0], cache.lengths).requires_grad
+    assert not layer.attn.step(x[:, 8], cache.k[0], cache.v[0], cache.lengths).requires_grad

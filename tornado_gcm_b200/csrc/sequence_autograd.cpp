@@ -1,7 +1,8 @@
 // torch.ops.tgcm.{gated_linear, qk_norm_rotary, window_attention}: the kernels'
 // forward passes with their backward passes attached.  The graph nodes are
 // native: a training step over short sequences is bound by the host, and a
-// node in Python costs several times what these kernels take.
+// node in Python costs several times what these kernels take.  The one-token step
+// has none and says so where one is wanted.
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/library.h>
 
@@ -171,6 +172,16 @@ at::Tensor window_attention_autograd(const at::Tensor& q, const at::Tensor& k, c
   return window_attention(q, k, v, window, sinks, causal, lengths, scale, err);
 }
 
+at::Tensor window_attention_step_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
+                                          at::Tensor& k_cache, at::Tensor& v_cache, const at::Tensor& lengths,
+                                          int64_t sinks, double scale) {
+  TORCH_CHECK(!at::GradMode::is_enabled() ||
+                  !(wants(q) || wants(k) || wants(v) || wants(k_cache) || wants(v_cache)),
+              "window_attention_step: no gradient; call it under torch.no_grad()");
+  at::AutoDispatchBelowADInplaceOrView below;
+  return window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks, scale);
+}
+
 }  // namespace
 }  // namespace tgcm
 
@@ -193,4 +204,5 @@ TORCH_LIBRARY_IMPL(tgcm, AutogradCUDA, m) {
   m.impl("gated_linear", &tgcm::gated_linear_autograd);
   m.impl("qk_norm_rotary", &tgcm::qk_norm_rotary_autograd);
   m.impl("window_attention", &tgcm::window_attention_autograd);
+  m.impl("window_attention_step", &tgcm::window_attention_step_autograd);
 }

@@ -1,4 +1,4 @@
-// Kernel entry points of the sequence operators that have a backward pass.
+// Kernel entry points of the sequence operators.
 #pragma once
 
 #include <ATen/ATen.h>
@@ -38,5 +38,9 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
                                              const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
                                              int64_t window, int64_t sinks, bool causal, const OptTensor& lengths,
                                              double scale, const OptTensor& err);
+
+// changes the caches in place; no backward pass
+at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache,
+                                 at::Tensor& v_cache, const at::Tensor& lengths, int64_t sinks, double scale);
 
 }  // namespace tgcm

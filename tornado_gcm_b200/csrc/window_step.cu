@@ -20,6 +20,7 @@
 // its part of the outputs through distributed shared memory: one launch, no
 // workspace, and a fixed order of the sums.
 #include "alloc.h"
+#include "sequence_ops.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>

@@ -6,7 +6,8 @@ layers see a sliding window of them and the first ``sinks`` tokens (static field
 rotation, may share key heads between query heads, and use a gated feed-forward block.  On the GPU everything between
 the projections runs in this framework's kernels, in the BF16 zone with fp32 master weights:
 ``ops.rotary.qk_norm_rotary``, ``ops.window_attention`` and ``ops.gated.gated_linear``; the plain projections are
-library products.  ``step`` runs the same block for one new token over a ring cache.
+library products.  ``step`` runs the same block for one new token over a ring cache, for forecasts: no gradient goes
+through it, nor through a cache.
 """
 
 from __future__ import annotations
@@ -101,6 +102,7 @@ class WindowSelfAttention(nn.Module):
         o = window_attention(q, k, v, window=self.window, sinks=self.sinks, causal=self.causal, lengths=lengths)
         return _linear(o.flatten(-2), self.out)
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, lengths: torch.Tensor,
              positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One token ``x (B, d_model)`` behind ``lengths`` earlier ones, at ``positions (B,)`` or, without, at
@@ -146,6 +148,7 @@ class SequenceBlock(nn.Module):
         x = x + self.attn(_zone(self.ln1(x)), lengths, positions, cache)
         return x + self.ffn(_zone(self.ln2(x)))
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor, k_cache, v_cache, lengths, positions=None) -> torch.Tensor:
         x = x + self.attn.step(_zone(self.ln1(x)), k_cache, v_cache, lengths, positions)
         return x + self.ffn(_zone(self.ln2(x)))
@@ -178,6 +181,7 @@ class SequenceTransformer(nn.Module):
                 cache.positions = last + (cache.lengths > 0)
         return self.final_ln(x)
 
+    @torch.no_grad()
     def step(self, x: torch.Tensor, cache: WindowCache, positions: Optional[torch.Tensor] = None) -> torch.Tensor:
         """One token ``(B, d_model)`` of every sequence; the cache takes it in.  ``positions (B,)``: where these tokens
         stand, if not right behind the last ones; later steps go on behind them.

@@ -96,11 +96,14 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     ``k_cache, v_cache``: ``(B, sinks + window, Hk, D)``, changed in place.  ``lengths``: int32 ``(B,)``, the tokens
     that each sequence had before this one (the caller adds one afterwards; calling again with the same lengths
     writes the same slots).  A negative length marks a sequence that takes no part: zeros, its cache untouched.
-    The result equals the last row of :func:`window_attention` with ``causal`` over the whole history.
+    The result equals the last row of :func:`window_attention` with ``causal`` over the whole history.  It has no
+    gradient: with gradients enabled and an input that requires one the call is refused.
     """
     scale = _scale(q, scale, "window_attention_step")
     if q.is_cuda:
         return _ext.op("window_attention_step")(q, k, v, k_cache, v_cache, lengths, int(sinks), scale)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, k_cache, v_cache)):
+        raise RuntimeError("window_attention_step: no gradient; call it under torch.no_grad()")
     cap = k_cache.shape[1]
     if not 0 <= sinks < cap:
         raise ValueError("window_attention_step: sinks must lie between 0 and the cache's slots")
@@ -123,8 +126,9 @@ def fill_window_cache(k: torch.Tensor, v: torch.Tensor, k_cache: torch.Tensor, v
     """Puts a whole history ``k, v (B, S, Hk, D)`` in the caches, as that many steps would have left them.
 
     ``lengths (B,)``: valid tokens of every sequence (what lies behind is not stored); a negative one leaves the
-    sequence's cache as it is.
+    sequence's cache as it is.  The caches hold values alone: no gradient reaches the history through them.
     """
+    k, v = k.detach(), v.detach()
     S, cap = k.shape[1], k_cache.shape[1]
     if not 0 <= sinks < cap:
         raise ValueError("fill_window_cache: sinks must lie between 0 and the cache's slots")
