@@ -19,6 +19,27 @@ pytestmark = [pytest.mark.gpu, pytest.mark.skipif(not torch.cuda.is_available(),
 BF = torch.bfloat16
 
 
+# ── precision ──────────────────────────────────────────────────────────────
+@pytest.mark.parametrize("D", [64, 128, 30])
+@pytest.mark.parametrize("S,window,sinks,causal,sharp", [
+    (300, 2, 0, True, 1), (300, 2, 1, False, 1), (300, 3, 0, True, 1), (300, 3, 1, True, 4), (1000, 2, 0, False, 1),
+    (1000, 3, 0, True, 4), (300, 200, 0, True, 4), (700, 64, 4, False, 4)])
+def test_window_attention_gradients_of_few_or_sharp_weights(D, S, window, sinks, causal, sharp):
+    """Two or three keys to a row, or weights close to one and zero: dP - delta cancels, whatever the sequence's length.
+    Three roundings to bf16: of the weights in the forward product, of dS, and of the result."""
+    from tornado_gcm_b200.ops.window_attention import window_attention
+
+    q, k, v = (_randn(2, S, h, D, seed=i, dtype=BF, scale=s).requires_grad_()
+               for i, (h, s) in enumerate(((4, sharp), (2, 1), (2, 1))))
+    do = _randn(2, S, 4, D, seed=5, dtype=BF)
+    grads = torch.autograd.grad(window_attention(q, k, v, window=window, sinks=sinks, causal=causal), [q, k, v], do)
+    r = [t.detach().double().requires_grad_() for t in (q, k, v)]
+    o64 = _attn64(*r, _see(S, window, sinks, causal, None, 2), D ** -0.5)
+    for n, a, b in zip(("dq", "dk", "dv"), grads, torch.autograd.grad(o64, r, do.double())):
+        _close(a, b, 3e-3, n)
+    _ext.check_error_flag(DEV)
+
+
 # ── derivatives ────────────────────────────────────────────────────────────
 @pytest.mark.parametrize("dtype", [torch.float32, BF])
 def test_window_step_has_no_gradient_and_says_so(dtype):

@@ -94,8 +94,8 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static at::Tensor forward(AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                             int64_t window, int64_t sinks, bool causal, const OptTensor& lengths, double scale,
                             const OptTensor& err) {
-    auto r = window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, err);
-    ctx->save_for_backward({q, k, v, r[0], r[1], undef_or(lengths)});
+    auto r = window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, true, err);
+    ctx->save_for_backward({q, k, v, r[0], r[1], undef_or(lengths), r[2]});
     keep(ctx, {window, sinks, causal, bits_of(scale)}, err);
     return r[0];
   }
@@ -103,8 +103,8 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const auto s = ctx->get_saved_variables();
     if (!g[0].defined()) return variable_list(9);
     const auto c = kept(ctx);
-    auto r = window_attention_bwd(rows_like(g[0], s[3]), s[0], s[1], s[2], s[3], s[4], c[0], c[1], c[2], opt(s[5]),
-                                  double_of(c[3]), flag_of(ctx));
+    auto r = window_attention_bwd(rows_like(g[0], s[3]), s[0], s[1], s[2], s[3], s[6], s[4], c[0], c[1], c[2],
+                                  opt(s[5]), double_of(c[3]), flag_of(ctx));
     variable_list out(9);
     for (int i = 0; i < 3; ++i) out[i] = r[i];
     return out;
@@ -161,7 +161,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rotary_autograd(
 
 at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
                             int64_t sinks, bool causal, const OptTensor& lengths, double scale, const OptTensor& err) {
-  return window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, err)[0];
+  return window_attention_fwd(q, k, v, window, sinks, causal, lengths, scale, false, err)[0];
 }
 at::Tensor window_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
                                      int64_t sinks, bool causal, const OptTensor& lengths, double scale,

@@ -29,14 +29,14 @@ std::vector<at::Tensor> qk_norm_rotary_bwd(const at::Tensor& dyq, const at::Tens
                                            const OptTensor& qw, const OptTensor& kw, int64_t norm, bool interleaved,
                                            double eps, std::array<bool, 4> need, const OptTensor& err);
 
-// o, lse
+// o, lse and, for a backward pass, what o's rounding left over (undefined in fp32 or without `train`)
 std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                              int64_t window, int64_t sinks, bool causal, const OptTensor& lengths,
-                                             double scale, const OptTensor& err);
+                                             double scale, bool train, const OptTensor& err);
 // dq, dk, dv
 std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
-                                             const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
-                                             int64_t window, int64_t sinks, bool causal, const OptTensor& lengths,
+                                             const at::Tensor& v, const at::Tensor& o, const at::Tensor& o_rest,
+                                             const at::Tensor& lse, int64_t window, int64_t sinks, bool causal, const OptTensor& lengths,
                                              double scale, const OptTensor& err);
 
 // changes the caches in place; no backward pass

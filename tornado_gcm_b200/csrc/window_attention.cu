@@ -10,6 +10,12 @@
 //   dv_j = sum_i p_ij dO_i,   ds_ij = p_ij (dO_i . v_j - delta_i) * scale,
 //   dq_i = sum_j ds_ij k_j,   dk_j = sum_i ds_ij q_i,
 // the sums over i running over every query head that shares the key head.
+// delta takes O as it was before its rounding to bf16: dO . v_j - delta is a
+// difference of nearly equal numbers where a row has few keys or one weight close
+// to 1, and O's rounding alone, 2^-9, would be more than dS's own there.  A forward
+// pass that a backward follows keeps the remainder as bf16 beside o (dq off by 2.4
+// to 2.8e-3 of its norm for every window and scores up to eight times as large; from
+// the rounded O 4.7e-3 at a window of 2 and 1e-2 with such scores, emulated in fp64).
 //
 // The work of these kernels is fp32 FMAs (2 D per pair and product); they reach
 // about a sixth of that rate (2 x 875 tokens, 32 + 8 heads of 40, window 319 to
@@ -71,6 +77,16 @@ __device__ __forceinline__ void load_share(const T* row, int D, int part, bool o
   for (int i = 0; i < N; ++i) {
     const int d = 4 * (part + 4 * (i / 4)) + i % 4;
     v[i] = (on && d < D) ? ldw(row + d) : 0.f;
+  }
+}
+// Remainders of the same values behind their rounding to T.
+template <typename T, int N>
+__device__ __forceinline__ void store_rest(T* row, int D, int part, bool on, const float (&v)[N], float f) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    const int d = 4 * (part + 4 * (i / 4)) + i % 4;
+    const float x = v[i] * f;
+    if (on && d < D) stw(row + d, x - __bfloat162float(__float2bfloat16(x)));
   }
 }
 template <typename T, int N>
@@ -255,8 +271,10 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_fwd_ke
   if (gid > 0) return;
   l = ls[0];
   const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
-  store_share<T, N>(static_cast<T*>(p.o) + ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D, p.D, part, on, acc,
-                    inv);
+  const long long orow = ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D;
+  store_share<T, N>(static_cast<T*>(p.o) + orow, p.D, part, on, acc, inv);
+  if constexpr (!std::is_same<T, float>::value)
+    if (p.o_rest != nullptr) store_rest<T, N>(static_cast<T*>(p.o_rest) + orow, p.D, part, on, acc, inv);
   if (on && part == 0)
     p.lse[(static_cast<long long>(b) * p.H + h) * p.S + i] = l == 0.f ? INFINITY : mb + log2f(l);
 }
@@ -284,6 +302,12 @@ __global__ void __launch_bounds__(RowShape<DP>::kGroups* kWinThreads) win_dq_ker
   load_share<T, N>(static_cast<const T*>(p.dout) + b * p.g_sb + i * p.g_ss + h * p.g_sh, p.D, part, on, g);
   load_share<T, N>(static_cast<const T*>(p.o) + orow, p.D, part, on, acc);
   float delta = 0.f;
+  if constexpr (!std::is_same<T, float>::value) {
+    float rest[N];
+    load_share<T, N>(static_cast<const T*>(p.o_rest) + orow, p.D, part, on, rest);
+#pragma unroll
+    for (int e = 0; e < N; ++e) acc[e] += rest[e];
+  }
 #pragma unroll
   for (int e = 0; e < N; ++e) {
     delta = fmaf(g[e], acc[e], delta);
@@ -463,20 +487,22 @@ int* flag_of(const c10::optional<at::Tensor>& err) {
 
 std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v,
                                              int64_t window, int64_t sinks, bool causal,
-                                             const c10::optional<at::Tensor>& lengths, double scale,
+                                             const c10::optional<at::Tensor>& lengths, double scale, bool train,
                                              const c10::optional<at::Tensor>& err) {
   WinParams p = params_of(q, k, v, window, sinks, causal, lengths, scale);
   c10::cuda::CUDAGuard guard(q.device());
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
   auto o = out_empty(q.sizes(), q.options());
+  auto rest = train && bf16 ? out_empty(q.sizes(), q.options()) : at::Tensor();
   auto lse = out_empty({p.B, p.H, p.S}, q.options().dtype(at::kFloat));
-  if (o.numel() == 0) return {o, lse};
+  if (o.numel() == 0) return {o, lse, rest};
   p.o = o.data_ptr();
+  p.o_rest = rest.defined() ? rest.data_ptr() : nullptr;
   p.lse = lse.data_ptr<float>();
   auto st = at::cuda::getCurrentCUDAStream();
-  const bool bf16 = q.scalar_type() == at::kBFloat16;
   if (window_sm100_takes(p, bf16)) {
     window_sm100_fwd(p, st, flag_of(err));
-    return {o, lse};
+    return {o, lse, rest};
   }
   by_dim(p.D, [&](auto dc) {
     constexpr int DP = decltype(dc)::value;
@@ -485,12 +511,12 @@ std::vector<at::Tensor> window_attention_fwd(const at::Tensor& q, const at::Tens
     else
       launch_rows<DP>(win_fwd_kernel<float, DP>, p, p.H, st);
   });
-  return {o, lse};
+  return {o, lse, rest};
 }
 
 std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::Tensor& q, const at::Tensor& k,
-                                             const at::Tensor& v, const at::Tensor& o, const at::Tensor& lse,
-                                             int64_t window, int64_t sinks, bool causal,
+                                             const at::Tensor& v, const at::Tensor& o, const at::Tensor& o_rest,
+                                             const at::Tensor& lse, int64_t window, int64_t sinks, bool causal,
                                              const c10::optional<at::Tensor>& lengths, double scale,
                                              const c10::optional<at::Tensor>& err) {
   WinParams p = params_of(q, k, v, window, sinks, causal, lengths, scale);
@@ -501,12 +527,17 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
                   lse.is_contiguous() && lse.scalar_type() == at::kFloat &&
                   lse.numel() == q.size(0) * q.size(1) * q.size(2),
               "window_attention backward: o and lse must be the forward's");
+  const bool bf16 = q.scalar_type() == at::kBFloat16;
+  TORCH_CHECK(!bf16 || (o_rest.defined() && o_rest.sizes() == q.sizes() && o_rest.is_contiguous() &&
+                        o_rest.scalar_type() == at::kBFloat16),
+              "window_attention backward: the forward must have kept o's remainder");
   c10::cuda::CUDAGuard guard(q.device());
   auto dq = out_empty(q.sizes(), q.options()), dk = out_empty(k.sizes(), k.options()),
        dv = out_empty(v.sizes(), v.options());
   if (q.numel() == 0) return {dq, dk.zero_(), dv.zero_()};
   auto delta = out_empty({p.B, p.H, p.S}, lse.options());
   p.o = o.data_ptr();
+  p.o_rest = bf16 ? o_rest.data_ptr() : nullptr;
   p.lse = lse.data_ptr<float>();
   p.dout = dout.data_ptr();
   p.g_sb = dout.stride(0), p.g_ss = dout.stride(1), p.g_sh = dout.stride(2);
@@ -515,7 +546,6 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
   p.dk = dk.data_ptr();
   p.dv = dv.data_ptr();
   auto st = at::cuda::getCurrentCUDAStream();
-  const bool bf16 = q.scalar_type() == at::kBFloat16;
   if (window_sm100_takes(p, bf16)) {
     window_sm100_bwd(p, st, flag_of(err));
     return {dq, dk, dv};

@@ -18,11 +18,12 @@ struct WinParams {
   long long k_sb, k_ss, k_sh;
   long long v_sb, v_ss, v_sh;
   void* o;                       // (B, S, H, D) contiguous
+  void* o_rest;                  // bf16, o's shape: what o lacks of O after its rounding; null unless a backward follows
   float* lse;                    // (B, H, S): log2 of the softmax sum, +inf for rows that see nothing
   // backward
   const void* dout;              // (B, S, H, D), unit stride along D
   long long g_sb, g_ss, g_sh;
-  float* delta;                  // (B, H, S): sum_d dO O
+  float* delta;                  // (B, H, S): sum_d dO O, with O = o + o_rest
   void *dq, *dk, *dv;            // contiguous, shapes of q, k, v
   const int* lengths;            // (B,) or null
   int B, S, H, Hk, D;

@@ -18,7 +18,7 @@
 // its TMEM and shared memory), and the next tile's scores are made while this
 // one's are worked on.  Only at D = 128 do dk and dv need all of TMEM.
 // Measured on 2 x 8192 tokens, 16 + 4 heads of 64, window 512, 4 sinks: forward 97
-// us, dq 131 us, dk/dv 183 us.  Eight softmax warps instead of four, smaller TMEM
+// us (112 with what the backward needs), dq 142 us, dk/dv 183 us.  Eight softmax warps instead of four, smaller TMEM
 // shares for three or four CTAs, and weights kept in TMEM in the backward were
 // each tried and took as long or longer.
 //   D <= 64:  forward 64-key tiles (2 x S, under P, 64, O 64 columns),
@@ -122,6 +122,16 @@ __device__ __forceinline__ uint32_t pack_f2(float a, float b) {
   return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// c plus the two bf16 values of w.
+__device__ __forceinline__ float2 add_packed(float2 c, uint32_t w) {
+  float2 d;
+  asm("{\n\t.reg .b16 l, h;\n\tmov.b32 {l, h}, %2;\n\t"
+      "add.rn.f32.bf16 %0, l, %3;\n\tadd.rn.f32.bf16 %1, h, %4;\n\t}"
+      : "=f"(d.x), "=f"(d.y)
+      : "r"(w), "f"(c.x), "f"(c.y));
+  return d;
+}
+
 __device__ __forceinline__ void load_row32(uint32_t taddr, float* s) {
   uint32_t r[32];
   tmem_ld_32x32b_x32(taddr, r);
@@ -152,9 +162,11 @@ __device__ __forceinline__ void store_rows(uint8_t* stage, __nv_bfloat16* dst, l
         *reinterpret_cast<uint4*>(dst + row * row_stride + d) = *stage_piece(stage, a, row, lane & 7);
     }
 }
-// TMEM columns [col, col + DP) of this thread's row, times f, to the staging tile.
-template <int DP>
-__device__ __forceinline__ void stage_row(uint8_t* stage, uint32_t taddr, bool have, float f, int row) {
+// TMEM columns [col, col + DP) of this thread's row, times f, to the staging tile; with REST what these values
+// times `exact` have beyond their rounded products with f.
+template <int DP, bool REST = false>
+__device__ __forceinline__ void stage_row(uint8_t* stage, uint32_t taddr, bool have, float f, int row,
+                                          float exact = 0.f) {
 #pragma unroll
   for (int c = 0; c < DP / 32; ++c) {
     float v[32];
@@ -166,10 +178,15 @@ __device__ __forceinline__ void stage_row(uint8_t* stage, uint32_t taddr, bool h
       for (int i = 0; i < 32; ++i) v[i] = 0.f;
     }
 #pragma unroll
+    for (int i = 0; i < 32; ++i) {
+      const float x = v[i] * f;
+      v[i] = REST ? v[i] * exact - __bfloat162float(__float2bfloat16(x)) : x;
+    }
+#pragma unroll
     for (int p = 0; p < 4; ++p)
       *stage_piece(stage, c >> 1, row, (c & 1) * 4 + p) =
-          make_uint4(pack_f2(v[8 * p] * f, v[8 * p + 1] * f), pack_f2(v[8 * p + 2] * f, v[8 * p + 3] * f),
-                     pack_f2(v[8 * p + 4] * f, v[8 * p + 5] * f), pack_f2(v[8 * p + 6] * f, v[8 * p + 7] * f));
+          make_uint4(pack_f2(v[8 * p], v[8 * p + 1]), pack_f2(v[8 * p + 2], v[8 * p + 3]),
+                     pack_f2(v[8 * p + 4], v[8 * p + 5]), pack_f2(v[8 * p + 6], v[8 * p + 7]));
   }
 }
 
@@ -242,7 +259,10 @@ struct FwdCfg {
   static constexpr uint32_t kO = kBufs * 64;                // TMEM columns: the scores first, P over them
 };
 
-template <int DP>
+// TRAIN: leaves o_rest for the backward pass.  delta = dO . O has to be the mean of dP under weights that add up
+// to one, or a weight near 1 brings its own rounding (2^-9 of dP) into a difference that is far smaller; so O for delta
+// is divided by the sum of the rounded weights, which were multiplied with V, and o by that of the exact ones, as without.
+template <int DP, bool TRAIN>
 __global__ void __launch_bounds__(kAttnThreads, 2)
     win_fwd_sm100(const __grid_constant__ AttnMaps maps, const __grid_constant__ WinParams p, int* err) {
   using C = FwdCfg<DP>;
@@ -376,7 +396,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     const float c = p.scale * kLog2e;
     const int w0 = i0 + q4 * 32, w1 = w0 + 31;  // this warp's queries
     float m = -INFINITY;                        // in the scaled base-2 domain
-    float2 l2 = make_float2(0.f, 0.f);
+    float2 l2 = make_float2(0.f, 0.f), r2 = l2;  // sums of the weights, and of the rounded ones
     bool ok = true;
     // tiles that all of this warp's queries see whole
     const int from = kt.n_sink + max(0, w1 - p.window + 1 - kt.lo + KT - 1) / KT;
@@ -413,6 +433,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
         f = ex2(m - mx);
         m = mx;
         l2 = mul2(l2, make_float2(f, f));
+        if constexpr (TRAIN) r2 = mul2(r2, make_float2(f, f));
         raise = true;
       }
       const float base = m == -INFINITY ? 0.f : m;
@@ -432,6 +453,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           }
           l2 = add2(l2, w);
           pk[e / 2] = pack_f2(w.x, w.y);
+          if constexpr (TRAIN) r2 = add_packed(r2, pk[e / 2]);
         }
       } else {
 #pragma unroll
@@ -444,6 +466,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
               w.y = ex2(w.y);
               l2 = add2(l2, w);
               pk[e / 2] = pack_f2(w.x, w.y);
+              if constexpr (TRAIN) r2 = add_packed(r2, pk[e / 2]);
             }
           }
       }
@@ -486,9 +509,15 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       // every product has read the queries: their tile is the staging tile now
       stage_row<DP>(smem, tmem + C::kO + lanes, kt.n > 0, inv, row);
       __syncwarp();
-      __nv_bfloat16* o = static_cast<__nv_bfloat16*>(p.o) +
-                         ((static_cast<long long>(b) * p.S + i0) * p.H + h) * p.D;
-      store_rows<DP>(smem, o, static_cast<long long>(p.H) * p.D, p.D, q4 * 32, 0, p.S - i0, lane);
+      const long long at = ((static_cast<long long>(b) * p.S + i0) * p.H + h) * p.D, stride = static_cast<long long>(p.H) * p.D;
+      store_rows<DP>(smem, static_cast<__nv_bfloat16*>(p.o) + at, stride, p.D, q4 * 32, 0, p.S - i0, lane);
+      if constexpr (TRAIN) {
+        const float r = r2.x + r2.y;
+        __syncwarp();  // the staging rows have been read
+        stage_row<DP, true>(smem, tmem + C::kO + lanes, kt.n > 0, inv, row, r > 0.f ? 1.f / r : (r == 0.f ? 0.f : r));
+        __syncwarp();
+        store_rows<DP>(smem, static_cast<__nv_bfloat16*>(p.o_rest) + at, stride, p.D, q4 * 32, 0, p.S - i0, lane);
+      }
       if (i < p.S)
         p.lse[(static_cast<long long>(b) * p.H + h) * p.S + i] = l == 0.f ? INFINITY : m + log2f(l);
     }
@@ -656,17 +685,20 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     float delta = 0.f, lse = INFINITY;
     if (i < p.S) {
       lse = p.lse[srow];
-      const uint4* o = reinterpret_cast<const uint4*>(
-          static_cast<const __nv_bfloat16*>(p.o) + ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D);
+      const long long orow = ((static_cast<long long>(b) * p.S + i) * p.H + h) * p.D;
+      const uint4* o = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.o) + orow);
+      const uint4* rest = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.o_rest) + orow);
       const uint4* g = reinterpret_cast<const uint4*>(static_cast<const __nv_bfloat16*>(p.dout) + b * p.g_sb +
                                                       i * p.g_ss + h * p.g_sh);
+#pragma unroll 4
       for (int d = 0; d < p.D / 8; ++d) {
-        const uint4 x = o[d], y = g[d];
-        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+        const uint4 x = o[d], z = rest[d], y = g[d];
+        const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, zs[4] = {z.x, z.y, z.z, z.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          delta = fmaf(__uint_as_float(xs[e] << 16), __uint_as_float(ys[e] << 16), delta);
-          delta = fmaf(__uint_as_float(xs[e] & 0xffff0000u), __uint_as_float(ys[e] & 0xffff0000u), delta);
+          delta = fmaf(__uint_as_float(xs[e] << 16) + __uint_as_float(zs[e] << 16), __uint_as_float(ys[e] << 16), delta);
+          delta = fmaf(__uint_as_float(xs[e] & 0xffff0000u) + __uint_as_float(zs[e] & 0xffff0000u),
+                       __uint_as_float(ys[e] & 0xffff0000u), delta);
         }
       }
       p.delta[srow] = delta;
@@ -696,8 +728,8 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       if (lane == 0) mbar_arrive(s_empty);
       const bool whole = j >= from && j < to;
       if (kt.n == 1) {
-        // The row's few keys are all here: delta from the weights themselves.  From O it would carry O's rounding
-        // to bf16, which is as large as dS's own when a row has two or three keys.
+        // The row's few keys are all here: delta from the weights themselves, without the forward's rounding of them
+        // to bf16, which is seen when a row has two or three keys (dq and dk off by 2.7 against 2.4e-3).
         const Sight si = whole ? words(~0ull) : sight_of(p, kt, L, i, j, j0);
         delta = 0.f;
 #pragma unroll
@@ -1185,12 +1217,12 @@ AttnMaps maps_of(const WinParams& p, int q_rows, int k_rows) {
   return m;
 }
 
-template <int DP>
+template <int DP, bool TRAIN>
 void fwd(const WinParams& p, cudaStream_t st, int* err) {
   using C = FwdCfg<DP>;
   static bool set[64] = {false};
-  allow_smem(win_fwd_sm100<DP>, C::kSmem, set);
-  win_fwd_sm100<DP><<<dim3((p.S + 127) / 128, p.H, p.B), kAttnThreads, C::kSmem, st>>>(maps_of(p, 128, C::KT), p, err);
+  allow_smem(win_fwd_sm100<DP, TRAIN>, C::kSmem, set);
+  win_fwd_sm100<DP, TRAIN><<<dim3((p.S + 127) / 128, p.H, p.B), kAttnThreads, C::kSmem, st>>>(maps_of(p, 128, C::KT), p, err);
   C10_CUDA_KERNEL_LAUNCH_CHECK();
 }
 
@@ -1251,10 +1283,11 @@ bool window_sm100_takes(const WinParams& p, bool bf16) {
 }
 
 void window_sm100_fwd(const WinParams& p, cudaStream_t st, int* err) {
+  const bool train = p.o_rest != nullptr;
   if (p.D <= 64)
-    fwd<64>(p, st, err);
+    train ? fwd<64, true>(p, st, err) : fwd<64, false>(p, st, err);
   else
-    fwd<128>(p, st, err);
+    train ? fwd<128, true>(p, st, err) : fwd<128, false>(p, st, err);
 }
 
 void window_sm100_bwd(const WinParams& p, cudaStream_t st, int* err) {
