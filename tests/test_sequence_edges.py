@@ -40,6 +40,29 @@ def test_window_attention_gradients_of_few_or_sharp_weights(D, S, window, sinks,
     _ext.check_error_flag(DEV)
 
 
+# ── what is not finite ─────────────────────────────────────────────────────
+@pytest.mark.parametrize("dtype,D", [(BF, 64), (BF, 128), (BF, 30), (torch.float32, 32)])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_whose_every_score_is_minus_infinity_give_zeros(dtype, D, causal):
+    from tornado_gcm_b200.ops.window_attention import window_attention, window_attention_step
+
+    B, S = 1, 600
+    q, k, v = (_randn(B, S, 1, D, seed=i, dtype=dtype) for i in range(3))
+    k[..., 3] = 1.0
+    cfg = dict(window=300, causal=causal)
+    rows = torch.tensor([0, 5, 100, 130, 400, 599], device=DEV)
+    q[:, rows] = 0.0
+    want = window_attention(q, k, v, **cfg)
+    q[:, rows, :, 3] = -math.inf
+    got = window_attention(q, k, v, **cfg)
+    assert (got[:, rows] == 0).all()
+    others = torch.ones(S, dtype=torch.bool, device=DEV).index_fill_(0, rows, False)
+    assert torch.equal(got[:, others], want[:, others])
+    lengths = torch.full((B,), S - 1, dtype=torch.int32, device=DEV)
+    o = window_attention_step(q[:, 5], k[:, 7], v[:, 7], k.clone(), v.clone(), lengths)
+    assert (o == 0).all()
+
+
 # ── derivatives ────────────────────────────────────────────────────────────
 @pytest.mark.parametrize("dtype", [torch.float32, BF])
 def test_window_step_has_no_gradient_and_says_so(dtype):

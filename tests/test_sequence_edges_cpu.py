@@ -187,3 +187,15 @@ def test_the_step_has_no_gradient_and_says_so():
     layer = m.layers[0]
     assert not layer.step(x[:, 8], cache.k[0], cache.v[0], cache.lengths).requires_grad
     assert not layer.attn.step(x[:, 8], cache.k[0], cache.v[0], cache.lengths).requires_grad
+
+
+def test_rows_whose_every_score_is_minus_infinity_give_zeros():
+    q, k, v = (_randn(1, 8, 1, 4, seed=i) for i in range(3))
+    k[..., 3] = 1.0
+    q[:, 2] = 0.0
+    want = window_attention(q, k, v, window=3)
+    q[:, 2, :, 3] = -math.inf
+    got = window_attention(q, k, v, window=3)
+    assert (got[:, 2] == 0).all() and torch.equal(got[:, 3:], want[:, 3:]) and torch.equal(got[:, :2], want[:, :2])
+    n = torch.full((1,), 7, dtype=torch.int32)
+    assert (window_attention_step(q[:, 2], k[:, 7], v[:, 7], k.clone(), v.clone(), n) == 0).all()

@@ -101,7 +101,8 @@ __device__ __forceinline__ float max_nan(float a, float b, float c) {
 // 2^t of two values on the FMA pipe: t = n + f with |f| <= 1/2 (n by adding and
 // taking away 1.5 * 2^23), a cubic for 2^f (least largest relative error on the
 // interval, 7.5e-5: a twentieth of a bf16 weight's rounding), n into the
-// exponent.  t below -126 gives 2^-126, and so does NaN.
+// exponent.  t below -126 gives 2^-126, and so does NaN: nothing beside a row's
+// largest weight, and rows that have none are set to zero at the end.
 __device__ __forceinline__ float2 ex2_poly2(float2 t) {
   t.x = fmaxf(t.x, -126.f);
   t.y = fmaxf(t.y, -126.f);
@@ -504,7 +505,11 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
     if (!ok) {
       *abort_flag = 1;
     } else {
-      const float l = l2.x + l2.y;
+      // Every score minus infinity: no weight (the polynomial's least value is not zero), as if nothing were in sight.
+      // A row that met NaN has a sum of NaN, whatever its maximum became afterwards.
+      const float sum = l2.x + l2.y;
+      const bool none = m == -INFINITY && sum == sum;
+      const float l = none ? 0.f : sum;
       const float inv = l > 0.f ? 1.f / l : (l == 0.f ? 0.f : l);
       // every product has read the queries: their tile is the staging tile now
       stage_row<DP>(smem, tmem + C::kO + lanes, kt.n > 0, inv, row);
@@ -512,7 +517,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       const long long at = ((static_cast<long long>(b) * p.S + i0) * p.H + h) * p.D, stride = static_cast<long long>(p.H) * p.D;
       store_rows<DP>(smem, static_cast<__nv_bfloat16*>(p.o) + at, stride, p.D, q4 * 32, 0, p.S - i0, lane);
       if constexpr (TRAIN) {
-        const float r = r2.x + r2.y;
+        const float r = none ? 0.f : r2.x + r2.y;
         __syncwarp();  // the staging rows have been read
         stage_row<DP, true>(smem, tmem + C::kO + lanes, kt.n > 0, inv, row, r > 0.f ? 1.f / r : (r == 0.f ? 0.f : r));
         __syncwarp();

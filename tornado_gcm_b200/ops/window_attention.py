@@ -41,7 +41,7 @@ def _torch_form(q, k, v, window, sinks, causal, lengths, scale):
     c = torch.float64 if q.dtype == torch.float64 else torch.float32
     qh, kh, vh = (t.transpose(1, 2).to(c) for t in (q, k.repeat_interleave(n, 2), v.repeat_interleave(n, 2)))
     s = (qh @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
-    dead = ~see.any(-1, keepdim=True)
+    dead = (s == -math.inf).all(-1, keepdim=True)
     p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
     if lengths is not None:  # what lies behind the end may hold anything
         at = torch.arange(q.shape[1], device=q.device)[None, None, :, None]
@@ -64,8 +64,8 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     """``(B, S, H, D)`` attention of ``q (B, S, H, D)`` over ``k, v (B, S, Hk, D)``; ``Hk`` divides ``H``.
 
     bf16 or fp32, ``D`` up to 128, any strides with a contiguous last axis.  ``lengths``: int32 ``(B,)``, the number
-    of valid keys of every sequence (what lies behind may hold anything, NaN included); a query that sees no key
-    gives zeros and no gradient, one that sees a score of NaN or plus infinity gives NaN.  ``scale`` (positive)
+    of valid keys of every sequence (what lies behind may hold anything, NaN included); a query that sees no key, or
+    scores of minus infinity alone, gives zeros and no gradient, one that sees a score of NaN or plus infinity gives NaN.  ``scale`` (positive)
     defaults to ``D ** -0.5``.
     """
     if window < 1:
@@ -115,7 +115,7 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     n = q.shape[1] // k.shape[1]
     kh, vh = (t.repeat_interleave(n, 2).transpose(1, 2).float() for t in (k_cache, v_cache))
     s = (q.float()[:, :, None] @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
-    dead = ~see.any(-1, keepdim=True)
+    dead = (s == -math.inf).all(-1, keepdim=True)
     p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
     vh = vh.masked_fill(~see.transpose(-1, -2), 0.0)
     return (p @ vh)[:, :, 0].to(q.dtype)
