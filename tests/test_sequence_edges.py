@@ -64,6 +64,53 @@ def test_rows_whose_every_score_is_minus_infinity_give_zeros(dtype, D, causal):
 
 
 # ── derivatives ────────────────────────────────────────────────────────────
+def _three():
+    """The operators that have a backward pass: a call, its differentiable inputs."""
+    from tornado_gcm_b200.ops.gated import gated_linear
+    from tornado_gcm_b200.ops.rotary import qk_norm_rotary, rotary_table
+    from tornado_gcm_b200.ops.window_attention import window_attention
+
+    table = rotary_table(40, 64, device=DEV)
+    return {
+        "gated": (lambda *t: (gated_linear(*t),), list(_gated_inputs(40, 64, 96, True))),
+        "qk": (lambda q, k, w: qk_norm_rotary(q, k, table, w, norm="rms"),
+               [_randn(2, 40, 4, 64, seed=1, dtype=BF), _randn(2, 40, 2, 64, seed=2, dtype=BF), 1 + _randn(64, seed=3, scale=0.1)]),
+        "attn": (lambda q, k, v: (window_attention(q, k, v, window=9, sinks=1),),
+                 [_randn(2, 40, h, 64, seed=h + i, dtype=BF) for i, h in enumerate((4, 2, 2))]),
+        "attn fp32": (lambda q, k, v: (window_attention(q, k, v, window=9, sinks=1),),
+                      [_randn(2, 40, h, 32, seed=h + i) for i, h in enumerate((4, 2, 2))]),
+    }
+
+
+NAMES = ["gated", "qk", "attn", "attn fp32"]
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_second_derivatives_are_refused(name):
+    call, ts = _three()[name]
+    ts = [t.requires_grad_() for t in ts]
+    ys = call(*ts)
+    plain = torch.autograd.grad(ys, ts, [torch.ones_like(y) for y in ys], retain_graph=True)
+    first = torch.autograd.grad(ys, ts, [torch.ones_like(y) for y in ys], create_graph=True)
+    assert all(torch.equal(a, b) for a, b in zip(plain, first))  # the first derivative is there all the same
+    for f in first:
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(f.float().square().sum(), ts, allow_unused=True, retain_graph=True)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("grad", [False, True])
+def test_forward_mode_is_refused(name, grad):
+    import torch.autograd.forward_ad as fwAD
+
+    call, ts = _three()[name]
+    for i in range(len(ts)):
+        with fwAD.dual_level(), torch.set_grad_enabled(grad):
+            duals = [fwAD.make_dual(t, torch.ones_like(t)) if j == i else t for j, t in enumerate(ts)]
+            with pytest.raises(NotImplementedError, match="no forward-mode"):
+                call(*duals)
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, BF])
 def test_window_step_has_no_gradient_and_says_so(dtype):
     from tornado_gcm_b200.ops.window_attention import window_attention_step

@@ -2,8 +2,11 @@
 // forward passes with their backward passes attached.  The graph nodes are
 // native: a training step over short sequences is bound by the host, and a
 // node in Python costs several times what these kernels take.  The one-token step
-// has none and says so where one is wanted.
+// has none and says so where one is wanted; so do all of them for forward-mode and
+// second derivatives.
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/library.h>
 
 #include <cstring>
@@ -20,6 +23,28 @@ bool wants(const at::Tensor& t) { return t.defined() && t.requires_grad(); }
 bool wants(const OptTensor& t) { return t.has_value() && wants(*t); }
 at::Tensor undef_or(const OptTensor& t) { return t.has_value() ? *t : at::Tensor(); }
 OptTensor opt(const at::Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); }
+
+bool dual(const at::Tensor& t) { return t.defined() && t._fw_grad(0).defined(); }
+bool dual(const OptTensor& t) { return t.has_value() && dual(*t); }
+template <class... T>
+void refuse_forward_mode(const char* name, const T&... inputs) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!(dual(inputs) || ...), name, ": no forward-mode derivative");
+}
+
+// A node's gradients under create_graph: they have no history, so one that says so takes its place.  `of`: the
+// node's inputs and the upstream gradients, on which the gradients depend.
+variable_list first_only(variable_list grads, const variable_list& of, const char* name) {
+  if (!at::GradMode::is_enabled()) return grads;
+  auto node = std::shared_ptr<torch::autograd::Error>(
+      new torch::autograd::Error(std::string(name) + ": no second derivative", torch::autograd::collect_next_edges(of)),
+      torch::autograd::deleteNode);
+  for (auto& g : grads)
+    if (g.defined()) {
+      g = g.detach();
+      torch::autograd::set_history(g, node);
+    }
+  return grads;
+}
 
 // The upstream gradient in the result's type with a contiguous last axis.
 at::Tensor rows_like(const at::Tensor& g, const at::Tensor& like) {
@@ -63,8 +88,9 @@ struct GatedLinear : torch::autograd::Function<GatedLinear> {
     const at::Tensor dh = g[0].scalar_type() == at::kBFloat16 ? g[0] : g[0].to(at::kBFloat16);
     auto r = gated_bwd(dh.size(1) == 1 || dh.stride(1) == 1 ? dh : dh.contiguous(), s[0], s[1], s[2], opt(s[3]),
                        opt(s[4]), c[0], c[1], c[2], c[3], c[4], flag_of(ctx));
-    return {r[0], r[1], r[2], s[3].defined() ? r[3] : at::Tensor(), s[4].defined() ? r[4] : at::Tensor(),
-            at::Tensor(), at::Tensor()};
+    return first_only({r[0], r[1], r[2], s[3].defined() ? r[3] : at::Tensor(), s[4].defined() ? r[4] : at::Tensor(),
+                       at::Tensor(), at::Tensor()},
+                      {g[0], s[0], s[1], s[2], s[3], s[4]}, "gated_linear");
   }
 };
 
@@ -86,7 +112,7 @@ struct QKNormRotary : torch::autograd::Function<QKNormRotary> {
     variable_list out(12);
     out[0] = r[0], out[1] = r[1];
     for (int i = 0; i < 4; ++i) out[4 + i] = r[2 + i];
-    return out;
+    return first_only(std::move(out), {g[0], g[1], s[0], s[1], s[4], s[5]}, "qk_norm_rotary");
   }
 };
 
@@ -107,7 +133,7 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
                                   opt(s[5]), double_of(c[3]), flag_of(ctx));
     variable_list out(9);
     for (int i = 0; i < 3; ++i) out[i] = r[i];
-    return out;
+    return first_only(std::move(out), {g[0], s[0], s[1], s[2]}, "window_attention");
   }
 };
 
@@ -120,6 +146,7 @@ at::Tensor gated_linear_autograd(const at::Tensor& x, const at::Tensor& wg, cons
   TORCH_CHECK_VALUE(x.dim() >= 1 && wg.dim() == 2 && wg.sizes() == wu.sizes() && x.size(-1) == wg.size(1),
                     "gated_linear: x (..., features) and two weights (hidden, features) expected");
   TORCH_CHECK_VALUE(bg.has_value() == bu.has_value(), "gated_linear: both biases or none");
+  refuse_forward_mode("gated_linear", x, wg, wu, bg, bu);
   // Other types are rounded to bf16 here, above autograd, so that gradients come back in the caller's type.
   auto bf = [](const at::Tensor& t) { return t.scalar_type() == at::kBFloat16 ? t : t.to(at::kBFloat16); };
   auto bf_opt = [&](const OptTensor& t) { return t.has_value() ? OptTensor(bf(*t)) : t; };
@@ -151,6 +178,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rotary_autograd(
     const at::Tensor& q, const at::Tensor& k, const OptTensor& table, const OptTensor& positions, const OptTensor& qw,
     const OptTensor& kw, const OptTensor& qb, const OptTensor& kb, int64_t norm, bool interleaved, double eps,
     const OptTensor& err) {
+  refuse_forward_mode("qk_norm_rotary", q, k, table, qw, kw, qb, kb);
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(qw) || wants(kw) || wants(qb) || wants(kb))) {
     auto r = QKNormRotary::apply(q, k, table, positions, qw, kw, qb, kb, norm, interleaved, eps, err);
     return {r[0], r[1]};
@@ -166,6 +194,7 @@ at::Tensor window_attention(const at::Tensor& q, const at::Tensor& k, const at::
 at::Tensor window_attention_autograd(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window,
                                      int64_t sinks, bool causal, const OptTensor& lengths, double scale,
                                      const OptTensor& err) {
+  refuse_forward_mode("window_attention", q, k, v);
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(v)))
     return WindowAttention::apply(q, k, v, window, sinks, causal, lengths, scale, err);
   at::AutoDispatchBelowADInplaceOrView below;
@@ -178,6 +207,7 @@ at::Tensor window_attention_step_autograd(const at::Tensor& q, const at::Tensor&
   TORCH_CHECK(!at::GradMode::is_enabled() ||
                   !(wants(q) || wants(k) || wants(v) || wants(k_cache) || wants(v_cache)),
               "window_attention_step: no gradient; call it under torch.no_grad()");
+  refuse_forward_mode("window_attention_step", q, k, v, k_cache, v_cache);
   at::AutoDispatchBelowADInplaceOrView below;
   return window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks, scale);
 }

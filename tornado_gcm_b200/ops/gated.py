@@ -24,7 +24,8 @@ def gated_linear(x: torch.Tensor, w_gate: torch.Tensor, w_up: torch.Tensor, b_ga
                  b_up: Optional[torch.Tensor] = None, *, activation: str = "silu") -> torch.Tensor:
     """``(…, F)`` from ``x (…, K)`` and the weights ``(F, K)``; ``activation`` one of ``ops.linear.ACT_CODES``.
 
-    On the GPU the result is BF16 and so is the arithmetic's input; on the CPU it has ``x``'s type.
+    On the GPU the result is BF16 and so is the arithmetic's input, and only first derivatives in reverse mode are
+    there (others are refused); on the CPU it has ``x``'s type.
     """
     act = ACT_CODES.get(activation)
     if act is None:

@@ -5,7 +5,8 @@ values, with optional scale and shift shared by the heads) and turns the first `
 of the token's position.  :func:`rotary_table` makes the cosines and sines once, in fp64, for whole-numbered or
 real positions (time steps, longitudes, level indices), with the two usual stretchings for sequences longer than
 those trained on.  Forward and backward are one kernel each for queries and keys together; the statistics and the
-parameter gradients are held in fp32, and the parameter gradients are added in a fixed order.
+parameter gradients are held in fp32, and the parameter gradients are added in a fixed order.  Second and forward-mode
+derivatives are refused on the GPU.
 """
 
 from __future__ import annotations

@@ -7,7 +7,8 @@ no score matrix is stored, and key tiles out of sight are never read.
 
 Kernels: ``csrc/window_attention_sm100.cu`` (bf16, tcgen05), ``csrc/window_attention.cu`` (fp32 and the shapes that
 the tensor cores do not take) and ``csrc/window_step.cu`` (one token over the cache).  Softmax statistics and sums
-are fp32; the gradients use no atomics, so a pass gives the same bits every time.
+are fp32; the gradients use no atomics, so a pass gives the same bits every time.  Second and forward-mode derivatives
+are refused on the GPU.
 """
 
 from __future__ import annotations
