@@ -63,6 +63,21 @@ def test_rows_whose_every_score_is_minus_infinity_give_zeros(dtype, D, causal):
     assert (o == 0).all()
 
 
+@pytest.mark.parametrize("T", [4, 300])
+def test_gated_relu_keeps_nan(T):
+    from tornado_gcm_b200.ops.gated import gated_linear
+
+    ts = [t.requires_grad_() for t in _gated_inputs(T, 64, 96, True)]
+    with torch.no_grad():
+        ts[3][7] = math.nan
+    h = gated_linear(*ts, activation="relu")
+    bad = torch.zeros(96, dtype=torch.bool, device=DEV)
+    bad[7] = True
+    assert torch.equal(h.isnan(), bad.expand(T, 96))
+    dwu = torch.autograd.grad(h, ts[2], torch.ones_like(h))[0]  # du = dh * act
+    assert torch.equal(dwu.isnan(), bad[:, None].expand(96, 64))
+
+
 # ── derivatives ────────────────────────────────────────────────────────────
 def _three():
     """The operators that have a backward pass: a call, its differentiable inputs."""

@@ -100,6 +100,9 @@ __device__ __forceinline__ float2 all2(float v) { return make_float2(v, v); }
 constexpr float kGeluC1 = 1.5957691216057308f, kGeluC3 = 0.044715f;
 constexpr float kLog2E = 1.4426950408889634f;
 
+// NaN stays NaN (a maximum would make it 0).
+__device__ __forceinline__ float2 relu2(float2 z) { return make_float2(z.x <= 0.f ? 0.f : z.x, z.y <= 0.f ? 0.f : z.y); }
+
 // act(z) of a pair of pre-activations
 template <int ACT>
 __device__ __forceinline__ float2 act_val2(float2 z) {
@@ -109,7 +112,7 @@ __device__ __forceinline__ float2 act_val2(float2 z) {
   } else if constexpr (ACT == kActSilu) {
     return mul2(z, sigmoid2(mul2(z, all2(-kLog2E))));
   } else if constexpr (ACT == kActRelu) {
-    return make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f));
+    return relu2(z);
   } else if constexpr (ACT == kActGelu) {
     return make_float2(gelu_erf_f(z.x), gelu_erf_f(z.y));
   } else if constexpr (ACT == kActTanh) {
@@ -136,8 +139,8 @@ __device__ __forceinline__ void act_both2(float2 z, float2* a, float2* da) {
     float2 t = mul2(*a, fma2(s, all2(-1.f), all2(1.f)));  // z s (1 - s)
     *da = ACT == kActGeluTanh ? fma2(t, slope, s) : add2(t, s);
   } else if constexpr (ACT == kActRelu) {
-    *a = make_float2(fmaxf(z.x, 0.f), fmaxf(z.y, 0.f));
-    *da = make_float2(z.x > 0.f ? 1.f : 0.f, z.y > 0.f ? 1.f : 0.f);
+    *a = relu2(z);
+    *da = make_float2(z.x <= 0.f ? 0.f : 1.f, z.y <= 0.f ? 0.f : 1.f);
   } else if constexpr (ACT == kActGelu) {
     const float2 c = make_float2(0.5f * (1.f + erff(z.x * 0.7071067811865476f)),
                                  0.5f * (1.f + erff(z.y * 0.7071067811865476f)));
