@@ -78,6 +78,26 @@ def test_gated_relu_keeps_nan(T):
     assert torch.equal(dwu.isnan(), bad[:, None].expand(96, 64))
 
 
+def test_padding_of_the_model_may_hold_anything():
+    from tornado_gcm_b200.models import sequence
+
+    torch.manual_seed(0)
+    m = sequence.SequenceEmulator(9, 3, statics=2, d_model=128, num_heads=2, num_layers=2, d_ff=80, window=30,
+                                  max_positions=256).to(DEV)
+    torch.nn.init.normal_(m.head.weight, std=0.1)
+    states, static = sequence.synthetic_columns(3, 150, 9, 3, device=DEV)
+    L = torch.tensor([150, 70, 0], dtype=torch.int32, device=DEV)
+    res = []
+    for junk in (0.0, math.nan):
+        s = states.clone()
+        s[1, 70:], s[2] = junk, junk
+        m.zero_grad()
+        loss = m.loss(s, static, L)
+        loss.backward()
+        res.append([loss.detach()] + [p.grad.clone() for p in m.parameters()])
+    assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(*res))
+
+
 # ── derivatives ────────────────────────────────────────────────────────────
 def _three():
     """The operators that have a backward pass: a call, its differentiable inputs."""

@@ -189,6 +189,34 @@ def test_the_step_has_no_gradient_and_says_so():
     assert not layer.attn.step(x[:, 8], cache.k[0], cache.v[0], cache.lengths).requires_grad
 
 
+def test_padding_of_the_model_may_hold_anything():
+    m = _emulator()
+    states, static = sequence.synthetic_columns(3, 16, 5, 3)
+    L = torch.tensor([16, 9, 0], dtype=torch.int32)
+    res = []
+    for junk in (0.0, math.nan, math.inf):
+        s = states.clone()
+        s[1, 9:], s[2] = junk, junk
+        m.zero_grad()
+        loss = m.loss(s, static, L)
+        loss.backward()
+        res.append([loss.detach()] + [p.grad.clone() for p in m.parameters()])
+    for other in res[1:]:
+        assert all(torch.isfinite(b).all() and torch.equal(a, b) for a, b in zip(res[0], other))
+    body = _body()
+    x = _randn(2, 12, 32, seed=4)
+    n = torch.tensor([12, 5], dtype=torch.int32)
+    res = []
+    for junk in (0.0, math.nan):
+        body.zero_grad()
+        y = x.clone()
+        y[1, 5:] = junk
+        out = body(y, n)
+        (out[0].sum() + out[1, :5].square().sum()).backward()
+        res.append([out.detach()[0], out.detach()[1, :5]] + [p.grad.clone() for p in body.parameters()])
+    assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(*res))
+
+
 def test_rows_whose_every_score_is_minus_infinity_give_zeros():
     q, k, v = (_randn(1, 8, 1, 4, seed=i) for i in range(3))
     k[..., 3] = 1.0

@@ -20,7 +20,7 @@ from typing import Optional
 import torch
 import torch.nn as nn
 
-from tornado_gcm_b200.neural.sequence_layers import SequenceTransformer, WindowCache
+from tornado_gcm_b200.neural.sequence_layers import SequenceTransformer, WindowCache, without_padding
 from tornado_gcm_b200.ops import _ext
 from tornado_gcm_b200.ops.gradnorm import clip_grad_norm
 
@@ -48,9 +48,10 @@ class SequenceEmulator(nn.Module):
     def forward(self, states: torch.Tensor, static: Optional[torch.Tensor] = None,
                 lengths: Optional[torch.Tensor] = None, cache: Optional[WindowCache] = None) -> torch.Tensor:
         """``states (B, T, features)`` and ``static (B, static_features)`` to the next state of every step.
-        ``lengths`` int32 ``(B,)``: valid states of each sequence (negative: it takes no part); ``cache`` takes the
-        valid history in."""
+        ``lengths`` int32 ``(B,)``: valid states of each sequence (negative: it takes no part), what lies behind is taken
+        for zeros; ``cache`` takes the valid history in."""
         if lengths is not None:
+            states = without_padding(states, lengths)
             lengths = torch.where(lengths < 0, lengths, lengths + self.statics)
         h = self.body(self._tokens(states, static), lengths, cache=cache)
         return states + self.head(h[:, self.statics:])
@@ -58,6 +59,8 @@ class SequenceEmulator(nn.Module):
     def loss(self, states: torch.Tensor, static: Optional[torch.Tensor] = None,
              lengths: Optional[torch.Tensor] = None) -> torch.Tensor:
         """Mean squared error of the predicted next states, over the valid ones."""
+        if lengths is not None:
+            states = without_padding(states, lengths)
         err = (self(states[:, :-1], static, None if lengths is None else (lengths - 1).clamp(min=0))
                - states[:, 1:]).square().mean(-1)
         if lengths is None:

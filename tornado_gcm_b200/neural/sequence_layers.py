@@ -29,6 +29,13 @@ def _linear(x: torch.Tensor, lin: nn.Linear) -> torch.Tensor:
     return F.linear(x, lin.weight.to(x.dtype), None if lin.bias is None else lin.bias.to(x.dtype))
 
 
+def without_padding(x: torch.Tensor, lengths: torch.Tensor) -> torch.Tensor:
+    """``x (B, S, features)`` with zeros behind each sequence's end, whatever was there: a product with a weight of zero
+    would carry NaN from it into gradients."""
+    behind = torch.arange(x.shape[1], device=x.device) >= lengths.to(x.device)[:, None]
+    return x.masked_fill(behind[..., None], 0.0)
+
+
 def _zone(x: torch.Tensor) -> torch.Tensor:
     return x.to(torch.bfloat16) if x.is_cuda else x
 
@@ -163,9 +170,12 @@ class SequenceTransformer(nn.Module):
         self.final_ln = nn.LayerNorm(d_model)
 
     def forward(self, x: torch.Tensor, lengths=None, positions=None, cache: Optional[WindowCache] = None) -> torch.Tensor:
-        """``cache`` takes the history in; with ``lengths`` each sequence's valid tokens only, so that its steps go on
+        """``lengths`` int32 ``(B,)``: valid tokens of each sequence; what lies behind may hold anything and is taken for
+        zeros.  ``cache`` takes the history in; with ``lengths`` each sequence's valid tokens only, so that its steps go on
         behind them (a negative length: the sequence takes no part).  ``positions``, ``(S,)`` or ``(B, S)``: those of
         the tokens; steps go on behind the last valid one (a sequence without tokens: at the first)."""
+        if lengths is not None:
+            x = without_padding(x, lengths)
         for i, layer in enumerate(self.layers):
             x = layer(x, lengths, positions, None if cache is None else (cache.k[i], cache.v[i]))
         if cache is not None:
