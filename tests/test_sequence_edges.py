@@ -78,6 +78,30 @@ def test_gated_relu_keeps_nan(T):
     assert torch.equal(dwu.isnan(), bad[:, None].expand(96, 64))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("norm", ["rms", "layer"])
+@pytest.mark.parametrize("H,Hk,D,R,S", [(5, 1, 64, 64, 30), (3, 2, 32, 16, 9), (1, 1, 16, 16, 70), (5, 3, 40, 20, 9)])
+def test_qk_norm_rotary_without_epsilon(H, Hk, D, R, S, norm, dtype):
+    """eps = 0 is sound where no head is constant; head counts that leave lanes of the last load idle."""
+    from tornado_gcm_b200.ops.rotary import qk_norm_rotary, rotary_table
+
+    q, k = (_randn(2, S, h, D, seed=h, dtype=dtype).requires_grad_() for h in (H, Hk))
+    w = [(1 + _randn(D, seed=s, scale=0.2)).requires_grad_() for s in (3, 4)]
+    b = [_randn(D, seed=s).requires_grad_() for s in (5, 6)] if norm == "layer" else [None, None]
+    table = rotary_table(S, R, device=DEV)
+    y = qk_norm_rotary(q, k, table, *w, *b, norm=norm, eps=0.0)
+    leaves = [t for t in (q, k, *w, *b) if t is not None]
+    up = [_randn(*t.shape, seed=9, dtype=dtype) for t in y]
+    grads = torch.autograd.grad(y, leaves, up)
+    r = {id(t): t.detach().double().requires_grad_() for t in leaves}
+    pos = torch.arange(S, device=DEV)
+    y64 = [_qk64(r[id(x)], r[id(w[i])], r.get(id(b[i])), table, pos, norm, False, 0.0) for i, x in enumerate((q, k))]
+    for a, c in zip(y, y64):
+        _close(a, c, TOL[dtype])
+    for i, (a, c) in enumerate(zip(grads, torch.autograd.grad(y64, list(r.values()), [u.double() for u in up]))):
+        _close(a, c, TOL[a.dtype], f"gradient {i}")
+
+
 def test_padding_of_the_model_may_hold_anything():
     from tornado_gcm_b200.models import sequence
 

@@ -271,7 +271,10 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? kRotBwdBlocks : kRotFwdBloc
           float q = 0.f;
 #pragma unroll
           for (int e = 0; e < V; ++e) q = fmaf(x[e], x[e], q);
-          r = rsqrtf(row_sum<LPR>(q) * inv_d + p.eps);
+          q = row_sum<LPR>(q);
+          // a lane group without a head takes part in the shuffles alone: 1 / sqrt(eps) of an eps of zero would put
+          // 0 * inf into the parameter sums
+          r = h < H ? rsqrtf(q * inv_d + p.eps) : 0.f;
         }
         if (!BWD) {
 #pragma unroll
