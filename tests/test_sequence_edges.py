@@ -102,6 +102,26 @@ def test_qk_norm_rotary_without_epsilon(H, Hk, D, R, S, norm, dtype):
         _close(a, c, TOL[a.dtype], f"gradient {i}")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+@pytest.mark.parametrize("D,R,inter", [(64, 32, False), (64, 32, True), (64, 30, True), (40, 20, False), (64, 0, False)])
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+def test_values_outside_the_rotation_pass_as_they_are(D, R, inter, bad, dtype):
+    from tornado_gcm_b200.ops.rotary import qk_norm_rotary, rotary_table
+
+    q = _randn(1, 5, 3, D, seed=1, dtype=dtype)
+    q[0, 2, 1, R + 3] = bad
+    q.requires_grad_()
+    table = rotary_table(5, R, device=DEV) if R else None
+    up = _randn(1, 5, 3, D, seed=2, dtype=dtype)
+    up[0, 2, 1, R + 3] = bad
+    y, _ = qk_norm_rotary(q, q.detach(), table, norm="none", interleaved=inter)
+    (g,) = torch.autograd.grad(y, q, up)
+    for a, src in ((y, q), (g, up)):
+        odd = ~torch.isfinite(a)
+        assert int(odd.sum()) == 1 and bool(odd[0, 2, 1, R + 3])
+        assert torch.equal(a[..., R:].nan_to_num(9.0, 8.0), src.detach()[..., R:].nan_to_num(9.0, 8.0))
+
+
 def test_padding_of_the_model_may_hold_anything():
     from tornado_gcm_b200.models import sequence
 

@@ -149,21 +149,26 @@ __device__ __forceinline__ float row_sum(float x) {
 }
 
 // Turns the lane's vector.  Half layout: element e of lanes [0, R/2/V) pairs
-// with element e of the lane R/2/V further; cs holds this element's pair.
+// with element e of the lane R/2/V further; cs holds this element's pair.  The
+// lane's first `turned` elements take part (half layout: all or none); the others
+// stay as they are, infinities and NaN among them.
 template <int V>
-__device__ __forceinline__ void turn(float (&v)[V], const float (&c)[V], const float (&s)[V], bool inter, int partner) {
+__device__ __forceinline__ void turn(float (&v)[V], const float (&c)[V], const float (&s)[V], bool inter, int partner,
+                                     int turned) {
   if (inter) {
 #pragma unroll
     for (int e = 0; e < V; e += 2) {
       const float a = v[e], b = v[e + 1];
-      v[e] = a * c[e] - b * s[e];
-      v[e + 1] = b * c[e] + a * s[e];
+      if (e < turned) {
+        v[e] = a * c[e] - b * s[e];
+        v[e + 1] = b * c[e] + a * s[e];
+      }
     }
-  } else {  // s carries the sign: -sin for first halves, +sin for second ones, 0 outside
+  } else {  // s carries the sign: -sin for first halves, +sin for second ones
 #pragma unroll
     for (int e = 0; e < V; ++e) {
       const float o = __shfl_sync(0xffffffffu, v[e], partner);
-      v[e] = v[e] * c[e] + o * s[e];
+      if (turned > 0) v[e] = v[e] * c[e] + o * s[e];
     }
   }
 }
@@ -196,6 +201,7 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? kRotBwdBlocks : kRotFwdBloc
   const int hl = half / V;
   const bool first = live && d0 < half, second = live && d0 >= half && d0 < p.R;
   const int partner = p.interleaved ? lane : (first ? lane + hl : (second ? lane - hl : lane));
+  const int turned = live ? min(V, max(0, p.R - d0)) : 0;
   const int H = hs.H;
   const int step = hs.blocks * kRotWarps, tokens = static_cast<int>(p.tokens);
   int t = block * kRotWarps + warp;
@@ -226,7 +232,7 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? kRotBwdBlocks : kRotFwdBloc
     float c[V], sn[V];
 #pragma unroll
     for (int e = 0; e < V; ++e) c[e] = 1.f, sn[e] = 0.f;
-    if (live && d0 < p.R) {
+    if (turned > 0) {
       const float2* row = p.table + static_cast<long long>(at) * half;
       const float dir = BWD ? -1.f : 1.f;
       if (p.interleaved) {
@@ -279,12 +285,12 @@ __global__ void __launch_bounds__(kRotThreads, BWD ? kRotBwdBlocks : kRotFwdBloc
         if (!BWD) {
 #pragma unroll
           for (int e = 0; e < V; ++e) x[e] = fmaf(x[e] * r, sw[d0 + e], sb[d0 + e]);
-          turn<V>(x, c, sn, p.interleaved, partner);
+          turn<V>(x, c, sn, p.interleaved, partner, turned);
           if (on) *reinterpret_cast<uint4*>(yt + h * p.D) = pack16<T>(x);
         } else {
           float g[V];
           unpack16<T>(gu[u], g);
-          turn<V>(g, c, sn, p.interleaved, partner);
+          turn<V>(g, c, sn, p.interleaved, partner, turned);
           if (p.norm != kNormNone) {
             float m1 = 0.f, m2 = 0.f;
 #pragma unroll
