@@ -217,6 +217,21 @@ def test_padding_of_the_model_may_hold_anything():
     assert all(torch.isfinite(a).all() and torch.equal(a, b) for a, b in zip(*res))
 
 
+@pytest.mark.parametrize("causal", [True, False])
+def test_gradients_with_keys_behind_the_end_that_hold_anything(causal):
+    q, k, v = (_randn(2, 9, h, 4, seed=i, dtype=torch.float64) for i, h in enumerate((2, 1, 1)))
+    lengths = torch.tensor([9, 4], dtype=torch.int32)
+    res = []
+    for junk in (0.0, math.nan, math.inf):
+        ts = [q.clone(), k.clone(), v.clone()]
+        ts[1][1, 4:], ts[2][1, 4:] = junk, junk
+        ts = [t.requires_grad_() for t in ts]
+        o = window_attention(*ts, window=3, sinks=1, causal=causal, lengths=lengths)
+        res.append([o, *torch.autograd.grad(o.square().sum(), ts)])
+    for other in res[1:]:
+        assert all(torch.isfinite(b).all() and torch.equal(a, b) for a, b in zip(res[0], other))
+
+
 def test_rows_whose_every_score_is_minus_infinity_give_zeros():
     q, k, v = (_randn(1, 8, 1, 4, seed=i) for i in range(3))
     k[..., 3] = 1.0

@@ -41,12 +41,12 @@ def _torch_form(q, k, v, window, sinks, causal, lengths, scale):
     n = q.shape[2] // k.shape[2]
     c = torch.float64 if q.dtype == torch.float64 else torch.float32
     qh, kh, vh = (t.transpose(1, 2).to(c) for t in (q, k.repeat_interleave(n, 2), v.repeat_interleave(n, 2)))
+    if lengths is not None:  # what lies behind the end may hold anything
+        behind = (torch.arange(q.shape[1], device=q.device) >= lengths.to(q.device)[:, None])[:, None, :, None]
+        kh, vh = kh.masked_fill(behind, 0.0), vh.masked_fill(behind, 0.0)
     s = (qh @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
     dead = (s == -math.inf).all(-1, keepdim=True)
     p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
-    if lengths is not None:  # what lies behind the end may hold anything
-        at = torch.arange(q.shape[1], device=q.device)[None, None, :, None]
-        vh = vh.masked_fill(at >= lengths.to(q.device)[:, None, None, None], 0.0)
     return (p @ vh).transpose(1, 2).to(q.dtype)
 
 
