@@ -242,3 +242,13 @@ def test_rows_whose_every_score_is_minus_infinity_give_zeros():
     assert (got[:, 2] == 0).all() and torch.equal(got[:, 3:], want[:, 3:]) and torch.equal(got[:, :2], want[:, :2])
     n = torch.full((1,), 7, dtype=torch.int32)
     assert (window_attention_step(q[:, 2], k[:, 7], v[:, 7], k.clone(), v.clone(), n) == 0).all()
+
+
+def test_positions_outside_the_table_are_refused():
+    q = _randn(1, 2, 1, 4, seed=1)
+    table = rotary_table(8, 4)
+    for pos in ([-1, 0], [0, 8]):
+        with pytest.raises(IndexError):
+            qk_norm_rotary(q, q, table, norm="none", positions=torch.tensor(pos))
+    with pytest.raises(ValueError):
+        qk_norm_rotary(q, q, table[:1], norm="none")

@@ -54,6 +54,10 @@ def _torch_form(q, k, table, positions, qw, kw, qb, kb, norm, interleaved, eps):
     out = []
     cs = None
     if table is not None and table.shape[1]:
+        if positions is None and q.shape[1] > table.shape[0]:
+            raise ValueError(f"qk_norm_rotary: the table has {table.shape[0]} positions, the sequence {q.shape[1]}")
+        if positions is not None and bool((positions < 0).any()):
+            raise IndexError("qk_norm_rotary: a position is negative")
         cs = table[: q.shape[1]] if positions is None else table[positions.long()]
         cs = cs.unsqueeze(-3)  # (…, S, 1, R/2, 2)
     for x, w, b in ((q, qw, qb), (k, kw, kb)):
@@ -91,7 +95,7 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tenso
     ``table``: :func:`rotary_table`; its width sets how much of the head turns, ``None`` turns nothing.
     ``positions``: rows of the table, int32 or int64, ``(B, S)`` or ``(S,)``; ``None`` means 0 … S-1.  A position
     outside the table is reported through the device error flag (:func:`tornado_gcm_b200.ops._ext.check_error_flag`)
-    and takes the nearest row.  ``norm``: ``"layer"``, ``"rms"`` or ``"none"``; weights and shifts are fp32 vectors
+    and takes the nearest row; on the CPU it raises ``IndexError``.  ``norm``: ``"layer"``, ``"rms"`` or ``"none"``; weights and shifts are fp32 vectors
     of ``D`` values.  ``interleaved``: pairs are neighbours (2i, 2i+1) instead of (i, i + rotary_dim/2).
     """
     if norm not in NORM_CODES:
