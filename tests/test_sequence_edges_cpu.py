@@ -252,3 +252,14 @@ def test_positions_outside_the_table_are_refused():
             qk_norm_rotary(q, q, table, norm="none", positions=torch.tensor(pos))
     with pytest.raises(ValueError):
         qk_norm_rotary(q, q, table[:1], norm="none")
+
+
+def test_the_step_computes_in_its_inputs_type():
+    q, k, v = (_randn(2, h, 8, seed=i, dtype=torch.float64) for i, h in enumerate((4, 2, 2)))
+    kc, vc = (_randn(2, 6, 2, 8, seed=i, dtype=torch.float64) for i in (5, 6))
+    n = torch.tensor([3, 20], dtype=torch.int32)
+    o = window_attention_step(q, k, v, kc, vc, n, sinks=1)
+    for b, seen in enumerate((4, 6)):
+        kk, vv = (t[b, :seen].repeat_interleave(2, 1) for t in (kc, vc))
+        p = torch.softmax(torch.einsum("hd,nhd->hn", q[b], kk) * 8 ** -0.5, -1)
+        assert torch.allclose(o[b], torch.einsum("hn,nhd->hd", p, vv), atol=1e-14)

@@ -114,8 +114,9 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
     k_cache[on, slot], v_cache[on, slot] = k[on], v[on]
     see = torch.arange(cap)[None, None, None] <= at[:, None, None, None]
     n = q.shape[1] // k.shape[1]
-    kh, vh = (t.repeat_interleave(n, 2).transpose(1, 2).float() for t in (k_cache, v_cache))
-    s = (q.float()[:, :, None] @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
+    c = torch.float64 if q.dtype == torch.float64 else torch.float32
+    kh, vh = (t.repeat_interleave(n, 2).transpose(1, 2).to(c) for t in (k_cache, v_cache))
+    s = (q.to(c)[:, :, None] @ kh.transpose(-1, -2) * scale).masked_fill(~see, -math.inf)
     dead = (s == -math.inf).all(-1, keepdim=True)
     p = torch.softmax(s.masked_fill(dead, 0.0), -1).masked_fill(dead, 0.0)
     vh = vh.masked_fill(~see.transpose(-1, -2), 0.0)
