@@ -262,4 +262,4 @@ def test_the_step_computes_in_its_inputs_type():
     for b, seen in enumerate((4, 6)):
         kk, vv = (t[b, :seen].repeat_interleave(2, 1) for t in (kc, vc))
         p = torch.softmax(torch.einsum("hd,nhd->hn", q[b], kk) * 8 ** -0.5, -1)
-        assert torch.allclose(o[b], torch.einsum("hn,nhd->hd", p, vv), atol=1e-14)
+        assert torch.allclose(o[b], torch.einsum("hn,nhd->hd", p, vv), rtol=0, atol=1e-14)
