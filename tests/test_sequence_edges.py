@@ -206,6 +206,17 @@ def test_window_step_has_no_gradient_and_says_so(dtype):
             assert torch.equal(window_attention_step(*ts, n), want)
 
 
+def test_caches_whose_sequences_share_memory_are_refused():
+    from tornado_gcm_b200.ops.window_attention import window_attention_step
+
+    q = _randn(3, 1, 32, seed=1)
+    own, shared = torch.zeros(3, 6, 1, 32, device=DEV), torch.zeros(1, 6, 1, 32, device=DEV).expand(3, 6, 1, 32)
+    n = torch.zeros(3, dtype=torch.int32, device=DEV)
+    for kc, vc in ((shared, own), (own, shared)):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            window_attention_step(q, q, q, kc, vc, n)
+
+
 # ── the model's caches ─────────────────────────────────────────────────────
 def _body():
     from tornado_gcm_b200.neural.sequence_layers import SequenceTransformer

@@ -263,3 +263,12 @@ def test_the_step_computes_in_its_inputs_type():
         kk, vv = (t[b, :seen].repeat_interleave(2, 1) for t in (kc, vc))
         p = torch.softmax(torch.einsum("hd,nhd->hn", q[b], kk) * 8 ** -0.5, -1)
         assert torch.allclose(o[b], torch.einsum("hn,nhd->hd", p, vv), rtol=0, atol=1e-14)
+
+
+def test_caches_whose_sequences_share_memory_are_refused():
+    q = _randn(3, 1, 8, seed=1)
+    own, shared = torch.zeros(3, 6, 1, 8), torch.zeros(1, 6, 1, 8).expand(3, 6, 1, 8)
+    n = torch.zeros(3, dtype=torch.int32)
+    for kc, vc in ((shared, own), (own, shared)):
+        with pytest.raises(RuntimeError, match="single memory location"):
+            window_attention_step(q, q, q, kc, vc, n)

@@ -23,6 +23,7 @@
 #include "sequence_ops.h"
 
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <torch/library.h>
@@ -568,6 +569,7 @@ at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const
     TORCH_CHECK(t->device() == q.device() && t->scalar_type() == q.scalar_type() && t->dim() == 4 &&
                     t->size(0) == B && t->size(2) == Hk && t->size(3) == D && (D == 1 || t->stride(3) == 1),
                 "window_attention_step: the caches must be (batch, sinks + window, key heads, head_dim) of q's type");
+    at::assert_no_internal_overlap(*t);  // sequences would overwrite each other's slots
   }
   TORCH_CHECK(k_cache.size(1) == v_cache.size(1), "window_attention_step: the caches differ in slots");
   const int64_t cap = k_cache.size(1);

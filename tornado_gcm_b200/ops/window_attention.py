@@ -105,6 +105,9 @@ def window_attention_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, k_c
         return _ext.op("window_attention_step")(q, k, v, k_cache, v_cache, lengths, int(sinks), scale)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (q, k, v, k_cache, v_cache)):
         raise RuntimeError("window_attention_step: no gradient; call it under torch.no_grad()")
+    for t in (k_cache, v_cache):
+        if any(n > 1 and s == 0 for n, s in zip(t.shape, t.stride())):
+            raise RuntimeError("window_attention_step: cache elements share a single memory location")
     cap = k_cache.shape[1]
     if not 0 <= sinks < cap:
         raise ValueError("window_attention_step: sinks must lie between 0 and the cache's slots")
