@@ -206,6 +206,39 @@ def test_window_step_has_no_gradient_and_says_so(dtype):
             assert torch.equal(window_attention_step(*ts, n), want)
 
 
+def test_writes_are_seen_by_autograd():
+    """A value that a graph has saved and an operator then overwrites is an error, not a wrong gradient."""
+    from tornado_gcm_b200.ops.gradnorm import clip_grad_norm
+    from tornado_gcm_b200.ops.window_attention import window_attention, window_attention_step
+
+    w = torch.ones((), device=DEV, requires_grad=True)
+    q = _randn(2, 1, 32, seed=1)
+    kc, vc = torch.zeros(2, 6, 1, 32, device=DEV), torch.zeros(2, 6, 1, 32, device=DEV)
+    n = torch.zeros(2, dtype=torch.int32, device=DEV)
+    for cache in (kc, vc):
+        y = (cache * w).sum()
+        window_attention_step(q, q, q, kc, vc, n)
+        with pytest.raises(RuntimeError, match="modified by an inplace"):
+            y.backward()
+    g, o = _randn(100, seed=2), torch.empty(100, device=DEV)
+    y = (g * w).sum()
+    clip_grad_norm([g], 0.1)
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    y = (o * w).sum()
+    before = g._version
+    clip_grad_norm([g], 0.1, out=[o])
+    assert g._version == before
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+    a = _randn(2, 9, 1, 32, seed=3).requires_grad_()
+    lengths = torch.full((2,), 9, dtype=torch.int32, device=DEV)
+    y = window_attention(a, a, a, window=3, lengths=lengths).sum()
+    lengths -= 1
+    with pytest.raises(RuntimeError, match="modified by an inplace"):
+        y.backward()
+
+
 def test_caches_whose_sequences_share_memory_are_refused():
     from tornado_gcm_b200.ops.window_attention import window_attention_step
 

@@ -23,6 +23,7 @@
 // itself, so no counter, no atomic and no second barrier is needed and two
 // calls give the same bits.
 #include "alloc.h"
+#include "sequence_ops.h"
 
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>

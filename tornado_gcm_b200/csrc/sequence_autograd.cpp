@@ -31,6 +31,11 @@ void refuse_forward_mode(const char* name, const T&... inputs) {
   TORCH_CHECK_NOT_IMPLEMENTED(!(dual(inputs) || ...), name, ": no forward-mode derivative");
 }
 
+// A graph that has saved t finds that it has changed since.
+void written(const at::Tensor& t) {
+  if (!t.is_inference()) torch::autograd::impl::bump_version(t);
+}
+
 // A node's gradients under create_graph: they have no history, so one that says so takes its place.  `of`: the
 // node's inputs and the upstream gradients, on which the gradients depend.
 variable_list first_only(variable_list grads, const variable_list& of, const char* name) {
@@ -208,8 +213,24 @@ at::Tensor window_attention_step_autograd(const at::Tensor& q, const at::Tensor&
                   !(wants(q) || wants(k) || wants(v) || wants(k_cache) || wants(v_cache)),
               "window_attention_step: no gradient; call it under torch.no_grad()");
   refuse_forward_mode("window_attention_step", q, k, v, k_cache, v_cache);
-  at::AutoDispatchBelowADInplaceOrView below;
-  return window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks, scale);
+  at::Tensor o;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    o = window_attention_step(q, k, v, k_cache, v_cache, lengths, sinks, scale);
+  }
+  written(k_cache);
+  written(v_cache);
+  return o;
+}
+
+at::Tensor clip_grad_norm_autograd(at::TensorList grads, at::TensorList out, double max_norm) {
+  at::Tensor norm;
+  {
+    at::AutoDispatchBelowADInplaceOrView below;
+    norm = clip_grad_norm(grads, out, max_norm);
+  }
+  for (const auto& t : out.empty() ? grads : out) written(t);
+  return norm;
 }
 
 }  // namespace
@@ -235,4 +256,5 @@ TORCH_LIBRARY_IMPL(tgcm, AutogradCUDA, m) {
   m.impl("qk_norm_rotary", &tgcm::qk_norm_rotary_autograd);
   m.impl("window_attention", &tgcm::window_attention_autograd);
   m.impl("window_attention_step", &tgcm::window_attention_step_autograd);
+  m.impl("clip_grad_norm", &tgcm::clip_grad_norm_autograd);
 }

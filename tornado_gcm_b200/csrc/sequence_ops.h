@@ -43,4 +43,7 @@ std::vector<at::Tensor> window_attention_bwd(const at::Tensor& dout, const at::T
 at::Tensor window_attention_step(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, at::Tensor& k_cache,
                                  at::Tensor& v_cache, const at::Tensor& lengths, int64_t sinks, double scale);
 
+// the norm; clips into `out`, or in place where that is empty; no backward pass
+at::Tensor clip_grad_norm(at::TensorList grads, at::TensorList out, double max_norm);
+
 }  // namespace tgcm

@@ -53,7 +53,6 @@ def clip_grad_norm(grads: Iterable[torch.Tensor], max_norm: float,
     if not grads:
         return torch.zeros(())
     if grads[0].is_cuda:
-        # the operator changes its arguments in place below autograd's sight, as an optimizer does
         return _ext.op("clip_grad_norm")(grads, [] if out is None else out_list, float(max_norm))
     with torch.no_grad():
         for g, o in zip(grads, out_list):
