@@ -252,7 +252,7 @@ __device__ __forceinline__ void clear_rows(uint8_t* tile, int rows, int first, i
 template <int DP>
 struct FwdCfg {
   static constexpr int KT = 64;
-  static constexpr int kBufs = 2;   // score tiles in flight
+  static constexpr int kBufs = 2;   // score tiles: one is made while the other is worked on
   static constexpr int kSlots = 4;
   static constexpr int kSlot = KT * DP * 2;
   static constexpr int kQ = 128 * DP * 2;
@@ -369,7 +369,7 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
       };
       bool go = warp_wait(q_full, 0, err, kErrTimeoutFull) && scores(0);
       for (int j = 0; j < kt.n && go; ++j) {
-        if (C::kBufs == 2 && j + 1 < kt.n && !(go = scores(j + 1))) break;
+        if (j + 1 < kt.n && !(go = scores(j + 1))) break;
         const int it = 2 * j + 1, s = it % C::kSlots;
         int j0, cols;
         key_tile<KT>(kt, j, &j0, &cols);
@@ -387,7 +387,6 @@ __global__ void __launch_bounds__(kAttnThreads, 2)
           if (j + 1 == kt.n) tc_commit(all_done);
         }
         __syncwarp();
-        if (C::kBufs == 1 && j + 1 < kt.n) go = scores(j + 1);
       }
       if (!go) *abort_flag = 1;
     }
