@@ -301,3 +301,99 @@ def test_forecast_past_the_table_of_positions():
         res.append(m.forecast(states, static, steps=40))
     assert torch.equal(*res)
     _ext.check_error_flag(DEV)
+
+
+# ── graphs, streams, broadcast gradients ───────────────────────────────────
+def _pass(call, ts):
+    ys = call(*ts)
+    ups = [torch.linspace(-1, 1, y.numel(), device=DEV).to(y.dtype).view_as(y) for y in ys]
+    grads = torch.autograd.grad(ys, ts, ups)
+    return [y.detach() for y in ys] + list(grads)  # a graph kept alive would tie the capture to this stream
+
+
+@pytest.mark.parametrize("name", NAMES)
+def test_training_pass_in_a_graph_and_on_another_stream(name):
+    call, ts = _three()[name]
+    ts = [t.requires_grad_() for t in ts]
+    want = _pass(call, ts)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = _pass(call, ts)
+    s.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(want, got))
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = _pass(call, ts)
+    with torch.no_grad():
+        for t in ts:
+            t.mul_(0.75)
+    for _ in range(2):
+        g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(_pass(call, ts), captured))
+    _ext.check_error_flag(DEV)
+
+
+def test_wide_gated_pass_in_a_graph():
+    """Sizes that split dW over the tokens, so every kernel of the pass is captured, with its place in the order."""
+    from tornado_gcm_b200.ops.gated import gated_linear
+
+    ts = [t.requires_grad_() for t in _gated_inputs(4096, 128, 264, True)]
+    call = lambda *t: (gated_linear(*t, activation="gelu_tanh"),)  # noqa: E731
+    _pass(call, ts)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = _pass(call, ts) + _pass(call, ts)
+    for _ in range(3):
+        g.replay()
+    torch.cuda.synchronize()
+    want = _pass(call, ts)
+    assert all(torch.equal(a, b) for a, b in zip(want + want, captured))
+    _ext.check_error_flag(DEV)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, BF])
+def test_steps_in_a_graph_and_on_another_stream(dtype):
+    from tornado_gcm_b200.ops.window_attention import window_attention_step
+
+    q, k, v = (_randn(3, h, 64, seed=i, dtype=dtype) for i, h in enumerate((4, 2, 2)))
+    fresh = lambda: [torch.zeros(3, 12, 2, 64, dtype=dtype, device=DEV) for _ in range(2)]  # noqa: E731
+    n = torch.tensor([0, 5, 30], dtype=torch.int32, device=DEV)
+
+    def steps(kc, vc, n):
+        outs = []
+        for _ in range(4):
+            outs.append(window_attention_step(q, k, v, kc, vc, n, sinks=2))
+            n += 1
+        return outs
+
+    a, b, c = fresh(), fresh(), fresh()
+    want = steps(*a, n.clone())
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        got = steps(*b, n.clone())
+    s.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want + a, got + b))
+    m = n.clone()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        captured = steps(*c, m)
+    g.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, y) for x, y in zip(want + a, captured + c)) and torch.equal(m, n + 4)
+
+
+@pytest.mark.parametrize("name", NAMES)
+@pytest.mark.parametrize("axis", [0, 1])
+def test_gradients_that_are_broadcast(name, axis):
+    """A mean over tokens or sequences hands back a gradient with a stride of zero."""
+    call, ts = _three()[name]
+    ts = [t.requires_grad_() for t in ts]
+    ys = call(*ts)
+    ups = [_randn(*y.shape, seed=7, dtype=y.dtype).select(axis, 0).unsqueeze(axis) for y in ys]
+    got = torch.autograd.grad(ys, ts, [u.expand_as(y) for u, y in zip(ups, ys)], retain_graph=True)
+    want = torch.autograd.grad(ys, ts, [u.expand_as(y).contiguous() for u, y in zip(ups, ys)])
+    for i, (a, b) in enumerate(zip(got, want)):
+        _close(a, b, TOL[a.dtype], f"gradient {i}")
