@@ -13,10 +13,11 @@
 // block takes chunks of kChunk elements, strided by the grid; a chunk never
 // spans two tensors and is found by bisection in the list of first chunks.
 //
-// The sum is fp64, and the squares never overflow or vanish (in fp32 they would
-// above 1.8e19 and below 1e-23, which a diverging or a nearly converged model
-// reaches): the squares of one 16-byte vector are added in fp32, and a vector
-// whose sum leaves [1e-30, 1e37] is done over in fp64.  Converting every value
+// The squares of one 16-byte vector are added in fp32 (relative error of such a
+// sum below 5e-7), the vectors' sums in fp64.  No square overflows or vanishes (in
+// fp32 they would above 1.8e19 and below 1e-23, which a diverging or a nearly
+// converged model reaches): a vector whose sum leaves [1e-30, 1e37], one of zeros
+// among them, is done over in fp64.  Converting every value
 // would bound the bf16 pass: the unit converts 16 values a cycle and SM, and DRAM
 // brings 12 (800 MB: 146 us so).
 // Every block of pass 2 adds the partial sums of pass 1 in one fixed order

@@ -45,7 +45,7 @@ constexpr int kRotWarps = kRotThreads / 32;
 constexpr int kRotMaxDim = 256;
 constexpr int kRotBatch = 2;  // heads that a lane group asks for at once
 // Resident blocks of an SM: more of them spill (8192 x 2 tokens, 16 + 4 heads of 64: forward 28 us with 3, 36 us
-// with 4; adjoint 47 us with 2, 54 us with 3).
+// with 4; adjoint 47 us with 2, 54 us with 3; 30 and 49 us since values outside the rotation are left alone).
 constexpr int kRotFwdBlocks = 3, kRotBwdBlocks = 2;
 
 enum NormKind : int { kNormNone = 0, kNormRms = 1, kNormLayer = 2 };

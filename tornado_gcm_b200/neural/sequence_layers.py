@@ -170,10 +170,11 @@ class SequenceTransformer(nn.Module):
         self.final_ln = nn.LayerNorm(d_model)
 
     def forward(self, x: torch.Tensor, lengths=None, positions=None, cache: Optional[WindowCache] = None) -> torch.Tensor:
-        """``lengths`` int32 ``(B,)``: valid tokens of each sequence; what lies behind may hold anything and is taken for
-        zeros.  ``cache`` takes the history in; with ``lengths`` each sequence's valid tokens only, so that its steps go on
-        behind them (a negative length: the sequence takes no part).  ``positions``, ``(S,)`` or ``(B, S)``: those of
-        the tokens; steps go on behind the last valid one (a sequence without tokens: at the first)."""
+        """``lengths`` int32 ``(B,)``: valid tokens of each sequence; what lies behind may hold anything and is taken
+        for zeros.  ``cache`` takes the history in; with ``lengths`` each sequence's valid tokens only, so that its
+        steps go on behind them (a negative length: the sequence takes no part).  ``positions``, ``(S,)`` or
+        ``(B, S)``: those of the tokens; steps go on behind the last valid one (a sequence without tokens: at the
+        first)."""
         if lengths is not None:
             x = without_padding(x, lengths)
         for i, layer in enumerate(self.layers):

@@ -2,8 +2,9 @@
 
 ``norm = sqrt(Σ g²)`` over every gradient, ``g ← g · min(1, max_norm / (norm + 1e-6))`` — the rule of
 ``torch.nn.utils.clip_grad_norm_`` — in one read for the norm and one read and write for the result, whatever
-the number of tensors.  The squares are summed in fp64 in a fixed order, so the norm neither overflows nor
-depends on the run.  Nothing synchronises with the host: the norm stays a 0-d device tensor, and a call can be
+the number of tensors.  The squares of 16 bytes of values are added in fp32 (in fp64 where they leave its range) and
+from there on in fp64, in a fixed order, so the norm neither overflows nor depends on the run.  The calls have no
+gradient; the tensors they write may not overlap each other or gradients still to be read.  Nothing synchronises with the host: the norm stays a 0-d device tensor, and a call can be
 captured in a CUDA graph.
 
 With ``out`` the clipped gradients go to other buffers of the same shapes: bf16 gradients can be widened to the

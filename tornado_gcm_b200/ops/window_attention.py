@@ -65,9 +65,12 @@ def window_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, windo
     """``(B, S, H, D)`` attention of ``q (B, S, H, D)`` over ``k, v (B, S, Hk, D)``; ``Hk`` divides ``H``.
 
     bf16 or fp32, ``D`` up to 128, any strides with a contiguous last axis.  ``lengths``: int32 ``(B,)``, the number
-    of valid keys of every sequence (what lies behind may hold anything, NaN included); a query that sees no key, or
-    scores of minus infinity alone, gives zeros and no gradient, one that sees a score of NaN or plus infinity gives NaN.  ``scale`` (positive)
-    defaults to ``D ** -0.5``.
+    of valid keys of every sequence (keys and values behind may hold anything, NaN included; the queries there are
+    computed like any other, and what they hold reaches the gradients of the keys they see).  A query that sees no
+    key, or scores of minus infinity alone, gives zeros and no gradient, one that sees a score of NaN or plus infinity
+    gives NaN.  A valid key's value, or in the backward pass any operand, that is not finite may also reach what lies
+    in one block of 128 tokens with those that see it: the tensor cores multiply whole tiles, masked weights being
+    zeros.  ``scale`` (positive) defaults to ``D ** -0.5``.
     """
     if window < 1:
         raise ValueError(f"window_attention: the window must hold at least the token itself, got {window}")

@@ -233,7 +233,7 @@ class GCMTrainer:
         (one host synchronisation; 0 leaves the check to the caller, see
         :meth:`check_device_errors`).
         ``native_clip``: clip with :func:`tornado_gcm_b200.ops.gradnorm.clip_grad_norm` (two
-        launches for all parameters, fp64 sum) instead of ``torch.nn.utils.clip_grad_norm_``;
+        launches for up to 960 tensors, partial sums in fp64) instead of ``torch.nn.utils.clip_grad_norm_``;
         the sharded optimizer clips its own chunk either way."""
         self.gcm = gcm
         params = [p for p in gcm.parameters() if p.requires_grad]
