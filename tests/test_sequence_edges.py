@@ -206,6 +206,21 @@ def test_window_step_has_no_gradient_and_says_so(dtype):
             assert torch.equal(window_attention_step(*ts, n), want)
 
 
+def test_a_table_that_requires_a_gradient_is_refused():
+    """The kernels have none for the table; on the CPU it can be learned."""
+    from tornado_gcm_b200.ops.rotary import qk_norm_rotary, rotary_table
+
+    q = _randn(1, 6, 2, 32, seed=1)
+    want = qk_norm_rotary(q, q, rotary_table(6, 32, device=DEV), norm="rms")
+    table = rotary_table(6, 32, device=DEV).requires_grad_()
+    for x in (q, q.clone().requires_grad_()):
+        with pytest.raises(RuntimeError, match="no gradient for the table"):
+            qk_norm_rotary(x, x, table, norm="rms")
+        with torch.no_grad():
+            got = qk_norm_rotary(x, x, table, norm="rms")
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
 def test_writes_are_seen_by_autograd():
     """A value that a graph has saved and an operator then overwrites is an error, not a wrong gradient."""
     from tornado_gcm_b200.ops.gradnorm import clip_grad_norm

@@ -184,6 +184,7 @@ std::tuple<at::Tensor, at::Tensor> qk_norm_rotary_autograd(
     const OptTensor& kw, const OptTensor& qb, const OptTensor& kb, int64_t norm, bool interleaved, double eps,
     const OptTensor& err) {
   refuse_forward_mode("qk_norm_rotary", q, k, table, qw, kw, qb, kb);
+  TORCH_CHECK(!at::GradMode::is_enabled() || !wants(table), "qk_norm_rotary: no gradient for the table");
   if (at::GradMode::is_enabled() && (wants(q) || wants(k) || wants(qw) || wants(kw) || wants(qb) || wants(kb))) {
     auto r = QKNormRotary::apply(q, k, table, positions, qw, kw, qb, kb, norm, interleaved, eps, err);
     return {r[0], r[1]};

@@ -92,7 +92,8 @@ def qk_norm_rotary(q: torch.Tensor, k: torch.Tensor, table: Optional[torch.Tenso
     """Normalised and rotated ``q (B, S, H, D)`` and ``k (B, S, Hk, D)`` (bf16 or fp32, any strides with a
     contiguous last axis: slices of a packed projection need no copy).
 
-    ``table``: :func:`rotary_table`; its width sets how much of the head turns, ``None`` turns nothing.
+    ``table``: :func:`rotary_table`; its width sets how much of the head turns, ``None`` turns nothing.  On the GPU it
+    has no gradient, and one that requires it is refused.
     ``positions``: rows of the table, int32 or int64, ``(B, S)`` or ``(S,)``; ``None`` means 0 … S-1.  A position
     outside the table is reported through the device error flag (:func:`tornado_gcm_b200.ops._ext.check_error_flag`)
     and takes the nearest row; on the CPU it raises ``IndexError``.  ``norm``: ``"layer"``, ``"rms"`` or ``"none"``; weights and shifts are fp32 vectors
